@@ -1,0 +1,159 @@
+// What the forward and backward kernels of attention over visible key ranges share: parameters,
+// the score of a (query, key) pair, bit masks of visible keys, tensor maps.
+#pragma once
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <climits>
+
+#include "gemm_kernel.cuh"
+#include "kernels_doc.h"
+
+namespace oxi {
+namespace {
+
+constexpr int DA_THREADS = 320;  // TMA warp, MMA warp, 8 softmax / epilogue warps
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct DaParams {
+  int B, S, Hq, Hk, Dqk, Dv, nt;
+  float scale;
+  float x_scale;  // scale, or scale / cap: what the dot product is multiplied by before tanh
+  float c_log2;   // factor of x in the exponent of 2: scale * log2 e, or cap * log2 e
+  int causal;
+  const float* slopes;
+  const int* lo;
+  const int* hi;
+  const int4* qt;
+  const int4* kt;
+  int* status;
+};
+
+// tanh(x) = sign(x) (1 - d) with d = 2 / (1 + e^(2|x|)): two special-function operations, absolute
+// error a few 1e-7 (the score is cap times it, so its error is far below that of the bf16
+// probabilities).  Its derivative 1 - tanh^2 = d (2 - d) keeps its relative accuracy at the cap,
+// where 1 - t * t would be nothing but rounding.
+__device__ __forceinline__ float tanh_rest(float x) {
+  return __fdividef(2.f, 1.f + ex2_approx(fabsf(x) * (2.f * LOG2E)));
+}
+__device__ __forceinline__ float tanh_ex2(float x) { return copysignf(1.f - tanh_rest(x), x); }
+__device__ __forceinline__ float tanh_ex2(float x, float& derivative) {
+  const float d = tanh_rest(x);
+  derivative = fmaf(-d, d, 2.f * d);
+  return copysignf(1.f - d, x);
+}
+
+// Visible keys of a row within 32 consecutive keys from k: bit t is key k + t in [lo, hi).
+__device__ __forceinline__ uint32_t range_bits(int lo, int hi, int k) {
+  const int a = max(lo - k, 0), e = min(hi - k, 32);
+  if (e <= a) return 0u;
+  return (0xffffffffu << a) & (0xffffffffu >> (32 - e));
+}
+
+struct TileRange {
+  int begin, end;
+};
+// Key tiles that a query tile looks at.
+__device__ __forceinline__ TileRange key_tiles(const DaParams& p, int b, int qt) {
+  if (qt >= p.nt) return {0, 0};
+  if (!p.qt) return {0, p.causal ? min(qt + 1, p.nt) : p.nt};
+  const int4 t = __ldg(p.qt + (int64_t)b * p.nt + qt);
+  if (t.y <= t.x) return {0, 0};
+  return {t.x / DA_TILE, (t.y + DA_TILE - 1) / DA_TILE};
+}
+// Query tiles that look at a key tile.
+__device__ __forceinline__ TileRange query_tiles(const DaParams& p, int b, int kt) {
+  if (!p.kt) return {p.causal ? kt : 0, p.nt};
+  const int4 t = __ldg(p.kt + (int64_t)b * p.nt + kt);
+  return {t.x, t.y};
+}
+// Visible keys of one token (none for one past the end of the row).
+__device__ __forceinline__ TileRange key_range(const DaParams& p, int b, int i) {
+  if (i >= p.S) return {0, 0};
+  if (!p.lo) return {0, p.causal ? i + 1 : p.S};
+  return {__ldg(p.lo + (int64_t)b * p.S + i), __ldg(p.hi + (int64_t)b * p.S + i)};
+}
+__device__ __forceinline__ bool tile_has_pad(const DaParams& p, int b, int kt) {
+  return p.kt && __ldg(&p.kt[(int64_t)b * p.nt + kt].z) != 0;
+}
+
+__device__ __forceinline__ uint64_t da_kmajor_desc(uint32_t base, int kk, uint32_t block_bytes) {
+  return umma_desc_sw128(base + (kk >> 2) * block_bytes + (kk & 3) * 32, 16, 1024);
+}
+
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* tmap, uint64_t* bar, int c0, int c1, int c2,
+                                            int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+// Zero the rows of a 128-row operand tile (BLOCKS blocks of 64 columns, 128 bytes a row) that hold padding tokens: their
+// contents may be anything, and 0 x NaN would reach rows that do not see them.  n threads, this one t.
+template <int BLOCKS>
+__device__ __forceinline__ void zero_pad_rows(uint8_t* tile, const DaParams& p, int b, int pos0, int t, int n) {
+  for (int r = t; r < DA_TILE; r += n) {
+    const TileRange v = key_range(p, b, pos0 + r);
+    if (v.end > v.begin) continue;
+#pragma unroll 1
+    for (int q = 0; q < BLOCKS * 8; ++q)
+      *reinterpret_cast<uint4*>(tile + (q >> 3) * (DA_TILE * 128) + r * 128 + (q & 7) * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
+}
+
+// Tensor map over [B, S, H, D]: boxes of 64 columns x 128 tokens of one head, 128-byte swizzle.
+// Columns past D and tokens past S read as zero, so a head width need not be a multiple of 64 and
+// a row's last tile never reads the next row.
+inline CUtensorMap da_tmap(const DaTensor& t, int B, int S, int H, int D) {
+  OXI_CHECK((reinterpret_cast<uintptr_t>(t.ptr) & 15) == 0, "TMA base must be 16-byte aligned");
+  OXI_CHECK(t.sb % 8 == 0 && t.ss % 8 == 0 && t.sh % 8 == 0 && D % 8 == 0, "TMA strides must be multiples of 16 bytes");
+  ensure_current_context();
+  CUtensorMap m;
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)S, (cuuint64_t)B};
+  cuuint64_t strides[3] = {(cuuint64_t)(t.sh * 2), (cuuint64_t)(t.ss * 2), (cuuint64_t)(t.sb * 2)};
+  cuuint32_t box[4] = {64, 1, DA_TILE, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = get_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(t.ptr), dims, strides, box,
+                               estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  OXI_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (attention operand) failed: ", (int)r);
+  return m;
+}
+
+inline DaParams da_params(const DaShape& s, int* status) {
+  DaParams p;
+  p.B = s.B; p.S = s.S; p.Hq = s.Hq; p.Hk = s.Hk; p.Dqk = s.Dqk; p.Dv = s.Dv;
+  p.nt = (s.S + DA_TILE - 1) / DA_TILE;
+  p.scale = s.scale;
+  p.x_scale = s.cap > 0.f ? s.scale / s.cap : s.scale;
+  p.c_log2 = (s.cap > 0.f ? s.cap : s.scale) * LOG2E;
+  p.causal = s.causal;
+  p.slopes = s.slopes;
+  p.lo = s.lo; p.hi = s.hi;
+  p.qt = reinterpret_cast<const int4*>(s.qt);
+  p.kt = reinterpret_cast<const int4*>(s.kt);
+  p.status = status;
+  return p;
+}
+
+inline void da_check(const DaShape& s) {
+  OXI_CHECK(da_supported(s.Dqk, s.Dv), "attention over key ranges: head widths (qk ", s.Dqk, ", v ", s.Dv,
+            ") must be multiples of 8 up to 128");
+  OXI_CHECK(s.Hk > 0 && s.Hq % s.Hk == 0, "query heads ", s.Hq, " must be a multiple of key heads ", s.Hk);
+  OXI_CHECK(s.scale > 0.f && s.cap >= 0.f, "scale must be positive and the cap not negative");
+  OXI_CHECK(s.B <= 65535 && s.Hq <= 65535, "batch and heads of at most 65535");
+  OXI_CHECK((s.lo != nullptr) == (s.hi != nullptr) && (s.lo != nullptr) == (s.qt != nullptr) &&
+                (s.lo != nullptr) == (s.kt != nullptr), "ranges and tile tables come together");
+}
+
+// Shared memory attribute of a kernel, set before every launch: it belongs to the current device.
+template <typename K>
+inline void da_smem(K kern, int bytes) {
+  OXI_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+}
+
+}  // namespace
+}  // namespace oxi

@@ -7,6 +7,7 @@
 #include "kernels.h"
 #include "kernels_ew.h"
 #include "kernels_attn.h"
+#include "kernels_doc.h"
 #include "kernels_comm.h"
 #include "kernels_mla.h"
 #include "kernels_ssm.h"
@@ -347,6 +348,113 @@ void flash_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor 
 
 bool flash_supported(int64_t Dqk, int64_t Dv, bool backward) {
   return backward ? oxi::fa_bwd_supported((int)Dqk, (int)Dv) : oxi::fa_supported((int)Dqk, (int)Dv);
+}
+
+// ------------------------------------------------------------ attention over visible key ranges
+std::vector<torch::Tensor> document_mask(torch::Tensor tokens, c10::optional<torch::Tensor> prefix,
+                                         c10::optional<int64_t> separator, c10::optional<int64_t> pad, bool causal) {
+  OXI_CHECK(tokens.is_cuda() && tokens.dim() == 2 && tokens.scalar_type() == torch::kInt64 &&
+                  (tokens.stride(1) == 1 || tokens.size(1) <= 1), "document_mask: tokens must be CUDA int64 [B, S] rows");
+  c10::cuda::CUDAGuard g(tokens.device());
+  const int64_t B = tokens.size(0), S = tokens.size(1);
+  OXI_CHECK(S <= oxi::DOC_MAX_SEQ, "document_mask: rows of at most ", oxi::DOC_MAX_SEQ, " tokens, got ", S);
+  const uint8_t* pre = nullptr;
+  int64_t ldp = 0;
+  if (prefix.has_value() && prefix->defined()) {
+    OXI_CHECK(prefix->device() == tokens.device() && prefix->sizes() == tokens.sizes() &&
+                    prefix->scalar_type() == torch::kBool && (prefix->stride(1) == 1 || S <= 1),
+                "document_mask: prefix must be bool like the tokens, on their device");
+    OXI_CHECK(causal, "document_mask: a prefix needs a causal mask");
+    pre = reinterpret_cast<const uint8_t*>(prefix->data_ptr<bool>());
+    ldp = prefix->stride(0);
+  }
+  const int64_t nt = (S + oxi::DA_TILE - 1) / oxi::DA_TILE;
+  auto opt = torch::TensorOptions().dtype(torch::kInt32).device(tokens.device());
+  auto lo = torch::empty({B, S}, opt), hi = torch::empty({B, S}, opt);
+  auto qt = torch::empty({B, nt, 4}, opt), kt = torch::empty({B, nt, 4}, opt);
+  oxi::launch_document_mask(tokens.data_ptr<int64_t>(), tokens.stride(0), pre, ldp, (int)B, (int)S,
+                            separator.has_value(), separator.value_or(0), pad.has_value(), pad.value_or(0), causal,
+                            lo.data_ptr<int>(), hi.data_ptr<int>(), qt.data_ptr<int>(), kt.data_ptr<int>(), stream());
+  return {lo, hi, qt, kt};
+}
+
+oxi::DaTensor da_tensor(const torch::Tensor& t, const torch::Tensor& like, const char* what) {
+  OXI_CHECK(t.is_cuda() && t.device() == like.device(), "attention: ", what, " must be on the device of q");
+  OXI_CHECK(t.dim() == 4 && t.scalar_type() == torch::kBFloat16 && t.stride(3) == 1, "attention: ", what,
+              " must be bf16 [B, S, H, D] with unit inner stride");
+  return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
+}
+
+oxi::DaShape da_shape(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, double scale, double cap,
+                      const c10::optional<torch::Tensor>& slopes, bool causal,
+                      const std::vector<torch::Tensor>& mask) {
+  oxi::DaShape s{};
+  OXI_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "attention: q, k, v must be [B, S, H, D]");
+  s.B = (int)q.size(0); s.S = (int)q.size(1); s.Hq = (int)q.size(2); s.Hk = (int)k.size(2);
+  s.Dqk = (int)q.size(3); s.Dv = (int)v.size(3);
+  OXI_CHECK(k.size(0) == s.B && v.size(0) == s.B && k.size(1) == s.S && v.size(1) == s.S && v.size(2) == s.Hk &&
+                  k.size(3) == s.Dqk, "attention: q, k, v do not go together");
+  OXI_CHECK(s.Hk > 0 && s.Hq % s.Hk == 0, "attention: query heads must be a multiple of key heads");
+  s.scale = (float)scale;
+  s.cap = (float)cap;
+  s.causal = causal;
+  if (slopes.has_value() && slopes->defined()) {
+    OXI_CHECK(slopes->device() == q.device() && slopes->scalar_type() == torch::kFloat32 && slopes->dim() == 1 &&
+                    slopes->numel() == s.Hq && slopes->is_contiguous(), "attention: alibi must be f32 [Hq] on q's device");
+    s.slopes = slopes->data_ptr<float>();
+  }
+  if (!mask.empty()) {
+    OXI_CHECK(mask.size() == 4, "attention: mask = lo, hi, query tiles, key tiles");
+    const int64_t nt = (s.S + oxi::DA_TILE - 1) / oxi::DA_TILE;
+    for (size_t i = 0; i < 4; ++i) {
+      const auto& m = mask[i];
+      OXI_CHECK(m.device() == q.device() && m.scalar_type() == torch::kInt32 && m.is_contiguous() &&
+                      m.numel() == (i < 2 ? (int64_t)s.B * s.S : (int64_t)s.B * nt * 4),
+                  "attention: the mask was built for another batch or device");
+    }
+    s.lo = mask[0].data_ptr<int>(); s.hi = mask[1].data_ptr<int>();
+    s.qt = mask[2].data_ptr<int>(); s.kt = mask[3].data_ptr<int>();
+  }
+  return s;
+}
+
+std::vector<torch::Tensor> doc_attn_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, double scale, double cap,
+                                        c10::optional<torch::Tensor> slopes, bool causal,
+                                        std::vector<torch::Tensor> mask, torch::Tensor status) {
+  c10::cuda::CUDAGuard g(q.device());
+  const oxi::DaShape s = da_shape(q, k, v, scale, cap, slopes, causal, mask);
+  const auto tq = da_tensor(q, q, "q"), tk = da_tensor(k, q, "k"), tv = da_tensor(v, q, "v");
+  auto o = torch::empty({s.B, s.S, s.Hq, s.Dv}, q.options());
+  auto lse2 = torch::empty({s.B, s.Hq, s.S}, q.options().dtype(torch::kFloat32));
+  oxi::launch_da_fwd(s, tq, tk, tv, {o.data_ptr(), (int64_t)s.Hq * s.Dv}, lse2.data_ptr<float>(), status_ptr(status),
+                     stream());
+  return {o, lse2};
+}
+
+// dq, dk, dv: bf16 [B * S, H * D] views with unit inner stride (columns of one buffer, say)
+void doc_attn_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o, torch::Tensor dout,
+                  torch::Tensor lse2, double scale, double cap, c10::optional<torch::Tensor> slopes, bool causal,
+                  std::vector<torch::Tensor> mask, torch::Tensor dq, torch::Tensor dk, torch::Tensor dv,
+                  torch::Tensor status) {
+  c10::cuda::CUDAGuard g(q.device());
+  const oxi::DaShape s = da_shape(q, k, v, scale, cap, slopes, causal, mask);
+  const auto tq = da_tensor(q, q, "q"), tk = da_tensor(k, q, "k"), tv = da_tensor(v, q, "v"),
+             to = da_tensor(o, q, "o"), td = da_tensor(dout, q, "dout");
+  OXI_CHECK(o.sizes() == dout.sizes() && o.size(0) == s.B && o.size(1) == s.S && o.size(2) == s.Hq &&
+                  o.size(3) == s.Dv, "attention backward: o and dout must be [B, S, Hq, Dv]");
+  OXI_CHECK(lse2.device() == q.device() && lse2.scalar_type() == torch::kFloat32 && lse2.is_contiguous() &&
+                  lse2.numel() == (int64_t)s.B * s.Hq * s.S, "attention backward: lse2");
+  const int64_t rows = (int64_t)s.B * s.S;
+  const int64_t cols[3] = {(int64_t)s.Hq * s.Dqk, (int64_t)s.Hk * s.Dqk, (int64_t)s.Hk * s.Dv};
+  const torch::Tensor outs[3] = {dq, dk, dv};
+  for (int i = 0; i < 3; ++i)
+    OXI_CHECK(outs[i].device() == q.device() && outs[i].scalar_type() == torch::kBFloat16 && outs[i].dim() == 2 &&
+                  outs[i].size(0) == rows && outs[i].size(1) == cols[i] && outs[i].stride(1) == 1,
+              "attention backward: gradients must be bf16 [B * S, H * D] on q's device");
+  auto delta = torch::empty_like(lse2);
+  oxi::launch_da_bwd(s, tq, tk, tv, to, td, lse2.data_ptr<float>(), delta.data_ptr<float>(),
+                     {dq.data_ptr(), dq.stride(0)}, {dk.data_ptr(), dk.stride(0)}, {dv.data_ptr(), dv.stride(0)},
+                     status_ptr(status), stream());
 }
 
 // ------------------------------------------------------------ NVLink DDP runtime
@@ -1180,6 +1288,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ce_bwd", &ce_bwd, "in-place softmax-minus-onehot gradient of the logits (of a column chunk from col0)",
         py::arg("logits"), py::arg("V"), py::arg("lse"), py::arg("targets"), py::arg("gscale"), py::arg("inv_count"),
         py::arg("col0") = 0);
+  m.def("document_mask", &document_mask, "visible key ranges and tile tables of packed documents");
+  m.def("doc_attn_fwd", &doc_attn_fwd, "attention over visible key ranges, forward");
+  m.def("doc_attn_bwd", &doc_attn_bwd, "attention over visible key ranges, backward");
+  m.def("doc_attn_supported", [](int64_t Dqk, int64_t Dv) { return oxi::da_supported((int)Dqk, (int)Dv); });
   m.def("embed_fwd", &embed_fwd, "embedding gather");
   m.def("embed_bwd", &embed_bwd, "embedding scatter-add into f32 grad");
   m.def("rope_bwd_to", &rope_bwd_to, "out-of-place RoPE backward (+ copy of the unrotated columns)");

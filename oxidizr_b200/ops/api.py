@@ -171,14 +171,36 @@ def swiglu_mlp(x, w_gu, w_down, resid=None):
     return y if resid is None else resid + y
 
 
-def attention(q, k, v, scale: float, causal: bool = True):
-    from .attention import attention as _att
-    return _att(q, k, v, scale, causal)
+def document_mask(tokens, separator=None, pad=None, prefix=None, causal: bool = True):
+    """Visible keys of a batch of packed documents, for the attention of every layer.
+
+    tokens [B, S]: document ids (a document is a run of one id; negative ids are padding), or, with
+    ``separator``, token ids whose documents end with that token (``pad``: a token id that is padding).
+    ``prefix`` (bool [B, S]): the leading flagged run of each document is visible to all of it.
+    """
+    from .doc_attention import document_mask as _dm
+    return _dm(tokens, separator, pad, prefix, causal)
 
 
-def attention_qkv(qkv, Hq: int, Hk: int, D: int, scale: float, causal: bool = True):
-    from .attention import attention_qkv as _aq
-    return _aq(qkv, Hq, Hk, D, scale, causal)
+def attention(q, k, v, scale: float, causal: bool = True, mask=None, softcap: float = 0.0, alibi=None):
+    """q [B, S, Hq, Dqk], k [B, S, Hk, Dqk], v [B, S, Hk, Dv] -> [B, S, Hq, Dv].  ``mask`` from
+    document_mask, ``softcap`` c: scores pass through c tanh(./c), ``alibi`` f32 [Hq]: slopes of a bias
+    -slope |i - j| added after the cap."""
+    if mask is None and not softcap and alibi is None:
+        from .attention import attention as _att
+        return _att(q, k, v, scale, causal)
+    from .doc_attention import attention as _doc
+    return _doc(q, k, v, scale, causal, mask, softcap or 0.0, alibi)
+
+
+def attention_qkv(qkv, Hq: int, Hk: int, D: int, scale: float, causal: bool = True, mask=None, softcap: float = 0.0,
+                  alibi=None):
+    """``attention`` from the fused [B, S, (Hq + 2 Hk) D] projection; returns [B, S, Hq D]."""
+    if mask is None and not softcap and alibi is None:
+        from .attention import attention_qkv as _aq
+        return _aq(qkv, Hq, Hk, D, scale, causal)
+    from .doc_attention import attention_qkv as _doc
+    return _doc(qkv, Hq, Hk, D, scale, causal, mask, softcap or 0.0, alibi)
 
 
 def linear_cross_entropy(x, w, targets, ignore_index: int = -100):

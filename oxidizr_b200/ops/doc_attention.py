@@ -1,0 +1,199 @@
+"""Causal attention over packed documents: visible key ranges, capped scores, a distance bias.
+
+A block of training tokens holds several documents one after another.  ``document_mask`` turns a
+batch into the range of keys that each token sees: its own document up to itself, or, for a
+document that opens with a prompt, at least that prompt.  Attention over it is
+
+    z_ij = scale q_i . k_j,  u = cap tanh(z / cap) (without a cap: z),  a = u - slope_h |i - j|
+    o_i  = sum_{lo_i <= j < hi_i} softmax(a_i)_j v_j
+
+and a token that sees nothing (padding) gets zeros and passes no gradient on.  What padding rows of
+q, k, v and the output's gradient hold does not matter, not even NaN.
+
+bf16 CUDA tensors with head widths that are multiples of 8 up to 128 run csrc/doc_attn_fwd.cu and
+csrc/doc_attn_bwd.cu; everything else runs the statement of the same math in ``ops.reference``.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import reference as R
+
+MAX_SEQ = 1 << 18  # DOC_MAX_SEQ of csrc/kernels_doc.h: the bit masks of a row stay in shared memory
+
+
+@dataclass(frozen=True)
+class DocMask:
+    """Visible keys of a batch: token i of row b sees keys ``lo[b, i] <= j < hi[b, i]`` (int32 [B, S]).
+
+    On CUDA ``qt`` / ``kt`` are the tile tables that the kernels walk.  One mask serves every layer
+    of the step it was built for.
+    """
+    lo: torch.Tensor
+    hi: torch.Tensor
+    qt: Optional[torch.Tensor]
+    kt: Optional[torch.Tensor]
+    causal: bool
+
+    def tensors(self):
+        return [self.lo, self.hi, self.qt, self.kt]
+
+
+def document_mask(tokens: torch.Tensor, separator: Optional[int] = None, pad: Optional[int] = None,
+                  prefix: Optional[torch.Tensor] = None, causal: bool = True) -> DocMask:
+    if tokens.dim() != 2 or tokens.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"document_mask: tokens must be int64 or int32 [B, S], got {tokens.dtype} "
+                         f"{list(tokens.shape)}")
+    if pad is not None and separator is None:
+        raise ValueError("document_mask: pad goes with a separator; document ids mark padding by a negative id")
+    if prefix is not None:
+        if not causal:
+            raise ValueError("document_mask: a prefix needs a causal mask")
+        if prefix.dtype != torch.bool or prefix.shape != tokens.shape or prefix.device != tokens.device:
+            raise ValueError("document_mask: prefix must be bool, of the tokens' shape and on their device")
+    tokens = tokens.long()
+    if tokens.is_cuda:
+        if tokens.shape[1] > MAX_SEQ:
+            raise ValueError(f"document_mask: rows of at most {MAX_SEQ} tokens, got {tokens.shape[1]}")
+        from ._C import ext
+        if tokens.stride(1) != 1:
+            tokens = tokens.contiguous()
+        if prefix is not None and prefix.stride(1) != 1:
+            prefix = prefix.contiguous()
+        lo, hi, qt, kt = ext().document_mask(tokens, prefix, separator, pad, causal)
+        return DocMask(lo, hi, qt, kt, causal)
+    lo, hi = R.document_ranges(tokens, separator, pad, prefix, causal)
+    return DocMask(lo, hi, None, None, causal)
+
+
+def _kernel_ok(q, k, v) -> bool:
+    if not (q.is_cuda and q.dtype == torch.bfloat16 and k.dtype == q.dtype and v.dtype == q.dtype):
+        return False
+    from ._C import ext
+    return ext().doc_attn_supported(q.shape[-1], v.shape[-1])
+
+
+def _check(q, k, v, scale, causal, mask, softcap, alibi):
+    B, S, Hq, D = q.shape
+    Hk = k.shape[2]
+    if k.shape != (B, S, Hk, D) or v.shape[:3] != (B, S, Hk) or Hk == 0 or Hq % Hk:
+        raise ValueError(f"attention: q {list(q.shape)}, k {list(k.shape)}, v {list(v.shape)} do not go together")
+    if not scale > 0:
+        raise ValueError(f"attention: scale must be positive, got {scale}")
+    if not 0 <= softcap < float("inf"):
+        raise ValueError(f"attention: softcap must be a positive number, or 0 for none, got {softcap}")
+    if mask is not None:
+        if mask.lo.shape != (B, S) or mask.lo.device != q.device:
+            raise ValueError(f"attention: the mask is for {list(mask.lo.shape)} on {mask.lo.device}, "
+                             f"q for {[B, S]} on {q.device}")
+        if mask.causal != causal:
+            raise ValueError(f"attention: causal={causal} with a mask built for causal={mask.causal}")
+    if alibi is not None:
+        if alibi.shape != (Hq,) or alibi.device != q.device:
+            raise ValueError(f"attention: alibi must be one slope per query head [{Hq}] on {q.device}")
+        if alibi.requires_grad:
+            raise ValueError("attention: alibi slopes are constants, no gradient is computed for them")
+
+
+def _tma_view(t: torch.Tensor) -> torch.Tensor:
+    """t itself where the tensor maps can address it, else a contiguous copy.  The stride of a
+    dimension of one element is never used, and is replaced where it would not be a valid one."""
+    B, S, H, D = t.shape
+    st = list(t.stride())
+    for d in (0, 1, 2):
+        if t.shape[d] == 1:
+            st[d] = D
+    if st[3] == 1 and t.data_ptr() % 16 == 0 and all(s > 0 and s % 8 == 0 for s in st[:3]):
+        return t.as_strided(t.shape, st)
+    return t.contiguous()
+
+
+class DocAttention(torch.autograd.Function):
+    """q [B, S, Hq, Dqk], k [B, S, Hk, Dqk], v [B, S, Hk, Dv] views -> o [B, S, Hq, Dv]."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, scale: float, cap: float, slopes, causal: bool, mask):
+        o, lse2 = _fwd(q, k, v, scale, cap, slopes, causal, mask)
+        ctx.save_for_backward(q, k, v, o, lse2, slopes, *mask)
+        ctx.cfg = (scale, cap, causal)
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        q, k, v, o, lse2, slopes, *mask = ctx.saved_tensors
+        outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
+        _bwd(ctx, q, k, v, o, do, lse2, slopes, mask, [t.flatten(0, 1).flatten(1) for t in outs])
+        return (*outs, None, None, None, None, None)
+
+
+class DocAttentionQKV(torch.autograd.Function):
+    """The same from the fused projection [B, S, (Hq + 2 Hk) D] -> [B, S, Hq D]; the gradient is
+    written in the projection's layout, with no assembly of slices."""
+
+    @staticmethod
+    def forward(ctx, qkv, Hq: int, Hk: int, D: int, scale: float, cap: float, slopes, causal: bool, mask):
+        q, k, v = _heads(qkv, Hq, Hk, D)
+        o, lse2 = _fwd(q, k, v, scale, cap, slopes, causal, mask)
+        ctx.save_for_backward(qkv, o, lse2, slopes, *mask)
+        ctx.cfg, ctx.heads = (scale, cap, causal), (Hq, Hk, D)
+        return o.flatten(2)
+
+    @staticmethod
+    def backward(ctx, do):
+        qkv, o, lse2, slopes, *mask = ctx.saved_tensors
+        Hq, Hk, D = ctx.heads
+        q, k, v = _heads(qkv, Hq, Hk, D)
+        dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        d2 = dqkv.flatten(0, 1)
+        a, b = Hq * D, (Hq + Hk) * D
+        _bwd(ctx, q, k, v, o, do.reshape(o.shape), lse2, slopes, mask, [d2[:, :a], d2[:, a:b], d2[:, b:]])
+        return (dqkv, *[None] * 8)
+
+
+def _heads(qkv, Hq, Hk, D):
+    return (t.unflatten(-1, (-1, D)) for t in qkv.split([Hq * D, Hk * D, Hk * D], -1))
+
+
+def _fwd(q, k, v, scale, cap, slopes, causal, mask):
+    from ._C import ext, status
+    return ext().doc_attn_fwd(_tma_view(q), _tma_view(k), _tma_view(v), scale, cap, slopes, causal, list(mask),
+                              status(q.device))
+
+
+def _bwd(ctx, q, k, v, o, do, lse2, slopes, mask, outs):
+    from ._C import ext, status
+    scale, cap, causal = ctx.cfg
+    ext().doc_attn_bwd(_tma_view(q), _tma_view(k), _tma_view(v), o, _tma_view(do), lse2, scale, cap, slopes, causal,
+                       list(mask), *outs, status(q.device))
+
+
+def _reference(q, k, v, scale, causal, mask, softcap, alibi):
+    lo, hi = (mask.lo, mask.hi) if mask is not None else R.plain_ranges(q.shape[0], q.shape[1], causal, q.device)
+    o = R.attention_ranges(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), scale, lo, hi, softcap, alibi)
+    return o.transpose(1, 2)
+
+
+def _slopes(alibi):
+    return None if alibi is None else alibi.float().contiguous()
+
+
+def attention(q, k, v, scale: float, causal: bool = True, mask: Optional[DocMask] = None, softcap: float = 0.0,
+              alibi: Optional[torch.Tensor] = None) -> torch.Tensor:
+    _check(q, k, v, scale, causal, mask, softcap, alibi)
+    if _kernel_ok(q, k, v):
+        m = mask.tensors() if mask is not None else []
+        return DocAttention.apply(q, k, v, float(scale), float(softcap), _slopes(alibi), causal, m)
+    return _reference(q, k, v, scale, causal, mask, softcap, alibi)
+
+
+def attention_qkv(qkv, Hq: int, Hk: int, D: int, scale: float, causal: bool = True, mask: Optional[DocMask] = None,
+                  softcap: float = 0.0, alibi: Optional[torch.Tensor] = None) -> torch.Tensor:
+    q, k, v = _heads(qkv, Hq, Hk, D)
+    _check(q, k, v, scale, causal, mask, softcap, alibi)
+    if _kernel_ok(q, k, v):
+        m = mask.tensors() if mask is not None else []
+        return DocAttentionQKV.apply(qkv, Hq, Hk, D, float(scale), float(softcap), _slopes(alibi), causal, m)
+    return _reference(q, k, v, scale, causal, mask, softcap, alibi).flatten(2)

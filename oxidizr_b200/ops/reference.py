@@ -72,6 +72,70 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, c
     return torch.matmul(p, v)
 
 
+def plain_ranges(B: int, S: int, causal: bool, device) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Visible key ranges [lo, hi) of every token without documents."""
+    lo = torch.zeros(B, S, dtype=torch.int32, device=device)
+    hi = torch.arange(1, S + 1, dtype=torch.int32, device=device) if causal else torch.full_like(lo[0], S)
+    return lo, hi.expand(B, S)
+
+
+def document_ranges(tokens: torch.Tensor, separator: Optional[int] = None, pad: Optional[int] = None,
+                    prefix: Optional[torch.Tensor] = None, causal: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Visible key ranges [lo, hi) of packed documents, int32 [B, S].
+
+    A document is a run of equal ids, or with a separator what ends with it.  A token sees its document
+    up to itself (without ``causal``: all of it) and the document's leading run of ``prefix`` flags;
+    padding (a negative id, or the token ``pad``) sees nothing and is its own run.
+    """
+    B, S = tokens.shape
+    pos = torch.arange(S, device=tokens.device).expand(B, S)
+    is_pad = (tokens < 0) if separator is None else (
+        tokens == pad if pad is not None else torch.zeros_like(tokens, dtype=torch.bool))
+    start = torch.ones_like(is_pad)
+    if separator is None:
+        start[:, 1:] = tokens[:, 1:] != tokens[:, :-1]
+    else:
+        start[:, 1:] = (tokens[:, :-1] == separator) | (is_pad[:, 1:] != is_pad[:, :-1])
+    lo = torch.where(start, pos, torch.zeros_like(pos)).cummax(1).values if S else pos
+
+    def stop_after(stop):  # the next marked position above each token, else S
+        at = torch.where(stop, pos, torch.full_like(pos, S))
+        at = torch.cat([at[:, 1:], torch.full_like(at[:, :1], S)], 1)
+        return at.flip(1).cummin(1).values.flip(1) if S else at
+
+    if not causal:
+        hi = stop_after(start)
+    else:
+        hi = pos + 1
+        if prefix is not None:
+            end = torch.where(prefix, stop_after(start | ~prefix), pos)
+            hi = torch.maximum(hi, end.gather(1, lo))
+    return lo.masked_fill(is_pad, 0).int(), hi.masked_fill(is_pad, 0).int()
+
+
+def attention_ranges(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, lo: torch.Tensor,
+                     hi: torch.Tensor, cap: float = 0.0, slopes: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention on [B, H, S, D] in which token i sees the keys lo <= j < hi, scores pass through
+    ``cap tanh(./cap)`` and then lose ``slope_h |i - j|``.  A token that sees nothing is padding: its
+    rows are taken as zeros, its output is zero."""
+    dt = torch.float64 if q.dtype == torch.float64 else torch.float32
+    hq, hk, S = q.shape[1], k.shape[1], q.shape[2]
+    empty = (hi <= lo)[:, None, :, None]
+    qf, kf, vf = (t.to(dt).masked_fill(empty, 0.0) for t in (q, k, v))
+    if hk != hq:
+        kf, vf = kf.repeat_interleave(hq // hk, dim=1), vf.repeat_interleave(hq // hk, dim=1)
+    a = torch.matmul(qf, kf.transpose(-1, -2)) * scale
+    if cap:
+        a = cap * torch.tanh(a / cap)
+    pos = torch.arange(S, device=q.device)
+    if slopes is not None:
+        a = a - slopes.to(dt).view(-1, 1, 1) * (pos[:, None] - pos).abs()
+    sees = ((pos >= lo[..., None]) & (pos < hi[..., None]))[:, None]
+    # a row that sees nothing is given every key (its output is dropped): no NaN in either pass
+    p = torch.softmax(a.masked_fill(~(sees | empty), float("-inf")), -1)
+    return torch.matmul(p, vf).masked_fill(empty, 0.0).to(v.dtype)
+
+
 # --------------------------------------------------------- cross entropy
 def cross_entropy(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
     """candle_nn::loss::cross_entropy mean over tokens (trainer.rs:166-171)."""

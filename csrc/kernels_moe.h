@@ -33,12 +33,22 @@ void launch_gemm_grouped(int mode, int epi, const Mat& a, bool a_mn, const Mat& 
                          const int* seg_off, int64_t group_rows_b, void* out, int64_t ldo, void* out2, int64_t ldo2,
                          const void* aux, int64_t ldaux, int* status, cudaStream_t st,
                          const GroupedScatter* scatter = nullptr);
-// Router (router.cu): logits [T, E] (bf16 or f32, row stride ld) -> top-k
-// indices / weights [T, k], mean routing probability usage [E] (f32), and
-// optional per-expert selection counts [E].
-void launch_router_fwd(const void* logits, bool bf16, int64_t ld, int64_t T, int E, int k, int64_t* topi, float* topw,
-                       float* usage, int* counts, cudaStream_t st);
-void launch_router_bwd(const void* logits, bool bf16, int64_t ld, int64_t T, int E, int k, const int64_t* topi,
-                       const float* topw, const float* dtopw, const float* dusage, void* dlogits, int64_t ldd,
+// Router (router.cu): logits [T, E] (bf16 or f32, row stride ld) -> the chosen experts topi and their
+// weights topw [T, k], mean normalised score usage [E] and selection counts [E].
+constexpr int ROUTE_MAX_EXPERTS = 512, ROUTE_MAX_K = 32, ROUTE_MAX_GROUPS = 32;
+struct RouteArgs {
+  int k;
+  bool sigmoid;                        // scores: sigmoid, else softmax
+  int groups, top_groups, group_top;   // groups 1: every expert takes part
+  bool renorm;
+  float scale;
+};
+int64_t route_workspace(int64_t T, int E);  // bytes
+// bias [E] f32 or null: added to the scores for the choice alone
+void launch_router_fwd(const void* logits, bool bf16, int64_t ld, int64_t T, int E, const RouteArgs& a,
+                       const float* bias, int64_t* topi, float* topw, float* usage, int* counts, void* workspace,
+                       cudaStream_t st);
+void launch_router_bwd(const void* logits, bool bf16, int64_t ld, int64_t T, int E, const RouteArgs& a,
+                       const int64_t* topi, const float* dtopw, const float* dusage, void* dlogits, int64_t ldd,
                        cudaStream_t st);
 }  // namespace oxi

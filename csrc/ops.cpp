@@ -8,6 +8,7 @@
 #include "kernels_ew.h"
 #include "kernels_attn.h"
 #include "kernels_doc.h"
+#include "kernels_embed.h"
 #include "kernels_comm.h"
 #include "kernels_mla.h"
 #include "kernels_ssm.h"
@@ -216,18 +217,46 @@ void ce_bwd(torch::Tensor logits, int64_t V, torch::Tensor lse, torch::Tensor ta
 }
 
 // ------------------------------------------------------------ embedding / rope
-void embed_fwd(torch::Tensor ids, torch::Tensor w, torch::Tensor out) {
-  c10::cuda::CUDAGuard g(w.device());
-  TORCH_CHECK(ids.scalar_type() == torch::kInt64 && ids.is_contiguous(), "ids must be contiguous int64");
-  TORCH_CHECK(w.scalar_type() == torch::kBFloat16 && w.is_contiguous() && out.is_contiguous(), "embedding tensors");
-  oxi::launch_embed_fwd(ids.data_ptr<int64_t>(), w.data_ptr(), out.data_ptr(), ids.numel(), (int)w.size(1), stream());
+void check_embedding(const torch::Tensor& ids, const torch::Tensor& w, const char* what) {
+  OXI_CHECK(w.is_cuda() && w.dim() == 2 && w.is_contiguous() &&
+                (w.scalar_type() == torch::kBFloat16 || w.scalar_type() == torch::kFloat32),
+            "embedding: ", what, " must be contiguous bf16 or f32 [rows, H] on a GPU");
+  OXI_CHECK(ids.device() == w.device() && ids.scalar_type() == torch::kInt64 && ids.is_contiguous(),
+            "embedding: ids must be contiguous int64 on the same device");
 }
 
-void embed_bwd(torch::Tensor ids, torch::Tensor dy, torch::Tensor dw) {
+torch::Tensor embedding_fwd(torch::Tensor ids, torch::Tensor w, double scale, torch::Tensor status) {
+  check_embedding(ids, w, "w");
+  c10::cuda::CUDAGuard g(w.device());
+  auto out = torch::empty({ids.numel(), w.size(1)}, w.options());
+  oxi::launch_embedding_fwd(ids.data_ptr<int64_t>(), w.data_ptr(), out.data_ptr(),
+                            w.scalar_type() == torch::kBFloat16, ids.numel(), w.size(0), (int)w.size(1), (float)scale,
+                            status_ptr(status), stream());
+  return out;
+}
+
+// The gradient [V, H] of the looked-up rows: a new tensor of dy's type, or added to acc (f32 [V, H]).
+torch::Tensor embedding_bwd(torch::Tensor ids, torch::Tensor dy, int64_t V, double scale,
+                            c10::optional<torch::Tensor> acc) {
+  check_embedding(ids, dy, "dy");
   c10::cuda::CUDAGuard g(dy.device());
-  TORCH_CHECK(dw.scalar_type() == torch::kFloat32 && dw.is_contiguous() && dy.is_contiguous(), "embedding grad");
-  oxi::launch_embed_bwd(ids.data_ptr<int64_t>(), dy.data_ptr(), dw.data_ptr<float>(), ids.numel(), (int)dw.size(1),
-                        stream());
+  const int64_t T = ids.numel(), H = dy.size(1);
+  OXI_CHECK(dy.size(0) == T, "embedding gradient: one row of dy per id");
+  const bool add = acc.has_value() && acc->defined();
+  torch::Tensor dw;
+  if (add) {
+    dw = *acc;
+    OXI_CHECK(dw.device() == dy.device() && dw.scalar_type() == torch::kFloat32 && dw.is_contiguous() &&
+                  dw.dim() == 2 && dw.size(0) == V && dw.size(1) == H,
+              "embedding gradient: the accumulator must be contiguous f32 [V, H] on dy's device");
+  } else {
+    dw = torch::empty({V, H}, dy.options());
+  }
+  auto ws = torch::empty({oxi::embedding_bwd_workspace(T, (int)H)},
+                         torch::TensorOptions().dtype(torch::kUInt8).device(dy.device()));
+  oxi::launch_embedding_bwd(ids.data_ptr<int64_t>(), dy.data_ptr(), dy.scalar_type() == torch::kBFloat16,
+                            dw.data_ptr(), add, T, V, (int)H, (float)scale, ws.data_ptr(), stream());
+  return dw;
 }
 
 void rope_bwd(torch::Tensor x, int64_t ncols_rot, int64_t hd, torch::Tensor cos, torch::Tensor sin) {
@@ -1172,38 +1201,62 @@ std::vector<torch::Tensor> moe_permute(torch::Tensor x, torch::Tensor topi, int6
   return {counts, seg, pos, xp};
 }
 
-std::vector<torch::Tensor> router_fwd(torch::Tensor logits, int64_t k) {
+oxi::RouteArgs route_args(int64_t k, bool sigmoid, int64_t groups, int64_t top_groups, int64_t group_top, bool renorm,
+                          double scale) {
+  return {(int)k, sigmoid, (int)groups, (int)top_groups, (int)group_top, renorm, (float)scale};
+}
+
+void check_logits(const torch::Tensor& logits) {
+  OXI_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) == 1) &&
+                (logits.scalar_type() == torch::kBFloat16 || logits.scalar_type() == torch::kFloat32),
+            "router logits must be bf16/f32 [T, E] with unit inner stride");
+}
+
+std::vector<torch::Tensor> router_fwd(torch::Tensor logits, int64_t k, bool sigmoid, c10::optional<torch::Tensor> bias,
+                                      int64_t groups, int64_t top_groups, int64_t group_top, bool renorm,
+                                      double scale) {
+  check_logits(logits);
   c10::cuda::CUDAGuard g(logits.device());
-  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1 &&
-                  (logits.scalar_type() == torch::kBFloat16 || logits.scalar_type() == torch::kFloat32),
-              "router logits must be bf16/f32 [T, E] with unit inner stride");
   const int64_t T = logits.size(0), E = logits.size(1);
+  const float* bp = nullptr;
+  if (bias.has_value() && bias->defined()) {
+    OXI_CHECK(bias->device() == logits.device() && bias->scalar_type() == torch::kFloat32 && bias->is_contiguous() &&
+                  bias->numel() == E, "router bias must be f32 [E] on the logits' device");
+    bp = bias->data_ptr<float>();
+  }
+  OXI_CHECK(E <= oxi::ROUTE_MAX_EXPERTS && k >= 1 && k <= oxi::ROUTE_MAX_K, "router: E <= ", oxi::ROUTE_MAX_EXPERTS,
+            " and 1 <= k <= ", oxi::ROUTE_MAX_K);
   auto dev = logits.device();
   auto topi = torch::empty({T, k}, torch::TensorOptions().dtype(torch::kInt64).device(dev));
   auto topw = torch::empty({T, k}, torch::TensorOptions().dtype(torch::kFloat32).device(dev));
   auto usage = torch::empty({E}, torch::TensorOptions().dtype(torch::kFloat32).device(dev));
   auto counts = torch::empty({E}, torch::TensorOptions().dtype(torch::kInt32).device(dev));
+  auto ws = torch::empty({oxi::route_workspace(T, (int)E)}, torch::TensorOptions().dtype(torch::kUInt8).device(dev));
   oxi::launch_router_fwd(logits.data_ptr(), logits.scalar_type() == torch::kBFloat16, logits.stride(0), T, (int)E,
-                         (int)k, topi.data_ptr<int64_t>(), topw.data_ptr<float>(), usage.data_ptr<float>(),
-                         counts.data_ptr<int>(), stream());
+                         route_args(k, sigmoid, groups, top_groups, group_top, renorm, scale), bp,
+                         topi.data_ptr<int64_t>(), topw.data_ptr<float>(), usage.data_ptr<float>(),
+                         counts.data_ptr<int>(), ws.data_ptr(), stream());
   return {topi, topw, usage, counts};
 }
 
-torch::Tensor router_bwd(torch::Tensor logits, torch::Tensor topi, torch::Tensor topw, torch::Tensor dtopw,
-                         c10::optional<torch::Tensor> dusage) {
+torch::Tensor router_bwd(torch::Tensor logits, torch::Tensor topi, torch::Tensor dtopw,
+                         c10::optional<torch::Tensor> dusage, bool sigmoid, bool renorm, double scale) {
+  check_logits(logits);
   c10::cuda::CUDAGuard g(logits.device());
-  TORCH_CHECK(topi.is_contiguous() && topw.is_contiguous() && dtopw.is_contiguous() &&
-                  dtopw.scalar_type() == torch::kFloat32 && dtopw.numel() == topw.numel(), "router bwd operands");
   const int64_t T = logits.size(0), E = logits.size(1), k = topi.size(1);
+  OXI_CHECK(topi.is_contiguous() && topi.scalar_type() == torch::kInt64 && dtopw.is_contiguous() &&
+                dtopw.scalar_type() == torch::kFloat32 && dtopw.numel() == T * k && topi.size(0) == T &&
+                topi.device() == logits.device() && dtopw.device() == logits.device(), "router backward operands");
   auto dl = torch::empty({T, E}, logits.options());
   const float* du = nullptr;
   if (dusage.has_value() && dusage->defined()) {
-    TORCH_CHECK(dusage->scalar_type() == torch::kFloat32 && dusage->is_contiguous() && dusage->numel() == E, "dusage");
+    OXI_CHECK(dusage->scalar_type() == torch::kFloat32 && dusage->is_contiguous() && dusage->numel() == E &&
+                  dusage->device() == logits.device(), "router backward: usage gradient");
     du = dusage->data_ptr<float>();
   }
   oxi::launch_router_bwd(logits.data_ptr(), logits.scalar_type() == torch::kBFloat16, logits.stride(0), T, (int)E,
-                         (int)k, topi.data_ptr<int64_t>(), topw.data_ptr<float>(), dtopw.data_ptr<float>(), du,
-                         dl.data_ptr(), dl.stride(0), stream());
+                         route_args(k, sigmoid, 1, 1, 1, renorm, scale), topi.data_ptr<int64_t>(),
+                         dtopw.data_ptr<float>(), du, dl.data_ptr(), dl.stride(0), stream());
   return dl;
 }
 
@@ -1292,8 +1345,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("doc_attn_fwd", &doc_attn_fwd, "attention over visible key ranges, forward");
   m.def("doc_attn_bwd", &doc_attn_bwd, "attention over visible key ranges, backward");
   m.def("doc_attn_supported", [](int64_t Dqk, int64_t Dv) { return oxi::da_supported((int)Dqk, (int)Dv); });
-  m.def("embed_fwd", &embed_fwd, "embedding gather");
-  m.def("embed_bwd", &embed_bwd, "embedding scatter-add into f32 grad");
+  m.def("embedding_fwd", &embedding_fwd, "scaled embedding lookup");
+  m.def("embedding_bwd", &embedding_bwd, "embedding gradient by sorted tokens");
   m.def("rope_bwd_to", &rope_bwd_to, "out-of-place RoPE backward (+ copy of the unrotated columns)");
   m.def("rope_bwd", &rope_bwd, "in-place inverse rotate-half RoPE");
   m.def("sqsum", &sqsum, "sum of squares (atomically added into out)");

@@ -1,8 +1,7 @@
-// Memory-bound training kernels: cross-entropy finish/backward, embedding
-// gather/scatter, RoPE backward, gradient-norm, clip coefficient and the flat
-// multi-tensor AdamW update.  All are single-pass over their data with 16-byte
+// Memory-bound training kernels: cross-entropy finish/backward, RoPE backward,
+// gradient-norm, clip coefficient and the flat multi-tensor AdamW update.  All are single-pass over their data with 16-byte
 // vector accesses; none synchronises with the host.
-// Upstream: cross-entropy trainer.rs:166-171 and model.rs:1002; embedding model.rs:964;
+// Upstream: cross-entropy trainer.rs:166-171 and model.rs:1002;
 // RoPE model.rs:68-117; gradient norm trainer.rs:560-574; AdamW trainer.rs:60-64,245 and
 // distributed/optimizer.rs:126-192.
 #include <cuda_bf16.h>
@@ -116,31 +115,6 @@ __global__ void __launch_bounds__(256) ce_bwd_kernel(__nv_bfloat16* __restrict__
       const float f = __bfloat162float(rp[c]);
       rp[c] = __float2bfloat16((__expf(f - l) - (c == t ? 1.f : 0.f)) * sc);
     }
-  }
-}
-
-// --------------------------------------------------------------- embedding
-__global__ void embed_fwd_kernel(const int64_t* __restrict__ ids, const __nv_bfloat16* __restrict__ w,
-                                 __nv_bfloat16* __restrict__ out, int64_t rows, int H) {
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-  if (row >= rows) return;
-  const int lane = threadIdx.x & 31;
-  const uint4* src = reinterpret_cast<const uint4*>(w + ids[row] * (int64_t)H);
-  uint4* dst = reinterpret_cast<uint4*>(out + row * (int64_t)H);
-  for (int i = lane; i < H / 8; i += 32) dst[i] = src[i];
-}
-
-__global__ void embed_bwd_kernel(const int64_t* __restrict__ ids, const __nv_bfloat16* __restrict__ dy,
-                                 float* __restrict__ dw, int64_t rows, int H) {
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-  if (row >= rows) return;
-  const int lane = threadIdx.x & 31;
-  const __nv_bfloat162* src = reinterpret_cast<const __nv_bfloat162*>(dy + row * (int64_t)H);
-  float* dst = dw + ids[row] * (int64_t)H;
-  for (int i = lane; i < H / 4; i += 32) {
-    const float2 a = __bfloat1622float2(src[2 * i]);
-    const float2 b = __bfloat1622float2(src[2 * i + 1]);
-    atomicAdd(reinterpret_cast<float4*>(dst) + i, make_float4(a.x, a.y, b.x, b.y));
   }
 }
 
@@ -370,22 +344,6 @@ void launch_ce_bwd(void* logits, int64_t ld, int64_t V, int64_t rows, const floa
   dim3 grid(gx, (unsigned)rows);
   ce_bwd_kernel<<<grid, 256, 0, st>>>(reinterpret_cast<__nv_bfloat16*>(logits), ld, V, lse, targets, gscale,
                                       inv_count, col0);
-  OXI_CUDA_CHECK(cudaGetLastError());
-}
-
-void launch_embed_fwd(const int64_t* ids, const void* w, void* out, int64_t rows, int H, cudaStream_t st) {
-  if (!rows) return;
-  OXI_CHECK(H % 8 == 0, "embedding width must be a multiple of 8");
-  embed_fwd_kernel<<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(ids, reinterpret_cast<const __nv_bfloat16*>(w),
-                                                                 reinterpret_cast<__nv_bfloat16*>(out), rows, H);
-  OXI_CUDA_CHECK(cudaGetLastError());
-}
-
-void launch_embed_bwd(const int64_t* ids, const void* dy, float* dw, int64_t rows, int H, cudaStream_t st) {
-  if (!rows) return;
-  OXI_CHECK(H % 8 == 0, "embedding width must be a multiple of 8");
-  embed_bwd_kernel<<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(ids, reinterpret_cast<const __nv_bfloat16*>(dy), dw,
-                                                                 rows, H);
   OXI_CUDA_CHECK(cudaGetLastError());
 }
 

@@ -22,11 +22,19 @@ def _native(t: torch.Tensor) -> bool:
     return t.is_cuda and t.dtype == torch.bfloat16
 
 
-def embedding(ids: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
-    if _native(w):
+def embedding(ids: torch.Tensor, w: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """w[ids] * scale for integer ids of any shape and w [V, H].  bf16 and f32 weights on the GPU run
+    csrc/embed.cu; there an id outside [0, V) gives a zero row, no gradient, and a bounds error in the
+    status word (``ops._C.check_status``)."""
+    if ids.dtype not in (torch.int64, torch.int32) or w.dim() != 2 or ids.device != w.device:
+        raise ValueError(f"embedding: int64 or int32 ids and w [V, H] on one device, got {ids.dtype} on {ids.device}, "
+                         f"{list(w.shape)} on {w.device}")
+    ids = ids.long()
+    if w.is_cuda and w.dtype in (torch.bfloat16, torch.float32):
         from .fused import Embedding
-        return Embedding.apply(ids, w)
-    return F.embedding(ids, w)
+        return Embedding.apply(ids, w, float(scale))
+    y = F.embedding(ids, w)
+    return y if scale == 1.0 else (y.to(R.wide(w.dtype)) * scale).to(w.dtype)
 
 
 def rmsnorm(x, w, eps: float = 1e-5):
@@ -201,6 +209,40 @@ def attention_qkv(qkv, Hq: int, Hk: int, D: int, scale: float, causal: bool = Tr
         return _aq(qkv, Hq, Hk, D, scale, causal)
     from .doc_attention import attention_qkv as _doc
     return _doc(qkv, Hq, Hk, D, scale, causal, mask, softcap or 0.0, alibi)
+
+
+def route_topk(logits, k: int, score: str = "softmax", bias=None, groups: int = 1, top_groups: int = 1,
+               group_top: int = 2, renorm: bool = True, scale: float = 1.0):
+    """Choose k of E experts per token from router logits [T, E].
+
+    s = softmax or sigmoid of the logits.  The choice goes by s + ``bias`` ([E], the choice alone: it has
+    no gradient and is not in the weights): with ``groups`` > 1 the ``top_groups`` groups of neighbouring
+    experts with the largest sum of their ``group_top`` best take part, and of those the k best experts,
+    largest first; of equals the lowest index.  Weights are s of the chosen, divided by their sum with
+    ``renorm``, times ``scale``.
+
+    Returns (topi [T, k] int64, topw [T, k] f32, usage [E] f32: the mean over the tokens of s / sum s,
+    counts [E] int32); topw and usage carry gradients to the logits.
+    """
+    if logits.dim() != 2 or not logits.is_floating_point():
+        raise ValueError(f"route_topk: logits must be floating point [T, E], got {logits.dtype} {list(logits.shape)}")
+    E = logits.shape[1]
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError(f"route_topk: score must be softmax or sigmoid, got {score!r}")
+    if groups < 1 or E % groups or not 1 <= top_groups <= groups or group_top < 1:
+        raise ValueError(f"route_topk: {E} experts in {groups} groups of which {top_groups} stay (ranked by their "
+                         f"{group_top} best)")
+    if not 1 <= k <= top_groups * (E // groups):
+        raise ValueError(f"route_topk: cannot choose {k} of {top_groups * (E // groups)} experts")
+    if bias is not None:
+        if bias.shape != (E,) or bias.device != logits.device:
+            raise ValueError(f"route_topk: bias must be one value per expert [{E}] on {logits.device}")
+        bias = bias.detach().float().contiguous()
+    if logits.is_cuda:
+        from .moe_kernels import RouterTopK, router_ok
+        if router_ok(logits, k, groups):
+            return RouterTopK.apply(logits, k, score, bias, groups, top_groups, group_top, bool(renorm), float(scale))
+    return R.route_topk(logits, k, score, bias, groups, top_groups, group_top, renorm, scale)
 
 
 def linear_cross_entropy(x, w, targets, ignore_index: int = -100):

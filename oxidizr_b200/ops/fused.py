@@ -78,13 +78,15 @@ def _c(t: torch.Tensor) -> torch.Tensor:
 
 # ---------------------------------------------------------------- embedding
 class Embedding(torch.autograd.Function):
+    """w[ids] * scale; the gradient sums each row's tokens in f32 in their order, by sorting them
+    (csrc/embed.cu), so it is the same from run to run."""
+
     @staticmethod
-    def forward(ctx, ids, w):
+    def forward(ctx, ids, w, scale: float = 1.0):
         ids_f = _c(ids.reshape(-1))
-        out = torch.empty(ids_f.numel(), w.shape[1], dtype=w.dtype, device=w.device)
-        ext().embed_fwd(ids_f, w, out)
+        out = ext().embedding_fwd(ids_f, _c(w), scale, status(w.device))
         ctx.save_for_backward(ids_f)
-        ctx.w = w
+        ctx.w, ctx.scale = w, scale
         return out.view(*ids.shape, w.shape[1])
 
     @staticmethod
@@ -94,12 +96,10 @@ class Embedding(torch.autograd.Function):
         dy = _c(dy.reshape(-1, w.shape[1]))
         mg = getattr(w, "main_grad", None)
         if mg is not None:
-            ext().embed_bwd(ids, dy, mg.view(w.shape))
+            ext().embedding_bwd(ids, dy, w.shape[0], ctx.scale, mg.view(w.shape))
             _ready(w)
-            return None, None
-        g = torch.zeros(w.shape, dtype=torch.float32, device=w.device)
-        ext().embed_bwd(ids, dy, g)
-        return None, g.to(w.dtype)
+            return None, None, None
+        return None, ext().embedding_bwd(ids, dy, w.shape[0], ctx.scale, None), None
 
 
 # ------------------------------------------------------------------- norms

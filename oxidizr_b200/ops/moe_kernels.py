@@ -105,27 +105,35 @@ def grouped_ok(x: torch.Tensor, w_gu: torch.Tensor) -> bool:
 
 
 class RouterTopK(torch.autograd.Function):
-    """Softmax router + top-k + renormalised weights + mean probability (csrc/router.cu).
+    """The router of csrc/router.cu: scores, choice, weights, mean normalised score and counts.
 
-    Returns ``(topi [T,k] int64, topw [T,k] f32, usage [E] f32, counts [E] int32)``;
-    ``usage`` (mean routing probability per expert) and ``topw`` carry gradients.
+    Returns ``(topi [T,k] int64, topw [T,k] f32, usage [E] f32, counts [E] int32)``; ``usage`` and
+    ``topw`` carry gradients.  The options are those of ``ops.api.route_topk``.
     """
 
     @staticmethod
-    def forward(ctx, logits, k: int):
-        topi, topw, usage, counts = ext().router_fwd(logits, int(k))
-        ctx.save_for_backward(logits, topi, topw)
+    def forward(ctx, logits, k: int, score: str = "softmax", bias=None, groups: int = 1, top_groups: int = 1,
+                group_top: int = 2, renorm: bool = True, scale: float = 1.0):
+        if logits.stride(1) != 1:
+            logits = logits.contiguous()
+        topi, topw, usage, counts = ext().router_fwd(logits, int(k), score == "sigmoid", bias, groups, top_groups,
+                                                     group_top, renorm, scale)
+        ctx.save_for_backward(logits, topi)
+        ctx.cfg = (score == "sigmoid", renorm, scale)
         ctx.mark_non_differentiable(topi, counts)
         return topi, topw, usage, counts
 
     @staticmethod
     def backward(ctx, _dtopi, dtopw, dusage, _dcounts):
-        logits, topi, topw = ctx.saved_tensors
-        dtopw = torch.zeros_like(topw) if dtopw is None else dtopw.float().contiguous()
+        logits, topi = ctx.saved_tensors
+        dtopw = torch.zeros(topi.shape, device=topi.device) if dtopw is None else dtopw.float().contiguous()
         du = None if dusage is None else dusage.float().contiguous()
-        return ext().router_bwd(logits, topi, topw, dtopw, du), None
+        return ext().router_bwd(logits, topi, dtopw, du, *ctx.cfg), *[None] * 8
 
 
-def router_ok(logits, k: int) -> bool:
-    return (logits.is_cuda and logits.dim() == 2 and logits.shape[1] <= 256 and k <= 16
-            and logits.dtype in (torch.bfloat16, torch.float32) and hasattr(ext(), "router_fwd"))
+ROUTE_MAX_EXPERTS, ROUTE_MAX_K, ROUTE_MAX_GROUPS = 512, 32, 32  # csrc/kernels_moe.h
+
+
+def router_ok(logits, k: int, groups: int = 1) -> bool:
+    return (logits.is_cuda and logits.dim() == 2 and logits.shape[1] <= ROUTE_MAX_EXPERTS and k <= ROUTE_MAX_K
+            and groups <= ROUTE_MAX_GROUPS and logits.dtype in (torch.bfloat16, torch.float32))

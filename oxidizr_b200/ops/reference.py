@@ -13,6 +13,11 @@ import torch
 import torch.nn.functional as F
 
 
+def wide(dtype: torch.dtype) -> torch.dtype:
+    """The type that values of ``dtype`` are computed in: f64 for f64, else f32."""
+    return torch.float64 if dtype == torch.float64 else torch.float32
+
+
 # ------------------------------------------------------------------ norms
 def rmsnorm(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-5) -> torch.Tensor:
     """model.rs:22-31: f32 internal ``x / sqrt(mean(x^2) + eps)``, cast back, then ``* weight``."""
@@ -326,3 +331,41 @@ def adamw_step(p, g, m, v, step: int, lr: float, beta1=0.9, beta2=0.999, eps=1e-
     upd = (m / bc1) / ((v / bc2).sqrt() + eps)
     p.sub_(lr * upd + lr * wd * p)
     return p
+
+
+# ----------------------------------------------------------------- routing
+def route_topk(logits: torch.Tensor, k: int, score: str = "softmax", bias: Optional[torch.Tensor] = None,
+               groups: int = 1, top_groups: int = 1, group_top: int = 2, renorm: bool = True, scale: float = 1.0):
+    """Top-k routing (model.rs:541-556 is softmax scores without bias and groups): the choice in f64, where
+    scores next to each other keep their order, the weights and their gradient in the logits' wide type."""
+    T, E = logits.shape
+
+    def scores(x):
+        return torch.softmax(x, -1) if score == "softmax" else torch.sigmoid(x)
+
+    with torch.no_grad():
+        x = logits.detach().double()
+        # without a bias the order of the scores is that of the logits
+        b = scores(x) + (0.0 if bias is None else bias.double())
+        order = (x if bias is None else b).nan_to_num(nan=-math.inf, posinf=math.inf, neginf=-math.inf)
+        if groups > 1:
+            n = E // groups
+            best = order.view(T, groups, n).sort(dim=-1, descending=True, stable=True).indices[..., :group_top]
+            rank = b.view(T, groups, n).gather(-1, best).sum(-1)
+            keep = rank.sort(dim=-1, descending=True, stable=True).indices[:, :top_groups]
+            stays = torch.zeros(T, groups, dtype=torch.bool, device=x.device).scatter_(1, keep, True)
+            # two-key order: the experts of the groups that go come after all others
+            first = order.sort(dim=-1, descending=True, stable=True).indices
+            gone = (~stays).to(torch.uint8).repeat_interleave(n, 1).gather(1, first)
+            topi = first.gather(1, gone.sort(dim=-1, stable=True).indices)[:, :k]
+        else:
+            topi = order.sort(dim=-1, descending=True, stable=True).indices[:, :k]
+        topi = topi.contiguous()
+    s = scores(logits.to(wide(logits.dtype)))
+    topw = s.gather(1, topi)
+    if renorm:
+        total = topw.sum(-1, keepdim=True)
+        topw = torch.where(total > 0, topw / torch.where(total > 0, total, torch.ones_like(total)), torch.zeros_like(topw))
+    usage = (s / s.sum(-1, keepdim=True)).mean(0) if T else s.sum(0)
+    counts = torch.bincount(topi.reshape(-1), minlength=E).to(torch.int32)
+    return topi, topw * scale, usage, counts

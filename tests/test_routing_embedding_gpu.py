@@ -1,0 +1,268 @@
+"""Expert routing and the scaled embedding on the GPU, against 64-bit statements.
+
+Tolerances count roundings: f32 values are off by at most 2^-24 of themselves, bf16 by 2^-8.
+"""
+import pytest
+import torch
+
+from oxidizr_b200.ops import api
+from oxidizr_b200.ops import reference as R
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = 2.0 ** -24, 2.0 ** -8
+
+
+def finish():
+    from oxidizr_b200.ops._C import check_status
+    torch.cuda.synchronize()
+    check_status("cuda")
+
+
+# ------------------------------------------------------------------ routing
+def route_both(x, k, dw, du, **kw):
+    leaf = x.detach().requires_grad_(True)
+    got = api.route_topk(leaf, k, **kw)
+    got = [t.detach() for t in got] + list(torch.autograd.grad(got[1:3], leaf, (dw, du)))
+    wide = x.detach().double().requires_grad_(True)
+    want = R.route_topk(wide, k, kw.get("score", "softmax"), kw.get("bias"), kw.get("groups", 1), kw.get("top_groups", 1),
+                        kw.get("group_top", 2), kw.get("renorm", True), kw.get("scale", 1.0))
+    want = [t.detach() for t in want] + list(torch.autograd.grad(want[1:3], wide, (dw.double(), du.double())))
+    return got, want
+
+
+def check_route(x, k, dw, du, **kw):
+    got, want = route_both(x, k, dw, du, **kw)
+    T, E = x.shape
+    assert torch.equal(got[0], want[0]) and torch.equal(got[3], want[3])
+    # an exponential is good to 2 steps, its sum over E terms to log E more, a quotient or two: 24 steps
+    assert ((got[1].double() - want[1]).abs() <= 24 * F32 * want[1].abs() + 1e-30).all()
+    # usage adds T positive terms, in runs of at most T / 32 after one another
+    assert ((got[2].double() - want[2]).abs() <= (24 + 2 * (T // 32 + 32)) * F32 * want[2].abs() + 1e-30).all()
+    # the gradient is a difference of sums: its parts in absolute values bound what f32 does to it
+    s = torch.softmax(x.double(), -1) if kw.get("score", "softmax") == "softmax" else torch.sigmoid(x.double())
+    S = s.sum(-1, keepdim=True)
+    sel = s.gather(1, want[0])
+    n = sel.sum(-1, keepdim=True) if kw.get("renorm", True) else torch.ones_like(S)
+    g = dw.double().abs() * kw.get("scale", 1.0) / n
+    g = g + (g * sel).sum(-1, keepdim=True) / n
+    part = torch.zeros_like(s).scatter_add_(1, want[0], g)
+    u = du.double().abs() / T
+    part = part + (u + (u * s).sum(-1, keepdim=True) / S) / S
+    size = s * (part + (s * part).sum(-1, keepdim=True))
+    step = BF16 if x.dtype == torch.bfloat16 else F32
+    assert ((got[4].double() - want[4]).abs() <= step * want[4].abs() + 64 * F32 * size + 1e-30).all()
+    finish()
+
+
+@pytest.mark.parametrize("T,E,k", [(1, 1, 1), (3, 2, 2), (100, 5, 3), (257, 32, 4), (64, 33, 8), (500, 64, 8), (77, 100, 16),
+                                   (300, 256, 8), (200, 257, 9), (50, 512, 32)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_routing(T, E, k, score, biased, dt):
+    g = torch.Generator(device="cuda").manual_seed(T + E)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    check_route((rnd(T, E) * 1.5).to(dt), k, rnd(T, k), rnd(E), score=score, renorm=(T % 2 == 0), scale=1.5,
+                bias=rnd(E) * (0.1 if score == "sigmoid" else 0.3 / E) if biased else None)
+
+
+@pytest.mark.parametrize("E,groups,top_groups,group_top,k", [(8, 8, 3, 2, 3), (12, 4, 2, 2, 5), (64, 8, 4, 2, 8), (96, 3, 1, 1, 8),
+                                                             (160, 8, 3, 2, 6), (256, 8, 4, 2, 8), (256, 2, 1, 3, 8),
+                                                             (512, 32, 7, 2, 16), (320, 32, 9, 2, 12)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [False, True])
+def test_grouped_routing(E, groups, top_groups, group_top, k, score, biased):
+    T = 301
+    g = torch.Generator(device="cuda").manual_seed(E + groups)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    check_route(rnd(T, E).bfloat16(), k, rnd(T, k), rnd(E), score=score, groups=groups, top_groups=top_groups,
+                group_top=group_top, scale=2.5, bias=rnd(E) * (0.1 if score == "sigmoid" else 0.3 / E) if biased else None)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_near_ties_are_decided_in_64_bits(score):
+    """Scores whose order f32 cannot tell: pairs a rounding step of a bias apart, and exact ties."""
+    T, E, k = 512, 64, 8
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = (torch.randint(-3, 4, (T, E), generator=g, device="cuda").float() / 2)
+    s = torch.softmax(x[0].double(), -1) if score == "softmax" else torch.sigmoid(x[0].double())
+    # bias that makes the first token's scores all but equal in f32, in no particular order in f64
+    bias = (s.max() - s).float()
+    dw, du = torch.randn(T, k, device="cuda"), torch.randn(E, device="cuda")
+    x[1::2] = x[0]
+    check_route(x, k, dw, du, score=score, bias=bias)
+    check_route(x, k, dw, du, score=score, bias=torch.zeros(E, device="cuda"))
+    check_route(x, k, dw, du, score=score)
+    check_route(x, k, dw, du, score=score, bias=bias, groups=8, top_groups=3)
+    check_route(torch.zeros_like(x), k, dw, du, score=score, groups=8, top_groups=3)
+
+
+def test_masked_experts_and_extreme_logits():
+    """Experts shut out by a logit of -inf, and logits far out, where exponentials vanish."""
+    T, E, k = 40, 48, 4
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn(T, E, generator=g, device="cuda") * 20
+    x[:, 5:20] = -float("inf")
+    topi, topw, usage, counts = api.route_topk(x, k)
+    ti, tw, tu, tc = R.route_topk(x.double(), k)
+    assert torch.equal(topi, ti) and torch.equal(counts, tc) and (counts[5:20] == 0).all() and (usage[5:20] == 0).all()
+    assert ((topw.double() - tw).abs() <= 64 * F32 * tw + 1e-30).all()
+    topi, topw, _, _ = api.route_topk(x, k, "sigmoid")
+    assert torch.equal(topi, ti) and torch.isfinite(topw).all()
+    # bias of -inf: never chosen while others are left
+    bias = torch.zeros(E, device="cuda")
+    bias[::2] = -float("inf")
+    topi = api.route_topk(x.clamp(min=-1e4), k, "sigmoid", bias)[0]
+    assert (topi % 2 == 1).all()
+    finish()
+
+
+def test_routing_layouts_streams_and_graphs():
+    T, E, k = 130, 64, 8
+    g = torch.Generator(device="cuda").manual_seed(3)
+    wide = torch.randn(T, 3 * E + 1, generator=g, device="cuda").bfloat16()
+    x = wide[:, E + 1:2 * E + 1]
+    dw, du = torch.randn(T, k, device="cuda"), torch.randn(E, device="cuda")
+    kw = dict(score="sigmoid", bias=torch.randn(E, device="cuda") * 0.1, groups=4, top_groups=2)
+    check_route(x, k, dw, du, **kw)
+    check_route(x.t().contiguous().t(), k, dw, du, **kw)
+    want = route_both(x, k, dw, du, **kw)[0]
+    # one of the two outputs alone passes a gradient
+    leaf = x.detach().requires_grad_(True)
+    out = api.route_topk(leaf, k, **kw)
+    (a,) = torch.autograd.grad(out[1], leaf, dw, retain_graph=True)
+    (b,) = torch.autograd.grad(out[2], leaf, du)
+    assert (a.float() + b.float() - want[4].float()).abs().max() <= 4 * BF16 * want[4].abs().max()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = [t.detach() for t in api.route_topk(x, k, **kw)]
+    torch.cuda.current_stream().wait_stream(s)
+    for p, q in zip(other, want):
+        assert torch.equal(p, q)  # usage too: the same sums in the same order
+    static = x.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = api.route_topk(static, k, **kw)
+    static.copy_(x.flip(0))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], want[0].flip(0)) and torch.equal(out[3], want[3])
+    empty = api.route_topk(x[:0], k, **kw)
+    assert empty[0].shape == (0, k) and (empty[2] == 0).all() and (empty[3] == 0).all()
+    finish()
+
+
+def test_larger_routers_take_the_stated_math():
+    x = torch.randn(9, 600, device="cuda")
+    topi, topw, usage, counts = api.route_topk(x, 40)
+    ti, tw, tu, tc = R.route_topk(x.double(), 40)
+    assert torch.equal(topi, ti) and torch.equal(counts, tc)
+    assert ((topw.double() - tw).abs() <= 64 * F32 * tw).all()
+
+
+# ------------------------------------------------------------------ embedding
+def check_embedding(ids, V, H, dt, scale, seed=0, misalign=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    w = torch.randn(V, H, generator=g, device="cuda").to(dt)
+    flat = torch.randn(ids.numel() * H + misalign, generator=g, device="cuda").to(dt)
+    dy = flat[misalign:].view(*ids.shape, H)
+    step = BF16 if dt == torch.bfloat16 else F32
+    leaf = w.detach().requires_grad_(True)
+    y = api.embedding(ids, leaf, scale=scale)
+    want = w.double()[ids] * scale
+    assert ((y.double() - want).abs() <= (step + F32) * want.abs()).all()
+    (dw,) = torch.autograd.grad(y, leaf, dy)
+    sums = torch.zeros(V, H, dtype=torch.float64, device="cuda")
+    mags = torch.zeros_like(sums)
+    sums.index_add_(0, ids.flatten(), dy.double().view(-1, H) * scale)
+    mags.index_add_(0, ids.flatten(), dy.double().abs().view(-1, H) * abs(scale))
+    n = torch.bincount(ids.flatten(), minlength=V)[:, None].double()
+    # f32 sums of n terms, the scale, and the rounding to the result's type
+    tol = step * sums.abs() + (n + 2) * F32 * mags * (1 + step)
+    assert dw.dtype == dt and ((dw.double() - sums).abs() <= tol).all()
+    assert (dw[n[:, 0] == 0] == 0).all()
+    (again,) = torch.autograd.grad(api.embedding(ids, leaf, scale=scale), leaf, dy)
+    assert torch.equal(dw, again)
+    # into main_grad, as the optimizer's buffer takes it
+    p = torch.nn.Parameter(w.clone())
+    p.main_grad = torch.randn(V, H, generator=g, device="cuda")
+    before = p.main_grad.clone()
+    api.embedding(ids, p, scale=scale).backward(dy)
+    assert p.grad is None
+    acc = before.double() + sums
+    assert ((p.main_grad.double() - acc).abs() <= (n + 2) * F32 * mags + F32 * acc.abs()).all()
+    assert torch.equal(p.main_grad[n[:, 0] == 0], before[n[:, 0] == 0])
+    finish()
+
+
+@pytest.mark.parametrize("T,V,H", [(1, 1, 8), (1, 1000, 64), (31, 5, 8), (32, 3, 256), (33, 50, 264), (1000, 511, 128),
+                                   (1024, 512, 96), (1025, 513, 1000), (5000, 128354, 64), (40000, 300, 16)])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_embedding(T, V, H, dt):
+    g = torch.Generator().manual_seed(T)
+    ids = (torch.rand(T, generator=g) ** 3 * V).long().clamp(max=V - 1).cuda()
+    check_embedding(ids, V, H, dt, 1.0 if T % 2 else 11.5)
+
+
+@pytest.mark.parametrize("H", [1, 7, 20, 132])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_embedding_odd_widths(H, dt):
+    ids = torch.randint(0, 40, (3, 77), device="cuda")
+    check_embedding(ids, 40, H, dt, 0.5)
+
+
+def test_embedding_runs_of_one_token():
+    """Segments that end at, before and after a block's edge, fill many blocks, or are all there is."""
+    for runs in ([(3, 32), (4, 32)], [(3, 31), (4, 33), (5, 1)], [(9, 5000)], [(0, 1), (1, 70), (2, 64), (3, 1), (4, 300)],
+                 [(7, 96), (8, 32), (9, 1)]):
+        ids = torch.cat([torch.full((n,), v) for v, n in runs]).cuda()
+        perm = torch.randperm(ids.numel(), generator=torch.Generator().manual_seed(1)).cuda()
+        check_embedding(ids, 10, 72, torch.bfloat16, 1.0)
+        check_embedding(ids[perm], 10, 72, torch.float32, 1.0)
+
+
+def test_embedding_misaligned_gradient():
+    check_embedding(torch.randint(0, 9, (50,), device="cuda"), 9, 64, torch.bfloat16, 1.0, misalign=1)
+
+
+def test_embedding_ids_out_of_range():
+    from oxidizr_b200.ops._C import read_status
+    w = torch.randn(6, 16, device="cuda").bfloat16().requires_grad_(True)
+    ids = torch.tensor([5, -1, 6, 2, 10 ** 12, 5], device="cuda")
+    y = api.embedding(ids, w)
+    assert read_status("cuda") == 3  # reported, and cleared for the next call
+    ok = torch.tensor([True, False, False, True, False, True], device="cuda")
+    assert torch.equal(y[ok], w.detach()[ids[ok]]) and (y[~ok] == 0).all()
+    (g,) = torch.autograd.grad(y, w, torch.ones_like(y))
+    assert g[5].eq(2).all() and g[2].eq(1).all() and (g[[0, 1, 3, 4]] == 0).all()
+    finish()
+
+
+def test_embedding_empty_and_captured():
+    w = torch.randn(30, 64, device="cuda").bfloat16().requires_grad_(True)
+    y = api.embedding(torch.zeros(2, 0, dtype=torch.int64, device="cuda"), w)
+    (g,) = torch.autograd.grad(y, w, torch.zeros_like(y))
+    assert y.shape == (2, 0, 64) and (g == 0).all()
+    # an eager graph of the leaf that outlives the capture would keep its gradient on the eager stream
+    del y, g
+    ids = torch.randint(0, 30, (4, 200), device="cuda")
+    other = torch.randint(0, 30, (4, 200), device="cuda")
+    dy = torch.randn(4, 200, 64, device="cuda").bfloat16()
+
+    def step(i):
+        y = api.embedding(i, w, scale=8.0)
+        return [y, *torch.autograd.grad(y, w, dy)]
+
+    want = [[t.detach().clone() for t in step(i)] for i in (ids, other)]
+    static = ids.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    for i, ref in ((other, want[1]), (ids, want[0])):
+        static.copy_(i)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, ref):
+            assert torch.equal(a, b)
+    finish()

@@ -12,7 +12,6 @@
 namespace oxi {
 namespace {
 
-constexpr int DA_THREADS = 320;  // TMA warp, MMA warp, 8 softmax / epilogue warps
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct DaParams {
@@ -53,13 +52,12 @@ __device__ __forceinline__ uint32_t range_bits(int lo, int hi, int k) {
 struct TileRange {
   int begin, end;
 };
-// Key tiles that a query tile looks at.
-__device__ __forceinline__ TileRange key_tiles(const DaParams& p, int b, int qt) {
-  if (qt >= p.nt) return {0, 0};
-  if (!p.qt) return {0, p.causal ? min(qt + 1, p.nt) : p.nt};
+// Steps of n keys that a query tile looks at.
+__device__ __forceinline__ TileRange key_steps(const DaParams& p, int b, int qt, int n) {
+  if (!p.qt) return {0, ((p.causal ? min((qt + 1) * DA_TILE, p.S) : p.S) + n - 1) / n};
   const int4 t = __ldg(p.qt + (int64_t)b * p.nt + qt);
   if (t.y <= t.x) return {0, 0};
-  return {t.x / DA_TILE, (t.y + DA_TILE - 1) / DA_TILE};
+  return {t.x / n, (t.y + n - 1) / n};
 }
 // Query tiles that look at a key tile.
 __device__ __forceinline__ TileRange query_tiles(const DaParams& p, int b, int kt) {
@@ -90,31 +88,38 @@ __device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* tmap, ui
       : "memory");
 }
 
-// Zero the rows of a 128-row operand tile (BLOCKS blocks of 64 columns, 128 bytes a row) that hold padding tokens: their
-// contents may be anything, and 0 x NaN would reach rows that do not see them.  n threads, this one t.
-template <int BLOCKS>
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+// Zero the rows of an operand tile (ROWS tokens from pos0, BLOCKS blocks of 64 columns, 128 bytes a row) that
+// hold padding tokens: their contents may be anything, and 0 x NaN would reach rows that do not see them.
+// n threads, this one t.
+template <int BLOCKS, int ROWS>
 __device__ __forceinline__ void zero_pad_rows(uint8_t* tile, const DaParams& p, int b, int pos0, int t, int n) {
-  for (int r = t; r < DA_TILE; r += n) {
+  for (int r = t; r < ROWS; r += n) {
     const TileRange v = key_range(p, b, pos0 + r);
     if (v.end > v.begin) continue;
 #pragma unroll 1
     for (int q = 0; q < BLOCKS * 8; ++q)
-      *reinterpret_cast<uint4*>(tile + (q >> 3) * (DA_TILE * 128) + r * 128 + (q & 7) * 16) = make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4*>(tile + (q >> 3) * (ROWS * 128) + r * 128 + (q & 7) * 16) = make_uint4(0, 0, 0, 0);
   }
   fence_proxy_async_smem();
 }
 
-// Tensor map over [B, S, H, D]: boxes of 64 columns x 128 tokens of one head, 128-byte swizzle.
+// Tensor map over [B, S, H, D]: boxes of 64 columns x `rows` tokens of one head, 128-byte swizzle.
 // Columns past D and tokens past S read as zero, so a head width need not be a multiple of 64 and
 // a row's last tile never reads the next row.
-inline CUtensorMap da_tmap(const DaTensor& t, int B, int S, int H, int D) {
+inline CUtensorMap da_tmap(const DaTensor& t, int B, int S, int H, int D, int rows = DA_TILE) {
   OXI_CHECK((reinterpret_cast<uintptr_t>(t.ptr) & 15) == 0, "TMA base must be 16-byte aligned");
   OXI_CHECK(t.sb % 8 == 0 && t.ss % 8 == 0 && t.sh % 8 == 0 && D % 8 == 0, "TMA strides must be multiples of 16 bytes");
   ensure_current_context();
   CUtensorMap m;
   cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)S, (cuuint64_t)B};
   cuuint64_t strides[3] = {(cuuint64_t)(t.sh * 2), (cuuint64_t)(t.ss * 2), (cuuint64_t)(t.sb * 2)};
-  cuuint32_t box[4] = {64, 1, DA_TILE, 1};
+  cuuint32_t box[4] = {64, 1, (cuuint32_t)rows, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = get_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(t.ptr), dims, strides, box,
                                estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,

@@ -6,95 +6,81 @@
 // Two kernels that each own their outputs, so no gradient is summed with atomics and the results do
 // not depend on the order in which CTAs run; each recomputes S and dP (seven tile products where one
 // kernel with an atomic dQ has five):
-//   dQ:     one CTA per (128 queries, query head, batch), over key tiles
+//   dQ:     one CTA per (128 queries, query head, batch), over key steps of 64
 //   dK, dV: one CTA per (128 keys, key head, batch), over the query heads of the group and query tiles
 // Both keep their accumulators in TMEM and feed dS (and P^T) to the tensor cores from TMEM, written by
 // the softmax warps over the scores they were computed from.
+//
+// delta is formed in the dQ kernel, from the rounded o, and is off by what that rounding does.  The
+// row's sum of P (dP - delta) would be zero with the true one: the dQ kernel adds it up as it goes,
+// and the dK / dV kernel behind it gets the corrected delta.
 #include "doc_attn.cuh"
 
 namespace oxi {
 namespace {
 
-// ------------------------------------------------------------------ delta
-// delta[b, h, s] = sum_d dO o, one warp per 32 / (Dv / 8) rows: every thread reads 16 bytes of each.
-__global__ void __launch_bounds__(256) da_delta_kernel(const __nv_bfloat16* __restrict__ o, int64_t osb, int64_t oss,
-                                                       int64_t osh, const __nv_bfloat16* __restrict__ d, int64_t dsb,
-                                                       int64_t dss, int64_t dsh, int B, int S, int Hq, int Dv,
-                                                       float* __restrict__ delta) {
-  const int lane = threadIdx.x & 31;
-  const int64_t rows = (int64_t)B * S * Hq;
-  for (int64_t row = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; row < rows; row += (int64_t)gridDim.x * 8) {
-    const int h = (int)(row % Hq);
-    const int64_t t = row / Hq, b = t / S, s = t % S;
-    float sum = 0.f;
-    if (lane * 8 < Dv) {
-      const uint4 x = *reinterpret_cast<const uint4*>(o + b * osb + s * oss + h * osh + lane * 8);
-      const uint4 y = *reinterpret_cast<const uint4*>(d + b * dsb + s * dss + h * dsh + lane * 8);
-      const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 a = unpack_bf16(xw[i]), c = unpack_bf16(yw[i]);
-        sum = fmaf(a.x, c.x, fmaf(a.y, c.y, sum));
-      }
-    }
-#pragma unroll
-    for (int q = 8; q > 0; q >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, q);
-    if (lane == 0) delta[(b * Hq + h) * S + s] = sum;
-  }
-}
-
 // ------------------------------------------------------------------ dQ
+constexpr int DQ_KEYS = 64;
+constexpr int DQ_THREADS = 320;  // TMA warp, MMA warp, 8 softmax warps: 32 query rows x 32 keys each
+
 template <int DQP, int DVP>
 struct DaDqSmem {
   static constexpr int KBQ = DQP / 64, KBV = DVP / 64;
-  static constexpr int BLK = DA_TILE * 128;
-  static constexpr int Q_BYTES = KBQ * BLK, V_BYTES = KBV * BLK;
-  static constexpr int ST = 2;  // K / V stages
+  static constexpr int QBLK = DA_TILE * 128, KBLK = DQ_KEYS * 128;
+  static constexpr int Q_BYTES = KBQ * QBLK, DO_BYTES = KBV * QBLK, K_BYTES = KBQ * KBLK, V_BYTES = KBV * KBLK;
+  static constexpr int KST = 2, VST = 1;  // K_i is held until its dQ product, V_i only until dP_i
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_DO = OFF_Q + Q_BYTES;
-  static constexpr int OFF_K = OFF_DO + V_BYTES;
-  static constexpr int OFF_V = OFF_K + ST * Q_BYTES;
-  static constexpr int OFF_BAR = OFF_V + ST * V_BYTES;
-  static constexpr int TOTAL = OFF_BAR + 256 + 1024;
-  static_assert(TOTAL <= 232448, "shared memory budget");
+  static constexpr int OFF_K = OFF_DO + DO_BYTES;
+  static constexpr int OFF_V = OFF_K + KST * K_BYTES;
+  static constexpr int OFF_BAR = OFF_V + VST * V_BYTES;
+  // two CTAs of the widest heads fill the SM's shared memory: there is no room to align the base by
+  // hand, it has to be on a 1024-byte boundary (the kernel checks)
+  static constexpr int TOTAL = OFF_BAR + 256;
+  static_assert(2 * (TOTAL + 1024) <= 233472, "two CTAs per SM");
 };
 
-// One column half (64 keys) of a 128 x 128 tile per warp, 32 query rows; TMEM: dQ, two S buffers, dP.
+// Two CTAs on an SM: one's softmax runs while the tensor cores work for the other.  TMEM: dQ, S (then dS), dP.
 template <int DQP, int DVP, bool CAP, bool ALIBI>
-__global__ void __launch_bounds__(DA_THREADS, 1)
+__global__ void __launch_bounds__(DQ_THREADS, 2)
     da_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO, DaParams p,
-                 const float* __restrict__ lse2, const float* __restrict__ delta, __nv_bfloat16* __restrict__ dq,
-                 int64_t ld) {
+                 DaTensor o_in, DaTensor do_in, const float* __restrict__ lse2, float* __restrict__ delta,
+                 __nv_bfloat16* __restrict__ dq, int64_t ld) {
   using L = DaDqSmem<DQP, DVP>;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0) record_error(p.status, OXI_ERR_BOUNDS);
+    return;
+  }
   uint8_t *sQ = smem + L::OFF_Q, *sDO = smem + L::OFF_DO, *sK = smem + L::OFF_K, *sV = smem + L::OFF_V;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* q_full = bars + 0;
-  uint64_t* kv_full = bars + 1;   // [2]
-  uint64_t* kv_empty = bars + 3;  // [2]
-  uint64_t* s_full = bars + 5;    // S and dP of a key tile
-  uint64_t* dp_free = bars + 6;   // dP has been read into registers
-  uint64_t* ds_full = bars + 7;
-  uint64_t* all_done = bars + 8;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 9);
+  uint64_t* k_full = bars + 1;   // [2]
+  uint64_t* k_empty = bars + 3;  // [2]
+  uint64_t* v_full = bars + 5;
+  uint64_t* v_empty = bars + 6;
+  uint64_t* s_full = bars + 7;
+  uint64_t* dp_full = bars + 8;
+  uint64_t* ds_full = bars + 9;
+  uint64_t* all_done = bars + 10;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 11);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int qt = gridDim.z - 1 - blockIdx.z, h = blockIdx.x, b = blockIdx.y;
   const int hk = h / (p.Hq / p.Hk);
-  const TileRange kr = key_tiles(p, b, qt);
-  const int n = kr.end - kr.begin;
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
     }
+    mbar_init(v_full, 1);
+    mbar_init(v_empty, 1);
     mbar_init(s_full, 1);
-    mbar_init(dp_free, 8);
+    mbar_init(dp_full, 1);
     mbar_init(ds_full, 8);
     mbar_init(all_done, 1);
     *abort_flag = 0;
@@ -105,72 +91,78 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
     tma_prefetch_desc(&tmDO);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
+    tmem_alloc(tmem_slot, 256);
     tmem_relinquish();
   }
+  const TileRange kr = key_steps(p, b, qt, DQ_KEYS);
+  const int n = kr.end - kr.begin;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const uint32_t TM_DQ = tmem, TM_S = tmem + 128, TM_DP = tmem + 384;
+  const uint32_t TM_DQ = tmem, TM_S = tmem + 128, TM_DP = tmem + 192;
 
   if (warp == 0) {
     if (lane == 0 && n > 0) {
-      mbar_arrive_expect_tx(q_full, L::Q_BYTES + L::V_BYTES);
+      mbar_arrive_expect_tx(q_full, L::Q_BYTES + L::DO_BYTES);
 #pragma unroll
-      for (int kb = 0; kb < L::KBQ; ++kb) tma_load_4d(sQ + kb * L::BLK, &tmQ, q_full, kb * 64, h, qt * DA_TILE, b);
+      for (int kb = 0; kb < L::KBQ; ++kb) tma_load_4d(sQ + kb * L::QBLK, &tmQ, q_full, kb * 64, h, qt * DA_TILE, b);
 #pragma unroll
-      for (int kb = 0; kb < L::KBV; ++kb) tma_load_4d(sDO + kb * L::BLK, &tmDO, q_full, kb * 64, h, qt * DA_TILE, b);
-      int i = 0;
-      for (; i < n; ++i) {
-        const int st = i % L::ST;
-        if (!mbar_wait(&kv_empty[st], ((i / L::ST) & 1) ^ 1, abort_flag, p.status)) break;
-        mbar_arrive_expect_tx(&kv_full[st], L::Q_BYTES + L::V_BYTES);
+      for (int kb = 0; kb < L::KBV; ++kb) tma_load_4d(sDO + kb * L::QBLK, &tmDO, q_full, kb * 64, h, qt * DA_TILE, b);
+      int ki = 0, vi = 0;
+      for (; ki < n; ++ki) {
+        const int st = ki % L::KST;
+        if (!mbar_wait(&k_empty[st], ((ki / L::KST) & 1) ^ 1, abort_flag, p.status)) break;
+        mbar_arrive_expect_tx(&k_full[st], L::K_BYTES);
 #pragma unroll
         for (int kb = 0; kb < L::KBQ; ++kb)
-          tma_load_4d(sK + st * L::Q_BYTES + kb * L::BLK, &tmK, &kv_full[st], kb * 64, hk, (kr.begin + i) * DA_TILE, b);
+          tma_load_4d(sK + st * L::K_BYTES + kb * L::KBLK, &tmK, &k_full[st], kb * 64, hk, (kr.begin + ki) * DQ_KEYS, b);
+        // V_{j} behind K_{j+1}
+        bool ok = true;
+        for (; ok && vi < n && (vi < ki || ki == n - 1); ++vi) {
+          ok = mbar_wait(v_empty, (vi & 1) ^ 1, abort_flag, p.status);
+          if (!ok) break;
+          mbar_arrive_expect_tx(v_full, L::V_BYTES);
 #pragma unroll
-        for (int kb = 0; kb < L::KBV; ++kb)
-          tma_load_4d(sV + st * L::V_BYTES + kb * L::BLK, &tmV, &kv_full[st], kb * 64, hk, (kr.begin + i) * DA_TILE, b);
+          for (int kb = 0; kb < L::KBV; ++kb)
+            tma_load_4d(sV + kb * L::KBLK, &tmV, v_full, kb * 64, hk, (kr.begin + vi) * DQ_KEYS, b);
+        }
+        if (!ok) { ++ki; break; }
       }
       mbar_wait(q_full, 0, nullptr, p.status);
-      for (int u = max(0, i - L::ST); u < i; ++u) mbar_wait(&kv_full[u % L::ST], (u / L::ST) & 1, nullptr, p.status);
+      for (int i = max(0, ki - L::KST); i < ki; ++i) mbar_wait(&k_full[i % L::KST], (i / L::KST) & 1, nullptr, p.status);
+      if (vi > 0) mbar_wait(v_full, (vi - 1) & 1, nullptr, p.status);
     }
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0 && n > 0) {
-      constexpr uint32_t ID_S = umma_idesc_bf16(DA_TILE, DA_TILE, false, false);
+      constexpr uint32_t ID_S = umma_idesc_bf16(DA_TILE, DQ_KEYS, false, false);
       constexpr uint32_t ID_Q = umma_idesc_bf16(DA_TILE, DQP, false, true);
       const int nkq = (p.Dqk + 15) / 16, nkv = (p.Dv + 15) / 16;
-      const uint32_t aQ = smem_u32(sQ), aDO = smem_u32(sDO);
+      const uint32_t aQ = smem_u32(sQ), aDO = smem_u32(sDO), aV = smem_u32(sV);
       bool ok = mbar_wait(q_full, 0, abort_flag, p.status);
-      // S_i into buffer i & 1, which last held dS_{i-2}, read by a product issued before; dP_i once
-      // the softmax warps have read dP_{i-1}
-      auto issue = [&](int i) -> bool {
-        const int st = i % L::ST;
-        if (!mbar_wait(&kv_full[st], (i / L::ST) & 1, abort_flag, p.status)) return false;
+      for (int i = 0; i < n && ok; ++i) {
+        // S_i over dS_{i-1}, read by the product issued just before; dP_{i-1} has been read as well
+        // (its softmax warps have handed dS over)
+        const uint32_t aK = smem_u32(sK + (i % L::KST) * L::K_BYTES);
+        if (!mbar_wait(&k_full[i % L::KST], (i / L::KST) & 1, abort_flag, p.status)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t aK = smem_u32(sK + st * L::Q_BYTES), aV = smem_u32(sV + st * L::V_BYTES);
         for (int kk = 0; kk < nkq; ++kk)
-          tc_mma_f16(TM_S + (i & 1) * 128, da_kmajor_desc(aQ, kk, L::BLK), da_kmajor_desc(aK, kk, L::BLK), ID_S, kk != 0);
-        if (i > 0 && !mbar_wait(dp_free, (i - 1) & 1, abort_flag, p.status)) return false;
+          tc_mma_f16(TM_S, da_kmajor_desc(aQ, kk, L::QBLK), da_kmajor_desc(aK, kk, L::KBLK), ID_S, kk != 0);
+        tc_commit(s_full);
+        if (!mbar_wait(v_full, i & 1, abort_flag, p.status)) { ok = false; break; }
         tc_fence_after();
         for (int kk = 0; kk < nkv; ++kk)
-          tc_mma_f16(TM_DP, da_kmajor_desc(aDO, kk, L::BLK), da_kmajor_desc(aV, kk, L::BLK), ID_S, kk != 0);
-        tc_commit(s_full);
-        return true;
-      };
-      if (ok) ok = issue(0);
-      for (int i = 0; i < n && ok; ++i) {
-        if (i + 1 < n && !issue(i + 1)) { ok = false; break; }
+          tc_mma_f16(TM_DP, da_kmajor_desc(aDO, kk, L::QBLK), da_kmajor_desc(aV, kk, L::KBLK), ID_S, kk != 0);
+        tc_commit(dp_full);
+        tc_commit(v_empty);
         if (!mbar_wait(ds_full, i & 1, abort_flag, p.status)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t aK = smem_u32(sK + (i % L::ST) * L::Q_BYTES);
 #pragma unroll
-        for (int kk = 0; kk < DA_TILE / 16; ++kk)  // keys 0..63 in columns 0..31, 64..127 in columns 64..95
-          tc_mma_f16_ts(TM_DQ, TM_S + (i & 1) * 128 + (kk < 4 ? kk * 8 : 64 + (kk - 4) * 8),
-                        umma_desc_sw128(aK + kk * 2048, L::BLK, 1024), ID_Q, (i | kk) != 0);
-        tc_commit(&kv_empty[i % L::ST]);
+        for (int kk = 0; kk < DQ_KEYS / 16; ++kk)  // keys 0..31 in columns 0..15, 32..63 in columns 32..47
+          tc_mma_f16_ts(TM_DQ, TM_S + (kk >> 1) * 32 + (kk & 1) * 8, umma_desc_sw128(aK + kk * 2048, L::KBLK, 1024), ID_Q,
+                        (i | kk) != 0);
+        tc_commit(&k_empty[i % L::KST]);
         if (i == n - 1) tc_commit(all_done);
       }
     }
@@ -182,61 +174,88 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
     const TileRange vis = key_range(p, b, qpos);
     const int all_lo = __reduce_max_sync(0xffffffffu, vis.begin), all_hi = __reduce_min_sync(0xffffffffu, vis.end);
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_addr = TM_S + lane_base + half * 32, dp_addr = TM_DP + lane_base + half * 32;
+    const bool in = qpos < p.S;
     const int64_t vi = ((int64_t)b * p.Hq + h) * p.S + qpos;
-    const float ls = qpos < p.S ? lse2[vi] : INFINITY, dl = qpos < p.S ? delta[vi] : 0.f;
+    const float ls = in ? lse2[vi] : INFINITY;
+    float dl = 0.f;  // delta of the row, formed while the first tiles load
+    if (in) {
+      const __nv_bfloat16* orow = reinterpret_cast<const __nv_bfloat16*>(o_in.ptr) + b * o_in.sb + qpos * o_in.ss + h * o_in.sh;
+      const __nv_bfloat16* drow = reinterpret_cast<const __nv_bfloat16*>(do_in.ptr) + b * do_in.sb + qpos * do_in.ss + h * do_in.sh;
+      for (int c = 0; c < p.Dv; c += 8) {
+        const uint4 x = __ldg(reinterpret_cast<const uint4*>(orow + c)), y = __ldg(reinterpret_cast<const uint4*>(drow + c));
+        const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 a = unpack_bf16(xw[e]), g = unpack_bf16(yw[e]);
+          dl = fmaf(a.x, g.x, fmaf(a.y, g.y, dl));
+        }
+      }
+    }
     const float slope2 = ALIBI ? __ldg(p.slopes + h) * LOG2E : 0.f;
     const float C = ALIBI ? 1.f : p.c_log2;
+    float rest = 0.f;  // sum of P (dP - delta) over this thread's keys
     bool ok = true;
     for (int i = 0; i < n; ++i) {
-      const int k0 = (kr.begin + i) * DA_TILE + half * 64;
+      const int k0 = (kr.begin + i) * DQ_KEYS + half * 32;
+      const bool padded = tile_has_pad(p, b, k0 / DA_TILE);
       if (!mbar_wait(s_full, i & 1, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
-      const uint32_t s_addr = TM_S + (i & 1) * 128 + lane_base + half * 64;
-      uint32_t x[2][32], d[2][32];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        tmem_ld32(s_addr + c * 32, x[c]);
-        tmem_ld32(TM_DP + lane_base + half * 64 + c * 32, d[c]);
-      }
+      uint32_t x[32];
+      tmem_ld32(s_addr, x);
       tc_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(dp_free);
-      const bool masked = !(all_lo <= k0 && k0 + 64 <= all_hi);
+      const bool masked = !(all_lo <= k0 && k0 + 32 <= all_hi);
+      const uint32_t bits = masked ? range_bits(vis.begin, vis.end, k0) : 0xffffffffu;
+      const float fd = (float)(qpos - k0);
+      float f[CAP ? 32 : 1];
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        float v = __uint_as_float(x[e]);
+        if (CAP) v = tanh_ex2(v * p.x_scale, f[e]);
+        if (ALIBI) v = fmaf(-slope2, fabsf(fd - (float)e), v * p.c_log2);
+        x[e] = __float_as_uint(ex2_approx(fmaf(v, C, -ls)));
+      }
+      if (!mbar_wait(dp_full, i & 1, abort_flag, p.status)) { ok = false; break; }
+      tc_fence_after();
+      float rs[2] = {0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const float fd = (float)(qpos - (k0 + c * 32));
-        const uint32_t bits = masked ? range_bits(vis.begin, vis.end, k0 + c * 32) : 0xffffffffu;
+        uint32_t d[16], pk[8];
+        tmem_ld16(dp_addr + c * 16, d);
+        tc_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          float v = __uint_as_float(x[c][e]), f = 1.f;
-          if (CAP) v = tanh_ex2(v * p.x_scale, f);
-          if (ALIBI) v = fmaf(-slope2, fabsf(fd - (float)e), v * p.c_log2);
-          float ds = ex2_approx(fmaf(v, C, -ls)) * (__uint_as_float(d[c][e]) - dl);
-          if (CAP) ds *= f;
-          x[c][e] = __float_as_uint(ds);
+        for (int e = 0; e < 16; ++e) {
+          const int t = c * 16 + e;
+          float g = __uint_as_float(x[t]) * (__uint_as_float(d[e]) - dl);
+          if (masked) g = ((bits >> t) & 1u) ? g : 0.f;
+          rs[e & 1] += g;
+          if (CAP) {
+            g *= f[t];
+            if (masked) g = ((bits >> t) & 1u) ? g : 0.f;  // a hidden score may be NaN, and f with it
+          }
+          d[e] = __float_as_uint(g);
         }
-        if (masked) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!((bits >> e) & 1u)) x[c][e] = 0u;
-        }
-        uint32_t pk[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) pk[e] = pack_bf16(__uint_as_float(x[c][2 * e]), __uint_as_float(x[c][2 * e + 1]));
-        tmem_st16(s_addr + c * 16, pk);
+        for (int e = 0; e < 8; ++e) pk[e] = pack_bf16(__uint_as_float(d[2 * e]), __uint_as_float(d[2 * e + 1]));
+        tmem_st8(s_addr + c * 8, pk);
       }
+      rest += rs[0] + rs[1];
       // S_i has read K_i: rows of padding become zero before the dQ product reads them
-      if (tile_has_pad(p, b, kr.begin + i))
-        zero_pad_rows<L::KBQ>(sK + (i % L::ST) * L::Q_BYTES, p, b, (kr.begin + i) * DA_TILE, half * 128 + r, 256);
+      if (padded)
+        zero_pad_rows<L::KBQ, DQ_KEYS>(sK + (i % L::KST) * L::K_BYTES, p, b, (kr.begin + i) * DQ_KEYS, half * 128 + r, 256);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(ds_full);
     }
     if (ok && n > 0 && !mbar_wait(all_done, 0, abort_flag, p.status)) ok = false;
+    // the halves' rests meet in shared memory: every product has completed, so K's ring is free
+    float* s_rest = reinterpret_cast<float*>(sK);
+    if (ok) s_rest[half * DA_TILE + r] = rest;
+    asm volatile("bar.sync 1, 256;" ::: "memory");  // reached by every softmax warp
     if (ok) {
       tc_fence_after();
+      if (half == 0 && in) delta[vi] = dl + (s_rest[r] + s_rest[DA_TILE + r]);
       __nv_bfloat16* row = dq + ((int64_t)b * p.S + qpos) * ld + (int64_t)h * p.Dqk;
 #pragma unroll 1
       for (int c = half; c < DQP / 32; c += 2) {
@@ -248,7 +267,7 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
 #pragma unroll
           for (int e = 0; e < 32; ++e) w[e] = 0u;
         }
-        if (qpos < p.S) {
+        if (in) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             if (c * 32 + q * 8 < p.Dqk) {
@@ -268,11 +287,13 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, 256);
   }
 }
 
 // ------------------------------------------------------------------ dK, dV
+constexpr int DKV_THREADS = 64 + 512;  // TMA warp, MMA warp, 16 softmax warps: 32 keys x 32 queries each
+
 template <int DQP, int DVP>
 struct DaDkvSmem {
   static constexpr int KBQ = DQP / 64, KBV = DVP / 64;
@@ -290,14 +311,22 @@ struct DaDkvSmem {
   static_assert(TOTAL <= 232448, "shared memory budget");
 };
 
+// Where a CTA's dK, dV go: bf16 rows, or (split > 1) f32 parts [split][B, Hk, S, Dqk + Dv]
+struct DkvOut {
+  __nv_bfloat16 *dk, *dv;
+  int64_t ldk, ldv;
+  float* part;
+  int splits;
+};
+
 // Transposed tiles: TMEM lanes are keys, columns queries.  TMEM: dV, dK, S^T (then P^T), dP^T (then dS^T).
-// A warp owns 32 keys and 64 of the tile's queries.
+// While the softmax warps turn dP^T into dS^T the tensor cores add P^T dO to dV and form the next S^T;
+// while they turn that into P^T, dS^T Q and the next dP^T.
 template <int DQP, int DVP, bool CAP, bool ALIBI>
-__global__ void __launch_bounds__(DA_THREADS, 1)
+__global__ void __launch_bounds__(DKV_THREADS, 1)
     da_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO, DaParams p,
-                  const float* __restrict__ lse2, const float* __restrict__ delta, __nv_bfloat16* __restrict__ dk,
-                  int64_t ldk, __nv_bfloat16* __restrict__ dv, int64_t ldv) {
+                  const float* __restrict__ lse2, const float* __restrict__ delta, DkvOut out) {
   using L = DaDkvSmem<DQP, DVP>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -318,10 +347,8 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   // the first key tiles have the most (causal) queries and start first
-  const int kt = blockIdx.z, hk = blockIdx.x, b = blockIdx.y;
+  const int kt = blockIdx.z, hk = blockIdx.x / out.splits, part = blockIdx.x % out.splits, b = blockIdx.y;
   const int group = p.Hq / p.Hk;
-  const TileRange qr = query_tiles(p, b, kt);
-  const int ni = qr.end - qr.begin, n = group * ni;
 
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
@@ -332,8 +359,8 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
     }
     mbar_init(s_full, 1);
     mbar_init(dp_full, 1);
-    mbar_init(p_full, 8);
-    mbar_init(ds_full, 8);
+    mbar_init(p_full, 16);
+    mbar_init(ds_full, 16);
     mbar_init(all_done, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -346,6 +373,10 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
+  // this CTA's share of the (query head, query tile) pairs that see the key tile
+  const TileRange qr = query_tiles(p, b, kt);
+  const int ni = qr.end - qr.begin, total = group * ni;
+  const int first = (int)((int64_t)total * part / out.splits), n = (int)((int64_t)total * (part + 1) / out.splits) - first;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -364,7 +395,7 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
       int it = 0;
       for (; it < n; ++it) {
         const int st = it % L::ST;
-        const int h = hk * group + it / ni, q0 = (qr.begin + it % ni) * DA_TILE;
+        const int h = hk * group + (first + it) / ni, q0 = (qr.begin + (first + it) % ni) * DA_TILE;
         const bool ok = mbar_wait(&q_empty[st], ((it / L::ST) & 1) ^ 1, abort_flag, p.status);
         if (!__all_sync(0xffffffffu, ok)) break;
         if (lane == 0) {
@@ -417,6 +448,8 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
           tc_mma_f16(TM_DP, da_kmajor_desc(aV, kk, L::BLK), da_kmajor_desc(a_do(it), kk, L::BLK), ID_S, kk != 0);
         tc_commit(dp_full);
       };
+      // queries 16 kk ..: 32 queries a softmax warp, as bf16 in the first half of its columns
+      auto a_t = [&](uint32_t t, int kk) { return t + (kk >> 1) * 32 + (kk & 1) * 8; };
       auto wait_q = [&](int it) { return mbar_wait(&q_full[it % L::ST], (it / L::ST) & 1, abort_flag, p.status); };
       if (ok) ok = wait_q(0);
       if (ok) {
@@ -428,9 +461,8 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
         if (!mbar_wait(p_full, it & 1, abort_flag, p.status)) { ok = false; break; }
         tc_fence_after();
 #pragma unroll
-        for (int kk = 0; kk < DA_TILE / 16; ++kk)  // queries 0..63 in columns 0..31, 64..127 in columns 64..95
-          tc_mma_f16_ts(TM_DV, TM_S + (kk < 4 ? kk * 8 : 64 + (kk - 4) * 8),
-                        umma_desc_sw128(a_do(it) + kk * 2048, L::BLK, 1024), ID_V, (it | kk) != 0);
+        for (int kk = 0; kk < DA_TILE / 16; ++kk)
+          tc_mma_f16_ts(TM_DV, a_t(TM_S, kk), umma_desc_sw128(a_do(it) + kk * 2048, L::BLK, 1024), ID_V, (it | kk) != 0);
         if (it + 1 < n) {
           if (!wait_q(it + 1)) { ok = false; break; }
           tc_fence_after();
@@ -440,8 +472,7 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < DA_TILE / 16; ++kk)
-          tc_mma_f16_ts(TM_DK, TM_DP + (kk < 4 ? kk * 8 : 64 + (kk - 4) * 8),
-                        umma_desc_sw128(a_q(it) + kk * 2048, L::BLK, 1024), ID_K, (it | kk) != 0);
+          tc_mma_f16_ts(TM_DK, a_t(TM_DP, kk), umma_desc_sw128(a_q(it) + kk * 2048, L::BLK, 1024), ID_K, (it | kk) != 0);
         tc_commit(&q_empty[it % L::ST]);
         if (it + 1 < n) issue_dp(it + 1);
         else tc_commit(all_done);
@@ -449,15 +480,16 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int quarter = warp & 3, sub = (warp - 2) >> 2;  // 32 keys, 32 queries
     const int r = quarter * 32 + lane;
     const int kpos = kt * DA_TILE + r;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const uint32_t s_addr = TM_S + lane_base + sub * 32, dp_addr = TM_DP + lane_base + sub * 32;
     const float C = ALIBI ? 1.f : p.c_log2;
     bool ok = true;
     for (int it = 0; it < n; ++it) {
       const int st = it % L::ST, u = it / L::ST;
-      const int h = hk * group + it / ni, qi = qr.begin + it % ni, q0 = qi * DA_TILE;
+      const int h = hk * group + (first + it) / ni, qi = qr.begin + (first + it) % ni, q0 = qi * DA_TILE;
       // every query of the tile sees every key of this warp?
       bool masked;
       bool padded = false;
@@ -470,45 +502,49 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
         masked = (p.causal && q0 < kt * DA_TILE + DA_TILE) || kt * DA_TILE + DA_TILE > p.S || q0 + DA_TILE > p.S;
       }
       const float slope2 = ALIBI ? __ldg(p.slopes + h) * LOG2E : 0.f;
-      const float* vec = s_vec + st * 4 * DA_TILE + half * 64;
-      const int* ivec = reinterpret_cast<const int*>(vec);
+      const float4* vec = reinterpret_cast<const float4*>(s_vec + st * 4 * DA_TILE + sub * 32);
+      const int4* ivec = reinterpret_cast<const int4*>(vec);
+      const float fd = (float)(q0 + sub * 32 - kpos);
       if (!mbar_wait(&vec_full[st], u & 1, abort_flag, p.status) ||
           !mbar_wait(s_full, it & 1, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
-      uint32_t x[2][32];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) tmem_ld32(TM_S + lane_base + half * 64 + c * 32, x[c]);
+      uint32_t x[32], pk[16];
+      tmem_ld32(s_addr, x);
       tc_wait_ld();
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float fd = (float)(q0 + half * 64 + c * 32 - kpos);
-        uint32_t pk[16];
+      for (int e = 0; e < 32; e += 4) {
+        const float4 l4 = vec[e / 4];
+        const float ls[4] = {l4.x, l4.y, l4.z, l4.w};
+        float pr[4], w[4];
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          float pr[2];
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            float v = __uint_as_float(x[c][e + g]), f = 1.f;
-            if (CAP) v = tanh_ex2(v * p.x_scale, f);
-            if (ALIBI) v = fmaf(-slope2, fabsf(fd + (float)(e + g)), v * p.c_log2);
-            float pp = ex2_approx(fmaf(v, C, -vec[c * 32 + e + g]));
-            if (masked) {
-              const int q = c * 32 + e + g;
-              const bool sees = ivec[2 * DA_TILE + q] <= kpos && kpos < ivec[3 * DA_TILE + q];
-              pp = sees ? pp : 0.f;
-              if (CAP) f = sees ? f : 0.f;  // the score of a hidden pair may be NaN
-            }
-            pr[g] = pp;
-            x[c][e + g] = __float_as_uint(CAP ? pp * f : pp);
-          }
-          pk[e / 2] = pack_bf16(pr[0], pr[1]);
+        for (int g = 0; g < 4; ++g) {
+          float v = __uint_as_float(x[e + g]);
+          w[g] = 1.f;
+          if (CAP) v = tanh_ex2(v * p.x_scale, w[g]);
+          if (ALIBI) v = fmaf(-slope2, fabsf(fd + (float)(e + g)), v * p.c_log2);
+          pr[g] = ex2_approx(fmaf(v, C, -ls[g]));
+          w[g] = CAP ? pr[g] * w[g] : pr[g];
         }
-        tmem_st16(TM_S + lane_base + half * 64 + c * 16, pk);
+        if (masked) {
+          const int4 lo = ivec[2 * DA_TILE / 4 + e / 4], hi = ivec[3 * DA_TILE / 4 + e / 4];
+          const int lo4[4] = {lo.x, lo.y, lo.z, lo.w}, hi4[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const bool sees = lo4[g] <= kpos && kpos < hi4[g];
+            pr[g] = sees ? pr[g] : 0.f;
+            w[g] = sees ? w[g] : 0.f;  // the score of a hidden pair may be NaN
+          }
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) x[e + g] = __float_as_uint(w[g]);
+        pk[e / 2] = pack_bf16(pr[0], pr[1]);
+        pk[e / 2 + 1] = pack_bf16(pr[2], pr[3]);
       }
+      tmem_st16(s_addr, pk);
       if (padded) {
         if (!mbar_wait(&q_full[st], u & 1, abort_flag, p.status)) { ok = false; break; }
-        zero_pad_rows<L::KBV>(sDO + st * L::V_BYTES, p, b, q0, half * 128 + r, 256);
-        zero_pad_rows<L::KBQ>(sQ + st * L::Q_BYTES, p, b, q0, half * 128 + r, 256);
+        zero_pad_rows<L::KBV, DA_TILE>(sDO + st * L::V_BYTES, p, b, q0, sub * 128 + r, 512);
+        zero_pad_rows<L::KBQ, DA_TILE>(sQ + st * L::Q_BYTES, p, b, q0, sub * 128 + r, 512);
       }
       tc_wait_st();
       tc_fence_before();
@@ -516,26 +552,24 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
       if (lane == 0) mbar_arrive(p_full);
       if (!mbar_wait(dp_full, it & 1, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
-      uint32_t d[2][32];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) tmem_ld32(TM_DP + lane_base + half * 64 + c * 32, d[c]);
+      uint32_t d[32];
+      tmem_ld32(dp_addr, d);
       tc_wait_ld();
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t pk[16];
+      for (int e = 0; e < 32; e += 4) {
+        const float4 d4 = vec[DA_TILE / 4 + e / 4];
+        const float dl[4] = {d4.x, d4.y, d4.z, d4.w};
+        float ds[4];
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          float ds[2];
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const float w = __uint_as_float(x[c][e + g]);
-            ds[g] = w * (__uint_as_float(d[c][e + g]) - vec[DA_TILE + c * 32 + e + g]);
-            if (masked && w == 0.f) ds[g] = 0.f;  // a hidden pair adds nothing, whatever dP is
-          }
-          pk[e / 2] = pack_bf16(ds[0], ds[1]);
+        for (int g = 0; g < 4; ++g) {
+          const float w = __uint_as_float(x[e + g]);
+          ds[g] = w * (__uint_as_float(d[e + g]) - dl[g]);
+          if (masked) ds[g] = w == 0.f ? 0.f : ds[g];  // a hidden pair adds nothing, whatever dP is
         }
-        tmem_st16(TM_DP + lane_base + half * 64 + c * 16, pk);
+        pk[e / 2] = pack_bf16(ds[0], ds[1]);
+        pk[e / 2 + 1] = pack_bf16(ds[2], ds[3]);
       }
+      tmem_st16(dp_addr, pk);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -547,12 +581,10 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
 #pragma unroll 1
       for (int which = 0; which < 2; ++which) {
         const int width = which ? p.Dqk : p.Dv;
-        __nv_bfloat16* row = which ? dk + ((int64_t)b * p.S + kpos) * ldk + (int64_t)hk * p.Dqk
-                                   : dv + ((int64_t)b * p.S + kpos) * ldv + (int64_t)hk * p.Dv;
         const float f = which ? p.scale : 1.f;
         const uint32_t src = (which ? TM_DK : TM_DV) + lane_base;
 #pragma unroll 1
-        for (int c = half; c < (which ? DQP : DVP) / 32; c += 2) {
+        for (int c = sub; c < (which ? DQP : DVP) / 32; c += 4) {
           uint32_t w[32];
           if (n > 0) {
             tmem_ld32(src + c * 32, w);
@@ -561,7 +593,19 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
 #pragma unroll
             for (int e = 0; e < 32; ++e) w[e] = 0u;
           }
-          if (kpos < p.S) {
+          if (kpos >= p.S) continue;
+          if (out.splits > 1) {
+            float* row = out.part + ((((int64_t)part * p.B + b) * p.Hk + hk) * p.S + kpos) * (p.Dqk + p.Dv) +
+                         (which ? p.Dv : 0) + c * 32;
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              if (c * 32 + q * 4 < width)
+                *reinterpret_cast<float4*>(row + q * 4) =
+                    make_float4(__uint_as_float(w[q * 4]) * f, __uint_as_float(w[q * 4 + 1]) * f,
+                                __uint_as_float(w[q * 4 + 2]) * f, __uint_as_float(w[q * 4 + 3]) * f);
+          } else {
+            __nv_bfloat16* row = which ? out.dk + ((int64_t)b * p.S + kpos) * out.ldk + (int64_t)hk * p.Dqk
+                                       : out.dv + ((int64_t)b * p.S + kpos) * out.ldv + (int64_t)hk * p.Dv;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
               if (c * 32 + q * 8 < width) {
@@ -585,11 +629,33 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
   }
 }
 
+// dK, dV = the splits' parts added in order; 8 columns a thread
+__global__ void __launch_bounds__(256) da_join_kernel(const float* __restrict__ part, int splits, int B, int S, int Hk,
+                                                      int Dqk, int Dv, __nv_bfloat16* __restrict__ dk, int64_t ldk,
+                                                      __nv_bfloat16* __restrict__ dv, int64_t ldv) {
+  const int vec = (Dqk + Dv) / 8;
+  const int64_t total = (int64_t)B * Hk * S * vec;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int c = (int)(i % vec) * 8;
+    const int64_t row = i / vec, s = row % S, bh = row / S, h = bh % Hk, b = bh / Hk;
+    float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < splits; ++q) {
+      const float4* src = reinterpret_cast<const float4*>(part + ((int64_t)q * B * Hk * S + row) * (Dqk + Dv) + c);
+      const float4 x = __ldg(src), y = __ldg(src + 1);
+      a[0] += x.x; a[1] += x.y; a[2] += x.z; a[3] += x.w;
+      a[4] += y.x; a[5] += y.y; a[6] += y.z; a[7] += y.w;
+    }
+    __nv_bfloat16* dst = c < Dv ? dv + (b * S + s) * ldv + h * Dv + c : dk + (b * S + s) * ldk + h * Dqk + (c - Dv);
+    *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(a[4], a[5]),
+                                                pack_bf16(a[6], a[7]));
+  }
+}
+
 struct BwdArgs {
   DaShape s;
   DaTensor q, k, v, o, dout;
   const float* lse2;
-  float* delta;
+  float *delta, *part;
   DaOut dq, dk, dv;
   int* status;
   cudaStream_t st;
@@ -598,20 +664,33 @@ struct BwdArgs {
 template <int DQP, int DVP, bool CAP, bool ALIBI>
 void launch_bwd_t(const BwdArgs& a) {
   const DaShape& s = a.s;
-  const CUtensorMap tq = da_tmap(a.q, s.B, s.S, s.Hq, s.Dqk), tk = da_tmap(a.k, s.B, s.S, s.Hk, s.Dqk),
-                    tv = da_tmap(a.v, s.B, s.S, s.Hk, s.Dv), td = da_tmap(a.dout, s.B, s.S, s.Hq, s.Dv);
+  const CUtensorMap tq = da_tmap(a.q, s.B, s.S, s.Hq, s.Dqk), td = da_tmap(a.dout, s.B, s.S, s.Hq, s.Dv),
+                    tk = da_tmap(a.k, s.B, s.S, s.Hk, s.Dqk), tv = da_tmap(a.v, s.B, s.S, s.Hk, s.Dv),
+                    tk64 = da_tmap(a.k, s.B, s.S, s.Hk, s.Dqk, DQ_KEYS), tv64 = da_tmap(a.v, s.B, s.S, s.Hk, s.Dv, DQ_KEYS);
   const DaParams p = da_params(s, a.status);
   auto kq = da_dq_kernel<DQP, DVP, CAP, ALIBI>;
   auto kkv = da_dkv_kernel<DQP, DVP, CAP, ALIBI>;
   da_smem(kq, DaDqSmem<DQP, DVP>::TOTAL);
   da_smem(kkv, DaDkvSmem<DQP, DVP>::TOTAL);
-  kkv<<<dim3(s.Hk, s.B, p.nt), DA_THREADS, DaDkvSmem<DQP, DVP>::TOTAL, a.st>>>(
-      tq, tk, tv, td, p, a.lse2, a.delta, reinterpret_cast<__nv_bfloat16*>(a.dk.ptr), a.dk.ld,
-      reinterpret_cast<__nv_bfloat16*>(a.dv.ptr), a.dv.ld);
+  kq<<<dim3(s.Hq, s.B, p.nt), DQ_THREADS, DaDqSmem<DQP, DVP>::TOTAL, a.st>>>(
+      tq, tk64, tv64, td, p, a.o, a.dout, a.lse2, a.delta, reinterpret_cast<__nv_bfloat16*>(a.dq.ptr), a.dq.ld);
   OXI_CUDA_CHECK(cudaGetLastError());
-  kq<<<dim3(s.Hq, s.B, p.nt), DA_THREADS, DaDqSmem<DQP, DVP>::TOTAL, a.st>>>(
-      tq, tk, tv, td, p, a.lse2, a.delta, reinterpret_cast<__nv_bfloat16*>(a.dq.ptr), a.dq.ld);
+  DkvOut out;
+  out.dk = reinterpret_cast<__nv_bfloat16*>(a.dk.ptr);
+  out.dv = reinterpret_cast<__nv_bfloat16*>(a.dv.ptr);
+  out.ldk = a.dk.ld;
+  out.ldv = a.dv.ld;
+  out.part = a.part;
+  out.splits = da_bwd_splits(s.B, s.S, s.Hq, s.Hk);
+  kkv<<<dim3(s.Hk * out.splits, s.B, p.nt), DKV_THREADS, DaDkvSmem<DQP, DVP>::TOTAL, a.st>>>(tq, tk, tv, td, p, a.lse2,
+                                                                                             a.delta, out);
   OXI_CUDA_CHECK(cudaGetLastError());
+  if (out.splits > 1) {
+    const int64_t threads = (int64_t)s.B * s.Hk * s.S * ((s.Dqk + s.Dv) / 8);
+    da_join_kernel<<<(unsigned)std::min<int64_t>((threads + 255) / 256, 148 * 16), 256, 0, a.st>>>(
+        a.part, out.splits, s.B, s.S, s.Hk, s.Dqk, s.Dv, out.dk, out.ldk, out.dv, out.ldv);
+    OXI_CUDA_CHECK(cudaGetLastError());
+  }
 }
 
 template <int DQP, int DVP>
@@ -622,21 +701,26 @@ void launch_bwd_d(const BwdArgs& a) {
 
 }  // namespace
 
+// A key tile's CTA walks every query head of its group: with few key heads and rows the CTAs are few
+// and, under causality, as unequal as can be.  Then each tile's work is cut into parts of its own.
+int da_bwd_splits(int B, int S, int Hq, int Hk) {
+  const int64_t tiles = (S + DA_TILE - 1) / DA_TILE, ctas = tiles * B * Hk, most = tiles * (Hq / Hk);
+  if (ctas >= 2 * 148 || most < 8) return 1;
+  return (int)std::min<int64_t>(std::min<int64_t>((4 * 148 + ctas - 1) / ctas, most / 4), 8);
+}
+
 void launch_da_bwd(const DaShape& s, const DaTensor& q, const DaTensor& k, const DaTensor& v, const DaTensor& o,
-                   const DaTensor& dout, const float* lse2, float* delta, const DaOut& dq, const DaOut& dk,
+                   const DaTensor& dout, const float* lse2, float* delta, float* part, const DaOut& dq, const DaOut& dk,
                    const DaOut& dv, int* status, cudaStream_t st) {
   if (s.B == 0 || s.S == 0 || s.Hq == 0) return;
   da_check(s);
   for (const DaOut* t : {&dq, &dk, &dv})
     OXI_CHECK((reinterpret_cast<uintptr_t>(t->ptr) & 15) == 0 && t->ld % 8 == 0, "16-byte aligned gradient rows");
-  OXI_CHECK((reinterpret_cast<uintptr_t>(o.ptr) & 15) == 0 && o.sb % 8 == 0 && o.ss % 8 == 0 && o.sh % 8 == 0,
-            "16-byte aligned output rows");
-  const int64_t rows = (int64_t)s.B * s.S * s.Hq;
-  da_delta_kernel<<<(unsigned)std::min<int64_t>((rows + 7) / 8, 148 * 16), 256, 0, st>>>(
-      reinterpret_cast<const __nv_bfloat16*>(o.ptr), o.sb, o.ss, o.sh, reinterpret_cast<const __nv_bfloat16*>(dout.ptr),
-      dout.sb, dout.ss, dout.sh, s.B, s.S, s.Hq, s.Dv, delta);
-  OXI_CUDA_CHECK(cudaGetLastError());
-  const BwdArgs a{s, q, k, v, o, dout, lse2, delta, dq, dk, dv, status, st};
+  for (const DaTensor* t : {&o, &dout})
+    OXI_CHECK((reinterpret_cast<uintptr_t>(t->ptr) & 15) == 0 && t->sb % 8 == 0 && t->ss % 8 == 0 && t->sh % 8 == 0,
+              "16-byte aligned rows of the output and its gradient");
+  OXI_CHECK(da_bwd_splits(s.B, s.S, s.Hq, s.Hk) == 1 || part != nullptr, "attention backward needs its parts' workspace");
+  const BwdArgs a{s, q, k, v, o, dout, lse2, delta, part, dq, dk, dv, status, st};
   if (s.Dqk <= 64 && s.Dv <= 64) launch_bwd_d<64, 64>(a);
   else if (s.Dv <= 64) launch_bwd_d<128, 64>(a);
   else launch_bwd_d<128, 128>(a);

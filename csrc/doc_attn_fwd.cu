@@ -3,38 +3,41 @@
 //   z_ij = scale q_i . k_j,  u = cap tanh(z / cap) (or z),  a = u - slope_h |i - j|
 //   o_i  = sum_{lo_i <= j < hi_i} softmax(a_i)_j v_j      (a row that sees nothing: 0)
 //
-// One CTA per (256 queries, query head, batch): two query tiles of 128 that take turns, so that
-// one tile's softmax runs while the tensor cores work for the other.  K/V tiles of 128 keys stream
-// through a TMA ring and serve both.  Per tile and key tile:
-//   S  = Q K^T              tcgen05.mma into TMEM
-//   P  = 2^(S - m)          one thread per query row, 128 keys in registers, no exchange between
+// One CTA per (128 queries, query head, batch), two CTAs on an SM: while one is between its tiles, or
+// at its start or end (documents are short, so that is often), the other works.  Q stays in shared
+// memory; K/V tiles of 64 keys stream through TMA rings.  Per step of 64 keys:
+//   S  = Q K^T              tcgen05.mma into one of two TMEM buffers, a step ahead
+//   P  = 2^(S - m)          one thread per query row, its 64 keys in registers, no exchange between
 //                           threads; P (bf16) goes back over S in TMEM
 //   O += P V                tcgen05.mma with A = P from TMEM
 // The running maximum m moves (and O is rescaled in TMEM) only when it grows by more than 2^8.
-// Key tiles outside the bounds of a query tile's ranges are not loaded or computed; a tile that
-// is wholly visible to a warp's 32 rows is computed without a mask.
-// Warps: 0 TMA, 1 MMA + TMEM owner, 2..5 softmax of query tile 0, 6..9 of query tile 1.
+// Steps outside the bounds of the query tile's ranges are not loaded or computed; a step that is
+// wholly visible to a warp's 32 rows is computed without a mask.
+// Warps: 0 TMA, 1 MMA + TMEM owner, 2..5 softmax and output.
 #include "doc_attn.cuh"
 
 namespace oxi {
 namespace {
 
+constexpr int FW_KEYS = 64;
+constexpr int FW_THREADS = 192;
+
 template <int DQP, int DVP>
 struct DaFwdSmem {
   static constexpr int KBQ = DQP / 64, KBV = DVP / 64;
-  static constexpr int BLK = DA_TILE * 128;  // 128 rows x 64 columns
-  static constexpr int Q_BYTES = KBQ * BLK, V_BYTES = KBV * BLK;
+  static constexpr int QBLK = DA_TILE * 128, KBLK = FW_KEYS * 128;  // blocks of 64 columns
+  static constexpr int Q_BYTES = KBQ * QBLK, K_BYTES = KBQ * KBLK, V_BYTES = KBV * KBLK;
   static constexpr int KST = 2, VST = 2;
-  static constexpr int OFF_Q = 0;                          // [2] query tiles
-  static constexpr int OFF_K = OFF_Q + 2 * Q_BYTES;
-  static constexpr int OFF_V = OFF_K + KST * Q_BYTES;
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_K = OFF_Q + Q_BYTES;
+  static constexpr int OFF_V = OFF_K + KST * K_BYTES;
   static constexpr int OFF_BAR = OFF_V + VST * V_BYTES;
   static constexpr int TOTAL = OFF_BAR + 256 + 1024;
-  static_assert(TOTAL <= 232448, "shared memory budget");
+  static_assert(2 * (TOTAL + 1024) <= 233472, "two CTAs per SM");
 };
 
 template <int DQP, int DVP, bool CAP, bool ALIBI>
-__global__ void __launch_bounds__(DA_THREADS, 1)
+__global__ void __launch_bounds__(FW_THREADS, 2)
     da_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, DaParams p, __nv_bfloat16* __restrict__ o_out, int64_t ldo,
                   float* __restrict__ lse2) {
@@ -46,25 +49,20 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
   uint8_t* sV = smem + L::OFF_V;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* q_full = bars + 0;
-  uint64_t* k_full = bars + 1;    // [2]
-  uint64_t* k_empty = bars + 3;   // [2]
-  uint64_t* v_full = bars + 5;    // [2]
-  uint64_t* v_empty = bars + 7;   // [2]
-  uint64_t* s_full = bars + 9;    // [2] per query tile
-  uint64_t* p_full = bars + 11;   // [2]
-  uint64_t* pv_done = bars + 13;  // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
+  uint64_t* k_full = bars + 1;   // [2]
+  uint64_t* k_empty = bars + 3;  // [2]
+  uint64_t* v_full = bars + 5;   // [2]
+  uint64_t* v_empty = bars + 7;  // [2]
+  uint64_t* s_full = bars + 9;   // [2] per S buffer
+  uint64_t* p_full = bars + 11;  // [2]
+  uint64_t* pv_done = bars + 13;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   // the query tile is the slowest grid index and runs backwards: the longest causal rows start first
-  const int pair = gridDim.z - 1 - blockIdx.z;
-  const int h = blockIdx.x, b = blockIdx.y;
+  const int qt = gridDim.z - 1 - blockIdx.z, h = blockIdx.x, b = blockIdx.y;
   const int hk = h / (p.Hq / p.Hk);
-  const TileRange r0 = key_tiles(p, b, 2 * pair), r1 = key_tiles(p, b, 2 * pair + 1);
-  const bool a0 = r0.end > r0.begin, a1 = r1.end > r1.begin;
-  const int j_begin = a0 && a1 ? min(r0.begin, r1.begin) : (a0 ? r0.begin : r1.begin);
-  const int j_end = a0 && a1 ? max(r0.end, r1.end) : (a0 ? r0.end : r1.end);
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -75,8 +73,8 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
       mbar_init(&v_empty[i], 1);
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
-      mbar_init(&pv_done[i], 1);
     }
+    mbar_init(pv_done, 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
@@ -84,40 +82,42 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
     tma_prefetch_desc(&tmV);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
+    tmem_alloc(tmem_slot, 256);
     tmem_relinquish();
   }
+  const TileRange kr = key_steps(p, b, qt, FW_KEYS);
+  const int n = kr.end - kr.begin;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  auto tm_s = [&](int t) { return tmem + t * DA_TILE; };
-  auto tm_o = [&](int t) { return tmem + 2 * DA_TILE + t * DVP; };
-  const int n = j_end - j_begin;
+  const uint32_t TM_S = tmem, TM_O = tmem + 2 * FW_KEYS;
 
   if (warp == 0) {
     if (lane == 0 && n > 0) {
-      mbar_arrive_expect_tx(q_full, 2 * L::Q_BYTES);
+      mbar_arrive_expect_tx(q_full, L::Q_BYTES);
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int kb = 0; kb < L::KBQ; ++kb)
-          tma_load_4d(sQ + t * L::Q_BYTES + kb * L::BLK, &tmQ, q_full, kb * 64, h, (2 * pair + t) * DA_TILE, b);
+      for (int kb = 0; kb < L::KBQ; ++kb) tma_load_4d(sQ + kb * L::QBLK, &tmQ, q_full, kb * 64, h, qt * DA_TILE, b);
       int ki = 0, vi = 0;
       for (; ki < n; ++ki) {
         const int st = ki % L::KST;
         if (!mbar_wait(&k_empty[st], ((ki / L::KST) & 1) ^ 1, abort_flag, p.status)) break;
-        mbar_arrive_expect_tx(&k_full[st], L::Q_BYTES);
+        mbar_arrive_expect_tx(&k_full[st], L::K_BYTES);
 #pragma unroll
         for (int kb = 0; kb < L::KBQ; ++kb)
-          tma_load_4d(sK + st * L::Q_BYTES + kb * L::BLK, &tmK, &k_full[st], kb * 64, hk, (j_begin + ki) * DA_TILE, b);
-        const int sv = vi % L::VST;
-        if (!mbar_wait(&v_empty[sv], ((vi / L::VST) & 1) ^ 1, abort_flag, p.status)) { ++ki; break; }
-        mbar_arrive_expect_tx(&v_full[sv], L::V_BYTES);
+          tma_load_4d(sK + st * L::K_BYTES + kb * L::KBLK, &tmK, &k_full[st], kb * 64, hk, (kr.begin + ki) * FW_KEYS, b);
+        // V_j is asked for once K_{j+1} has been: K is needed a step earlier
+        bool ok = true;
+        for (; ok && vi < n && (vi < ki || ki == n - 1); ++vi) {
+          const int sv = vi % L::VST;
+          ok = mbar_wait(&v_empty[sv], ((vi / L::VST) & 1) ^ 1, abort_flag, p.status);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&v_full[sv], L::V_BYTES);
 #pragma unroll
-        for (int kb = 0; kb < L::KBV; ++kb)
-          tma_load_4d(sV + sv * L::V_BYTES + kb * L::BLK, &tmV, &v_full[sv], kb * 64, hk, (j_begin + vi) * DA_TILE, b);
-        ++vi;
+          for (int kb = 0; kb < L::KBV; ++kb)
+            tma_load_4d(sV + sv * L::V_BYTES + kb * L::KBLK, &tmV, &v_full[sv], kb * 64, hk, (kr.begin + vi) * FW_KEYS, b);
+        }
+        if (!ok) { ++ki; break; }
       }
       // leave no copy in flight into shared memory
       mbar_wait(q_full, 0, nullptr, p.status);
@@ -127,85 +127,65 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0 && n > 0) {
-      constexpr uint32_t ID_S = umma_idesc_bf16(DA_TILE, DA_TILE, false, false);
+      constexpr uint32_t ID_S = umma_idesc_bf16(DA_TILE, FW_KEYS, false, false);
       constexpr uint32_t ID_O = umma_idesc_bf16(DA_TILE, DVP, false, true);
       const int nkk = (p.Dqk + 15) / 16;
-      const TileRange rt[2] = {r0, r1};
-      int done[2] = {0, 0};  // PV products issued per query tile
+      const uint32_t aQ = smem_u32(sQ);
       bool ok = mbar_wait(q_full, 0, abort_flag, p.status);
-      auto active = [&](int t, int j) { return j >= rt[t].begin && j < rt[t].end; };
-      // S of query tile t and key tile j_begin + i (in stage i % KST, already waited for); its
-      // buffer last held P of the previous key tile, read by the PV product issued before
-      auto issue_s = [&](int t, int i) {
-        const uint32_t aQ = smem_u32(sQ + t * L::Q_BYTES), aK = smem_u32(sK + (i % L::KST) * L::Q_BYTES);
-        for (int kk = 0; kk < nkk; ++kk)
-          tc_mma_f16(tm_s(t), da_kmajor_desc(aQ, kk, L::BLK), da_kmajor_desc(aK, kk, L::BLK), ID_S, kk != 0);
-        tc_commit(&s_full[t]);
-      };
-      auto wait_k = [&](int i) {
-        return mbar_wait(&k_full[i % L::KST], (i / L::KST) & 1, abort_flag, p.status);
-      };
-      if (ok) ok = wait_k(0);
-      if (ok) {
+      // S_i's buffer last held P_{i-2}, read by a product issued before
+      auto issue_s = [&](int i) -> bool {
+        if (!mbar_wait(&k_full[i % L::KST], (i / L::KST) & 1, abort_flag, p.status)) return false;
         tc_fence_after();
-        for (int t = 0; t < 2; ++t)
-          if (active(t, j_begin)) issue_s(t, 0);
-        tc_commit(&k_empty[0]);
-      }
+        const uint32_t aK = smem_u32(sK + (i % L::KST) * L::K_BYTES);
+        for (int kk = 0; kk < nkk; ++kk)
+          tc_mma_f16(TM_S + (i & 1) * FW_KEYS, da_kmajor_desc(aQ, kk, L::QBLK), da_kmajor_desc(aK, kk, L::KBLK), ID_S,
+                     kk != 0);
+        tc_commit(&s_full[i & 1]);
+        tc_commit(&k_empty[i % L::KST]);
+        return true;
+      };
+      if (ok) ok = issue_s(0);
       for (int i = 0; i < n && ok; ++i) {
-        const int j = j_begin + i;
-        if (i + 1 < n && !wait_k(i + 1)) { ok = false; break; }
-        if (!mbar_wait(&v_full[i % L::VST], (i / L::VST) & 1, abort_flag, p.status)) { ok = false; break; }
+        if (i + 1 < n && !issue_s(i + 1)) { ok = false; break; }
+        if (!mbar_wait(&v_full[i % L::VST], (i / L::VST) & 1, abort_flag, p.status) ||
+            !mbar_wait(&p_full[i & 1], (i >> 1) & 1, abort_flag, p.status)) { ok = false; break; }
+        tc_fence_after();
         const uint32_t aV = smem_u32(sV + (i % L::VST) * L::V_BYTES);
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (active(t, j)) {
-            if (!mbar_wait(&p_full[t], done[t] & 1, abort_flag, p.status)) { ok = false; break; }
-            tc_fence_after();
 #pragma unroll
-            for (int kk = 0; kk < DA_TILE / 16; ++kk)
-              tc_mma_f16_ts(tm_o(t), tm_s(t) + kk * 8, umma_desc_sw128(aV + kk * 2048, L::BLK, 1024), ID_O,
-                            (done[t] | kk) != 0);
-            tc_commit(&pv_done[t]);
-            ++done[t];
-          }
-          if (i + 1 < n && active(t, j + 1)) {
-            tc_fence_after();
-            issue_s(t, i + 1);
-          }
-        }
+        for (int kk = 0; kk < FW_KEYS / 16; ++kk)
+          tc_mma_f16_ts(TM_O, TM_S + (i & 1) * FW_KEYS + kk * 8, umma_desc_sw128(aV + kk * 2048, L::KBLK, 1024), ID_O,
+                        (i | kk) != 0);
+        tc_commit(pv_done);
         tc_commit(&v_empty[i % L::VST]);
-        if (i + 1 < n) tc_commit(&k_empty[(i + 1) % L::KST]);
       }
     }
     __syncwarp();
   } else {
-    const int t = (warp - 2) >> 2;  // query tile of this warp
-    const int quarter = warp & 3;   // TMEM lanes a warp may read: 32 * (warp % 4)
+    const int quarter = warp & 3;  // TMEM lanes a warp may read: 32 * (warp % 4)
     const int r = quarter * 32 + lane;
-    const TileRange rt = t == 0 ? r0 : r1;
-    const int qpos = (2 * pair + t) * DA_TILE + r;
+    const int qpos = qt * DA_TILE + r;
     const TileRange vis = key_range(p, b, qpos);
-    // keys that all / any rows of the warp see
+    // keys that all rows of the warp see
     const int all_lo = __reduce_max_sync(0xffffffffu, vis.begin), all_hi = __reduce_min_sync(0xffffffffu, vis.end);
-    const uint32_t s_addr = tm_s(t) + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t o_addr = tm_o(t) + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const float slope2 = ALIBI ? __ldg(p.slopes + h) * LOG2E : 0.f;
     const float C = ALIBI ? 1.f : p.c_log2;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    const int nj = rt.end - rt.begin;
-    for (int i = 0; i < nj; ++i) {
-      const int j = rt.begin + i, k0 = j * DA_TILE;
-      if (!mbar_wait(&s_full[t], i & 1, abort_flag, p.status)) { ok = false; break; }
+    for (int i = 0; i < n; ++i) {
+      const int k0 = (kr.begin + i) * FW_KEYS;
+      const bool padded = tile_has_pad(p, b, k0 / DA_TILE);
+      const uint32_t s_addr = TM_S + (i & 1) * FW_KEYS + lane_base;
+      if (!mbar_wait(&s_full[i & 1], (i >> 1) & 1, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
-      uint32_t x[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, x[c]);
+      uint32_t x[2][32];
+      tmem_ld32(s_addr, x[0]);
+      tmem_ld32(s_addr + 32, x[1]);
       tc_wait_ld();
-      const bool masked = !(all_lo <= k0 && k0 + DA_TILE <= all_hi);
+      const bool masked = !(all_lo <= k0 && k0 + FW_KEYS <= all_hi);
       float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         if (CAP || ALIBI) {
           const float fd = (float)(qpos - (k0 + c * 32));
 #pragma unroll
@@ -233,22 +213,22 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
       m = m_new;
       if (i > 0 && __any_sync(0xffffffffu, move)) {
         // O belongs to the previous product until it completes
-        if (!mbar_wait(&pv_done[t], (i - 1) & 1, abort_flag, p.status)) { ok = false; break; }
+        if (!mbar_wait(pv_done, (i - 1) & 1, abort_flag, p.status)) { ok = false; break; }
         tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < DVP / 32; ++c) {
           uint32_t w[32];
-          tmem_ld32(o_addr + c * 32, w);
+          tmem_ld32(TM_O + lane_base + c * 32, w);
           tc_wait_ld();
 #pragma unroll
           for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * alpha);
-          tmem_st32(o_addr + c * 32, w);
+          tmem_st32(TM_O + lane_base + c * 32, w);
         }
         tc_wait_st();
       }
       float rs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < 2; ++c) {
         uint32_t pk[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
@@ -260,20 +240,17 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
         tmem_st16(s_addr + c * 16, pk);
       }
       l = l * alpha + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
-      if (tile_has_pad(p, b, j)) {
-        // V_j has landed before its product may read it; rows of padding become zero
-        if (!mbar_wait(&v_full[(j - j_begin) % L::VST], ((j - j_begin) / L::VST) & 1, abort_flag, p.status)) {
-          ok = false;
-          break;
-        }
-        zero_pad_rows<L::KBV>(sV + ((j - j_begin) % L::VST) * L::V_BYTES, p, b, k0, r, 128);
+      if (padded) {
+        // V_i has landed before its product may read it; rows of padding become zero
+        if (!mbar_wait(&v_full[i % L::VST], (i / L::VST) & 1, abort_flag, p.status)) { ok = false; break; }
+        zero_pad_rows<L::KBV, FW_KEYS>(sV + (i % L::VST) * L::V_BYTES, p, b, k0, r, 128);
       }
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[t]);
+      if (lane == 0) mbar_arrive(&p_full[i & 1]);
     }
-    if (ok && nj > 0 && !mbar_wait(&pv_done[t], (nj - 1) & 1, abort_flag, p.status)) ok = false;
+    if (ok && n > 0 && !mbar_wait(pv_done, (n - 1) & 1, abort_flag, p.status)) ok = false;
     if (ok) {
       tc_fence_after();
       const bool valid = qpos < p.S;
@@ -282,8 +259,8 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
 #pragma unroll 1
       for (int c = 0; c < DVP / 32; ++c) {
         uint32_t w[32];
-        if (nj > 0) {
-          tmem_ld32(o_addr + c * 32, w);
+        if (n > 0) {
+          tmem_ld32(TM_O + lane_base + c * 32, w);
           tc_wait_ld();
         } else {
 #pragma unroll
@@ -312,7 +289,7 @@ __global__ void __launch_bounds__(DA_THREADS, 1)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, 256);
   }
 }
 
@@ -320,12 +297,12 @@ template <int DQP, int DVP, bool CAP, bool ALIBI>
 void launch_fwd_t(const DaShape& s, const DaTensor& q, const DaTensor& k, const DaTensor& v, const DaOut& o,
                   float* lse2, int* status, cudaStream_t st) {
   using L = DaFwdSmem<DQP, DVP>;
-  const CUtensorMap tq = da_tmap(q, s.B, s.S, s.Hq, s.Dqk), tk = da_tmap(k, s.B, s.S, s.Hk, s.Dqk),
-                    tv = da_tmap(v, s.B, s.S, s.Hk, s.Dv);
+  const CUtensorMap tq = da_tmap(q, s.B, s.S, s.Hq, s.Dqk), tk = da_tmap(k, s.B, s.S, s.Hk, s.Dqk, FW_KEYS),
+                    tv = da_tmap(v, s.B, s.S, s.Hk, s.Dv, FW_KEYS);
   auto kern = da_fwd_kernel<DQP, DVP, CAP, ALIBI>;
   da_smem(kern, L::TOTAL);
-  const dim3 grid(s.Hq, s.B, (s.S + 2 * DA_TILE - 1) / (2 * DA_TILE));
-  kern<<<grid, DA_THREADS, L::TOTAL, st>>>(tq, tk, tv, da_params(s, status), reinterpret_cast<__nv_bfloat16*>(o.ptr),
+  const dim3 grid(s.Hq, s.B, (s.S + DA_TILE - 1) / DA_TILE);
+  kern<<<grid, FW_THREADS, L::TOTAL, st>>>(tq, tk, tv, da_params(s, status), reinterpret_cast<__nv_bfloat16*>(o.ptr),
                                            o.ld, lse2);
   OXI_CUDA_CHECK(cudaGetLastError());
 }

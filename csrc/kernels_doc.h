@@ -41,8 +41,10 @@ bool da_supported(int Dqk, int Dv);
 // o [B*S, Hq*Dv] bf16; lse2 [B, Hq, S] f32: log2 of the row's sum of 2^score (+inf for a row that sees nothing)
 void launch_da_fwd(const DaShape& s, const DaTensor& q, const DaTensor& k, const DaTensor& v, const DaOut& o,
                    float* lse2, int* status, cudaStream_t st);
-// dq, dk, dv from dout [B, S, Hq, Dv]; delta [B, Hq, S] f32 is scratch.
+// dq, dk, dv from dout [B, S, Hq, Dv].  delta [B, Hq, S] f32 is scratch, and part too: with
+// da_bwd_splits > 1 that many f32 [B, Hk, S, Dqk + Dv].
+int da_bwd_splits(int B, int S, int Hq, int Hk);
 void launch_da_bwd(const DaShape& s, const DaTensor& q, const DaTensor& k, const DaTensor& v, const DaTensor& o,
-                   const DaTensor& dout, const float* lse2, float* delta, const DaOut& dq, const DaOut& dk,
+                   const DaTensor& dout, const float* lse2, float* delta, float* part, const DaOut& dq, const DaOut& dk,
                    const DaOut& dv, int* status, cudaStream_t st);
 }  // namespace oxi

@@ -481,7 +481,11 @@ void doc_attn_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tens
                   outs[i].size(0) == rows && outs[i].size(1) == cols[i] && outs[i].stride(1) == 1,
               "attention backward: gradients must be bf16 [B * S, H * D] on q's device");
   auto delta = torch::empty_like(lse2);
+  const int splits = oxi::da_bwd_splits(s.B, s.S, s.Hq, s.Hk);
+  torch::Tensor part;
+  if (splits > 1) part = torch::empty({splits, (int64_t)s.B * s.Hk * s.S, s.Dqk + s.Dv}, lse2.options());
   oxi::launch_da_bwd(s, tq, tk, tv, to, td, lse2.data_ptr<float>(), delta.data_ptr<float>(),
+                     splits > 1 ? part.data_ptr<float>() : nullptr,
                      {dq.data_ptr(), dq.stride(0)}, {dk.data_ptr(), dk.stride(0)}, {dv.data_ptr(), dv.stride(0)},
                      status_ptr(status), stream());
 }

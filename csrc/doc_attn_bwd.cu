@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(DQ_THREADS, 2)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 11);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   const int qt = gridDim.z - 1 - blockIdx.z, h = blockIdx.x, b = blockIdx.y;
   const int hk = h / (p.Hq / p.Hk);
 
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(DQ_THREADS, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   const uint32_t TM_DQ = tmem, TM_S = tmem + 128, TM_DP = tmem + 192;
 
   if (warp == 0) {
@@ -135,35 +135,36 @@ __global__ void __launch_bounds__(DQ_THREADS, 2)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
+    if (n > 0) {
+      const uint32_t lead = elect_lead();
       constexpr uint32_t ID_S = umma_idesc_bf16(DA_TILE, DQ_KEYS, false, false);
       constexpr uint32_t ID_Q = umma_idesc_bf16(DA_TILE, DQP, false, true);
       const int nkq = (p.Dqk + 15) / 16, nkv = (p.Dv + 15) / 16;
       const uint32_t aQ = smem_u32(sQ), aDO = smem_u32(sDO), aV = smem_u32(sV);
-      bool ok = mbar_wait(q_full, 0, abort_flag, p.status);
+      bool ok = warp_wait(q_full, 0, abort_flag, p.status);
       for (int i = 0; i < n && ok; ++i) {
         // S_i over dS_{i-1}, read by the product issued just before; dP_{i-1} has been read as well
         // (its softmax warps have handed dS over)
         const uint32_t aK = smem_u32(sK + (i % L::KST) * L::K_BYTES);
-        if (!mbar_wait(&k_full[i % L::KST], (i / L::KST) & 1, abort_flag, p.status)) { ok = false; break; }
+        if (!warp_wait(&k_full[i % L::KST], (i / L::KST) & 1, abort_flag, p.status)) { ok = false; break; }
         tc_fence_after();
         for (int kk = 0; kk < nkq; ++kk)
-          tc_mma_f16(TM_S, da_kmajor_desc(aQ, kk, L::QBLK), da_kmajor_desc(aK, kk, L::KBLK), ID_S, kk != 0);
-        tc_commit(s_full);
-        if (!mbar_wait(v_full, i & 1, abort_flag, p.status)) { ok = false; break; }
+          da_mma(lead, TM_S, da_kmajor_desc(aQ, kk, L::QBLK), da_kmajor_desc(aK, kk, L::KBLK), ID_S, kk != 0);
+        da_commit(lead, s_full);
+        if (!warp_wait(v_full, i & 1, abort_flag, p.status)) { ok = false; break; }
         tc_fence_after();
         for (int kk = 0; kk < nkv; ++kk)
-          tc_mma_f16(TM_DP, da_kmajor_desc(aDO, kk, L::QBLK), da_kmajor_desc(aV, kk, L::KBLK), ID_S, kk != 0);
-        tc_commit(dp_full);
-        tc_commit(v_empty);
-        if (!mbar_wait(ds_full, i & 1, abort_flag, p.status)) { ok = false; break; }
+          da_mma(lead, TM_DP, da_kmajor_desc(aDO, kk, L::QBLK), da_kmajor_desc(aV, kk, L::KBLK), ID_S, kk != 0);
+        da_commit(lead, dp_full);
+        da_commit(lead, v_empty);
+        if (!warp_wait(ds_full, i & 1, abort_flag, p.status)) { ok = false; break; }
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < DQ_KEYS / 16; ++kk)  // keys 0..31 in columns 0..15, 32..63 in columns 32..47
-          tc_mma_f16_ts(TM_DQ, TM_S + (kk >> 1) * 32 + (kk & 1) * 8, umma_desc_sw128(aK + kk * 2048, L::KBLK, 1024), ID_Q,
+          da_mma_ts(lead, TM_DQ, TM_S + (kk >> 1) * 32 + (kk & 1) * 8, umma_desc_sw128(aK + kk * 2048, L::KBLK, 1024), ID_Q,
                         (i | kk) != 0);
-        tc_commit(&k_empty[i % L::KST]);
-        if (i == n - 1) tc_commit(all_done);
+        da_commit(lead, &k_empty[i % L::KST]);
+        if (i == n - 1) da_commit(lead, all_done);
       }
     }
     __syncwarp();
@@ -345,7 +346,7 @@ __global__ void __launch_bounds__(DKV_THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 12);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   // the first key tiles have the most (causal) queries and start first
   const int kt = blockIdx.z, hk = blockIdx.x / out.splits, part = blockIdx.x % out.splits, b = blockIdx.y;
   const int group = p.Hq / p.Hk;
@@ -380,7 +381,7 @@ __global__ void __launch_bounds__(DKV_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   const uint32_t TM_DV = tmem, TM_DK = tmem + 128, TM_S = tmem + 256, TM_DP = tmem + 384;
 
   if (warp == 0) {
@@ -428,29 +429,30 @@ __global__ void __launch_bounds__(DKV_THREADS, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
+    if (n > 0) {
+      const uint32_t lead = elect_lead();
       constexpr uint32_t ID_S = umma_idesc_bf16(DA_TILE, DA_TILE, false, false);
       constexpr uint32_t ID_V = umma_idesc_bf16(DA_TILE, DVP, false, true);
       constexpr uint32_t ID_K = umma_idesc_bf16(DA_TILE, DQP, false, true);
       const int nkq = (p.Dqk + 15) / 16, nkv = (p.Dv + 15) / 16;
       const uint32_t aK = smem_u32(sK), aV = smem_u32(sV);
-      bool ok = mbar_wait(kv_full, 0, abort_flag, p.status);
+      bool ok = warp_wait(kv_full, 0, abort_flag, p.status);
       auto a_q = [&](int it) { return smem_u32(sQ + (it % L::ST) * L::Q_BYTES); };
       auto a_do = [&](int it) { return smem_u32(sDO + (it % L::ST) * L::V_BYTES); };
       // S^T over P^T of the pair before, dP^T over its dS^T: both read by products issued before
       auto issue_s = [&](int it) {
         for (int kk = 0; kk < nkq; ++kk)
-          tc_mma_f16(TM_S, da_kmajor_desc(aK, kk, L::BLK), da_kmajor_desc(a_q(it), kk, L::BLK), ID_S, kk != 0);
-        tc_commit(s_full);
+          da_mma(lead, TM_S, da_kmajor_desc(aK, kk, L::BLK), da_kmajor_desc(a_q(it), kk, L::BLK), ID_S, kk != 0);
+        da_commit(lead, s_full);
       };
       auto issue_dp = [&](int it) {
         for (int kk = 0; kk < nkv; ++kk)
-          tc_mma_f16(TM_DP, da_kmajor_desc(aV, kk, L::BLK), da_kmajor_desc(a_do(it), kk, L::BLK), ID_S, kk != 0);
-        tc_commit(dp_full);
+          da_mma(lead, TM_DP, da_kmajor_desc(aV, kk, L::BLK), da_kmajor_desc(a_do(it), kk, L::BLK), ID_S, kk != 0);
+        da_commit(lead, dp_full);
       };
       // queries 16 kk ..: 32 queries a softmax warp, as bf16 in the first half of its columns
       auto a_t = [&](uint32_t t, int kk) { return t + (kk >> 1) * 32 + (kk & 1) * 8; };
-      auto wait_q = [&](int it) { return mbar_wait(&q_full[it % L::ST], (it / L::ST) & 1, abort_flag, p.status); };
+      auto wait_q = [&](int it) { return warp_wait(&q_full[it % L::ST], (it / L::ST) & 1, abort_flag, p.status); };
       if (ok) ok = wait_q(0);
       if (ok) {
         tc_fence_after();
@@ -458,24 +460,24 @@ __global__ void __launch_bounds__(DKV_THREADS, 1)
         issue_dp(0);
       }
       for (int it = 0; it < n && ok; ++it) {
-        if (!mbar_wait(p_full, it & 1, abort_flag, p.status)) { ok = false; break; }
+        if (!warp_wait(p_full, it & 1, abort_flag, p.status)) { ok = false; break; }
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < DA_TILE / 16; ++kk)
-          tc_mma_f16_ts(TM_DV, a_t(TM_S, kk), umma_desc_sw128(a_do(it) + kk * 2048, L::BLK, 1024), ID_V, (it | kk) != 0);
+          da_mma_ts(lead, TM_DV, a_t(TM_S, kk), umma_desc_sw128(a_do(it) + kk * 2048, L::BLK, 1024), ID_V, (it | kk) != 0);
         if (it + 1 < n) {
           if (!wait_q(it + 1)) { ok = false; break; }
           tc_fence_after();
           issue_s(it + 1);
         }
-        if (!mbar_wait(ds_full, it & 1, abort_flag, p.status)) { ok = false; break; }
+        if (!warp_wait(ds_full, it & 1, abort_flag, p.status)) { ok = false; break; }
         tc_fence_after();
 #pragma unroll
         for (int kk = 0; kk < DA_TILE / 16; ++kk)
-          tc_mma_f16_ts(TM_DK, a_t(TM_DP, kk), umma_desc_sw128(a_q(it) + kk * 2048, L::BLK, 1024), ID_K, (it | kk) != 0);
-        tc_commit(&q_empty[it % L::ST]);
+          da_mma_ts(lead, TM_DK, a_t(TM_DP, kk), umma_desc_sw128(a_q(it) + kk * 2048, L::BLK, 1024), ID_K, (it | kk) != 0);
+        da_commit(lead, &q_empty[it % L::ST]);
         if (it + 1 < n) issue_dp(it + 1);
-        else tc_commit(all_done);
+        else da_commit(lead, all_done);
       }
     }
     __syncwarp();

@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   // the query tile is the slowest grid index and runs backwards: the longest causal rows start first
   const int qt = gridDim.z - 1 - blockIdx.z, h = blockIdx.x, b = blockIdx.y;
   const int hk = h / (p.Hq / p.Hk);
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = uniform(*tmem_slot);
   const uint32_t TM_S = tmem, TM_O = tmem + 2 * FW_KEYS;
 
   if (warp == 0) {
@@ -126,37 +126,38 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
+    if (n > 0) {
+      const uint32_t lead = elect_lead();
       constexpr uint32_t ID_S = umma_idesc_bf16(DA_TILE, FW_KEYS, false, false);
       constexpr uint32_t ID_O = umma_idesc_bf16(DA_TILE, DVP, false, true);
       const int nkk = (p.Dqk + 15) / 16;
       const uint32_t aQ = smem_u32(sQ);
-      bool ok = mbar_wait(q_full, 0, abort_flag, p.status);
+      bool ok = warp_wait(q_full, 0, abort_flag, p.status);
       // S_i's buffer last held P_{i-2}, read by a product issued before
       auto issue_s = [&](int i) -> bool {
-        if (!mbar_wait(&k_full[i % L::KST], (i / L::KST) & 1, abort_flag, p.status)) return false;
+        if (!warp_wait(&k_full[i % L::KST], (i / L::KST) & 1, abort_flag, p.status)) return false;
         tc_fence_after();
         const uint32_t aK = smem_u32(sK + (i % L::KST) * L::K_BYTES);
         for (int kk = 0; kk < nkk; ++kk)
-          tc_mma_f16(TM_S + (i & 1) * FW_KEYS, da_kmajor_desc(aQ, kk, L::QBLK), da_kmajor_desc(aK, kk, L::KBLK), ID_S,
+          da_mma(lead, TM_S + (i & 1) * FW_KEYS, da_kmajor_desc(aQ, kk, L::QBLK), da_kmajor_desc(aK, kk, L::KBLK), ID_S,
                      kk != 0);
-        tc_commit(&s_full[i & 1]);
-        tc_commit(&k_empty[i % L::KST]);
+        da_commit(lead, &s_full[i & 1]);
+        da_commit(lead, &k_empty[i % L::KST]);
         return true;
       };
       if (ok) ok = issue_s(0);
       for (int i = 0; i < n && ok; ++i) {
         if (i + 1 < n && !issue_s(i + 1)) { ok = false; break; }
-        if (!mbar_wait(&v_full[i % L::VST], (i / L::VST) & 1, abort_flag, p.status) ||
-            !mbar_wait(&p_full[i & 1], (i >> 1) & 1, abort_flag, p.status)) { ok = false; break; }
+        if (!warp_wait(&v_full[i % L::VST], (i / L::VST) & 1, abort_flag, p.status) ||
+            !warp_wait(&p_full[i & 1], (i >> 1) & 1, abort_flag, p.status)) { ok = false; break; }
         tc_fence_after();
         const uint32_t aV = smem_u32(sV + (i % L::VST) * L::V_BYTES);
 #pragma unroll
         for (int kk = 0; kk < FW_KEYS / 16; ++kk)
-          tc_mma_f16_ts(TM_O, TM_S + (i & 1) * FW_KEYS + kk * 8, umma_desc_sw128(aV + kk * 2048, L::KBLK, 1024), ID_O,
+          da_mma_ts(lead, TM_O, TM_S + (i & 1) * FW_KEYS + kk * 8, umma_desc_sw128(aV + kk * 2048, L::KBLK, 1024), ID_O,
                         (i | kk) != 0);
-        tc_commit(pv_done);
-        tc_commit(&v_empty[i % L::VST]);
+        da_commit(lead, pv_done);
+        da_commit(lead, &v_empty[i % L::VST]);
       }
     }
     __syncwarp();

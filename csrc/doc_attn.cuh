@@ -32,14 +32,38 @@ struct DaParams {
 // error a few 1e-7 (the score is cap times it, so its error is far below that of the bf16
 // probabilities).  Its derivative 1 - tanh^2 = d (2 - d) keeps its relative accuracy at the cap,
 // where 1 - t * t would be nothing but rounding.
-__device__ __forceinline__ float tanh_rest(float x) {
-  return __fdividef(2.f, 1.f + ex2_approx(fabsf(x) * (2.f * LOG2E)));
-}
-__device__ __forceinline__ float tanh_ex2(float x) { return copysignf(1.f - tanh_rest(x), x); }
-__device__ __forceinline__ float tanh_ex2(float x, float& derivative) {
-  const float d = tanh_rest(x);
+__device__ __forceinline__ float tanh_wide(float x, float& derivative) {
+  const float d = __fdividef(2.f, 1.f + ex2_approx(fabsf(x) * (2.f * LOG2E)));
   derivative = fmaf(-d, d, 2.f * d);
   return copysignf(1.f - d, x);
+}
+// tanh(x) = x P(x^2) for |x| <= 1: the minimax polynomial of degree 5 in x^2 for the relative error,
+// 6e-7.  It costs no special-function operation: with the exponential of the softmax that unit would
+// have three to do per score, and sets the kernels' time (a 128 x 128 tile has 16384 scores, the unit
+// does 16 a clock, the tile's products take 1024 clocks in the forward).
+__device__ __forceinline__ float tanh_near(float x, float& derivative) {
+  const float y = x * x;
+  float r = fmaf(y, -0.003067060373723507f, 0.016743114218115807f);
+  r = fmaf(r, y, -0.051605675369501114f);
+  r = fmaf(r, y, 0.13281433284282684f);
+  r = fmaf(r, y, -0.3332904279232025f);
+  r = fmaf(r, y, 0.9999994039535522f);
+  const float t = x * r;
+  derivative = fmaf(-t, t, 1.f);
+  return t;
+}
+template <bool NEAR>
+__device__ __forceinline__ float tanh_score(float x, float& derivative) {
+  return NEAR ? tanh_near(x, derivative) : tanh_wide(x, derivative);
+}
+// Scores of the whole warp are within the polynomial's range (a score of 0.76 of the cap): scores of
+// a model are, nearly always; a warp with a larger one takes the other form.
+template <int N>
+__device__ __forceinline__ bool warp_near(const uint32_t (&x)[N], float x_scale) {
+  float m[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int e = 0; e < N; ++e) m[e & 3] = fmaxf(m[e & 3], fabsf(__uint_as_float(x[e])));
+  return __all_sync(0xffffffffu, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * x_scale <= 1.f);
 }
 
 // Visible keys of a row within 32 consecutive keys from k: bit t is key k + t in [lo, hi).
@@ -120,8 +144,31 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 // the same value in every lane, in a uniform register
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
 
-__device__ __forceinline__ uint64_t da_kmajor_desc(uint32_t base, int kk, uint32_t block_bytes) {
-  return umma_desc_sw128(base + (kk >> 2) * block_bytes + (kk & 3) * 32, 16, 1024);
+// Matrix descriptors of 128-byte swizzled tiles in shared memory, as base + constant: the address field
+// is the low word's low 14 bits (in units of 16 bytes; shared memory ends below 2^18), so a slice's
+// offset is added to the low word alone.  Built slice by slice at run time they took longer than the
+// products (125 clocks each, where 128 x 64 x 16 takes 49).
+struct DaDesc {
+  uint32_t lo, hi;
+  __device__ __forceinline__ uint64_t at(uint32_t bytes) const {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo + (bytes >> 4)), "r"(hi));
+    return d;
+  }
+};
+__device__ __forceinline__ DaDesc da_desc(uint32_t addr, uint32_t lbo) {
+  const uint64_t d = umma_desc_sw128(addr, lbo, 1024);
+  return {(uint32_t)d, (uint32_t)(d >> 32)};
+}
+// D = A B^T of two K-major tiles (rows of 64-column blocks of A_BLK / B_BLK bytes) over the first
+// 16 * nk of COLS columns; fresh: D is overwritten.
+template <int COLS, int A_BLK, int B_BLK>
+__device__ __forceinline__ void da_mma_kk(uint32_t lead, uint32_t d_tmem, const DaDesc& a, const DaDesc& b, uint32_t idesc,
+                                          int nk) {
+#pragma unroll
+  for (int kk = 0; kk < COLS / 16; ++kk)
+    if (kk < nk)
+      da_mma(lead, d_tmem, a.at((kk >> 2) * A_BLK + (kk & 3) * 32), b.at((kk >> 2) * B_BLK + (kk & 3) * 32), idesc, kk != 0);
 }
 
 __device__ __forceinline__ void tma_load_4d(void* smem_dst, const void* tmap, uint64_t* bar, int c0, int c1, int c2,

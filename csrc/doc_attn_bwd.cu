@@ -40,7 +40,9 @@ struct DaDqSmem {
   static_assert(2 * (TOTAL + 1024) <= 233472, "two CTAs per SM");
 };
 
-// Two CTAs on an SM: one's softmax runs while the tensor cores work for the other.  TMEM: dQ, S (then dS), dP.
+// Two CTAs on an SM: one's softmax runs while the tensor cores work for the other.  TMEM: dQ, S, dP (then
+// dS): S is free for the next step as soon as it has been read, so that the next S is formed while this
+// step's exponentials are.
 template <int DQP, int DVP, bool CAP, bool ALIBI>
 __global__ void __launch_bounds__(DQ_THREADS, 2)
     da_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -64,7 +66,8 @@ __global__ void __launch_bounds__(DQ_THREADS, 2)
   uint64_t* dp_full = bars + 8;
   uint64_t* ds_full = bars + 9;
   uint64_t* all_done = bars + 10;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 11);
+  uint64_t* s_free = bars + 11;  // S has been read into registers
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 12);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
@@ -82,6 +85,7 @@ __global__ void __launch_bounds__(DQ_THREADS, 2)
     mbar_init(s_full, 1);
     mbar_init(dp_full, 1);
     mbar_init(ds_full, 8);
+    mbar_init(s_free, 8);
     mbar_init(all_done, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -140,31 +144,37 @@ __global__ void __launch_bounds__(DQ_THREADS, 2)
       constexpr uint32_t ID_S = umma_idesc_bf16(DA_TILE, DQ_KEYS, false, false);
       constexpr uint32_t ID_Q = umma_idesc_bf16(DA_TILE, DQP, false, true);
       const int nkq = (p.Dqk + 15) / 16, nkv = (p.Dv + 15) / 16;
-      const uint32_t aQ = smem_u32(sQ), aDO = smem_u32(sDO), aV = smem_u32(sV);
+      const DaDesc dQ = da_desc(smem_u32(sQ), 16), dDO = da_desc(smem_u32(sDO), 16), dV = da_desc(smem_u32(sV), 16);
       bool ok = warp_wait(q_full, 0, abort_flag, p.status);
-      for (int i = 0; i < n && ok; ++i) {
-        // S_i over dS_{i-1}, read by the product issued just before; dP_{i-1} has been read as well
-        // (its softmax warps have handed dS over)
-        const uint32_t aK = smem_u32(sK + (i % L::KST) * L::K_BYTES);
-        if (!warp_wait(&k_full[i % L::KST], (i / L::KST) & 1, abort_flag, p.status)) { ok = false; break; }
+      auto issue_s = [&](int i) -> bool {
+        if (!warp_wait(&k_full[i % L::KST], (i / L::KST) & 1, abort_flag, p.status)) return false;
         tc_fence_after();
-        for (int kk = 0; kk < nkq; ++kk)
-          da_mma(lead, TM_S, da_kmajor_desc(aQ, kk, L::QBLK), da_kmajor_desc(aK, kk, L::KBLK), ID_S, kk != 0);
+        da_mma_kk<DQP, L::QBLK, L::KBLK>(lead, TM_S, dQ, da_desc(smem_u32(sK + (i % L::KST) * L::K_BYTES), 16), ID_S, nkq);
         da_commit(lead, s_full);
-        if (!warp_wait(v_full, i & 1, abort_flag, p.status)) { ok = false; break; }
+        return true;
+      };
+      // over dS_{i-1}, read by the product issued just before
+      auto issue_dp = [&](int i) -> bool {
+        if (!warp_wait(v_full, i & 1, abort_flag, p.status)) return false;
         tc_fence_after();
-        for (int kk = 0; kk < nkv; ++kk)
-          da_mma(lead, TM_DP, da_kmajor_desc(aDO, kk, L::QBLK), da_kmajor_desc(aV, kk, L::KBLK), ID_S, kk != 0);
+        da_mma_kk<DVP, L::QBLK, L::KBLK>(lead, TM_DP, dDO, dV, ID_S, nkv);
         da_commit(lead, dp_full);
         da_commit(lead, v_empty);
+        return true;
+      };
+      if (ok) ok = issue_s(0) && issue_dp(0);
+      for (int i = 0; i < n && ok; ++i) {
+        if (i + 1 < n && (!warp_wait(s_free, i & 1, abort_flag, p.status) || !issue_s(i + 1))) { ok = false; break; }
         if (!warp_wait(ds_full, i & 1, abort_flag, p.status)) { ok = false; break; }
         tc_fence_after();
+        const DaDesc dK = da_desc(smem_u32(sK + (i % L::KST) * L::K_BYTES), L::KBLK);
 #pragma unroll
         for (int kk = 0; kk < DQ_KEYS / 16; ++kk)  // keys 0..31 in columns 0..15, 32..63 in columns 32..47
-          da_mma_ts(lead, TM_DQ, TM_S + (kk >> 1) * 32 + (kk & 1) * 8, umma_desc_sw128(aK + kk * 2048, L::KBLK, 1024), ID_Q,
-                        (i | kk) != 0);
+          da_mma_ts(lead, TM_DQ, TM_DP + (kk >> 1) * 32 + (kk & 1) * 8, dK.at(kk * 2048), ID_Q,
+                    (i | kk) != 0);
         da_commit(lead, &k_empty[i % L::KST]);
-        if (i == n - 1) da_commit(lead, all_done);
+        if (i + 1 < n) ok = issue_dp(i + 1);
+        else da_commit(lead, all_done);
       }
     }
     __syncwarp();
@@ -205,14 +215,25 @@ __global__ void __launch_bounds__(DQ_THREADS, 2)
       uint32_t x[32];
       tmem_ld32(s_addr, x);
       tc_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_free);
       const bool masked = !(all_lo <= k0 && k0 + 32 <= all_hi);
       const uint32_t bits = masked ? range_bits(vis.begin, vis.end, k0) : 0xffffffffu;
       const float fd = (float)(qpos - k0);
       float f[CAP ? 32 : 1];
+      if (CAP) {
+        if (warp_near<32>(x, p.x_scale)) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(tanh_near(__uint_as_float(x[e]) * p.x_scale, f[e]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(tanh_wide(__uint_as_float(x[e]) * p.x_scale, f[e]));
+        }
+      }
 #pragma unroll
       for (int e = 0; e < 32; ++e) {
         float v = __uint_as_float(x[e]);
-        if (CAP) v = tanh_ex2(v * p.x_scale, f[e]);
         if (ALIBI) v = fmaf(-slope2, fabsf(fd - (float)e), v * p.c_log2);
         x[e] = __float_as_uint(ex2_approx(fmaf(v, C, -ls)));
       }
@@ -238,7 +259,7 @@ __global__ void __launch_bounds__(DQ_THREADS, 2)
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) pk[e] = pack_bf16(__uint_as_float(d[2 * e]), __uint_as_float(d[2 * e + 1]));
-        tmem_st8(s_addr + c * 8, pk);
+        tmem_st8(dp_addr + c * 8, pk);
       }
       rest += rs[0] + rs[1];
       // S_i has read K_i: rows of padding become zero before the dQ product reads them
@@ -293,26 +314,27 @@ __global__ void __launch_bounds__(DQ_THREADS, 2)
 }
 
 // ------------------------------------------------------------------ dK, dV
-constexpr int DKV_THREADS = 64 + 512;  // TMA warp, MMA warp, 16 softmax warps: 32 keys x 32 queries each
+constexpr int KV_QUERIES = 64;
+constexpr int DKV_THREADS = 64 + 512;  // TMA warp, MMA warp, two groups of 8 softmax warps
 
 template <int DQP, int DVP>
 struct DaDkvSmem {
   static constexpr int KBQ = DQP / 64, KBV = DVP / 64;
-  static constexpr int BLK = DA_TILE * 128;
-  static constexpr int Q_BYTES = KBQ * BLK, V_BYTES = KBV * BLK;
-  static constexpr int ST = 2;  // Q / dO stages
-  static constexpr int VEC_BYTES = 4 * DA_TILE * 4;  // lse2, delta, lo, hi of a query tile
+  static constexpr int BLK = DA_TILE * 128, QBLK = KV_QUERIES * 128;
+  static constexpr int K_BYTES = KBQ * BLK, V_BYTES = KBV * BLK, Q_BYTES = KBQ * QBLK, DO_BYTES = KBV * QBLK;
+  static constexpr int ST = 4;  // Q / dO stages
+  static constexpr int VEC = 4 * KV_QUERIES;  // lse2, delta, lo, hi of a step's queries
   static constexpr int OFF_K = 0;
-  static constexpr int OFF_V = OFF_K + Q_BYTES;
+  static constexpr int OFF_V = OFF_K + K_BYTES;
   static constexpr int OFF_Q = OFF_V + V_BYTES;
   static constexpr int OFF_DO = OFF_Q + ST * Q_BYTES;
-  static constexpr int OFF_VEC = OFF_DO + ST * V_BYTES;
-  static constexpr int OFF_BAR = OFF_VEC + ST * VEC_BYTES;
+  static constexpr int OFF_VEC = OFF_DO + ST * DO_BYTES;
+  static constexpr int OFF_BAR = OFF_VEC + ST * VEC * 4;
   static constexpr int TOTAL = OFF_BAR + 256 + 1024;
   static_assert(TOTAL <= 232448, "shared memory budget");
 };
 
-// Where a CTA's dK, dV go: bf16 rows, or (split > 1) f32 parts [split][B, Hk, S, Dqk + Dv]
+// Where a CTA's dK, dV go: bf16 rows, or (splits > 1) f32 parts [split][B, Hk, S, Dv + Dqk]
 struct DkvOut {
   __nv_bfloat16 *dk, *dv;
   int64_t ldk, ldv;
@@ -320,9 +342,10 @@ struct DkvOut {
   int splits;
 };
 
-// Transposed tiles: TMEM lanes are keys, columns queries.  TMEM: dV, dK, S^T (then P^T), dP^T (then dS^T).
-// While the softmax warps turn dP^T into dS^T the tensor cores add P^T dO to dV and form the next S^T;
-// while they turn that into P^T, dS^T Q and the next dP^T.
+// Transposed tiles: TMEM lanes are keys, columns the 64 queries of a step.  TMEM: dV, dK, two buffers of S^T
+// (then P^T) and of dP^T (then dS^T).  The softmax warps are two groups that take the steps in turn, each with
+// its buffers: while a group works on its step the tensor cores work for the other's.  A warp owns 32 keys and
+// 32 queries.
 template <int DQP, int DVP, bool CAP, bool ALIBI>
 __global__ void __launch_bounds__(DKV_THREADS, 1)
     da_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -332,18 +355,18 @@ __global__ void __launch_bounds__(DKV_THREADS, 1)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sK = smem + L::OFF_K, *sV = smem + L::OFF_V, *sQ = smem + L::OFF_Q, *sDO = smem + L::OFF_DO;
-  float* s_vec = reinterpret_cast<float*>(smem + L::OFF_VEC);  // [stage][4][128]
+  float* s_vec = reinterpret_cast<float*>(smem + L::OFF_VEC);  // [stage][4][64]
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* kv_full = bars + 0;
-  uint64_t* q_full = bars + 1;     // [2] Q, dO tiles
-  uint64_t* q_empty = bars + 3;    // [2]
-  uint64_t* vec_full = bars + 5;   // [2] the tile's vectors
-  uint64_t* s_full = bars + 7;
-  uint64_t* dp_full = bars + 8;
-  uint64_t* p_full = bars + 9;
-  uint64_t* ds_full = bars + 10;
-  uint64_t* all_done = bars + 11;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 12);
+  uint64_t* q_full = bars + 1;     // [4] Q, dO tiles
+  uint64_t* q_empty = bars + 5;    // [4]
+  uint64_t* vec_full = bars + 9;   // [4] the step's vectors
+  uint64_t* s_full = bars + 13;    // [2] per buffer
+  uint64_t* dp_full = bars + 15;   // [2]
+  uint64_t* p_full = bars + 17;    // [2]
+  uint64_t* ds_full = bars + 19;   // [2]
+  uint64_t* all_done = bars + 21;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
@@ -353,15 +376,17 @@ __global__ void __launch_bounds__(DKV_THREADS, 1)
 
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < L::ST; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
       mbar_init(&vec_full[i], 32);
     }
-    mbar_init(s_full, 1);
-    mbar_init(dp_full, 1);
-    mbar_init(p_full, 16);
-    mbar_init(ds_full, 16);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&dp_full[i], 1);
+      mbar_init(&p_full[i], 8);
+      mbar_init(&ds_full[i], 8);
+    }
     mbar_init(all_done, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -374,9 +399,11 @@ __global__ void __launch_bounds__(DKV_THREADS, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  // this CTA's share of the (query head, query tile) pairs that see the key tile
-  const TileRange qr = query_tiles(p, b, kt);
-  const int ni = qr.end - qr.begin, total = group * ni;
+  // this CTA's share of the (query head, 64 queries) steps that see the key tile
+  TileRange qr = query_tiles(p, b, kt);
+  qr.begin *= 2;
+  qr.end = min(qr.end * 2, (p.S + KV_QUERIES - 1) / KV_QUERIES);
+  const int ni = max(qr.end - qr.begin, 0), total = group * ni;
   const int first = (int)((int64_t)total * part / out.splits), n = (int)((int64_t)total * (part + 1) / out.splits) - first;
   tc_fence_before();
   __syncthreads();
@@ -387,40 +414,44 @@ __global__ void __launch_bounds__(DKV_THREADS, 1)
   if (warp == 0) {
     if (n > 0) {
       if (lane == 0) {
-        mbar_arrive_expect_tx(kv_full, L::Q_BYTES + L::V_BYTES);
+        mbar_arrive_expect_tx(kv_full, L::K_BYTES + L::V_BYTES);
 #pragma unroll
         for (int kb = 0; kb < L::KBQ; ++kb) tma_load_4d(sK + kb * L::BLK, &tmK, kv_full, kb * 64, hk, kt * DA_TILE, b);
 #pragma unroll
         for (int kb = 0; kb < L::KBV; ++kb) tma_load_4d(sV + kb * L::BLK, &tmV, kv_full, kb * 64, hk, kt * DA_TILE, b);
       }
+      int h = hk * group + first / ni, qi = first % ni;
       int it = 0;
       for (; it < n; ++it) {
         const int st = it % L::ST;
-        const int h = hk * group + (first + it) / ni, q0 = (qr.begin + (first + it) % ni) * DA_TILE;
-        const bool ok = mbar_wait(&q_empty[st], ((it / L::ST) & 1) ^ 1, abort_flag, p.status);
-        if (!__all_sync(0xffffffffu, ok)) break;
+        const int q0 = (qr.begin + qi) * KV_QUERIES;
+        if (!warp_wait(&q_empty[st], ((it / L::ST) & 1) ^ 1, abort_flag, p.status)) break;
         if (lane == 0) {
-          mbar_arrive_expect_tx(&q_full[st], L::Q_BYTES + L::V_BYTES);
+          mbar_arrive_expect_tx(&q_full[st], L::Q_BYTES + L::DO_BYTES);
 #pragma unroll
           for (int kb = 0; kb < L::KBQ; ++kb)
-            tma_load_4d(sQ + st * L::Q_BYTES + kb * L::BLK, &tmQ, &q_full[st], kb * 64, h, q0, b);
+            tma_load_4d(sQ + st * L::Q_BYTES + kb * L::QBLK, &tmQ, &q_full[st], kb * 64, h, q0, b);
 #pragma unroll
           for (int kb = 0; kb < L::KBV; ++kb)
-            tma_load_4d(sDO + st * L::V_BYTES + kb * L::BLK, &tmDO, &q_full[st], kb * 64, h, q0, b);
+            tma_load_4d(sDO + st * L::DO_BYTES + kb * L::QBLK, &tmDO, &q_full[st], kb * 64, h, q0, b);
         }
-        float* vec = s_vec + st * 4 * DA_TILE;
+        float* vec = s_vec + st * L::VEC;
         const int64_t base = ((int64_t)b * p.Hq + h) * p.S;
 #pragma unroll
-        for (int c = 0; c < DA_TILE / 32; ++c) {
+        for (int c = 0; c < KV_QUERIES / 32; ++c) {
           const int q = c * 32 + lane, qpos = q0 + q;
           const bool in = qpos < p.S;
           const TileRange v = key_range(p, b, qpos);
           vec[q] = in ? __ldg(lse2 + base + qpos) : INFINITY;
-          vec[DA_TILE + q] = in ? __ldg(delta + base + qpos) : 0.f;
-          reinterpret_cast<int*>(vec)[2 * DA_TILE + q] = v.begin;
-          reinterpret_cast<int*>(vec)[3 * DA_TILE + q] = v.end;
+          vec[KV_QUERIES + q] = in ? __ldg(delta + base + qpos) : 0.f;
+          reinterpret_cast<int*>(vec)[2 * KV_QUERIES + q] = v.begin;
+          reinterpret_cast<int*>(vec)[3 * KV_QUERIES + q] = v.end;
         }
         mbar_arrive(&vec_full[st]);
+        if (++qi == ni) {
+          qi = 0;
+          ++h;
+        }
       }
       if (lane == 0) {
         mbar_wait(kv_full, 0, nullptr, p.status);
@@ -431,135 +462,149 @@ __global__ void __launch_bounds__(DKV_THREADS, 1)
   } else if (warp == 1) {
     if (n > 0) {
       const uint32_t lead = elect_lead();
-      constexpr uint32_t ID_S = umma_idesc_bf16(DA_TILE, DA_TILE, false, false);
+      constexpr uint32_t ID_S = umma_idesc_bf16(DA_TILE, KV_QUERIES, false, false);
       constexpr uint32_t ID_V = umma_idesc_bf16(DA_TILE, DVP, false, true);
       constexpr uint32_t ID_K = umma_idesc_bf16(DA_TILE, DQP, false, true);
       const int nkq = (p.Dqk + 15) / 16, nkv = (p.Dv + 15) / 16;
-      const uint32_t aK = smem_u32(sK), aV = smem_u32(sV);
+      const DaDesc dK = da_desc(smem_u32(sK), 16), dV = da_desc(smem_u32(sV), 16);
       bool ok = warp_wait(kv_full, 0, abort_flag, p.status);
       auto a_q = [&](int it) { return smem_u32(sQ + (it % L::ST) * L::Q_BYTES); };
-      auto a_do = [&](int it) { return smem_u32(sDO + (it % L::ST) * L::V_BYTES); };
-      // S^T over P^T of the pair before, dP^T over its dS^T: both read by products issued before
-      auto issue_s = [&](int it) {
-        for (int kk = 0; kk < nkq; ++kk)
-          da_mma(lead, TM_S, da_kmajor_desc(aK, kk, L::BLK), da_kmajor_desc(a_q(it), kk, L::BLK), ID_S, kk != 0);
-        da_commit(lead, s_full);
+      auto a_do = [&](int it) { return smem_u32(sDO + (it % L::ST) * L::DO_BYTES); };
+      // S^T over P^T of two steps before, dP^T over its dS^T: both read by products issued before
+      auto issue_s = [&](int it) -> bool {
+        if (!warp_wait(&q_full[it % L::ST], (it / L::ST) & 1, abort_flag, p.status)) return false;
+        tc_fence_after();
+        da_mma_kk<DQP, L::BLK, L::QBLK>(lead, TM_S + (it & 1) * KV_QUERIES, dK, da_desc(a_q(it), 16), ID_S, nkq);
+        da_commit(lead, &s_full[it & 1]);
+        return true;
       };
       auto issue_dp = [&](int it) {
-        for (int kk = 0; kk < nkv; ++kk)
-          da_mma(lead, TM_DP, da_kmajor_desc(aV, kk, L::BLK), da_kmajor_desc(a_do(it), kk, L::BLK), ID_S, kk != 0);
-        da_commit(lead, dp_full);
+        da_mma_kk<DVP, L::BLK, L::QBLK>(lead, TM_DP + (it & 1) * KV_QUERIES, dV, da_desc(a_do(it), 16), ID_S, nkv);
+        da_commit(lead, &dp_full[it & 1]);
       };
       // queries 16 kk ..: 32 queries a softmax warp, as bf16 in the first half of its columns
-      auto a_t = [&](uint32_t t, int kk) { return t + (kk >> 1) * 32 + (kk & 1) * 8; };
-      auto wait_q = [&](int it) { return warp_wait(&q_full[it % L::ST], (it / L::ST) & 1, abort_flag, p.status); };
-      if (ok) ok = wait_q(0);
-      if (ok) {
-        tc_fence_after();
-        issue_s(0);
-        issue_dp(0);
+      auto a_t = [&](uint32_t t, int it, int kk) { return t + (it & 1) * KV_QUERIES + (kk >> 1) * 32 + (kk & 1) * 8; };
+      for (int it = 0; it < 2 && it < n && ok; ++it) {
+        ok = issue_s(it);
+        if (ok) issue_dp(it);
       }
       for (int it = 0; it < n && ok; ++it) {
-        if (!warp_wait(p_full, it & 1, abort_flag, p.status)) { ok = false; break; }
+        if (!warp_wait(&p_full[it & 1], (it >> 1) & 1, abort_flag, p.status)) { ok = false; break; }
+        tc_fence_after();
+        const DaDesc dDO = da_desc(a_do(it), L::QBLK), dQ = da_desc(a_q(it), L::QBLK);
+#pragma unroll
+        for (int kk = 0; kk < KV_QUERIES / 16; ++kk)
+          da_mma_ts(lead, TM_DV, a_t(TM_S, it, kk), dDO.at(kk * 2048), ID_V,
+                    (it | kk) != 0);
+        if (it + 2 < n && !issue_s(it + 2)) { ok = false; break; }
+        if (!warp_wait(&ds_full[it & 1], (it >> 1) & 1, abort_flag, p.status)) { ok = false; break; }
         tc_fence_after();
 #pragma unroll
-        for (int kk = 0; kk < DA_TILE / 16; ++kk)
-          da_mma_ts(lead, TM_DV, a_t(TM_S, kk), umma_desc_sw128(a_do(it) + kk * 2048, L::BLK, 1024), ID_V, (it | kk) != 0);
-        if (it + 1 < n) {
-          if (!wait_q(it + 1)) { ok = false; break; }
-          tc_fence_after();
-          issue_s(it + 1);
-        }
-        if (!warp_wait(ds_full, it & 1, abort_flag, p.status)) { ok = false; break; }
-        tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < DA_TILE / 16; ++kk)
-          da_mma_ts(lead, TM_DK, a_t(TM_DP, kk), umma_desc_sw128(a_q(it) + kk * 2048, L::BLK, 1024), ID_K, (it | kk) != 0);
+        for (int kk = 0; kk < KV_QUERIES / 16; ++kk)
+          da_mma_ts(lead, TM_DK, a_t(TM_DP, it, kk), dQ.at(kk * 2048), ID_K,
+                    (it | kk) != 0);
         da_commit(lead, &q_empty[it % L::ST]);
-        if (it + 1 < n) issue_dp(it + 1);
-        else da_commit(lead, all_done);
+        if (it + 2 < n) issue_dp(it + 2);
+        if (it + 1 == n) da_commit(lead, all_done);
       }
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3, sub = (warp - 2) >> 2;  // 32 keys, 32 queries
+    const int quarter = warp & 3, sub = (warp - 2) >> 2;  // 32 keys; half a group (or an output column block)
+    const int mine = sub >> 1, half = sub & 1;            // group, 32 queries
     const int r = quarter * 32 + lane;
     const int kpos = kt * DA_TILE + r;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    const uint32_t s_addr = TM_S + lane_base + sub * 32, dp_addr = TM_DP + lane_base + sub * 32;
+    const uint32_t s_addr = TM_S + mine * KV_QUERIES + lane_base + half * 32;
+    const uint32_t dp_addr = TM_DP + mine * KV_QUERIES + lane_base + half * 32;
     const float C = ALIBI ? 1.f : p.c_log2;
     bool ok = true;
-    for (int it = 0; it < n; ++it) {
-      const int st = it % L::ST, u = it / L::ST;
-      const int h = hk * group + (first + it) / ni, qi = qr.begin + (first + it) % ni, q0 = qi * DA_TILE;
-      // every query of the tile sees every key of this warp?
+    int h = 0, qi = 0;
+    if (n > mine) {
+      h = hk * group + (first + mine) / ni;
+      qi = (first + mine) % ni;
+    }
+    for (int it = mine; it < n; it += 2) {
+      const int st = it % L::ST, u = it / L::ST, ph = (it >> 1) & 1;
+      const int q0 = (qr.begin + qi) * KV_QUERIES;
+      // every query of the step sees every key of this warp?
       bool masked;
       bool padded = false;
       if (p.qt) {
-        const int4 t = __ldg(p.qt + (int64_t)b * p.nt + qi);
+        const int4 t = __ldg(p.qt + (int64_t)b * p.nt + q0 / DA_TILE);
         const int w0 = kt * DA_TILE + quarter * 32;
-        masked = !(t.z <= w0 && w0 + 32 <= t.w) || q0 + DA_TILE > p.S;
+        masked = !(t.z <= w0 && w0 + 32 <= t.w) || q0 + KV_QUERIES > p.S;
         padded = t.z == INT_MAX;
       } else {
-        masked = (p.causal && q0 < kt * DA_TILE + DA_TILE) || kt * DA_TILE + DA_TILE > p.S || q0 + DA_TILE > p.S;
+        masked = (p.causal && q0 < kt * DA_TILE + DA_TILE) || kt * DA_TILE + DA_TILE > p.S || q0 + KV_QUERIES > p.S;
       }
       const float slope2 = ALIBI ? __ldg(p.slopes + h) * LOG2E : 0.f;
-      const float4* vec = reinterpret_cast<const float4*>(s_vec + st * 4 * DA_TILE + sub * 32);
+      qi += 2;
+      while (qi >= ni) {
+        qi -= ni;
+        ++h;
+      }
+      const float4* vec = reinterpret_cast<const float4*>(s_vec + st * L::VEC + half * 32);
       const int4* ivec = reinterpret_cast<const int4*>(vec);
-      const float fd = (float)(q0 + sub * 32 - kpos);
+      const float fd = (float)(q0 + half * 32 - kpos);
       if (!mbar_wait(&vec_full[st], u & 1, abort_flag, p.status) ||
-          !mbar_wait(s_full, it & 1, abort_flag, p.status)) { ok = false; break; }
+          !mbar_wait(&s_full[mine], ph, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
       uint32_t x[32], pk[16];
       tmem_ld32(s_addr, x);
       tc_wait_ld();
+      // x becomes P times the cap's derivative, pk P
+      auto probabilities = [&](auto near) {
 #pragma unroll
-      for (int e = 0; e < 32; e += 4) {
-        const float4 l4 = vec[e / 4];
-        const float ls[4] = {l4.x, l4.y, l4.z, l4.w};
-        float pr[4], w[4];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float v = __uint_as_float(x[e + g]);
-          w[g] = 1.f;
-          if (CAP) v = tanh_ex2(v * p.x_scale, w[g]);
-          if (ALIBI) v = fmaf(-slope2, fabsf(fd + (float)(e + g)), v * p.c_log2);
-          pr[g] = ex2_approx(fmaf(v, C, -ls[g]));
-          w[g] = CAP ? pr[g] * w[g] : pr[g];
-        }
-        if (masked) {
-          const int4 lo = ivec[2 * DA_TILE / 4 + e / 4], hi = ivec[3 * DA_TILE / 4 + e / 4];
-          const int lo4[4] = {lo.x, lo.y, lo.z, lo.w}, hi4[4] = {hi.x, hi.y, hi.z, hi.w};
+        for (int e = 0; e < 32; e += 4) {
+          const float4 l4 = vec[e / 4];
+          const float ls[4] = {l4.x, l4.y, l4.z, l4.w};
+          float pr[4], w[4];
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            const bool sees = lo4[g] <= kpos && kpos < hi4[g];
-            pr[g] = sees ? pr[g] : 0.f;
-            w[g] = sees ? w[g] : 0.f;  // the score of a hidden pair may be NaN
+            float v = __uint_as_float(x[e + g]);
+            w[g] = 1.f;
+            if (CAP) v = tanh_score<decltype(near)::value>(v * p.x_scale, w[g]);
+            if (ALIBI) v = fmaf(-slope2, fabsf(fd + (float)(e + g)), v * p.c_log2);
+            pr[g] = ex2_approx(fmaf(v, C, -ls[g]));
+            w[g] = CAP ? pr[g] * w[g] : pr[g];
           }
-        }
+          if (masked) {
+            const int4 lo = ivec[2 * KV_QUERIES / 4 + e / 4], hi = ivec[3 * KV_QUERIES / 4 + e / 4];
+            const int lo4[4] = {lo.x, lo.y, lo.z, lo.w}, hi4[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-        for (int g = 0; g < 4; ++g) x[e + g] = __float_as_uint(w[g]);
-        pk[e / 2] = pack_bf16(pr[0], pr[1]);
-        pk[e / 2 + 1] = pack_bf16(pr[2], pr[3]);
-      }
+            for (int g = 0; g < 4; ++g) {
+              const bool sees = lo4[g] <= kpos && kpos < hi4[g];
+              pr[g] = sees ? pr[g] : 0.f;
+              w[g] = sees ? w[g] : 0.f;  // the score of a hidden pair may be NaN
+            }
+          }
+#pragma unroll
+          for (int g = 0; g < 4; ++g) x[e + g] = __float_as_uint(w[g]);
+          pk[e / 2] = pack_bf16(pr[0], pr[1]);
+          pk[e / 2 + 1] = pack_bf16(pr[2], pr[3]);
+        }
+      };
+      if (CAP && warp_near<32>(x, p.x_scale)) probabilities(std::true_type{});
+      else probabilities(std::false_type{});
       tmem_st16(s_addr, pk);
       if (padded) {
         if (!mbar_wait(&q_full[st], u & 1, abort_flag, p.status)) { ok = false; break; }
-        zero_pad_rows<L::KBV, DA_TILE>(sDO + st * L::V_BYTES, p, b, q0, sub * 128 + r, 512);
-        zero_pad_rows<L::KBQ, DA_TILE>(sQ + st * L::Q_BYTES, p, b, q0, sub * 128 + r, 512);
+        zero_pad_rows<L::KBV, KV_QUERIES>(sDO + st * L::DO_BYTES, p, b, q0, half * 128 + r, 256);
+        zero_pad_rows<L::KBQ, KV_QUERIES>(sQ + st * L::Q_BYTES, p, b, q0, half * 128 + r, 256);
       }
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full);
-      if (!mbar_wait(dp_full, it & 1, abort_flag, p.status)) { ok = false; break; }
+      if (lane == 0) mbar_arrive(&p_full[mine]);
+      if (!mbar_wait(&dp_full[mine], ph, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
       uint32_t d[32];
       tmem_ld32(dp_addr, d);
       tc_wait_ld();
 #pragma unroll
       for (int e = 0; e < 32; e += 4) {
-        const float4 d4 = vec[DA_TILE / 4 + e / 4];
+        const float4 d4 = vec[KV_QUERIES / 4 + e / 4];
         const float dl[4] = {d4.x, d4.y, d4.z, d4.w};
         float ds[4];
 #pragma unroll
@@ -575,7 +620,7 @@ __global__ void __launch_bounds__(DKV_THREADS, 1)
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ds_full);
+      if (lane == 0) mbar_arrive(&ds_full[mine]);
     }
     if (ok && n > 0 && !mbar_wait(all_done, 0, abort_flag, p.status)) ok = false;
     if (ok) {
@@ -668,7 +713,8 @@ void launch_bwd_t(const BwdArgs& a) {
   const DaShape& s = a.s;
   const CUtensorMap tq = da_tmap(a.q, s.B, s.S, s.Hq, s.Dqk), td = da_tmap(a.dout, s.B, s.S, s.Hq, s.Dv),
                     tk = da_tmap(a.k, s.B, s.S, s.Hk, s.Dqk), tv = da_tmap(a.v, s.B, s.S, s.Hk, s.Dv),
-                    tk64 = da_tmap(a.k, s.B, s.S, s.Hk, s.Dqk, DQ_KEYS), tv64 = da_tmap(a.v, s.B, s.S, s.Hk, s.Dv, DQ_KEYS);
+                    tk64 = da_tmap(a.k, s.B, s.S, s.Hk, s.Dqk, DQ_KEYS), tv64 = da_tmap(a.v, s.B, s.S, s.Hk, s.Dv, DQ_KEYS),
+                    tq64 = da_tmap(a.q, s.B, s.S, s.Hq, s.Dqk, KV_QUERIES), td64 = da_tmap(a.dout, s.B, s.S, s.Hq, s.Dv, KV_QUERIES);
   const DaParams p = da_params(s, a.status);
   auto kq = da_dq_kernel<DQP, DVP, CAP, ALIBI>;
   auto kkv = da_dkv_kernel<DQP, DVP, CAP, ALIBI>;
@@ -684,7 +730,7 @@ void launch_bwd_t(const BwdArgs& a) {
   out.ldv = a.dv.ld;
   out.part = a.part;
   out.splits = da_bwd_splits(s.B, s.S, s.Hq, s.Hk);
-  kkv<<<dim3(s.Hk * out.splits, s.B, p.nt), DKV_THREADS, DaDkvSmem<DQP, DVP>::TOTAL, a.st>>>(tq, tk, tv, td, p, a.lse2,
+  kkv<<<dim3(s.Hk * out.splits, s.B, p.nt), DKV_THREADS, DaDkvSmem<DQP, DVP>::TOTAL, a.st>>>(tq64, tk, tv, td64, p, a.lse2,
                                                                                              a.delta, out);
   OXI_CUDA_CHECK(cudaGetLastError());
   if (out.splits > 1) {

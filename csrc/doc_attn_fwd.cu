@@ -10,7 +10,11 @@
 //   P  = 2^(S - m)          one thread per query row, its 64 keys in registers, no exchange between
 //                           threads; P (bf16) goes back over S in TMEM
 //   O += P V                tcgen05.mma with A = P from TMEM
-// The running maximum m moves (and O is rescaled in TMEM) only when it grows by more than 2^8.
+// The reference m need not be the row's maximum, it has only to keep 2^(S - m) in range: a step takes
+// the m of the steps before it, so that its exponentials wait for no maximum, and the maximum found
+// meanwhile moves m (and rescales O in TMEM) for the next step when it is more than 8 above.  Only
+// where it is more than 60 above, or a row sees its first keys, is the step's own maximum used.
+// Scores capped at up to 60 log 2 need no maximum at all: m = 0.
 // Steps outside the bounds of the query tile's ranges are not loaded or computed; a step that is
 // wholly visible to a warp's 32 rows is computed without a mask.
 // Warps: 0 TMA, 1 MMA + TMEM owner, 2..5 softmax and output.
@@ -56,7 +60,8 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
   uint64_t* s_full = bars + 9;   // [2] per S buffer
   uint64_t* p_full = bars + 11;  // [2]
   uint64_t* pv_done = bars + 13;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
+  uint64_t* o_done = bars + 14;  // the last product
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
@@ -75,6 +80,7 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
       mbar_init(&p_full[i], 4);
     }
     mbar_init(pv_done, 1);
+    mbar_init(o_done, 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
@@ -131,16 +137,14 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
       constexpr uint32_t ID_S = umma_idesc_bf16(DA_TILE, FW_KEYS, false, false);
       constexpr uint32_t ID_O = umma_idesc_bf16(DA_TILE, DVP, false, true);
       const int nkk = (p.Dqk + 15) / 16;
-      const uint32_t aQ = smem_u32(sQ);
+      const DaDesc dQ = da_desc(smem_u32(sQ), 16);
       bool ok = warp_wait(q_full, 0, abort_flag, p.status);
       // S_i's buffer last held P_{i-2}, read by a product issued before
       auto issue_s = [&](int i) -> bool {
         if (!warp_wait(&k_full[i % L::KST], (i / L::KST) & 1, abort_flag, p.status)) return false;
         tc_fence_after();
-        const uint32_t aK = smem_u32(sK + (i % L::KST) * L::K_BYTES);
-        for (int kk = 0; kk < nkk; ++kk)
-          da_mma(lead, TM_S + (i & 1) * FW_KEYS, da_kmajor_desc(aQ, kk, L::QBLK), da_kmajor_desc(aK, kk, L::KBLK), ID_S,
-                     kk != 0);
+        da_mma_kk<DQP, L::QBLK, L::KBLK>(lead, TM_S + (i & 1) * FW_KEYS, dQ,
+                                         da_desc(smem_u32(sK + (i % L::KST) * L::K_BYTES), 16), ID_S, nkk);
         da_commit(lead, &s_full[i & 1]);
         da_commit(lead, &k_empty[i % L::KST]);
         return true;
@@ -151,13 +155,14 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
         if (!warp_wait(&v_full[i % L::VST], (i / L::VST) & 1, abort_flag, p.status) ||
             !warp_wait(&p_full[i & 1], (i >> 1) & 1, abort_flag, p.status)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t aV = smem_u32(sV + (i % L::VST) * L::V_BYTES);
+        const DaDesc dV = da_desc(smem_u32(sV + (i % L::VST) * L::V_BYTES), L::KBLK);
 #pragma unroll
         for (int kk = 0; kk < FW_KEYS / 16; ++kk)
-          da_mma_ts(lead, TM_O, TM_S + (i & 1) * FW_KEYS + kk * 8, umma_desc_sw128(aV + kk * 2048, L::KBLK, 1024), ID_O,
+          da_mma_ts(lead, TM_O, TM_S + (i & 1) * FW_KEYS + kk * 8, dV.at(kk * 2048), ID_O,
                         (i | kk) != 0);
         da_commit(lead, pv_done);
         da_commit(lead, &v_empty[i % L::VST]);
+        if (i + 1 == n) da_commit(lead, o_done);
       }
     }
     __syncwarp();
@@ -171,31 +176,59 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const float slope2 = ALIBI ? __ldg(p.slopes + h) * LOG2E : 0.f;
     const float C = ALIBI ? 1.f : p.c_log2;
-    float m = -INFINITY, l = 0.f;
+    const bool bounded = CAP && p.c_log2 <= 60.f;
+    float m = bounded ? 0.f : -INFINITY, m_next = m, l = 0.f;
     bool ok = true;
+    // O times 2^(m - m_new), m = m_new; O belongs to the product of step i - 1 until it completes.  Called
+    // behind S_i, which was issued after the product of step i - 2: pv_done's parity can only mean i - 1.
+    auto move = [&](int i, float m_new) -> bool {
+      const float alpha = m_new == m ? 1.f : ex2_approx(m - m_new);  // 2^-inf = 0 at a row's first keys
+      m = m_new;
+      l *= alpha;
+      if (i == 0) return true;
+      if (!mbar_wait(pv_done, (i - 1) & 1, abort_flag, p.status)) return false;
+      tc_fence_after();
+#pragma unroll 1
+      for (int c = 0; c < DVP / 32; ++c) {
+        uint32_t w[32];
+        tmem_ld32(TM_O + lane_base + c * 32, w);
+        tc_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * alpha);
+        tmem_st32(TM_O + lane_base + c * 32, w);
+      }
+      tc_wait_st();
+      return true;
+    };
     for (int i = 0; i < n; ++i) {
       const int k0 = (kr.begin + i) * FW_KEYS;
       const bool padded = tile_has_pad(p, b, k0 / DA_TILE);
       const uint32_t s_addr = TM_S + (i & 1) * FW_KEYS + lane_base;
       if (!mbar_wait(&s_full[i & 1], (i >> 1) & 1, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
+      if (!bounded && __any_sync(0xffffffffu, m_next > m) && !move(i, m_next)) { ok = false; break; }
       uint32_t x[2][32];
       tmem_ld32(s_addr, x[0]);
       tmem_ld32(s_addr + 32, x[1]);
       tc_wait_ld();
       const bool masked = !(all_lo <= k0 && k0 + FW_KEYS <= all_hi);
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        if (CAP || ALIBI) {
+        if (CAP) {
+          float unused;
+          if (warp_near<32>(x[c], p.x_scale)) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[c][e] = __float_as_uint(tanh_near(__uint_as_float(x[c][e]) * p.x_scale, unused));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[c][e] = __float_as_uint(tanh_wide(__uint_as_float(x[c][e]) * p.x_scale, unused));
+          }
+        }
+        if (ALIBI) {
           const float fd = (float)(qpos - (k0 + c * 32));
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            float v = __uint_as_float(x[c][e]);
-            if (CAP) v = tanh_ex2(v * p.x_scale);
-            if (ALIBI) v = fmaf(-slope2, fabsf(fd - (float)e), v * p.c_log2);
-            x[c][e] = __float_as_uint(v);
-          }
+          for (int e = 0; e < 32; ++e)
+            x[c][e] = __float_as_uint(fmaf(-slope2, fabsf(fd - (float)e), __uint_as_float(x[c][e]) * p.c_log2));
         }
         if (masked) {
           const uint32_t bits = range_bits(vis.begin, vis.end, k0 + c * 32);
@@ -203,44 +236,38 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
           for (int e = 0; e < 32; ++e)
             if (!((bits >> e) & 1u)) x[c][e] = 0xff800000u;  // -inf
         }
-#pragma unroll
-        for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(x[c][e]));
       }
-      const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * C;
-      const bool move = mt > m + 8.f;
-      const float m_new = move ? mt : m;
-      const float alpha = move ? ex2_approx(m - m_new) : 1.f;  // 2^-inf = 0 at a row's first keys
-      const float mref = m_new == -INFINITY ? 0.f : m_new;
-      m = m_new;
-      if (i > 0 && __any_sync(0xffffffffu, move)) {
-        // O belongs to the previous product until it completes
-        if (!mbar_wait(pv_done, (i - 1) & 1, abort_flag, p.status)) { ok = false; break; }
-        tc_fence_after();
-#pragma unroll 1
-        for (int c = 0; c < DVP / 32; ++c) {
-          uint32_t w[32];
-          tmem_ld32(TM_O + lane_base + c * 32, w);
-          tc_wait_ld();
+      uint32_t pk[2][16];
+      float rs[4];
+      auto exponentials = [&]() {
+        const float mref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) w[e] = __float_as_uint(__uint_as_float(w[e]) * alpha);
-          tmem_st32(TM_O + lane_base + c * 32, w);
+        for (int q = 0; q < 4; ++q) rs[q] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float a = ex2_approx(fmaf(__uint_as_float(x[c][e]), C, -mref));
+            const float bb = ex2_approx(fmaf(__uint_as_float(x[c][e + 1]), C, -mref));
+            rs[(e >> 1) & 3] += a + bb;
+            pk[c][e / 2] = pack_bf16(a, bb);
+          }
+      };
+      exponentials();
+      if (!bounded) {
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int e = 0; e < 64; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(x[e >> 5][e & 31]));
+        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * C;
+        if (__any_sync(0xffffffffu, m == -INFINITY ? mt > -INFINITY : mt > m + 60.f)) {
+          if (!move(i, fmaxf(mt, m))) { ok = false; break; }
+          exponentials();
         }
-        tc_wait_st();
+        m_next = mt > m + 8.f ? mt : m;
       }
-      float rs[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t pk[16];
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          const float a = ex2_approx(fmaf(__uint_as_float(x[c][e]), C, -mref));
-          const float bb = ex2_approx(fmaf(__uint_as_float(x[c][e + 1]), C, -mref));
-          rs[(e >> 1) & 3] += a + bb;
-          pk[e / 2] = pack_bf16(a, bb);
-        }
-        tmem_st16(s_addr + c * 16, pk);
-      }
-      l = l * alpha + ((rs[0] + rs[1]) + (rs[2] + rs[3]));
+      tmem_st16(s_addr, pk[0]);
+      tmem_st16(s_addr + 16, pk[1]);
+      l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
       if (padded) {
         // V_i has landed before its product may read it; rows of padding become zero
         if (!mbar_wait(&v_full[i % L::VST], (i / L::VST) & 1, abort_flag, p.status)) { ok = false; break; }
@@ -251,7 +278,7 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[i & 1]);
     }
-    if (ok && n > 0 && !mbar_wait(pv_done, (n - 1) & 1, abort_flag, p.status)) ok = false;
+    if (ok && n > 0 && !mbar_wait(o_done, 0, abort_flag, p.status)) ok = false;
     if (ok) {
       tc_fence_after();
       const bool valid = qpos < p.S;

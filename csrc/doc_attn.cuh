@@ -28,6 +28,44 @@ struct DaParams {
   int* status;
 };
 
+// Two f32 in a register pair: one instruction for both halves' arithmetic.  The softmax warps are bound
+// by the instructions they issue, not by the arithmetic units.
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2(float a) { return f2(a, a); }
+__device__ __forceinline__ uint64_t f2(uint32_t a, uint32_t b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t ex2_2(uint64_t x) {
+  const float2 v = unpack2(x);
+  return f2(ex2_approx(v.x), ex2_approx(v.y));
+}
+
 // tanh(x) = sign(x) (1 - d) with d = 2 / (1 + e^(2|x|)): two special-function operations, absolute
 // error a few 1e-7 (the score is cap times it, so its error is far below that of the bf16
 // probabilities).  Its derivative 1 - tanh^2 = d (2 - d) keeps its relative accuracy at the cap,
@@ -41,20 +79,25 @@ __device__ __forceinline__ float tanh_wide(float x, float& derivative) {
 // 6e-7.  It costs no special-function operation: with the exponential of the softmax that unit would
 // have three to do per score, and sets the kernels' time (a 128 x 128 tile has 16384 scores, the unit
 // does 16 a clock, the tile's products take 1024 clocks in the forward).
-__device__ __forceinline__ float tanh_near(float x, float& derivative) {
-  const float y = x * x;
-  float r = fmaf(y, -0.003067060373723507f, 0.016743114218115807f);
-  r = fmaf(r, y, -0.051605675369501114f);
-  r = fmaf(r, y, 0.13281433284282684f);
-  r = fmaf(r, y, -0.3332904279232025f);
-  r = fmaf(r, y, 0.9999994039535522f);
-  const float t = x * r;
-  derivative = fmaf(-t, t, 1.f);
-  return t;
-}
-template <bool NEAR>
-__device__ __forceinline__ float tanh_score(float x, float& derivative) {
-  return NEAR ? tanh_near(x, derivative) : tanh_wide(x, derivative);
+template <bool NEAR, bool DERIVATIVE>
+__device__ __forceinline__ uint64_t tanh2(uint64_t z, float x_scale, uint64_t& derivative) {
+  if (NEAR) {
+    const uint64_t x = mul2(z, f2(x_scale)), y = mul2(x, x);
+    uint64_t r = fma2(y, f2(-0.003067060373723507f), f2(0.016743114218115807f));
+    r = fma2(r, y, f2(-0.051605675369501114f));
+    r = fma2(r, y, f2(0.13281433284282684f));
+    r = fma2(r, y, f2(-0.3332904279232025f));
+    r = fma2(r, y, f2(0.9999994039535522f));
+    const uint64_t t = mul2(x, r);
+    if (DERIVATIVE) derivative = fma2(t, mul2(t, f2(-1.f)), f2(1.f));
+    return t;
+  }
+  const float2 v = unpack2(z);
+  float2 d, t;
+  t.x = tanh_wide(v.x * x_scale, d.x);
+  t.y = tanh_wide(v.y * x_scale, d.y);
+  derivative = f2(d.x, d.y);
+  return f2(t.x, t.y);
 }
 // Scores of the whole warp are within the polynomial's range (a score of 0.76 of the cap): scores of
 // a model are, nearly always; a warp with a larger one takes the other form.
@@ -62,7 +105,8 @@ template <int N>
 __device__ __forceinline__ bool warp_near(const uint32_t (&x)[N], float x_scale) {
   float m[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int e = 0; e < N; ++e) m[e & 3] = fmaxf(m[e & 3], fabsf(__uint_as_float(x[e])));
+  for (int e = 0; e < N; e += 2)
+    m[(e >> 1) & 3] = fmaxf(fmaxf(fabsf(__uint_as_float(x[e])), fabsf(__uint_as_float(x[e + 1]))), m[(e >> 1) & 3]);
   return __all_sync(0xffffffffu, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * x_scale <= 1.f);
 }
 
@@ -201,9 +245,49 @@ __device__ __forceinline__ void zero_pad_rows(uint8_t* tile, const DaParams& p, 
   fence_proxy_async_smem();
 }
 
+// The output tile of a warp (32 rows x COLS columns of f32 in TMEM, times f) as bf16: through its own
+// part of a staging tile in shared memory (laid out like an operand: blocks of 64 columns, 128 rows of
+// 128 bytes, swizzled) and out by TMA, 32 rows x 64 columns a store.  Rows past S and columns past D
+// are clipped by the tensor map.  (Written by each thread to its own row, the same tile took 4000 to
+// 9000 clocks.)  zero: the sums are taken as zeros.
+__device__ __forceinline__ void tma_store_4d(const void* tmap, const void* smem_src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(tmap)),
+               "r"(smem_u32(smem_src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
+}
+// one block of 64 columns (kb, of `width` columns) of rows 32 * quarter .. from token pos
+__device__ __forceinline__ void store_block(uint8_t* stage, uint32_t taddr, int kb, int width, int quarter, float f,
+                                            bool zero, bool nan, const void* tmap, int head, int pos, int S, int b) {
+  const int lane = threadIdx.x & 31;
+  uint8_t* slab = stage + kb * (DA_TILE * 128) + quarter * (32 * 128);
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t w[32];
+    tmem_ld32(taddr + kb * 64 + c * 32, w);
+    tc_wait_ld();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t u[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        u[e] = pack_bf16(__uint_as_float(w[q * 8 + 2 * e]) * f, __uint_as_float(w[q * 8 + 2 * e + 1]) * f);
+        if (zero) u[e] = nan ? 0x7fff7fffu : 0u;
+      }
+      sw128_store16(slab, lane, c * 4 + q, make_uint4(u[0], u[1], u[2], u[3]));
+    }
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0 && kb * 64 < width && pos + quarter * 32 < S) {
+    tma_store_4d(tmap, slab, kb * 64, head, pos + quarter * 32, b);
+    bulk_commit();
+  }
+}
+
 // Tensor map over [B, S, H, D]: boxes of 64 columns x `rows` tokens of one head, 128-byte swizzle.
-// Columns past D and tokens past S read as zero, so a head width need not be a multiple of 64 and
-// a row's last tile never reads the next row.
+// Columns past D and tokens past S read as zero (and are not written), so a head width need not be a
+// multiple of 64 and a row's last tile never touches the next row.
 inline CUtensorMap da_tmap(const DaTensor& t, int B, int S, int H, int D, int rows = DA_TILE) {
   OXI_CHECK((reinterpret_cast<uintptr_t>(t.ptr) & 15) == 0, "TMA base must be 16-byte aligned");
   OXI_CHECK(t.sb % 8 == 0 && t.ss % 8 == 0 && t.sh % 8 == 0 && D % 8 == 0, "TMA strides must be multiples of 16 bytes");
@@ -218,6 +302,9 @@ inline CUtensorMap da_tmap(const DaTensor& t, int B, int S, int H, int D, int ro
                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   OXI_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (attention operand) failed: ", (int)r);
   return m;
+}
+inline CUtensorMap da_tmap_out(const DaOut& o, int B, int S, int H, int D) {
+  return da_tmap({o.ptr, (int64_t)S * o.ld, o.ld, D}, B, S, H, D, 32);
 }
 
 inline DaParams da_params(const DaShape& s, int* status) {

@@ -6,8 +6,8 @@
 // Two kernels that each own their outputs, so no gradient is summed with atomics and the results do
 // not depend on the order in which CTAs run; each recomputes S and dP (seven tile products where one
 // kernel with an atomic dQ has five):
-//   dQ:     one CTA per (128 queries, query head, batch), over key steps of 64
-//   dK, dV: one CTA per (128 keys, key head, batch), over the query heads of the group and query tiles
+//   dQ:     one CTA per (128 queries, query head, batch), over steps of 64 keys
+//   dK, dV: one CTA per (128 keys, key head, batch), over the query heads of the group and steps of 64 queries
 // Both keep their accumulators in TMEM and feed dS (and P^T) to the tensor cores from TMEM, written by
 // the softmax warps over the scores they were computed from.
 //
@@ -21,53 +21,68 @@ namespace {
 
 // ------------------------------------------------------------------ dQ
 constexpr int DQ_KEYS = 64;
-constexpr int DQ_THREADS = 320;  // TMA warp, MMA warp, 8 softmax warps: 32 query rows x 32 keys each
+constexpr int DA_GROUPS_THREADS = 64 + 512;  // TMA warp, MMA warp, two groups of 8 softmax warps
 
 template <int DQP, int DVP>
 struct DaDqSmem {
   static constexpr int KBQ = DQP / 64, KBV = DVP / 64;
   static constexpr int QBLK = DA_TILE * 128, KBLK = DQ_KEYS * 128;
   static constexpr int Q_BYTES = KBQ * QBLK, DO_BYTES = KBV * QBLK, K_BYTES = KBQ * KBLK, V_BYTES = KBV * KBLK;
-  static constexpr int KST = 2, VST = 1;  // K_i is held until its dQ product, V_i only until dP_i
+  static constexpr int ST = 4;  // K / V stages
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_DO = OFF_Q + Q_BYTES;
   static constexpr int OFF_K = OFF_DO + DO_BYTES;
-  static constexpr int OFF_V = OFF_K + KST * K_BYTES;
-  static constexpr int OFF_BAR = OFF_V + VST * V_BYTES;
-  // two CTAs of the widest heads fill the SM's shared memory: there is no room to align the base by
-  // hand, it has to be on a 1024-byte boundary (the kernel checks)
-  static constexpr int TOTAL = OFF_BAR + 256;
-  static_assert(2 * (TOTAL + 1024) <= 233472, "two CTAs per SM");
+  static constexpr int OFF_V = OFF_K + ST * K_BYTES;
+  static constexpr int OFF_ROW = OFF_V + ST * V_BYTES;  // delta, and what it is off by, per row: [5][128] f32
+  static constexpr int OFF_BAR = OFF_ROW + 5 * DA_TILE * 4;
+  static constexpr int TOTAL = OFF_BAR + 256 + 1024;
+  static_assert(TOTAL <= 232448, "shared memory budget");
 };
 
-// Two CTAs on an SM: one's softmax runs while the tensor cores work for the other.  TMEM: dQ, S, dP (then
-// dS): S is free for the next step as soon as it has been read, so that the next S is formed while this
-// step's exponentials are.
-template <int DQP, int DVP, bool CAP, bool ALIBI>
-__global__ void __launch_bounds__(DQ_THREADS, 2)
-    da_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO, DaParams p,
-                 DaTensor o_in, DaTensor do_in, const float* __restrict__ lse2, float* __restrict__ delta,
-                 __nv_bfloat16* __restrict__ dq, int64_t ld) {
-  using L = DaDqSmem<DQP, DVP>;
-  extern __shared__ __align__(1024) uint8_t smem[];
-  if (smem_u32(smem) & 1023u) {
-    if (threadIdx.x == 0) record_error(p.status, OXI_ERR_BOUNDS);
-    return;
+// 128 rows of a K-major operand tile (COLS columns, blocks of 64) from shared memory into TMEM as the A operand of
+// a product: each thread its row, half the columns.
+template <int COLS>
+__device__ __forceinline__ void rows_to_tmem(const uint8_t* tile, uint32_t taddr, int r, int half) {
+  uint32_t w[COLS / 4];
+#pragma unroll
+  for (int c = 0; c < COLS / 16; ++c) {
+    const int chunk = half * (COLS / 16) + c;  // 8 columns
+    const uint4 v = *reinterpret_cast<const uint4*>(tile + (chunk >> 3) * (DA_TILE * 128) + r * 128 +
+                                                    (((chunk & 7) ^ (r & 7)) << 4));
+    w[4 * c] = v.x;
+    w[4 * c + 1] = v.y;
+    w[4 * c + 2] = v.z;
+    w[4 * c + 3] = v.w;
   }
+  if constexpr (COLS == 128) tmem_st32(taddr + half * 32, w);
+  else tmem_st16(taddr + half * 16, w);
+}
+
+// TMEM: dQ, Q and dO (as A operands: read from there a 128 x 64 x 16 product takes 33 clocks, with A from shared
+// memory 49), two buffers of S and of dP (then dS).  The softmax warps are two groups that take the steps of 64
+// keys in turn, each with its buffers: while a group works on its step the tensor cores work for the other's.  A
+// warp owns 32 queries and 32 keys.
+template <int DQP, int DVP, bool CAP, bool ALIBI>
+__global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
+    da_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
+                 const __grid_constant__ CUtensorMap tmDQ, DaParams p, DaTensor o_in, DaTensor do_in,
+                 const float* __restrict__ nlse2, float* __restrict__ ndelta) {
+  using L = DaDqSmem<DQP, DVP>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t *sQ = smem + L::OFF_Q, *sDO = smem + L::OFF_DO, *sK = smem + L::OFF_K, *sV = smem + L::OFF_V;
+  float* s_row = reinterpret_cast<float*>(smem + L::OFF_ROW);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* q_full = bars + 0;
-  uint64_t* k_full = bars + 1;   // [2]
-  uint64_t* k_empty = bars + 3;  // [2]
-  uint64_t* v_full = bars + 5;
-  uint64_t* v_empty = bars + 6;
-  uint64_t* s_full = bars + 7;
-  uint64_t* dp_full = bars + 8;
-  uint64_t* ds_full = bars + 9;
-  uint64_t* all_done = bars + 10;
-  uint64_t* s_free = bars + 11;  // S has been read into registers
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 12);
+  uint64_t* a_full = bars + 1;     // Q and dO are in TMEM
+  uint64_t* kv_full = bars + 2;    // [4]
+  uint64_t* kv_empty = bars + 6;   // [4]
+  uint64_t* s_full = bars + 10;    // [2] per buffer
+  uint64_t* dp_full = bars + 12;   // [2]
+  uint64_t* ds_full = bars + 14;   // [2]
+  uint64_t* all_done = bars + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
@@ -76,16 +91,16 @@ __global__ void __launch_bounds__(DQ_THREADS, 2)
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&k_full[i], 1);
-      mbar_init(&k_empty[i], 1);
+    mbar_init(a_full, 16);
+    for (int i = 0; i < L::ST; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
     }
-    mbar_init(v_full, 1);
-    mbar_init(v_empty, 1);
-    mbar_init(s_full, 1);
-    mbar_init(dp_full, 1);
-    mbar_init(ds_full, 8);
-    mbar_init(s_free, 8);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&dp_full[i], 1);
+      mbar_init(&ds_full[i], 8);
+    }
     mbar_init(all_done, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -95,7 +110,7 @@ __global__ void __launch_bounds__(DQ_THREADS, 2)
     tma_prefetch_desc(&tmDO);
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 256);
+    tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
   const TileRange kr = key_steps(p, b, qt, DQ_KEYS);
@@ -104,7 +119,7 @@ __global__ void __launch_bounds__(DQ_THREADS, 2)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = uniform(*tmem_slot);
-  const uint32_t TM_DQ = tmem, TM_S = tmem + 128, TM_DP = tmem + 192;
+  const uint32_t TM_DQ = tmem, TM_Q = tmem + 128, TM_DO = tmem + 192, TM_S = tmem + 256, TM_DP = tmem + 384;
 
   if (warp == 0) {
     if (lane == 0 && n > 0) {
@@ -113,29 +128,21 @@ __global__ void __launch_bounds__(DQ_THREADS, 2)
       for (int kb = 0; kb < L::KBQ; ++kb) tma_load_4d(sQ + kb * L::QBLK, &tmQ, q_full, kb * 64, h, qt * DA_TILE, b);
 #pragma unroll
       for (int kb = 0; kb < L::KBV; ++kb) tma_load_4d(sDO + kb * L::QBLK, &tmDO, q_full, kb * 64, h, qt * DA_TILE, b);
-      int ki = 0, vi = 0;
-      for (; ki < n; ++ki) {
-        const int st = ki % L::KST;
-        if (!mbar_wait(&k_empty[st], ((ki / L::KST) & 1) ^ 1, abort_flag, p.status)) break;
-        mbar_arrive_expect_tx(&k_full[st], L::K_BYTES);
+      int i = 0;
+      for (; i < n; ++i) {
+        const int st = i % L::ST;
+        if (!mbar_wait(&kv_empty[st], ((i / L::ST) & 1) ^ 1, abort_flag, p.status)) break;
+        mbar_arrive_expect_tx(&kv_full[st], L::K_BYTES + L::V_BYTES);
 #pragma unroll
         for (int kb = 0; kb < L::KBQ; ++kb)
-          tma_load_4d(sK + st * L::K_BYTES + kb * L::KBLK, &tmK, &k_full[st], kb * 64, hk, (kr.begin + ki) * DQ_KEYS, b);
-        // V_{j} behind K_{j+1}
-        bool ok = true;
-        for (; ok && vi < n && (vi < ki || ki == n - 1); ++vi) {
-          ok = mbar_wait(v_empty, (vi & 1) ^ 1, abort_flag, p.status);
-          if (!ok) break;
-          mbar_arrive_expect_tx(v_full, L::V_BYTES);
+          tma_load_4d(sK + st * L::K_BYTES + kb * L::KBLK, &tmK, &kv_full[st], kb * 64, hk, (kr.begin + i) * DQ_KEYS, b);
 #pragma unroll
-          for (int kb = 0; kb < L::KBV; ++kb)
-            tma_load_4d(sV + kb * L::KBLK, &tmV, v_full, kb * 64, hk, (kr.begin + vi) * DQ_KEYS, b);
-        }
-        if (!ok) { ++ki; break; }
+        for (int kb = 0; kb < L::KBV; ++kb)
+          tma_load_4d(sV + st * L::V_BYTES + kb * L::KBLK, &tmV, &kv_full[st], kb * 64, hk, (kr.begin + i) * DQ_KEYS, b);
       }
+      // leave no copy in flight into shared memory
       mbar_wait(q_full, 0, nullptr, p.status);
-      for (int i = max(0, ki - L::KST); i < ki; ++i) mbar_wait(&k_full[i % L::KST], (i / L::KST) & 1, nullptr, p.status);
-      if (vi > 0) mbar_wait(v_full, (vi - 1) & 1, nullptr, p.status);
+      for (int u = max(0, i - L::ST); u < i; ++u) mbar_wait(&kv_full[u % L::ST], (u / L::ST) & 1, nullptr, p.status);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -144,178 +151,203 @@ __global__ void __launch_bounds__(DQ_THREADS, 2)
       constexpr uint32_t ID_S = umma_idesc_bf16(DA_TILE, DQ_KEYS, false, false);
       constexpr uint32_t ID_Q = umma_idesc_bf16(DA_TILE, DQP, false, true);
       const int nkq = (p.Dqk + 15) / 16, nkv = (p.Dv + 15) / 16;
-      const DaDesc dQ = da_desc(smem_u32(sQ), 16), dDO = da_desc(smem_u32(sDO), 16), dV = da_desc(smem_u32(sV), 16);
-      bool ok = warp_wait(q_full, 0, abort_flag, p.status);
-      auto issue_s = [&](int i) -> bool {
-        if (!warp_wait(&k_full[i % L::KST], (i / L::KST) & 1, abort_flag, p.status)) return false;
+      // S_i over S_{i-2}, which its group has read; dP_i over dS_{i-2}, read by a product issued before
+      auto issue = [&](int i) -> bool {
+        if (!warp_wait(&kv_full[i % L::ST], (i / L::ST) & 1, abort_flag, p.status)) return false;
         tc_fence_after();
-        da_mma_kk<DQP, L::QBLK, L::KBLK>(lead, TM_S, dQ, da_desc(smem_u32(sK + (i % L::KST) * L::K_BYTES), 16), ID_S, nkq);
-        da_commit(lead, s_full);
+        const DaDesc dK = da_desc(smem_u32(sK + (i % L::ST) * L::K_BYTES), 16);
+        const DaDesc dV = da_desc(smem_u32(sV + (i % L::ST) * L::V_BYTES), 16);
+#pragma unroll
+        for (int kk = 0; kk < DQP / 16; ++kk)
+          if (kk < nkq)
+            da_mma_ts(lead, TM_S + (i & 1) * DQ_KEYS, TM_Q + kk * 8, dK.at((kk >> 2) * L::KBLK + (kk & 3) * 32), ID_S, kk != 0);
+        da_commit(lead, &s_full[i & 1]);
+#pragma unroll
+        for (int kk = 0; kk < DVP / 16; ++kk)
+          if (kk < nkv)
+            da_mma_ts(lead, TM_DP + (i & 1) * DQ_KEYS, TM_DO + kk * 8, dV.at((kk >> 2) * L::KBLK + (kk & 3) * 32), ID_S, kk != 0);
+        da_commit(lead, &dp_full[i & 1]);
         return true;
       };
-      // over dS_{i-1}, read by the product issued just before
-      auto issue_dp = [&](int i) -> bool {
-        if (!warp_wait(v_full, i & 1, abort_flag, p.status)) return false;
-        tc_fence_after();
-        da_mma_kk<DVP, L::QBLK, L::KBLK>(lead, TM_DP, dDO, dV, ID_S, nkv);
-        da_commit(lead, dp_full);
-        da_commit(lead, v_empty);
-        return true;
-      };
-      if (ok) ok = issue_s(0) && issue_dp(0);
+      bool ok = warp_wait(a_full, 0, abort_flag, p.status);
+      for (int i = 0; i < 2 && i < n && ok; ++i) ok = issue(i);
       for (int i = 0; i < n && ok; ++i) {
-        if (i + 1 < n && (!warp_wait(s_free, i & 1, abort_flag, p.status) || !issue_s(i + 1))) { ok = false; break; }
-        if (!warp_wait(ds_full, i & 1, abort_flag, p.status)) { ok = false; break; }
+        if (!warp_wait(&ds_full[i & 1], (i >> 1) & 1, abort_flag, p.status)) { ok = false; break; }
         tc_fence_after();
-        const DaDesc dK = da_desc(smem_u32(sK + (i % L::KST) * L::K_BYTES), L::KBLK);
+        const DaDesc dK = da_desc(smem_u32(sK + (i % L::ST) * L::K_BYTES), L::KBLK);
 #pragma unroll
         for (int kk = 0; kk < DQ_KEYS / 16; ++kk)  // keys 0..31 in columns 0..15, 32..63 in columns 32..47
-          da_mma_ts(lead, TM_DQ, TM_DP + (kk >> 1) * 32 + (kk & 1) * 8, dK.at(kk * 2048), ID_Q,
+          da_mma_ts(lead, TM_DQ, TM_DP + (i & 1) * DQ_KEYS + (kk >> 1) * 32 + (kk & 1) * 8, dK.at(kk * 2048), ID_Q,
                     (i | kk) != 0);
-        da_commit(lead, &k_empty[i % L::KST]);
-        if (i + 1 < n) ok = issue_dp(i + 1);
-        else da_commit(lead, all_done);
+        da_commit(lead, &kv_empty[i % L::ST]);
+        if (i + 2 < n) ok = issue(i + 2);
+        if (i + 1 == n) da_commit(lead, all_done);
       }
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const int quarter = warp & 3, sub = (warp - 2) >> 2;  // 32 queries; group and half of its keys
+    const int mine = sub >> 1, half = sub & 1;
     const int r = quarter * 32 + lane;
     const int qpos = qt * DA_TILE + r;
-    const TileRange vis = key_range(p, b, qpos);
-    const int all_lo = __reduce_max_sync(0xffffffffu, vis.begin), all_hi = __reduce_min_sync(0xffffffffu, vis.end);
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    const uint32_t s_addr = TM_S + lane_base + half * 32, dp_addr = TM_DP + lane_base + half * 32;
-    const bool in = qpos < p.S;
-    const int64_t vi = ((int64_t)b * p.Hq + h) * p.S + qpos;
-    const float ls = in ? lse2[vi] : INFINITY;
-    float dl = 0.f;  // delta of the row, formed while the first tiles load
-    if (in) {
-      const __nv_bfloat16* orow = reinterpret_cast<const __nv_bfloat16*>(o_in.ptr) + b * o_in.sb + qpos * o_in.ss + h * o_in.sh;
-      const __nv_bfloat16* drow = reinterpret_cast<const __nv_bfloat16*>(do_in.ptr) + b * do_in.sb + qpos * do_in.ss + h * do_in.sh;
-      for (int c = 0; c < p.Dv; c += 8) {
-        const uint4 x = __ldg(reinterpret_cast<const uint4*>(orow + c)), y = __ldg(reinterpret_cast<const uint4*>(drow + c));
-        const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+    bool ok = true;
+    // minus delta of 8 rows a warp, 16 bytes a lane: 2 rows at a time
+    {
+      const __nv_bfloat16* op = reinterpret_cast<const __nv_bfloat16*>(o_in.ptr) + b * o_in.sb + h * o_in.sh;
+      const __nv_bfloat16* dp = reinterpret_cast<const __nv_bfloat16*>(do_in.ptr) + b * do_in.sb + h * do_in.sh;
+      const int c = (lane & 15) * 8, row0 = (warp - 2) * 8 + (lane >> 4);
+      uint4 x[4], y[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 a = unpack_bf16(xw[e]), g = unpack_bf16(yw[e]);
-          dl = fmaf(a.x, g.x, fmaf(a.y, g.y, dl));
+      for (int g = 0; g < 4; ++g) {
+        const int64_t pos = qt * DA_TILE + row0 + 2 * g;
+        x[g] = y[g] = make_uint4(0, 0, 0, 0);
+        if (pos < p.S && c < p.Dv) {
+          x[g] = __ldg(reinterpret_cast<const uint4*>(op + pos * o_in.ss + c));
+          y[g] = __ldg(reinterpret_cast<const uint4*>(dp + pos * do_in.ss + c));
         }
       }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const uint32_t xw[4] = {x[g].x, x[g].y, x[g].z, x[g].w}, yw[4] = {y[g].x, y[g].y, y[g].z, y[g].w};
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 a = unpack_bf16(xw[e]), d = unpack_bf16(yw[e]);
+          sum = fmaf(a.x, d.x, fmaf(a.y, d.y, sum));
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if ((lane & 15) == 0) s_row[row0 + 2 * g] = -sum;
+      }
     }
+    if (n > 0) {
+      if (!mbar_wait(q_full, 0, abort_flag, p.status)) ok = false;
+      if (ok) {
+        if (mine == 0) rows_to_tmem<DQP>(sQ, TM_Q + lane_base, r, half);
+        else rows_to_tmem<DVP>(sDO, TM_DO + lane_base, r, half);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(a_full);
+      }
+    }
+    asm volatile("bar.sync 1, 512;" ::: "memory");  // delta's rows; reached by every softmax warp
+    const TileRange vis = key_range(p, b, qpos);
+    const int all_lo = __reduce_max_sync(0xffffffffu, vis.begin), all_hi = __reduce_min_sync(0xffffffffu, vis.end);
+    const uint32_t s_addr = TM_S + mine * DQ_KEYS + lane_base + half * 32;
+    const uint32_t dp_addr = TM_DP + mine * DQ_KEYS + lane_base + half * 32;
+    const bool in = qpos < p.S;
+    const int64_t vi = ((int64_t)b * p.Hq + h) * p.S + qpos;
+    const float nls = in ? nlse2[vi] : -INFINITY;
+    const float ndl = s_row[r];
     const float slope2 = ALIBI ? __ldg(p.slopes + h) * LOG2E : 0.f;
     const float C = ALIBI ? 1.f : p.c_log2;
     float rest = 0.f;  // sum of P (dP - delta) over this thread's keys
-    bool ok = true;
-    for (int i = 0; i < n; ++i) {
-      const int k0 = (kr.begin + i) * DQ_KEYS + half * 32;
+    for (int i = mine; i < n && ok; i += 2) {
+      const int k0 = (kr.begin + i) * DQ_KEYS + half * 32, ph = (i >> 1) & 1;
       const bool padded = tile_has_pad(p, b, k0 / DA_TILE);
-      if (!mbar_wait(s_full, i & 1, abort_flag, p.status)) { ok = false; break; }
+      if (!mbar_wait(&s_full[mine], ph, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
       uint32_t x[32];
       tmem_ld32(s_addr, x);
       tc_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(s_free);
       const bool masked = !(all_lo <= k0 && k0 + 32 <= all_hi);
       const uint32_t bits = masked ? range_bits(vis.begin, vis.end, k0) : 0xffffffffu;
       const float fd = (float)(qpos - k0);
-      float f[CAP ? 32 : 1];
-      if (CAP) {
-        if (warp_near<32>(x, p.x_scale)) {
+      uint64_t f[CAP ? 16 : 1];  // the cap's derivative
+      auto probabilities = [&](auto near) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(tanh_near(__uint_as_float(x[e]) * p.x_scale, f[e]));
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(tanh_wide(__uint_as_float(x[e]) * p.x_scale, f[e]));
+        for (int e = 0; e < 32; e += 2) {
+          uint64_t v = f2(x[e], x[e + 1]);
+          if (CAP) v = tanh2<decltype(near)::value, true>(v, p.x_scale, f[CAP ? e / 2 : 0]);
+          if (ALIBI) {
+            const float2 t = unpack2(v);
+            v = f2(fmaf(-slope2, fabsf(fd - (float)e), t.x * p.c_log2), fmaf(-slope2, fabsf(fd - (float)(e + 1)), t.y * p.c_log2));
+          }
+          const float2 pr = unpack2(ex2_2(fma2(v, f2(C), f2(nls))));
+          x[e] = __float_as_uint(pr.x);
+          x[e + 1] = __float_as_uint(pr.y);
         }
-      }
-#pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        float v = __uint_as_float(x[e]);
-        if (ALIBI) v = fmaf(-slope2, fabsf(fd - (float)e), v * p.c_log2);
-        x[e] = __float_as_uint(ex2_approx(fmaf(v, C, -ls)));
-      }
-      if (!mbar_wait(dp_full, i & 1, abort_flag, p.status)) { ok = false; break; }
+      };
+      if (CAP && warp_near<32>(x, p.x_scale)) probabilities(std::true_type{});
+      else probabilities(std::false_type{});
+      if (!mbar_wait(&dp_full[mine], ph, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
-      float rs[2] = {0.f, 0.f};
+      uint64_t rs = 0ull;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t d[16], pk[8];
         tmem_ld16(dp_addr + c * 16, d);
         tc_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int e = 0; e < 16; e += 2) {
           const int t = c * 16 + e;
-          float g = __uint_as_float(x[t]) * (__uint_as_float(d[e]) - dl);
-          if (masked) g = ((bits >> t) & 1u) ? g : 0.f;
-          rs[e & 1] += g;
-          if (CAP) {
-            g *= f[t];
-            if (masked) g = ((bits >> t) & 1u) ? g : 0.f;  // a hidden score may be NaN, and f with it
+          uint64_t g = mul2(f2(x[t], x[t + 1]), add2(f2(d[e], d[e + 1]), f2(ndl)));
+          if (masked) {  // a hidden pair adds nothing, whatever its score and dP are
+            const float2 u = unpack2(g);
+            g = f2(((bits >> t) & 1u) ? u.x : 0.f, ((bits >> (t + 1)) & 1u) ? u.y : 0.f);
           }
-          d[e] = __float_as_uint(g);
+          rs = add2(rs, g);
+          if (CAP) {
+            g = mul2(g, f[CAP ? t / 2 : 0]);
+            if (masked) {
+              const float2 u = unpack2(g);
+              g = f2(((bits >> t) & 1u) ? u.x : 0.f, ((bits >> (t + 1)) & 1u) ? u.y : 0.f);
+            }
+          }
+          const float2 u = unpack2(g);
+          pk[e / 2] = pack_bf16(u.x, u.y);
         }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) pk[e] = pack_bf16(__uint_as_float(d[2 * e]), __uint_as_float(d[2 * e + 1]));
         tmem_st8(dp_addr + c * 8, pk);
       }
-      rest += rs[0] + rs[1];
+      const float2 rv = unpack2(rs);
+      rest += rv.x + rv.y;
       // S_i has read K_i: rows of padding become zero before the dQ product reads them
       if (padded)
-        zero_pad_rows<L::KBQ, DQ_KEYS>(sK + (i % L::KST) * L::K_BYTES, p, b, (kr.begin + i) * DQ_KEYS, half * 128 + r, 256);
+        zero_pad_rows<L::KBQ, DQ_KEYS>(sK + (i % L::ST) * L::K_BYTES, p, b, (kr.begin + i) * DQ_KEYS, half * 128 + r, 256);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ds_full);
+      if (lane == 0) mbar_arrive(&ds_full[mine]);
     }
     if (ok && n > 0 && !mbar_wait(all_done, 0, abort_flag, p.status)) ok = false;
-    // the halves' rests meet in shared memory: every product has completed, so K's ring is free
-    float* s_rest = reinterpret_cast<float*>(sK);
-    if (ok) s_rest[half * DA_TILE + r] = rest;
-    asm volatile("bar.sync 1, 256;" ::: "memory");  // reached by every softmax warp
+    s_row[(1 + sub) * DA_TILE + r] = rest;
+    asm volatile("bar.sync 1, 512;" ::: "memory");  // reached by every softmax warp
     if (ok) {
       tc_fence_after();
-      if (half == 0 && in) delta[vi] = dl + (s_rest[r] + s_rest[DA_TILE + r]);
-      __nv_bfloat16* row = dq + ((int64_t)b * p.S + qpos) * ld + (int64_t)h * p.Dqk;
-#pragma unroll 1
-      for (int c = half; c < DQP / 32; c += 2) {
-        uint32_t w[32];
-        if (n > 0) {
-          tmem_ld32(TM_DQ + lane_base + c * 32, w);
-          tc_wait_ld();
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) w[e] = 0u;
-        }
-        if (in) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (c * 32 + q * 8 < p.Dqk) {
-              uint32_t u[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                u[e] = pack_bf16(__uint_as_float(w[q * 8 + 2 * e]) * p.scale,
-                                 __uint_as_float(w[q * 8 + 2 * e + 1]) * p.scale);
-              *reinterpret_cast<uint4*>(row + c * 32 + q * 8) = make_uint4(u[0], u[1], u[2], u[3]);
-            }
-          }
-        }
-      }
+      if (sub == 0 && in)
+        ndelta[vi] = ndl - ((s_row[DA_TILE + r] + s_row[2 * DA_TILE + r]) + (s_row[3 * DA_TILE + r] + s_row[4 * DA_TILE + r]));
+      // Q's tile in shared memory is free by now
+      if (sub < L::KBQ)
+        store_block(sQ, TM_DQ + lane_base, sub, p.Dqk, quarter, p.scale, n == 0, false, &tmDQ, h, qt * DA_TILE, p.S, b);
+      if (lane == 0) bulk_wait_read<0>();
     }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 256);
+    tmem_dealloc(tmem, 512);
   }
 }
 
 // ------------------------------------------------------------------ dK, dV
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const void* tmap, const void* smem_src, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(tmap)),
+               "r"(smem_u32(smem_src)), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+// this thread's arrival, once its copies so far have landed
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 constexpr int KV_QUERIES = 64;
-constexpr int DKV_THREADS = 64 + 512;  // TMA warp, MMA warp, two groups of 8 softmax warps
 
 template <int DQP, int DVP>
 struct DaDkvSmem {
@@ -323,7 +355,7 @@ struct DaDkvSmem {
   static constexpr int BLK = DA_TILE * 128, QBLK = KV_QUERIES * 128;
   static constexpr int K_BYTES = KBQ * BLK, V_BYTES = KBV * BLK, Q_BYTES = KBQ * QBLK, DO_BYTES = KBV * QBLK;
   static constexpr int ST = 4;  // Q / dO stages
-  static constexpr int VEC = 4 * KV_QUERIES;  // lse2, delta, lo, hi of a step's queries
+  static constexpr int VEC = 4 * KV_QUERIES;  // -lse2, -delta, lo, hi of a step's queries
   static constexpr int OFF_K = 0;
   static constexpr int OFF_V = OFF_K + K_BYTES;
   static constexpr int OFF_Q = OFF_V + V_BYTES;
@@ -334,23 +366,16 @@ struct DaDkvSmem {
   static_assert(TOTAL <= 232448, "shared memory budget");
 };
 
-// Where a CTA's dK, dV go: bf16 rows, or (splits > 1) f32 parts [split][B, Hk, S, Dv + Dqk]
-struct DkvOut {
-  __nv_bfloat16 *dk, *dv;
-  int64_t ldk, ldv;
-  float* part;
-  int splits;
-};
-
 // Transposed tiles: TMEM lanes are keys, columns the 64 queries of a step.  TMEM: dV, dK, two buffers of S^T
 // (then P^T) and of dP^T (then dS^T).  The softmax warps are two groups that take the steps in turn, each with
 // its buffers: while a group works on its step the tensor cores work for the other's.  A warp owns 32 keys and
 // 32 queries.
 template <int DQP, int DVP, bool CAP, bool ALIBI>
-__global__ void __launch_bounds__(DKV_THREADS, 1)
+__global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
     da_dkv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO, DaParams p,
-                  const float* __restrict__ lse2, const float* __restrict__ delta, DkvOut out) {
+                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
+                  const __grid_constant__ CUtensorMap tmDK, const __grid_constant__ CUtensorMap tmDV, DaParams p,
+                  const float* __restrict__ nlse2, const float* __restrict__ ndelta, int splits) {
   using L = DaDkvSmem<DQP, DVP>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -371,7 +396,7 @@ __global__ void __launch_bounds__(DKV_THREADS, 1)
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
   // the first key tiles have the most (causal) queries and start first
-  const int kt = blockIdx.z, hk = blockIdx.x / out.splits, part = blockIdx.x % out.splits, b = blockIdx.y;
+  const int kt = blockIdx.z, hk = blockIdx.x / splits, part = blockIdx.x % splits, b = blockIdx.y;
   const int group = p.Hq / p.Hk;
 
   if (threadIdx.x == 0) {
@@ -404,7 +429,7 @@ __global__ void __launch_bounds__(DKV_THREADS, 1)
   qr.begin *= 2;
   qr.end = min(qr.end * 2, (p.S + KV_QUERIES - 1) / KV_QUERIES);
   const int ni = max(qr.end - qr.begin, 0), total = group * ni;
-  const int first = (int)((int64_t)total * part / out.splits), n = (int)((int64_t)total * (part + 1) / out.splits) - first;
+  const int first = (int)((int64_t)total * part / splits), n = (int)((int64_t)total * (part + 1) / splits) - first;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -435,19 +460,22 @@ __global__ void __launch_bounds__(DKV_THREADS, 1)
           for (int kb = 0; kb < L::KBV; ++kb)
             tma_load_4d(sDO + st * L::DO_BYTES + kb * L::QBLK, &tmDO, &q_full[st], kb * 64, h, q0, b);
         }
-        float* vec = s_vec + st * L::VEC;
+        // the step's vectors, asynchronously as well (waited for here, their latency set the steps' pace)
+        const uint32_t vec = smem_u32(s_vec + st * L::VEC);
         const int64_t base = ((int64_t)b * p.Hq + h) * p.S;
 #pragma unroll
         for (int c = 0; c < KV_QUERIES / 32; ++c) {
           const int q = c * 32 + lane, qpos = q0 + q;
-          const bool in = qpos < p.S;
-          const TileRange v = key_range(p, b, qpos);
-          vec[q] = in ? __ldg(lse2 + base + qpos) : INFINITY;
-          vec[KV_QUERIES + q] = in ? __ldg(delta + base + qpos) : 0.f;
-          reinterpret_cast<int*>(vec)[2 * KV_QUERIES + q] = v.begin;
-          reinterpret_cast<int*>(vec)[3 * KV_QUERIES + q] = v.end;
+          const bool in = qpos < p.S;  // past the end: zeros, and no key is seen
+          const int64_t at = in ? qpos : 0;
+          cp_async4(vec + q * 4, nlse2 + base + at, in);
+          cp_async4(vec + (KV_QUERIES + q) * 4, ndelta + base + at, in);
+          if (p.lo) {
+            cp_async4(vec + (2 * KV_QUERIES + q) * 4, p.lo + (int64_t)b * p.S + at, in);
+            cp_async4(vec + (3 * KV_QUERIES + q) * 4, p.hi + (int64_t)b * p.S + at, in);
+          }
         }
-        mbar_arrive(&vec_full[st]);
+        cp_async_arrive(&vec_full[st]);
         if (++qi == ni) {
           qi = 0;
           ++h;
@@ -455,7 +483,10 @@ __global__ void __launch_bounds__(DKV_THREADS, 1)
       }
       if (lane == 0) {
         mbar_wait(kv_full, 0, nullptr, p.status);
-        for (int u = max(0, it - L::ST); u < it; ++u) mbar_wait(&q_full[u % L::ST], (u / L::ST) & 1, nullptr, p.status);
+        for (int u = max(0, it - L::ST); u < it; ++u) {
+          mbar_wait(&q_full[u % L::ST], (u / L::ST) & 1, nullptr, p.status);
+          mbar_wait(&vec_full[u % L::ST], (u / L::ST) & 1, nullptr, p.status);
+        }
       }
     }
     __syncwarp();
@@ -558,20 +589,37 @@ __global__ void __launch_bounds__(DKV_THREADS, 1)
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
           const float4 l4 = vec[e / 4];
-          const float ls[4] = {l4.x, l4.y, l4.z, l4.w};
+          const uint64_t nls[2] = {f2(l4.x, l4.y), f2(l4.z, l4.w)};
           float pr[4], w[4];
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            float v = __uint_as_float(x[e + g]);
-            w[g] = 1.f;
-            if (CAP) v = tanh_score<decltype(near)::value>(v * p.x_scale, w[g]);
-            if (ALIBI) v = fmaf(-slope2, fabsf(fd + (float)(e + g)), v * p.c_log2);
-            pr[g] = ex2_approx(fmaf(v, C, -ls[g]));
-            w[g] = CAP ? pr[g] * w[g] : pr[g];
+          for (int g = 0; g < 2; ++g) {
+            uint64_t v = f2(x[e + 2 * g], x[e + 2 * g + 1]), f = 0ull;
+            if (CAP) v = tanh2<decltype(near)::value, true>(v, p.x_scale, f);
+            if (ALIBI) {
+              const float2 t = unpack2(v);
+              const float d = fd + (float)(e + 2 * g);
+              v = f2(fmaf(-slope2, fabsf(d), t.x * p.c_log2), fmaf(-slope2, fabsf(d + 1.f), t.y * p.c_log2));
+            }
+            const uint64_t pp = ex2_2(fma2(v, f2(C), nls[g]));
+            const float2 p2 = unpack2(pp), w2 = unpack2(CAP ? mul2(pp, f) : pp);
+            pr[2 * g] = p2.x;
+            pr[2 * g + 1] = p2.y;
+            w[2 * g] = w2.x;
+            w[2 * g + 1] = w2.y;
           }
           if (masked) {
-            const int4 lo = ivec[2 * KV_QUERIES / 4 + e / 4], hi = ivec[3 * KV_QUERIES / 4 + e / 4];
-            const int lo4[4] = {lo.x, lo.y, lo.z, lo.w}, hi4[4] = {hi.x, hi.y, hi.z, hi.w};
+            int lo4[4] = {0, 0, 0, 0}, hi4[4];
+            if (p.lo) {
+              const int4 lo = ivec[2 * KV_QUERIES / 4 + e / 4], hi = ivec[3 * KV_QUERIES / 4 + e / 4];
+              lo4[0] = lo.x; lo4[1] = lo.y; lo4[2] = lo.z; lo4[3] = lo.w;
+              hi4[0] = hi.x; hi4[1] = hi.y; hi4[2] = hi.z; hi4[3] = hi.w;
+            } else {
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                const int q = q0 + half * 32 + e + g;
+                hi4[g] = q < p.S ? (p.causal ? q + 1 : p.S) : 0;
+              }
+            }
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
               const bool sees = lo4[g] <= kpos && kpos < hi4[g];
@@ -605,13 +653,12 @@ __global__ void __launch_bounds__(DKV_THREADS, 1)
 #pragma unroll
       for (int e = 0; e < 32; e += 4) {
         const float4 d4 = vec[KV_QUERIES / 4 + e / 4];
-        const float dl[4] = {d4.x, d4.y, d4.z, d4.w};
-        float ds[4];
+        const float2 a = unpack2(mul2(f2(x[e], x[e + 1]), add2(f2(d[e], d[e + 1]), f2(d4.x, d4.y))));
+        const float2 c = unpack2(mul2(f2(x[e + 2], x[e + 3]), add2(f2(d[e + 2], d[e + 3]), f2(d4.z, d4.w))));
+        float ds[4] = {a.x, a.y, c.x, c.y};
+        if (masked) {  // a hidden pair adds nothing, whatever dP is
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const float w = __uint_as_float(x[e + g]);
-          ds[g] = w * (__uint_as_float(d[e + g]) - dl[g]);
-          if (masked) ds[g] = w == 0.f ? 0.f : ds[g];  // a hidden pair adds nothing, whatever dP is
+          for (int g = 0; g < 4; ++g) ds[g] = x[e + g] == 0u ? 0.f : ds[g];
         }
         pk[e / 2] = pack_bf16(ds[0], ds[1]);
         pk[e / 2 + 1] = pack_bf16(ds[2], ds[3]);
@@ -625,47 +672,42 @@ __global__ void __launch_bounds__(DKV_THREADS, 1)
     if (ok && n > 0 && !mbar_wait(all_done, 0, abort_flag, p.status)) ok = false;
     if (ok) {
       tc_fence_after();
-#pragma unroll 1
-      for (int which = 0; which < 2; ++which) {
-        const int width = which ? p.Dqk : p.Dv;
-        const float f = which ? p.scale : 1.f;
-        const uint32_t src = (which ? TM_DK : TM_DV) + lane_base;
-#pragma unroll 1
-        for (int c = sub; c < (which ? DQP : DVP) / 32; c += 4) {
+      // every product has completed and every copy landed: shared memory is free for the output tiles
+      if (splits == 1) {
+        for (int o = sub; o < L::KBV + L::KBQ; o += 4) {  // dV's, then dK's blocks of 64 columns
+          if (o < L::KBV)
+            store_block(sV, TM_DV + lane_base, o, p.Dv, quarter, 1.f, n == 0, false, &tmDV, hk, kt * DA_TILE, p.S, b);
+          else
+            store_block(sK, TM_DK + lane_base, o - L::KBV, p.Dqk, quarter, p.scale, n == 0, false, &tmDK, hk, kt * DA_TILE,
+                        p.S, b);
+        }
+      } else {
+        // f32 parts: 32 columns a store, staged in the Q / dO ring
+        const int plane = (part * p.B + b) * p.Hk + hk;
+        for (int o = sub; o < (DVP + DQP) / 32; o += 4) {
+          const bool is_v = o < DVP / 32;
+          const int c = is_v ? o : o - DVP / 32;
+          uint8_t* slab = sQ + (o * 4 + quarter) * 4096;
           uint32_t w[32];
-          if (n > 0) {
-            tmem_ld32(src + c * 32, w);
-            tc_wait_ld();
-          } else {
+          tmem_ld32((is_v ? TM_DV : TM_DK) + lane_base + c * 32, w);
+          tc_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) w[e] = 0u;
+          for (int q = 0; q < 8; ++q) {
+            uint32_t v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              v[e] = n == 0 ? 0u : __float_as_uint(__uint_as_float(w[q * 4 + e]) * (is_v ? 1.f : p.scale));
+            sw128_store16(slab, lane, q, make_uint4(v[0], v[1], v[2], v[3]));
           }
-          if (kpos >= p.S) continue;
-          if (out.splits > 1) {
-            float* row = out.part + ((((int64_t)part * p.B + b) * p.Hk + hk) * p.S + kpos) * (p.Dqk + p.Dv) +
-                         (which ? p.Dv : 0) + c * 32;
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              if (c * 32 + q * 4 < width)
-                *reinterpret_cast<float4*>(row + q * 4) =
-                    make_float4(__uint_as_float(w[q * 4]) * f, __uint_as_float(w[q * 4 + 1]) * f,
-                                __uint_as_float(w[q * 4 + 2]) * f, __uint_as_float(w[q * 4 + 3]) * f);
-          } else {
-            __nv_bfloat16* row = which ? out.dk + ((int64_t)b * p.S + kpos) * out.ldk + (int64_t)hk * p.Dqk
-                                       : out.dv + ((int64_t)b * p.S + kpos) * out.ldv + (int64_t)hk * p.Dv;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              if (c * 32 + q * 8 < width) {
-                uint32_t o[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  o[e] = pack_bf16(__uint_as_float(w[q * 8 + 2 * e]) * f, __uint_as_float(w[q * 8 + 2 * e + 1]) * f);
-                *reinterpret_cast<uint4*>(row + c * 32 + q * 8) = make_uint4(o[0], o[1], o[2], o[3]);
-              }
-            }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && c * 32 < (is_v ? p.Dv : p.Dqk) && kt * DA_TILE + quarter * 32 < p.S) {
+            tma_store_3d(is_v ? &tmDV : &tmDK, slab, c * 32, kt * DA_TILE + quarter * 32, plane);
+            bulk_commit();
           }
         }
       }
+      if (lane == 0) bulk_wait_read<0>();
     }
   }
   tc_fence_before();
@@ -676,33 +718,51 @@ __global__ void __launch_bounds__(DKV_THREADS, 1)
   }
 }
 
-// dK, dV = the splits' parts added in order; 8 columns a thread
-__global__ void __launch_bounds__(256) da_join_kernel(const float* __restrict__ part, int splits, int B, int S, int Hk,
-                                                      int Dqk, int Dv, __nv_bfloat16* __restrict__ dk, int64_t ldk,
+// dV, dK = the splits' parts (f32 [split][B, Hk, S, D]) added in order; 8 columns a thread
+__global__ void __launch_bounds__(256) da_join_kernel(const float* __restrict__ part_v, const float* __restrict__ part_k,
+                                                      int splits, int B, int S, int Hk, int Dqk, int Dv,
+                                                      __nv_bfloat16* __restrict__ dk, int64_t ldk,
                                                       __nv_bfloat16* __restrict__ dv, int64_t ldv) {
   const int vec = (Dqk + Dv) / 8;
-  const int64_t total = (int64_t)B * Hk * S * vec;
+  const int64_t rows = (int64_t)B * Hk * S, total = rows * vec;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int c = (int)(i % vec) * 8;
+    const int c0 = (int)(i % vec) * 8;
+    const bool is_v = c0 < Dv;
+    const int c = is_v ? c0 : c0 - Dv, D = is_v ? Dv : Dqk;
     const int64_t row = i / vec, s = row % S, bh = row / S, h = bh % Hk, b = bh / Hk;
     float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int q = 0; q < splits; ++q) {
-      const float4* src = reinterpret_cast<const float4*>(part + ((int64_t)q * B * Hk * S + row) * (Dqk + Dv) + c);
+      const float4* src = reinterpret_cast<const float4*>((is_v ? part_v : part_k) + (q * rows + row) * D + c);
       const float4 x = __ldg(src), y = __ldg(src + 1);
       a[0] += x.x; a[1] += x.y; a[2] += x.z; a[3] += x.w;
       a[4] += y.x; a[5] += y.y; a[6] += y.z; a[7] += y.w;
     }
-    __nv_bfloat16* dst = c < Dv ? dv + (b * S + s) * ldv + h * Dv + c : dk + (b * S + s) * ldk + h * Dqk + (c - Dv);
+    __nv_bfloat16* dst = is_v ? dv + (b * S + s) * ldv + h * Dv + c : dk + (b * S + s) * ldk + h * Dqk + c;
     *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(a[4], a[5]),
                                                 pack_bf16(a[6], a[7]));
   }
 }
 
+// f32 [planes, S, D]: boxes of 32 columns x 32 rows
+inline CUtensorMap part_tmap(float* ptr, int64_t planes, int S, int D) {
+  ensure_current_context();
+  CUtensorMap m;
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)planes};
+  cuuint64_t strides[2] = {(cuuint64_t)D * 4, (cuuint64_t)S * D * 4};
+  cuuint32_t box[3] = {32, 32, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = get_encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, ptr, dims, strides, box, estr,
+                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  OXI_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (gradient parts) failed: ", (int)r);
+  return m;
+}
+
 struct BwdArgs {
   DaShape s;
   DaTensor q, k, v, o, dout;
-  const float* lse2;
-  float *delta, *part;
+  const float* nlse2;
+  float *ndelta, *part;
   DaOut dq, dk, dv;
   int* status;
   cudaStream_t st;
@@ -711,32 +771,32 @@ struct BwdArgs {
 template <int DQP, int DVP, bool CAP, bool ALIBI>
 void launch_bwd_t(const BwdArgs& a) {
   const DaShape& s = a.s;
+  const DaParams p = da_params(s, a.status);
   const CUtensorMap tq = da_tmap(a.q, s.B, s.S, s.Hq, s.Dqk), td = da_tmap(a.dout, s.B, s.S, s.Hq, s.Dv),
                     tk = da_tmap(a.k, s.B, s.S, s.Hk, s.Dqk), tv = da_tmap(a.v, s.B, s.S, s.Hk, s.Dv),
                     tk64 = da_tmap(a.k, s.B, s.S, s.Hk, s.Dqk, DQ_KEYS), tv64 = da_tmap(a.v, s.B, s.S, s.Hk, s.Dv, DQ_KEYS),
-                    tq64 = da_tmap(a.q, s.B, s.S, s.Hq, s.Dqk, KV_QUERIES), td64 = da_tmap(a.dout, s.B, s.S, s.Hq, s.Dv, KV_QUERIES);
-  const DaParams p = da_params(s, a.status);
+                    tq64 = da_tmap(a.q, s.B, s.S, s.Hq, s.Dqk, KV_QUERIES), td64 = da_tmap(a.dout, s.B, s.S, s.Hq, s.Dv, KV_QUERIES),
+                    tdq = da_tmap_out(a.dq, s.B, s.S, s.Hq, s.Dqk);
   auto kq = da_dq_kernel<DQP, DVP, CAP, ALIBI>;
   auto kkv = da_dkv_kernel<DQP, DVP, CAP, ALIBI>;
   da_smem(kq, DaDqSmem<DQP, DVP>::TOTAL);
   da_smem(kkv, DaDkvSmem<DQP, DVP>::TOTAL);
-  kq<<<dim3(s.Hq, s.B, p.nt), DQ_THREADS, DaDqSmem<DQP, DVP>::TOTAL, a.st>>>(
-      tq, tk64, tv64, td, p, a.o, a.dout, a.lse2, a.delta, reinterpret_cast<__nv_bfloat16*>(a.dq.ptr), a.dq.ld);
+  kq<<<dim3(s.Hq, s.B, p.nt), DA_GROUPS_THREADS, DaDqSmem<DQP, DVP>::TOTAL, a.st>>>(tq, tk64, tv64, td, tdq, p, a.o, a.dout,
+                                                                                    a.nlse2, a.ndelta);
   OXI_CUDA_CHECK(cudaGetLastError());
-  DkvOut out;
-  out.dk = reinterpret_cast<__nv_bfloat16*>(a.dk.ptr);
-  out.dv = reinterpret_cast<__nv_bfloat16*>(a.dv.ptr);
-  out.ldk = a.dk.ld;
-  out.ldv = a.dv.ld;
-  out.part = a.part;
-  out.splits = da_bwd_splits(s.B, s.S, s.Hq, s.Hk);
-  kkv<<<dim3(s.Hk * out.splits, s.B, p.nt), DKV_THREADS, DaDkvSmem<DQP, DVP>::TOTAL, a.st>>>(tq64, tk, tv, td64, p, a.lse2,
-                                                                                             a.delta, out);
+  const int splits = da_bwd_splits(s.B, s.S, s.Hq, s.Hk);
+  const int64_t planes = (int64_t)splits * s.B * s.Hk;
+  float* part_k = a.part ? a.part + planes * s.S * s.Dv : nullptr;
+  const CUtensorMap tdk = splits > 1 ? part_tmap(part_k, planes, s.S, s.Dqk) : da_tmap_out(a.dk, s.B, s.S, s.Hk, s.Dqk),
+                    tdv = splits > 1 ? part_tmap(a.part, planes, s.S, s.Dv) : da_tmap_out(a.dv, s.B, s.S, s.Hk, s.Dv);
+  kkv<<<dim3(s.Hk * splits, s.B, p.nt), DA_GROUPS_THREADS, DaDkvSmem<DQP, DVP>::TOTAL, a.st>>>(
+      tq64, tk, tv, td64, tdk, tdv, p, a.nlse2, a.ndelta, splits);
   OXI_CUDA_CHECK(cudaGetLastError());
-  if (out.splits > 1) {
+  if (splits > 1) {
     const int64_t threads = (int64_t)s.B * s.Hk * s.S * ((s.Dqk + s.Dv) / 8);
     da_join_kernel<<<(unsigned)std::min<int64_t>((threads + 255) / 256, 148 * 16), 256, 0, a.st>>>(
-        a.part, out.splits, s.B, s.S, s.Hk, s.Dqk, s.Dv, out.dk, out.ldk, out.dv, out.ldv);
+        a.part, part_k, splits, s.B, s.S, s.Hk, s.Dqk, s.Dv, reinterpret_cast<__nv_bfloat16*>(a.dk.ptr), a.dk.ld,
+        reinterpret_cast<__nv_bfloat16*>(a.dv.ptr), a.dv.ld);
     OXI_CUDA_CHECK(cudaGetLastError());
   }
 }
@@ -758,7 +818,7 @@ int da_bwd_splits(int B, int S, int Hq, int Hk) {
 }
 
 void launch_da_bwd(const DaShape& s, const DaTensor& q, const DaTensor& k, const DaTensor& v, const DaTensor& o,
-                   const DaTensor& dout, const float* lse2, float* delta, float* part, const DaOut& dq, const DaOut& dk,
+                   const DaTensor& dout, const float* nlse2, float* ndelta, float* part, const DaOut& dq, const DaOut& dk,
                    const DaOut& dv, int* status, cudaStream_t st) {
   if (s.B == 0 || s.S == 0 || s.Hq == 0) return;
   da_check(s);
@@ -768,7 +828,7 @@ void launch_da_bwd(const DaShape& s, const DaTensor& q, const DaTensor& k, const
     OXI_CHECK((reinterpret_cast<uintptr_t>(t->ptr) & 15) == 0 && t->sb % 8 == 0 && t->ss % 8 == 0 && t->sh % 8 == 0,
               "16-byte aligned rows of the output and its gradient");
   OXI_CHECK(da_bwd_splits(s.B, s.S, s.Hq, s.Hk) == 1 || part != nullptr, "attention backward needs its parts' workspace");
-  const BwdArgs a{s, q, k, v, o, dout, lse2, delta, part, dq, dk, dv, status, st};
+  const BwdArgs a{s, q, k, v, o, dout, nlse2, ndelta, part, dq, dk, dv, status, st};
   if (s.Dqk <= 64 && s.Dv <= 64) launch_bwd_d<64, 64>(a);
   else if (s.Dv <= 64) launch_bwd_d<128, 64>(a);
   else launch_bwd_d<128, 128>(a);

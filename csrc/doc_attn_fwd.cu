@@ -43,8 +43,8 @@ struct DaFwdSmem {
 template <int DQP, int DVP, bool CAP, bool ALIBI>
 __global__ void __launch_bounds__(FW_THREADS, 2)
     da_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                  const __grid_constant__ CUtensorMap tmV, DaParams p, __nv_bfloat16* __restrict__ o_out, int64_t ldo,
-                  float* __restrict__ lse2) {
+                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, DaParams p,
+                  float* __restrict__ nlse2) {
   using L = DaFwdSmem<DQP, DVP>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -215,14 +215,17 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         if (CAP) {
-          float unused;
-          if (warp_near<32>(x[c], p.x_scale)) {
+          uint64_t unused;
+          auto capped = [&](auto near) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) x[c][e] = __float_as_uint(tanh_near(__uint_as_float(x[c][e]) * p.x_scale, unused));
-          } else {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) x[c][e] = __float_as_uint(tanh_wide(__uint_as_float(x[c][e]) * p.x_scale, unused));
-          }
+            for (int e = 0; e < 32; e += 2) {
+              const float2 t = unpack2(tanh2<decltype(near)::value, false>(f2(x[c][e], x[c][e + 1]), p.x_scale, unused));
+              x[c][e] = __float_as_uint(t.x);
+              x[c][e + 1] = __float_as_uint(t.y);
+            }
+          };
+          if (warp_near<32>(x[c], p.x_scale)) capped(std::true_type{});
+          else capped(std::false_type{});
         }
         if (ALIBI) {
           const float fd = (float)(qpos - (k0 + c * 32));
@@ -238,26 +241,28 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
         }
       }
       uint32_t pk[2][16];
-      float rs[4];
+      uint64_t rs[4];
       auto exponentials = [&]() {
-        const float mref = m == -INFINITY ? 0.f : m;
+        const uint64_t mref = f2(m == -INFINITY ? 0.f : -m), cc = f2(C);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) rs[q] = 0.f;
+        for (int q = 0; q < 4; ++q) rs[q] = 0ull;
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float a = ex2_approx(fmaf(__uint_as_float(x[c][e]), C, -mref));
-            const float bb = ex2_approx(fmaf(__uint_as_float(x[c][e + 1]), C, -mref));
-            rs[(e >> 1) & 3] += a + bb;
-            pk[c][e / 2] = pack_bf16(a, bb);
+            const uint64_t pp = ex2_2(fma2(f2(x[c][e], x[c][e + 1]), cc, mref));
+            rs[(e >> 1) & 3] = add2(rs[(e >> 1) & 3], pp);
+            const float2 v = unpack2(pp);
+            pk[c][e / 2] = pack_bf16(v.x, v.y);
           }
       };
       exponentials();
       if (!bounded) {
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int e = 0; e < 64; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(x[e >> 5][e & 31]));
+        for (int e = 0; e < 64; e += 2)
+          mx[(e >> 1) & 3] = fmaxf(fmaxf(__uint_as_float(x[e >> 5][e & 31]), __uint_as_float(x[e >> 5][(e & 31) + 1])),
+                                   mx[(e >> 1) & 3]);
         const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * C;
         if (__any_sync(0xffffffffu, m == -INFINITY ? mt > -INFINITY : mt > m + 60.f)) {
           if (!move(i, fmaxf(mt, m))) { ok = false; break; }
@@ -267,7 +272,8 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
       }
       tmem_st16(s_addr, pk[0]);
       tmem_st16(s_addr + 16, pk[1]);
-      l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+      const float2 rsum = unpack2(add2(add2(rs[0], rs[1]), add2(rs[2], rs[3])));
+      l += rsum.x + rsum.y;
       if (padded) {
         // V_i has landed before its product may read it; rows of padding become zero
         if (!mbar_wait(&v_full[i % L::VST], (i / L::VST) & 1, abort_flag, p.status)) { ok = false; break; }
@@ -281,35 +287,14 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
     if (ok && n > 0 && !mbar_wait(o_done, 0, abort_flag, p.status)) ok = false;
     if (ok) {
       tc_fence_after();
-      const bool valid = qpos < p.S;
-      const float inv_l = l > 0.f ? 1.f / l : 0.f;
-      __nv_bfloat16* orow = o_out + ((int64_t)b * p.S + qpos) * ldo + (int64_t)h * p.Dv;
+      // a row that sees no key is zero; one whose scores are NaN stays NaN.  Q's tile is free by now
+      const bool some = l > 0.f;
 #pragma unroll 1
-      for (int c = 0; c < DVP / 32; ++c) {
-        uint32_t w[32];
-        if (n > 0) {
-          tmem_ld32(TM_O + lane_base + c * 32, w);
-          tc_wait_ld();
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) w[e] = 0u;
-        }
-        if (valid) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (c * 32 + q * 8 < p.Dv) {
-              uint32_t u[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                u[e] = l > 0.f ? pack_bf16(__uint_as_float(w[q * 8 + 2 * e]) * inv_l,
-                                           __uint_as_float(w[q * 8 + 2 * e + 1]) * inv_l)
-                               : (l == l ? 0u : 0x7fff7fffu);  // no visible key: 0; NaN scores stay NaN
-              *reinterpret_cast<uint4*>(orow + c * 32 + q * 8) = make_uint4(u[0], u[1], u[2], u[3]);
-            }
-          }
-        }
-      }
-      if (valid) lse2[((int64_t)b * p.Hq + h) * p.S + qpos] = l == 0.f ? INFINITY : m + log2f(l);
+      for (int kb = 0; kb < L::KBV; ++kb)
+        store_block(sQ, TM_O + lane_base, kb, p.Dv, quarter, some ? 1.f / l : 0.f, !some, l != l, &tmO, h, qt * DA_TILE,
+                    p.S, b);
+      if (qpos < p.S) nlse2[((int64_t)b * p.Hq + h) * p.S + qpos] = l == 0.f ? -INFINITY : -(m + log2f(l));
+      if (lane == 0) bulk_wait_read<0>();
     }
   }
 
@@ -323,27 +308,26 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
 
 template <int DQP, int DVP, bool CAP, bool ALIBI>
 void launch_fwd_t(const DaShape& s, const DaTensor& q, const DaTensor& k, const DaTensor& v, const DaOut& o,
-                  float* lse2, int* status, cudaStream_t st) {
+                  float* nlse2, int* status, cudaStream_t st) {
   using L = DaFwdSmem<DQP, DVP>;
   const CUtensorMap tq = da_tmap(q, s.B, s.S, s.Hq, s.Dqk), tk = da_tmap(k, s.B, s.S, s.Hk, s.Dqk, FW_KEYS),
-                    tv = da_tmap(v, s.B, s.S, s.Hk, s.Dv, FW_KEYS);
+                    tv = da_tmap(v, s.B, s.S, s.Hk, s.Dv, FW_KEYS), to = da_tmap_out(o, s.B, s.S, s.Hq, s.Dv);
   auto kern = da_fwd_kernel<DQP, DVP, CAP, ALIBI>;
   da_smem(kern, L::TOTAL);
   const dim3 grid(s.Hq, s.B, (s.S + DA_TILE - 1) / DA_TILE);
-  kern<<<grid, FW_THREADS, L::TOTAL, st>>>(tq, tk, tv, da_params(s, status), reinterpret_cast<__nv_bfloat16*>(o.ptr),
-                                           o.ld, lse2);
+  kern<<<grid, FW_THREADS, L::TOTAL, st>>>(tq, tk, tv, to, da_params(s, status), nlse2);
   OXI_CUDA_CHECK(cudaGetLastError());
 }
 
 template <int DQP, int DVP>
 void launch_fwd_d(const DaShape& s, const DaTensor& q, const DaTensor& k, const DaTensor& v, const DaOut& o,
-                  float* lse2, int* status, cudaStream_t st) {
+                  float* nlse2, int* status, cudaStream_t st) {
   if (s.cap > 0.f)
-    s.slopes ? launch_fwd_t<DQP, DVP, true, true>(s, q, k, v, o, lse2, status, st)
-             : launch_fwd_t<DQP, DVP, true, false>(s, q, k, v, o, lse2, status, st);
+    s.slopes ? launch_fwd_t<DQP, DVP, true, true>(s, q, k, v, o, nlse2, status, st)
+             : launch_fwd_t<DQP, DVP, true, false>(s, q, k, v, o, nlse2, status, st);
   else
-    s.slopes ? launch_fwd_t<DQP, DVP, false, true>(s, q, k, v, o, lse2, status, st)
-             : launch_fwd_t<DQP, DVP, false, false>(s, q, k, v, o, lse2, status, st);
+    s.slopes ? launch_fwd_t<DQP, DVP, false, true>(s, q, k, v, o, nlse2, status, st)
+             : launch_fwd_t<DQP, DVP, false, false>(s, q, k, v, o, nlse2, status, st);
 }
 
 }  // namespace
@@ -353,14 +337,14 @@ bool da_supported(int Dqk, int Dv) {
 }
 
 void launch_da_fwd(const DaShape& s, const DaTensor& q, const DaTensor& k, const DaTensor& v, const DaOut& o,
-                   float* lse2, int* status, cudaStream_t st) {
+                   float* nlse2, int* status, cudaStream_t st) {
   if (s.B == 0 || s.S == 0 || s.Hq == 0) return;
   da_check(s);
   OXI_CHECK((reinterpret_cast<uintptr_t>(o.ptr) & 15) == 0 && o.ld % 8 == 0, "16-byte aligned output rows");
   // kernels for widths of up to 64 and 128 columns: narrower heads are padded with zero columns
-  if (s.Dqk <= 64 && s.Dv <= 64) launch_fwd_d<64, 64>(s, q, k, v, o, lse2, status, st);
-  else if (s.Dv <= 64) launch_fwd_d<128, 64>(s, q, k, v, o, lse2, status, st);
-  else launch_fwd_d<128, 128>(s, q, k, v, o, lse2, status, st);
+  if (s.Dqk <= 64 && s.Dv <= 64) launch_fwd_d<64, 64>(s, q, k, v, o, nlse2, status, st);
+  else if (s.Dv <= 64) launch_fwd_d<128, 64>(s, q, k, v, o, nlse2, status, st);
+  else launch_fwd_d<128, 128>(s, q, k, v, o, nlse2, status, st);
 }
 
 }  // namespace oxi

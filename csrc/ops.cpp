@@ -454,15 +454,15 @@ std::vector<torch::Tensor> doc_attn_fwd(torch::Tensor q, torch::Tensor k, torch:
   const oxi::DaShape s = da_shape(q, k, v, scale, cap, slopes, causal, mask);
   const auto tq = da_tensor(q, q, "q"), tk = da_tensor(k, q, "k"), tv = da_tensor(v, q, "v");
   auto o = torch::empty({s.B, s.S, s.Hq, s.Dv}, q.options());
-  auto lse2 = torch::empty({s.B, s.Hq, s.S}, q.options().dtype(torch::kFloat32));
-  oxi::launch_da_fwd(s, tq, tk, tv, {o.data_ptr(), (int64_t)s.Hq * s.Dv}, lse2.data_ptr<float>(), status_ptr(status),
+  auto nlse2 = torch::empty({s.B, s.Hq, s.S}, q.options().dtype(torch::kFloat32));
+  oxi::launch_da_fwd(s, tq, tk, tv, {o.data_ptr(), (int64_t)s.Hq * s.Dv}, nlse2.data_ptr<float>(), status_ptr(status),
                      stream());
-  return {o, lse2};
+  return {o, nlse2};
 }
 
 // dq, dk, dv: bf16 [B * S, H * D] views with unit inner stride (columns of one buffer, say)
 void doc_attn_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o, torch::Tensor dout,
-                  torch::Tensor lse2, double scale, double cap, c10::optional<torch::Tensor> slopes, bool causal,
+                  torch::Tensor nlse2, double scale, double cap, c10::optional<torch::Tensor> slopes, bool causal,
                   std::vector<torch::Tensor> mask, torch::Tensor dq, torch::Tensor dk, torch::Tensor dv,
                   torch::Tensor status) {
   c10::cuda::CUDAGuard g(q.device());
@@ -471,8 +471,8 @@ void doc_attn_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tens
              to = da_tensor(o, q, "o"), td = da_tensor(dout, q, "dout");
   OXI_CHECK(o.sizes() == dout.sizes() && o.size(0) == s.B && o.size(1) == s.S && o.size(2) == s.Hq &&
                   o.size(3) == s.Dv, "attention backward: o and dout must be [B, S, Hq, Dv]");
-  OXI_CHECK(lse2.device() == q.device() && lse2.scalar_type() == torch::kFloat32 && lse2.is_contiguous() &&
-                  lse2.numel() == (int64_t)s.B * s.Hq * s.S, "attention backward: lse2");
+  OXI_CHECK(nlse2.device() == q.device() && nlse2.scalar_type() == torch::kFloat32 && nlse2.is_contiguous() &&
+                  nlse2.numel() == (int64_t)s.B * s.Hq * s.S, "attention backward: nlse2");
   const int64_t rows = (int64_t)s.B * s.S;
   const int64_t cols[3] = {(int64_t)s.Hq * s.Dqk, (int64_t)s.Hk * s.Dqk, (int64_t)s.Hk * s.Dv};
   const torch::Tensor outs[3] = {dq, dk, dv};
@@ -480,11 +480,11 @@ void doc_attn_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tens
     OXI_CHECK(outs[i].device() == q.device() && outs[i].scalar_type() == torch::kBFloat16 && outs[i].dim() == 2 &&
                   outs[i].size(0) == rows && outs[i].size(1) == cols[i] && outs[i].stride(1) == 1,
               "attention backward: gradients must be bf16 [B * S, H * D] on q's device");
-  auto delta = torch::empty_like(lse2);
+  auto ndelta = torch::empty_like(nlse2);
   const int splits = oxi::da_bwd_splits(s.B, s.S, s.Hq, s.Hk);
   torch::Tensor part;
-  if (splits > 1) part = torch::empty({splits, (int64_t)s.B * s.Hk * s.S, s.Dqk + s.Dv}, lse2.options());
-  oxi::launch_da_bwd(s, tq, tk, tv, to, td, lse2.data_ptr<float>(), delta.data_ptr<float>(),
+  if (splits > 1) part = torch::empty({splits, (int64_t)s.B * s.Hk * s.S, s.Dqk + s.Dv}, nlse2.options());
+  oxi::launch_da_bwd(s, tq, tk, tv, to, td, nlse2.data_ptr<float>(), ndelta.data_ptr<float>(),
                      splits > 1 ? part.data_ptr<float>() : nullptr,
                      {dq.data_ptr(), dq.stride(0)}, {dk.data_ptr(), dk.stride(0)}, {dv.data_ptr(), dv.stride(0)},
                      status_ptr(status), stream());

@@ -116,16 +116,16 @@ class DocAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, scale: float, cap: float, slopes, causal: bool, mask):
-        o, lse2 = _fwd(q, k, v, scale, cap, slopes, causal, mask)
-        ctx.save_for_backward(q, k, v, o, lse2, slopes, *mask)
+        o, nlse2 = _fwd(q, k, v, scale, cap, slopes, causal, mask)
+        ctx.save_for_backward(q, k, v, o, nlse2, slopes, *mask)
         ctx.cfg = (scale, cap, causal)
         return o
 
     @staticmethod
     def backward(ctx, do):
-        q, k, v, o, lse2, slopes, *mask = ctx.saved_tensors
+        q, k, v, o, nlse2, slopes, *mask = ctx.saved_tensors
         outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
-        _bwd(ctx, q, k, v, o, do, lse2, slopes, mask, [t.flatten(0, 1).flatten(1) for t in outs])
+        _bwd(ctx, q, k, v, o, do, nlse2, slopes, mask, [t.flatten(0, 1).flatten(1) for t in outs])
         return (*outs, None, None, None, None, None)
 
 
@@ -136,20 +136,20 @@ class DocAttentionQKV(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, Hq: int, Hk: int, D: int, scale: float, cap: float, slopes, causal: bool, mask):
         q, k, v = _heads(qkv, Hq, Hk, D)
-        o, lse2 = _fwd(q, k, v, scale, cap, slopes, causal, mask)
-        ctx.save_for_backward(qkv, o, lse2, slopes, *mask)
+        o, nlse2 = _fwd(q, k, v, scale, cap, slopes, causal, mask)
+        ctx.save_for_backward(qkv, o, nlse2, slopes, *mask)
         ctx.cfg, ctx.heads = (scale, cap, causal), (Hq, Hk, D)
         return o.flatten(2)
 
     @staticmethod
     def backward(ctx, do):
-        qkv, o, lse2, slopes, *mask = ctx.saved_tensors
+        qkv, o, nlse2, slopes, *mask = ctx.saved_tensors
         Hq, Hk, D = ctx.heads
         q, k, v = _heads(qkv, Hq, Hk, D)
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
         d2 = dqkv.flatten(0, 1)
         a, b = Hq * D, (Hq + Hk) * D
-        _bwd(ctx, q, k, v, o, do.reshape(o.shape), lse2, slopes, mask, [d2[:, :a], d2[:, a:b], d2[:, b:]])
+        _bwd(ctx, q, k, v, o, do.reshape(o.shape), nlse2, slopes, mask, [d2[:, :a], d2[:, a:b], d2[:, b:]])
         return (dqkv, *[None] * 8)
 
 
@@ -163,10 +163,10 @@ def _fwd(q, k, v, scale, cap, slopes, causal, mask):
                               status(q.device))
 
 
-def _bwd(ctx, q, k, v, o, do, lse2, slopes, mask, outs):
+def _bwd(ctx, q, k, v, o, do, nlse2, slopes, mask, outs):
     from ._C import ext, status
     scale, cap, causal = ctx.cfg
-    ext().doc_attn_bwd(_tma_view(q), _tma_view(k), _tma_view(v), o, _tma_view(do), lse2, scale, cap, slopes, causal,
+    ext().doc_attn_bwd(_tma_view(q), _tma_view(k), _tma_view(v), o, _tma_view(do), nlse2, scale, cap, slopes, causal,
                        list(mask), *outs, status(q.device))
 
 

@@ -102,12 +102,27 @@ __device__ __forceinline__ uint64_t tanh2(uint64_t z, float x_scale, uint64_t& d
 // Scores of the whole warp are within the polynomial's range (a score of 0.76 of the cap): scores of
 // a model are, nearly always; a warp with a larger one takes the other form.
 template <int N>
-__device__ __forceinline__ bool warp_near(const uint32_t (&x)[N], float x_scale) {
+__device__ __forceinline__ bool warp_near(const uint64_t (&x)[N], float x_scale) {
   float m[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int e = 0; e < N; e += 2)
-    m[(e >> 1) & 3] = fmaxf(fmaxf(fabsf(__uint_as_float(x[e])), fabsf(__uint_as_float(x[e + 1]))), m[(e >> 1) & 3]);
+  for (int e = 0; e < N; ++e) {
+    const float2 v = unpack2(x[e]);
+    m[e & 3] = fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), m[e & 3]);
+  }
   return __all_sync(0xffffffffu, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * x_scale <= 1.f);
+}
+// 32 columns of TMEM, as pairs
+__device__ __forceinline__ void tmem_ld_pairs(uint32_t taddr, uint64_t (&x)[16]) {
+  uint32_t w[32];
+  tmem_ld32(taddr, w);
+  tc_wait_ld();
+#pragma unroll
+  for (int e = 0; e < 16; ++e) x[e] = f2(w[2 * e], w[2 * e + 1]);
+}
+// Where a bit is not set, the element is v
+__device__ __forceinline__ uint64_t select2(uint64_t x, uint32_t bits, int e, float v) {
+  const float2 u = unpack2(x);
+  return f2(((bits >> e) & 1u) ? u.x : v, ((bits >> (e + 1)) & 1u) ? u.y : v);
 }
 
 // Visible keys of a row within 32 consecutive keys from k: bit t is key k + t in [lo, hi).

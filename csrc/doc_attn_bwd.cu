@@ -192,6 +192,11 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
     const int qpos = qt * DA_TILE + r;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     bool ok = true;
+    // what a row needs from memory, all in flight together
+    const TileRange vis = key_range(p, b, qpos);
+    const bool in = qpos < p.S;
+    const int64_t vi = ((int64_t)b * p.Hq + h) * p.S + qpos;
+    const float nls = in ? __ldg(nlse2 + vi) : -INFINITY;
     // minus delta of 8 rows a warp, 16 bytes a lane: 2 rows at a time
     {
       const __nv_bfloat16* op = reinterpret_cast<const __nv_bfloat16*>(o_in.ptr) + b * o_in.sb + h * o_in.sh;
@@ -233,13 +238,9 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
       }
     }
     asm volatile("bar.sync 1, 512;" ::: "memory");  // delta's rows; reached by every softmax warp
-    const TileRange vis = key_range(p, b, qpos);
     const int all_lo = __reduce_max_sync(0xffffffffu, vis.begin), all_hi = __reduce_min_sync(0xffffffffu, vis.end);
     const uint32_t s_addr = TM_S + mine * DQ_KEYS + lane_base + half * 32;
     const uint32_t dp_addr = TM_DP + mine * DQ_KEYS + lane_base + half * 32;
-    const bool in = qpos < p.S;
-    const int64_t vi = ((int64_t)b * p.Hq + h) * p.S + qpos;
-    const float nls = in ? nlse2[vi] : -INFINITY;
     const float ndl = s_row[r];
     const float slope2 = ALIBI ? __ldg(p.slopes + h) * LOG2E : 0.f;
     const float C = ALIBI ? 1.f : p.c_log2;
@@ -249,60 +250,52 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
       const bool padded = tile_has_pad(p, b, k0 / DA_TILE);
       if (!mbar_wait(&s_full[mine], ph, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
-      uint32_t x[32];
-      tmem_ld32(s_addr, x);
-      tc_wait_ld();
+      uint64_t x[16], f[CAP ? 16 : 1];  // scores, then P; the cap's derivative
+      tmem_ld_pairs(s_addr, x);
       const bool masked = !(all_lo <= k0 && k0 + 32 <= all_hi);
-      const uint32_t bits = masked ? range_bits(vis.begin, vis.end, k0) : 0xffffffffu;
-      const float fd = (float)(qpos - k0);
-      uint64_t f[CAP ? 16 : 1];  // the cap's derivative
       auto probabilities = [&](auto near) {
+        const float fd = (float)(qpos - k0);
 #pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          uint64_t v = f2(x[e], x[e + 1]);
-          if (CAP) v = tanh2<decltype(near)::value, true>(v, p.x_scale, f[CAP ? e / 2 : 0]);
-          if (ALIBI) {
-            const float2 t = unpack2(v);
-            v = f2(fmaf(-slope2, fabsf(fd - (float)e), t.x * p.c_log2), fmaf(-slope2, fabsf(fd - (float)(e + 1)), t.y * p.c_log2));
-          }
-          const float2 pr = unpack2(ex2_2(fma2(v, f2(C), f2(nls))));
-          x[e] = __float_as_uint(pr.x);
-          x[e + 1] = __float_as_uint(pr.y);
+        for (int e = 0; e < 16; ++e) {
+          uint64_t v = x[e];
+          if (CAP) v = tanh2<decltype(near)::value, true>(v, p.x_scale, f[CAP ? e : 0]);
+          if (ALIBI)
+            v = fma2(f2(-slope2), f2(fabsf(fd - (float)(2 * e)), fabsf(fd - (float)(2 * e + 1))), mul2(v, f2(p.c_log2)));
+          x[e] = ex2_2(fma2(v, f2(C), f2(nls)));
         }
       };
-      if (CAP && warp_near<32>(x, p.x_scale)) probabilities(std::true_type{});
+      if (CAP && warp_near(x, p.x_scale)) probabilities(std::true_type{});
       else probabilities(std::false_type{});
       if (!mbar_wait(&dp_full[mine], ph, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
-      uint64_t rs = 0ull;
+      // hidden pairs add nothing, whatever their scores and dP are
+      auto gradients = [&](auto some_hidden) {
+        constexpr bool HIDDEN = decltype(some_hidden)::value;
+        const uint32_t bits = HIDDEN ? range_bits(vis.begin, vis.end, k0) : 0u;
+        uint64_t rs = 0ull;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t d[16], pk[8];
-        tmem_ld16(dp_addr + c * 16, d);
-        tc_wait_ld();
+        for (int c = 0; c < 2; ++c) {
+          uint32_t d[16], pk[8];
+          tmem_ld16(dp_addr + c * 16, d);
+          tc_wait_ld();
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          const int t = c * 16 + e;
-          uint64_t g = mul2(f2(x[t], x[t + 1]), add2(f2(d[e], d[e + 1]), f2(ndl)));
-          if (masked) {  // a hidden pair adds nothing, whatever its score and dP are
+          for (int e = 0; e < 8; ++e) {
+            const int t = c * 8 + e;
+            uint64_t g = mul2(x[t], add2(f2(d[2 * e], d[2 * e + 1]), f2(ndl)));
+            if (HIDDEN) g = select2(g, bits, 2 * t, 0.f);
+            rs = add2(rs, g);
+            if (CAP) g = mul2(g, f[CAP ? t : 0]);
+            if (CAP && HIDDEN) g = select2(g, bits, 2 * t, 0.f);
             const float2 u = unpack2(g);
-            g = f2(((bits >> t) & 1u) ? u.x : 0.f, ((bits >> (t + 1)) & 1u) ? u.y : 0.f);
+            pk[e] = pack_bf16(u.x, u.y);
           }
-          rs = add2(rs, g);
-          if (CAP) {
-            g = mul2(g, f[CAP ? t / 2 : 0]);
-            if (masked) {
-              const float2 u = unpack2(g);
-              g = f2(((bits >> t) & 1u) ? u.x : 0.f, ((bits >> (t + 1)) & 1u) ? u.y : 0.f);
-            }
-          }
-          const float2 u = unpack2(g);
-          pk[e / 2] = pack_bf16(u.x, u.y);
+          tmem_st8(dp_addr + c * 8, pk);
         }
-        tmem_st8(dp_addr + c * 8, pk);
-      }
-      const float2 rv = unpack2(rs);
-      rest += rv.x + rv.y;
+        const float2 rv = unpack2(rs);
+        rest += rv.x + rv.y;
+      };
+      if (masked) gradients(std::true_type{});
+      else gradients(std::false_type{});
       // S_i has read K_i: rows of padding become zero before the dQ product reads them
       if (padded)
         zero_pad_rows<L::KBQ, DQ_KEYS>(sK + (i % L::ST) * L::K_BYTES, p, b, (kr.begin + i) * DQ_KEYS, half * 128 + r, 256);
@@ -581,60 +574,57 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
       if (!mbar_wait(&vec_full[st], u & 1, abort_flag, p.status) ||
           !mbar_wait(&s_full[mine], ph, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
-      uint32_t x[32], pk[16];
-      tmem_ld32(s_addr, x);
-      tc_wait_ld();
-      // x becomes P times the cap's derivative, pk P
-      auto probabilities = [&](auto near) {
+      uint64_t x[16];  // scores, then P times the cap's derivative
+      uint32_t pk[16];
+      tmem_ld_pairs(s_addr, x);
+      auto probabilities = [&](auto near, auto some_hidden) {
+        constexpr bool HIDDEN = decltype(some_hidden)::value;
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const float4 l4 = vec[e / 4];
+        for (int e = 0; e < 16; e += 2) {
+          const float4 l4 = vec[e / 2];
           const uint64_t nls[2] = {f2(l4.x, l4.y), f2(l4.z, l4.w)};
-          float pr[4], w[4];
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            uint64_t v = f2(x[e + 2 * g], x[e + 2 * g + 1]), f = 0ull;
-            if (CAP) v = tanh2<decltype(near)::value, true>(v, p.x_scale, f);
-            if (ALIBI) {
-              const float2 t = unpack2(v);
-              const float d = fd + (float)(e + 2 * g);
-              v = f2(fmaf(-slope2, fabsf(d), t.x * p.c_log2), fmaf(-slope2, fabsf(d + 1.f), t.y * p.c_log2));
-            }
-            const uint64_t pp = ex2_2(fma2(v, f2(C), nls[g]));
-            const float2 p2 = unpack2(pp), w2 = unpack2(CAP ? mul2(pp, f) : pp);
-            pr[2 * g] = p2.x;
-            pr[2 * g + 1] = p2.y;
-            w[2 * g] = w2.x;
-            w[2 * g + 1] = w2.y;
-          }
-          if (masked) {
-            int lo4[4] = {0, 0, 0, 0}, hi4[4];
+          uint32_t sees = 15u;
+          if (HIDDEN) {
+            int lo[4] = {0, 0, 0, 0}, hi[4];
             if (p.lo) {
-              const int4 lo = ivec[2 * KV_QUERIES / 4 + e / 4], hi = ivec[3 * KV_QUERIES / 4 + e / 4];
-              lo4[0] = lo.x; lo4[1] = lo.y; lo4[2] = lo.z; lo4[3] = lo.w;
-              hi4[0] = hi.x; hi4[1] = hi.y; hi4[2] = hi.z; hi4[3] = hi.w;
+              const int4 a = ivec[2 * KV_QUERIES / 4 + e / 2], c = ivec[3 * KV_QUERIES / 4 + e / 2];
+              lo[0] = a.x; lo[1] = a.y; lo[2] = a.z; lo[3] = a.w;
+              hi[0] = c.x; hi[1] = c.y; hi[2] = c.z; hi[3] = c.w;
             } else {
 #pragma unroll
               for (int g = 0; g < 4; ++g) {
-                const int q = q0 + half * 32 + e + g;
-                hi4[g] = q < p.S ? (p.causal ? q + 1 : p.S) : 0;
+                const int q = q0 + half * 32 + 2 * e + g;
+                hi[g] = q < p.S ? (p.causal ? q + 1 : p.S) : 0;
               }
             }
+            sees = 0u;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const bool sees = lo4[g] <= kpos && kpos < hi4[g];
-              pr[g] = sees ? pr[g] : 0.f;
-              w[g] = sees ? w[g] : 0.f;  // the score of a hidden pair may be NaN
-            }
+            for (int g = 0; g < 4; ++g) sees |= (lo[g] <= kpos && kpos < hi[g]) ? 1u << g : 0u;
           }
 #pragma unroll
-          for (int g = 0; g < 4; ++g) x[e + g] = __float_as_uint(w[g]);
-          pk[e / 2] = pack_bf16(pr[0], pr[1]);
-          pk[e / 2 + 1] = pack_bf16(pr[2], pr[3]);
+          for (int g = 0; g < 2; ++g) {
+            uint64_t v = x[e + g], f = 0ull;
+            if (CAP) v = tanh2<decltype(near)::value, true>(v, p.x_scale, f);
+            if (ALIBI) {
+              const float d = fd + (float)(2 * (e + g));
+              v = fma2(f2(-slope2), f2(fabsf(d), fabsf(d + 1.f)), mul2(v, f2(p.c_log2)));
+            }
+            uint64_t pp = ex2_2(fma2(v, f2(C), nls[g]));
+            if (HIDDEN) pp = select2(pp, sees, 2 * g, 0.f);
+            if (CAP) {
+              x[e + g] = mul2(pp, f);
+              if (HIDDEN) x[e + g] = select2(x[e + g], sees, 2 * g, 0.f);  // a hidden pair's score may be NaN
+            } else {
+              x[e + g] = pp;
+            }
+            const float2 u = unpack2(pp);
+            pk[e + g] = pack_bf16(u.x, u.y);
+          }
         }
       };
-      if (CAP && warp_near<32>(x, p.x_scale)) probabilities(std::true_type{});
-      else probabilities(std::false_type{});
+      const bool near = CAP && warp_near(x, p.x_scale);
+      if (masked) near ? probabilities(std::true_type{}, std::true_type{}) : probabilities(std::false_type{}, std::true_type{});
+      else near ? probabilities(std::true_type{}, std::false_type{}) : probabilities(std::false_type{}, std::false_type{});
       tmem_st16(s_addr, pk);
       if (padded) {
         if (!mbar_wait(&q_full[st], u & 1, abort_flag, p.status)) { ok = false; break; }
@@ -647,22 +637,27 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
       if (lane == 0) mbar_arrive(&p_full[mine]);
       if (!mbar_wait(&dp_full[mine], ph, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
-      uint32_t d[32];
-      tmem_ld32(dp_addr, d);
-      tc_wait_ld();
+      auto gradients = [&](auto some_hidden) {
+        uint64_t d[16];
+        tmem_ld_pairs(dp_addr, d);
 #pragma unroll
-      for (int e = 0; e < 32; e += 4) {
-        const float4 d4 = vec[KV_QUERIES / 4 + e / 4];
-        const float2 a = unpack2(mul2(f2(x[e], x[e + 1]), add2(f2(d[e], d[e + 1]), f2(d4.x, d4.y))));
-        const float2 c = unpack2(mul2(f2(x[e + 2], x[e + 3]), add2(f2(d[e + 2], d[e + 3]), f2(d4.z, d4.w))));
-        float ds[4] = {a.x, a.y, c.x, c.y};
-        if (masked) {  // a hidden pair adds nothing, whatever dP is
+        for (int e = 0; e < 16; e += 2) {
+          const float4 d4 = vec[KV_QUERIES / 4 + e / 2];
 #pragma unroll
-          for (int g = 0; g < 4; ++g) ds[g] = x[e + g] == 0u ? 0.f : ds[g];
+          for (int g = 0; g < 2; ++g) {
+            const uint64_t ds = mul2(x[e + g], add2(d[e + g], g ? f2(d4.z, d4.w) : f2(d4.x, d4.y)));
+            float2 u = unpack2(ds);
+            if (decltype(some_hidden)::value) {  // a hidden pair adds nothing, whatever dP is
+              const float2 w = unpack2(x[e + g]);
+              u.x = w.x == 0.f ? 0.f : u.x;
+              u.y = w.y == 0.f ? 0.f : u.y;
+            }
+            pk[e + g] = pack_bf16(u.x, u.y);
+          }
         }
-        pk[e / 2] = pack_bf16(ds[0], ds[1]);
-        pk[e / 2 + 1] = pack_bf16(ds[2], ds[3]);
-      }
+      };
+      if (masked) gradients(std::true_type{});
+      else gradients(std::false_type{});
       tmem_st16(dp_addr, pk);
       tc_wait_st();
       tc_fence_before();

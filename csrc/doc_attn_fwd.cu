@@ -207,10 +207,15 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
       if (!mbar_wait(&s_full[i & 1], (i >> 1) & 1, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
       if (!bounded && __any_sync(0xffffffffu, m_next > m) && !move(i, m_next)) { ok = false; break; }
-      uint32_t x[2][32];
-      tmem_ld32(s_addr, x[0]);
-      tmem_ld32(s_addr + 32, x[1]);
-      tc_wait_ld();
+      uint64_t x[2][16];
+      {
+        uint32_t w[2][32];
+        tmem_ld32(s_addr, w[0]);
+        tmem_ld32(s_addr + 32, w[1]);
+        tc_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x[e >> 4][e & 15] = f2(w[e >> 4][2 * (e & 15)], w[e >> 4][2 * (e & 15) + 1]);
+      }
       const bool masked = !(all_lo <= k0 && k0 + FW_KEYS <= all_hi);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -218,26 +223,22 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
           uint64_t unused;
           auto capped = [&](auto near) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const float2 t = unpack2(tanh2<decltype(near)::value, false>(f2(x[c][e], x[c][e + 1]), p.x_scale, unused));
-              x[c][e] = __float_as_uint(t.x);
-              x[c][e + 1] = __float_as_uint(t.y);
-            }
+            for (int e = 0; e < 16; ++e) x[c][e] = tanh2<decltype(near)::value, false>(x[c][e], p.x_scale, unused);
           };
-          if (warp_near<32>(x[c], p.x_scale)) capped(std::true_type{});
+          if (warp_near(x[c], p.x_scale)) capped(std::true_type{});
           else capped(std::false_type{});
         }
         if (ALIBI) {
           const float fd = (float)(qpos - (k0 + c * 32));
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            x[c][e] = __float_as_uint(fmaf(-slope2, fabsf(fd - (float)e), __uint_as_float(x[c][e]) * p.c_log2));
+          for (int e = 0; e < 16; ++e)
+            x[c][e] = fma2(f2(-slope2), f2(fabsf(fd - (float)(2 * e)), fabsf(fd - (float)(2 * e + 1))),
+                           mul2(x[c][e], f2(p.c_log2)));
         }
         if (masked) {
           const uint32_t bits = range_bits(vis.begin, vis.end, k0 + c * 32);
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!((bits >> e) & 1u)) x[c][e] = 0xff800000u;  // -inf
+          for (int e = 0; e < 16; ++e) x[c][e] = select2(x[c][e], bits, 2 * e, -INFINITY);
         }
       }
       uint32_t pk[2][16];
@@ -249,20 +250,21 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const uint64_t pp = ex2_2(fma2(f2(x[c][e], x[c][e + 1]), cc, mref));
-            rs[(e >> 1) & 3] = add2(rs[(e >> 1) & 3], pp);
+          for (int e = 0; e < 16; ++e) {
+            const uint64_t pp = ex2_2(fma2(x[c][e], cc, mref));
+            rs[e & 3] = add2(rs[e & 3], pp);
             const float2 v = unpack2(pp);
-            pk[c][e / 2] = pack_bf16(v.x, v.y);
+            pk[c][e] = pack_bf16(v.x, v.y);
           }
       };
       exponentials();
       if (!bounded) {
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int e = 0; e < 64; e += 2)
-          mx[(e >> 1) & 3] = fmaxf(fmaxf(__uint_as_float(x[e >> 5][e & 31]), __uint_as_float(x[e >> 5][(e & 31) + 1])),
-                                   mx[(e >> 1) & 3]);
+        for (int e = 0; e < 32; ++e) {
+          const float2 v = unpack2(x[e >> 4][e & 15]);
+          mx[e & 3] = fmaxf(fmaxf(v.x, v.y), mx[e & 3]);
+        }
         const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * C;
         if (__any_sync(0xffffffffu, m == -INFINITY ? mt > -INFINITY : mt > m + 60.f)) {
           if (!move(i, fmaxf(mt, m))) { ok = false; break; }

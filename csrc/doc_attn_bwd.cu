@@ -104,10 +104,15 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
     mbar_init(all_done, 1);
     *abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&tmQ);
+    // Q and dO at once: the rest of the start runs under their latency
+    mbar_arrive_expect_tx(q_full, L::Q_BYTES + L::DO_BYTES);
+#pragma unroll
+    for (int kb = 0; kb < L::KBQ; ++kb) tma_load_4d(sQ + kb * L::QBLK, &tmQ, q_full, kb * 64, h, qt * DA_TILE, b);
+#pragma unroll
+    for (int kb = 0; kb < L::KBV; ++kb) tma_load_4d(sDO + kb * L::QBLK, &tmDO, q_full, kb * 64, h, qt * DA_TILE, b);
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
-    tma_prefetch_desc(&tmDO);
+    tma_prefetch_desc(&tmDQ);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
@@ -122,12 +127,7 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
   const uint32_t TM_DQ = tmem, TM_Q = tmem + 128, TM_DO = tmem + 192, TM_S = tmem + 256, TM_DP = tmem + 384;
 
   if (warp == 0) {
-    if (lane == 0 && n > 0) {
-      mbar_arrive_expect_tx(q_full, L::Q_BYTES + L::DO_BYTES);
-#pragma unroll
-      for (int kb = 0; kb < L::KBQ; ++kb) tma_load_4d(sQ + kb * L::QBLK, &tmQ, q_full, kb * 64, h, qt * DA_TILE, b);
-#pragma unroll
-      for (int kb = 0; kb < L::KBV; ++kb) tma_load_4d(sDO + kb * L::QBLK, &tmDO, q_full, kb * 64, h, qt * DA_TILE, b);
+    if (lane == 0) {
       int i = 0;
       for (; i < n; ++i) {
         const int st = i % L::ST;
@@ -151,26 +151,32 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
       constexpr uint32_t ID_S = umma_idesc_bf16(DA_TILE, DQ_KEYS, false, false);
       constexpr uint32_t ID_Q = umma_idesc_bf16(DA_TILE, DQP, false, true);
       const int nkq = (p.Dqk + 15) / 16, nkv = (p.Dv + 15) / 16;
-      // S_i over S_{i-2}, which its group has read; dP_i over dS_{i-2}, read by a product issued before
-      auto issue = [&](int i) -> bool {
+      // over S_{i-2}, which its group has read before it handed dS_{i-2} over
+      auto issue_s = [&](int i) -> bool {
         if (!warp_wait(&kv_full[i % L::ST], (i / L::ST) & 1, abort_flag, p.status)) return false;
         tc_fence_after();
         const DaDesc dK = da_desc(smem_u32(sK + (i % L::ST) * L::K_BYTES), 16);
-        const DaDesc dV = da_desc(smem_u32(sV + (i % L::ST) * L::V_BYTES), 16);
 #pragma unroll
         for (int kk = 0; kk < DQP / 16; ++kk)
           if (kk < nkq)
             da_mma_ts(lead, TM_S + (i & 1) * DQ_KEYS, TM_Q + kk * 8, dK.at((kk >> 2) * L::KBLK + (kk & 3) * 32), ID_S, kk != 0);
         da_commit(lead, &s_full[i & 1]);
+        return true;
+      };
+      // over dS_{i-2}, read by a product issued before
+      auto issue_dp = [&](int i) {
+        const DaDesc dV = da_desc(smem_u32(sV + (i % L::ST) * L::V_BYTES), 16);
 #pragma unroll
         for (int kk = 0; kk < DVP / 16; ++kk)
           if (kk < nkv)
             da_mma_ts(lead, TM_DP + (i & 1) * DQ_KEYS, TM_DO + kk * 8, dV.at((kk >> 2) * L::KBLK + (kk & 3) * 32), ID_S, kk != 0);
         da_commit(lead, &dp_full[i & 1]);
-        return true;
       };
       bool ok = warp_wait(a_full, 0, abort_flag, p.status);
-      for (int i = 0; i < 2 && i < n && ok; ++i) ok = issue(i);
+      for (int i = 0; i < 2 && i < n && ok; ++i) {
+        ok = issue_s(i);
+        if (ok) issue_dp(i);
+      }
       for (int i = 0; i < n && ok; ++i) {
         if (!warp_wait(&ds_full[i & 1], (i >> 1) & 1, abort_flag, p.status)) { ok = false; break; }
         tc_fence_after();
@@ -180,7 +186,10 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
           da_mma_ts(lead, TM_DQ, TM_DP + (i & 1) * DQ_KEYS + (kk >> 1) * 32 + (kk & 1) * 8, dK.at(kk * 2048), ID_Q,
                     (i | kk) != 0);
         da_commit(lead, &kv_empty[i % L::ST]);
-        if (i + 2 < n) ok = issue(i + 2);
+        if (i + 2 < n) {
+          if (!issue_s(i + 2)) { ok = false; break; }
+          issue_dp(i + 2);
+        }
         if (i + 1 == n) da_commit(lead, all_done);
       }
     }
@@ -212,6 +221,15 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
           y[g] = __ldg(reinterpret_cast<const uint4*>(dp + pos * do_in.ss + c));
         }
       }
+      if (!mbar_wait(q_full, 0, abort_flag, p.status)) ok = false;
+      if (ok) {
+        if (mine == 0) rows_to_tmem<DQP>(sQ, TM_Q + lane_base, r, half);
+        else rows_to_tmem<DVP>(sDO, TM_DO + lane_base, r, half);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(a_full);
+      }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const uint32_t xw[4] = {x[g].x, x[g].y, x[g].z, x[g].w}, yw[4] = {y[g].x, y[g].y, y[g].z, y[g].w};
@@ -224,17 +242,6 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if ((lane & 15) == 0) s_row[row0 + 2 * g] = -sum;
-      }
-    }
-    if (n > 0) {
-      if (!mbar_wait(q_full, 0, abort_flag, p.status)) ok = false;
-      if (ok) {
-        if (mine == 0) rows_to_tmem<DQP>(sQ, TM_Q + lane_base, r, half);
-        else rows_to_tmem<DVP>(sDO, TM_DO + lane_base, r, half);
-        tc_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(a_full);
       }
     }
     asm volatile("bar.sync 1, 512;" ::: "memory");  // delta's rows; reached by every softmax warp
@@ -408,10 +415,16 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
     mbar_init(all_done, 1);
     *abort_flag = 0;
     fence_mbar_init();
+    // K and V at once: the rest of the start runs under their latency
+    mbar_arrive_expect_tx(kv_full, L::K_BYTES + L::V_BYTES);
+#pragma unroll
+    for (int kb = 0; kb < L::KBQ; ++kb) tma_load_4d(sK + kb * L::BLK, &tmK, kv_full, kb * 64, hk, kt * DA_TILE, b);
+#pragma unroll
+    for (int kb = 0; kb < L::KBV; ++kb) tma_load_4d(sV + kb * L::BLK, &tmV, kv_full, kb * 64, hk, kt * DA_TILE, b);
     tma_prefetch_desc(&tmQ);
-    tma_prefetch_desc(&tmK);
-    tma_prefetch_desc(&tmV);
     tma_prefetch_desc(&tmDO);
+    tma_prefetch_desc(&tmDK);
+    tma_prefetch_desc(&tmDV);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
@@ -430,16 +443,9 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
   const uint32_t TM_DV = tmem, TM_DK = tmem + 128, TM_S = tmem + 256, TM_DP = tmem + 384;
 
   if (warp == 0) {
+    int it = 0;
     if (n > 0) {
-      if (lane == 0) {
-        mbar_arrive_expect_tx(kv_full, L::K_BYTES + L::V_BYTES);
-#pragma unroll
-        for (int kb = 0; kb < L::KBQ; ++kb) tma_load_4d(sK + kb * L::BLK, &tmK, kv_full, kb * 64, hk, kt * DA_TILE, b);
-#pragma unroll
-        for (int kb = 0; kb < L::KBV; ++kb) tma_load_4d(sV + kb * L::BLK, &tmV, kv_full, kb * 64, hk, kt * DA_TILE, b);
-      }
       int h = hk * group + first / ni, qi = first % ni;
-      int it = 0;
       for (; it < n; ++it) {
         const int st = it % L::ST;
         const int q0 = (qr.begin + qi) * KV_QUERIES;
@@ -474,12 +480,13 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
           ++h;
         }
       }
-      if (lane == 0) {
-        mbar_wait(kv_full, 0, nullptr, p.status);
-        for (int u = max(0, it - L::ST); u < it; ++u) {
-          mbar_wait(&q_full[u % L::ST], (u / L::ST) & 1, nullptr, p.status);
-          mbar_wait(&vec_full[u % L::ST], (u / L::ST) & 1, nullptr, p.status);
-        }
+    }
+    if (lane == 0) {
+      // leave no copy in flight into shared memory
+      mbar_wait(kv_full, 0, nullptr, p.status);
+      for (int u = max(0, it - L::ST); u < it; ++u) {
+        mbar_wait(&q_full[u % L::ST], (u / L::ST) & 1, nullptr, p.status);
+        mbar_wait(&vec_full[u % L::ST], (u / L::ST) & 1, nullptr, p.status);
       }
     }
     __syncwarp();

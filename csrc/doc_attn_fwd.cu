@@ -83,9 +83,13 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
     mbar_init(o_done, 1);
     *abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&tmQ);
+    // Q at once: the rest of the start runs under its latency
+    mbar_arrive_expect_tx(q_full, L::Q_BYTES);
+#pragma unroll
+    for (int kb = 0; kb < L::KBQ; ++kb) tma_load_4d(sQ + kb * L::QBLK, &tmQ, q_full, kb * 64, h, qt * DA_TILE, b);
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
+    tma_prefetch_desc(&tmO);
   }
   if (warp == 1) {
     tmem_alloc(tmem_slot, 256);
@@ -100,10 +104,7 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
   const uint32_t TM_S = tmem, TM_O = tmem + 2 * FW_KEYS;
 
   if (warp == 0) {
-    if (lane == 0 && n > 0) {
-      mbar_arrive_expect_tx(q_full, L::Q_BYTES);
-#pragma unroll
-      for (int kb = 0; kb < L::KBQ; ++kb) tma_load_4d(sQ + kb * L::QBLK, &tmQ, q_full, kb * 64, h, qt * DA_TILE, b);
+    if (lane == 0) {
       int ki = 0, vi = 0;
       for (; ki < n; ++ki) {
         const int st = ki % L::KST;

@@ -49,6 +49,5 @@ void launch_router_fwd(const void* logits, bool bf16, int64_t ld, int64_t T, int
                        const float* bias, int64_t* topi, float* topw, float* usage, int* counts, void* workspace,
                        cudaStream_t st);
 void launch_router_bwd(const void* logits, bool bf16, int64_t ld, int64_t T, int E, const RouteArgs& a,
-                       const int64_t* topi, const float* dtopw, const float* dusage, void* dlogits, int64_t ldd,
-                       cudaStream_t st);
+                       const int64_t* topi, const float* dtopw, const float* dusage, void* dlogits, cudaStream_t st);
 }  // namespace oxi

@@ -4,6 +4,8 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <array>
+
 #include "kernels.h"
 #include "kernels_ew.h"
 #include "kernels_attn.h"
@@ -407,11 +409,35 @@ std::vector<torch::Tensor> document_mask(torch::Tensor tokens, c10::optional<tor
   return {lo, hi, qt, kt};
 }
 
-oxi::DaTensor da_tensor(const torch::Tensor& t, const torch::Tensor& like, const char* what) {
-  OXI_CHECK(t.is_cuda() && t.device() == like.device(), "attention: ", what, " must be on the device of q");
-  OXI_CHECK(t.dim() == 4 && t.scalar_type() == torch::kBFloat16 && t.stride(3) == 1, "attention: ", what,
-              " must be bf16 [B, S, H, D] with unit inner stride");
-  return {t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
+// An operand [B, S, H, D] that tensor maps can address, t itself or a contiguous copy.  The stride of a
+// dimension of one element is never used and need not be a valid one.
+struct DaOperand {
+  torch::Tensor t;
+  oxi::DaTensor d;
+};
+DaOperand da_operand(const torch::Tensor& t, const torch::Tensor& like, const char* what) {
+  OXI_CHECK(t.is_cuda() && t.device() == like.device(), "attention: ", what, " must be on the GPU of q");
+  OXI_CHECK(t.dim() == 4 && t.scalar_type() == torch::kBFloat16, "attention: ", what, " must be bf16 [B, S, H, D]");
+  DaOperand r;
+  r.t = t;
+  bool ok = t.stride(3) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+  for (int i = 0; i < 3 && ok; ++i) ok = t.size(i) == 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0);
+  if (!ok) r.t = t.contiguous();
+  int64_t st[3];
+  for (int i = 0; i < 3; ++i) st[i] = r.t.size(i) == 1 ? 8 : r.t.stride(i);
+  r.d = {r.t.data_ptr(), st[0], st[1], st[2]};
+  return r;
+}
+// q, k, v heads of a fused projection [B, S, (Hq + 2 Hk) D]
+std::array<torch::Tensor, 3> da_heads(const torch::Tensor& qkv, int64_t Hq, int64_t Hk, int64_t D) {
+  OXI_CHECK(qkv.dim() == 3 && Hq > 0 && Hk > 0 && D > 0 && qkv.size(2) == (Hq + 2 * Hk) * D,
+            "attention: qkv must be [B, S, (Hq + 2 Hk) D]");
+  const int64_t e = qkv.stride(2);
+  auto part = [&](int64_t first, int64_t heads) {
+    return qkv.as_strided({qkv.size(0), qkv.size(1), heads, D}, {qkv.stride(0), qkv.stride(1), D * e, e},
+                          qkv.storage_offset() + first * D * e);
+  };
+  return {part(0, Hq), part(Hq, Hk), part(Hq + Hk, Hk)};
 }
 
 oxi::DaShape da_shape(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, double scale, double cap,
@@ -422,14 +448,14 @@ oxi::DaShape da_shape(const torch::Tensor& q, const torch::Tensor& k, const torc
   s.B = (int)q.size(0); s.S = (int)q.size(1); s.Hq = (int)q.size(2); s.Hk = (int)k.size(2);
   s.Dqk = (int)q.size(3); s.Dv = (int)v.size(3);
   OXI_CHECK(k.size(0) == s.B && v.size(0) == s.B && k.size(1) == s.S && v.size(1) == s.S && v.size(2) == s.Hk &&
-                  k.size(3) == s.Dqk, "attention: q, k, v do not go together");
+                k.size(3) == s.Dqk, "attention: q, k, v do not go together");
   OXI_CHECK(s.Hk > 0 && s.Hq % s.Hk == 0, "attention: query heads must be a multiple of key heads");
   s.scale = (float)scale;
   s.cap = (float)cap;
   s.causal = causal;
   if (slopes.has_value() && slopes->defined()) {
     OXI_CHECK(slopes->device() == q.device() && slopes->scalar_type() == torch::kFloat32 && slopes->dim() == 1 &&
-                    slopes->numel() == s.Hq && slopes->is_contiguous(), "attention: alibi must be f32 [Hq] on q's device");
+                  slopes->numel() == s.Hq && slopes->is_contiguous(), "attention: alibi must be f32 [Hq] on q's device");
     s.slopes = slopes->data_ptr<float>();
   }
   if (!mask.empty()) {
@@ -438,8 +464,8 @@ oxi::DaShape da_shape(const torch::Tensor& q, const torch::Tensor& k, const torc
     for (size_t i = 0; i < 4; ++i) {
       const auto& m = mask[i];
       OXI_CHECK(m.device() == q.device() && m.scalar_type() == torch::kInt32 && m.is_contiguous() &&
-                      m.numel() == (i < 2 ? (int64_t)s.B * s.S : (int64_t)s.B * nt * 4),
-                  "attention: the mask was built for another batch or device");
+                    m.numel() == (i < 2 ? (int64_t)s.B * s.S : (int64_t)s.B * nt * 4),
+                "attention: the mask was built for another batch or device");
     }
     s.lo = mask[0].data_ptr<int>(); s.hi = mask[1].data_ptr<int>();
     s.qt = mask[2].data_ptr<int>(); s.kt = mask[3].data_ptr<int>();
@@ -450,44 +476,68 @@ oxi::DaShape da_shape(const torch::Tensor& q, const torch::Tensor& k, const torc
 std::vector<torch::Tensor> doc_attn_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, double scale, double cap,
                                         c10::optional<torch::Tensor> slopes, bool causal,
                                         std::vector<torch::Tensor> mask, torch::Tensor status) {
-  c10::cuda::CUDAGuard g(q.device());
   const oxi::DaShape s = da_shape(q, k, v, scale, cap, slopes, causal, mask);
-  const auto tq = da_tensor(q, q, "q"), tk = da_tensor(k, q, "k"), tv = da_tensor(v, q, "v");
+  const auto tq = da_operand(q, q, "q"), tk = da_operand(k, q, "k"), tv = da_operand(v, q, "v");
+  c10::cuda::CUDAGuard g(q.device());
   auto o = torch::empty({s.B, s.S, s.Hq, s.Dv}, q.options());
   auto nlse2 = torch::empty({s.B, s.Hq, s.S}, q.options().dtype(torch::kFloat32));
-  oxi::launch_da_fwd(s, tq, tk, tv, {o.data_ptr(), (int64_t)s.Hq * s.Dv}, nlse2.data_ptr<float>(), status_ptr(status),
-                     stream());
+  oxi::launch_da_fwd(s, tq.d, tk.d, tv.d, {o.data_ptr(), (int64_t)s.Hq * s.Dv}, nlse2.data_ptr<float>(),
+                     status_ptr(status), stream());
   return {o, nlse2};
 }
+std::vector<torch::Tensor> doc_attn_qkv_fwd(torch::Tensor qkv, int64_t Hq, int64_t Hk, int64_t D, double scale,
+                                            double cap, c10::optional<torch::Tensor> slopes, bool causal,
+                                            std::vector<torch::Tensor> mask, torch::Tensor status) {
+  const auto h = da_heads(qkv, Hq, Hk, D);
+  auto r = doc_attn_fwd(h[0], h[1], h[2], scale, cap, slopes, causal, mask, status);
+  r[0] = r[0].view({qkv.size(0), qkv.size(1), Hq * D});
+  return r;
+}
 
-// dq, dk, dv: bf16 [B * S, H * D] views with unit inner stride (columns of one buffer, say)
-void doc_attn_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o, torch::Tensor dout,
-                  torch::Tensor nlse2, double scale, double cap, c10::optional<torch::Tensor> slopes, bool causal,
-                  std::vector<torch::Tensor> mask, torch::Tensor dq, torch::Tensor dk, torch::Tensor dv,
-                  torch::Tensor status) {
-  c10::cuda::CUDAGuard g(q.device());
+void da_backward(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& o,
+                 const torch::Tensor& dout, const torch::Tensor& nlse2, double scale, double cap,
+                 const c10::optional<torch::Tensor>& slopes, bool causal, const std::vector<torch::Tensor>& mask,
+                 const oxi::DaOut& dq, const oxi::DaOut& dk, const oxi::DaOut& dv, const torch::Tensor& status) {
   const oxi::DaShape s = da_shape(q, k, v, scale, cap, slopes, causal, mask);
-  const auto tq = da_tensor(q, q, "q"), tk = da_tensor(k, q, "k"), tv = da_tensor(v, q, "v"),
-             to = da_tensor(o, q, "o"), td = da_tensor(dout, q, "dout");
+  const auto tq = da_operand(q, q, "q"), tk = da_operand(k, q, "k"), tv = da_operand(v, q, "v"),
+             to = da_operand(o, q, "o"), td = da_operand(dout, q, "the output's gradient");
   OXI_CHECK(o.sizes() == dout.sizes() && o.size(0) == s.B && o.size(1) == s.S && o.size(2) == s.Hq &&
-                  o.size(3) == s.Dv, "attention backward: o and dout must be [B, S, Hq, Dv]");
+                o.size(3) == s.Dv, "attention backward: o and its gradient must be [B, S, Hq, Dv]");
   OXI_CHECK(nlse2.device() == q.device() && nlse2.scalar_type() == torch::kFloat32 && nlse2.is_contiguous() &&
-                  nlse2.numel() == (int64_t)s.B * s.Hq * s.S, "attention backward: nlse2");
-  const int64_t rows = (int64_t)s.B * s.S;
-  const int64_t cols[3] = {(int64_t)s.Hq * s.Dqk, (int64_t)s.Hk * s.Dqk, (int64_t)s.Hk * s.Dv};
-  const torch::Tensor outs[3] = {dq, dk, dv};
-  for (int i = 0; i < 3; ++i)
-    OXI_CHECK(outs[i].device() == q.device() && outs[i].scalar_type() == torch::kBFloat16 && outs[i].dim() == 2 &&
-                  outs[i].size(0) == rows && outs[i].size(1) == cols[i] && outs[i].stride(1) == 1,
-              "attention backward: gradients must be bf16 [B * S, H * D] on q's device");
+                nlse2.numel() == (int64_t)s.B * s.Hq * s.S, "attention backward: nlse2");
   auto ndelta = torch::empty_like(nlse2);
   const int splits = oxi::da_bwd_splits(s.B, s.S, s.Hq, s.Hk);
   torch::Tensor part;
   if (splits > 1) part = torch::empty({splits, (int64_t)s.B * s.Hk * s.S, s.Dqk + s.Dv}, nlse2.options());
-  oxi::launch_da_bwd(s, tq, tk, tv, to, td, nlse2.data_ptr<float>(), ndelta.data_ptr<float>(),
-                     splits > 1 ? part.data_ptr<float>() : nullptr,
-                     {dq.data_ptr(), dq.stride(0)}, {dk.data_ptr(), dk.stride(0)}, {dv.data_ptr(), dv.stride(0)},
-                     status_ptr(status), stream());
+  oxi::launch_da_bwd(s, tq.d, tk.d, tv.d, to.d, td.d, nlse2.data_ptr<float>(), ndelta.data_ptr<float>(),
+                     splits > 1 ? part.data_ptr<float>() : nullptr, dq, dk, dv, status_ptr(status), stream());
+}
+std::vector<torch::Tensor> doc_attn_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o,
+                                        torch::Tensor dout, torch::Tensor nlse2, double scale, double cap,
+                                        c10::optional<torch::Tensor> slopes, bool causal,
+                                        std::vector<torch::Tensor> mask, torch::Tensor status) {
+  OXI_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "attention: q, k, v must be CUDA [B, S, H, D]");
+  c10::cuda::CUDAGuard g(q.device());
+  auto dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), q.options()),
+       dv = torch::empty(v.sizes(), q.options());
+  auto out = [](torch::Tensor& t) { return oxi::DaOut{t.data_ptr(), t.size(2) * t.size(3)}; };
+  da_backward(q, k, v, o, dout, nlse2, scale, cap, slopes, causal, mask, out(dq), out(dk), out(dv), status);
+  return {dq, dk, dv};
+}
+torch::Tensor doc_attn_qkv_bwd(torch::Tensor qkv, int64_t Hq, int64_t Hk, int64_t D, torch::Tensor o,
+                               torch::Tensor dout, torch::Tensor nlse2, double scale, double cap,
+                               c10::optional<torch::Tensor> slopes, bool causal, std::vector<torch::Tensor> mask,
+                               torch::Tensor status) {
+  const auto h = da_heads(qkv, Hq, Hk, D);
+  OXI_CHECK(qkv.is_cuda() && qkv.scalar_type() == torch::kBFloat16 && o.dim() == 3 && dout.sizes() == o.sizes() &&
+                o.size(2) == Hq * D, "attention backward: o and its gradient must be [B, S, Hq D]");
+  c10::cuda::CUDAGuard g(qkv.device());
+  auto dqkv = torch::empty(qkv.sizes(), qkv.options());
+  const int64_t ld = qkv.size(2);
+  auto* base = reinterpret_cast<uint16_t*>(dqkv.data_ptr());
+  da_backward(h[0], h[1], h[2], o.unflatten(2, {Hq, D}), dout.unflatten(2, {Hq, D}), nlse2, scale, cap, slopes, causal,
+              mask, {base, ld}, {base + Hq * D, ld}, {base + (Hq + Hk) * D, ld}, status);
+  return dqkv;
 }
 
 // ------------------------------------------------------------ NVLink DDP runtime
@@ -1251,7 +1301,7 @@ torch::Tensor router_bwd(torch::Tensor logits, torch::Tensor topi, torch::Tensor
   OXI_CHECK(topi.is_contiguous() && topi.scalar_type() == torch::kInt64 && dtopw.is_contiguous() &&
                 dtopw.scalar_type() == torch::kFloat32 && dtopw.numel() == T * k && topi.size(0) == T &&
                 topi.device() == logits.device() && dtopw.device() == logits.device(), "router backward operands");
-  auto dl = torch::empty({T, E}, logits.options());
+  auto dl = torch::empty({T, E}, logits.options());  // contiguous
   const float* du = nullptr;
   if (dusage.has_value() && dusage->defined()) {
     OXI_CHECK(dusage->scalar_type() == torch::kFloat32 && dusage->is_contiguous() && dusage->numel() == E &&
@@ -1260,7 +1310,7 @@ torch::Tensor router_bwd(torch::Tensor logits, torch::Tensor topi, torch::Tensor
   }
   oxi::launch_router_bwd(logits.data_ptr(), logits.scalar_type() == torch::kBFloat16, logits.stride(0), T, (int)E,
                          route_args(k, sigmoid, 1, 1, 1, renorm, scale), topi.data_ptr<int64_t>(),
-                         dtopw.data_ptr<float>(), du, dl.data_ptr(), dl.stride(0), stream());
+                         dtopw.data_ptr<float>(), du, dl.data_ptr(), stream());
   return dl;
 }
 
@@ -1348,6 +1398,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("document_mask", &document_mask, "visible key ranges and tile tables of packed documents");
   m.def("doc_attn_fwd", &doc_attn_fwd, "attention over visible key ranges, forward");
   m.def("doc_attn_bwd", &doc_attn_bwd, "attention over visible key ranges, backward");
+  m.def("doc_attn_qkv_fwd", &doc_attn_qkv_fwd, "the same from a fused projection");
+  m.def("doc_attn_qkv_bwd", &doc_attn_qkv_bwd, "its gradient in the projection's layout");
   m.def("doc_attn_supported", [](int64_t Dqk, int64_t Dv) { return oxi::da_supported((int)Dqk, (int)Dv); });
   m.def("embedding_fwd", &embedding_fwd, "scaled embedding lookup");
   m.def("embedding_bwd", &embedding_bwd, "embedding gradient by sorted tokens");

@@ -15,7 +15,12 @@
 //   ds_j += scale (dw_j - sum_i dw_i s_i / n) / n for the chosen (n = sum of the chosen s; renorm),
 //   ds   += (g - sum_e g_e s_e / S) / S,  then dx = s (ds - sum s ds) or ds s (1 - s).
 //
-// Sums over tokens (usage, counts) are per-CTA partials joined in a fixed order: no atomics.
+// A lane holds EPL neighbouring experts, so that a row is one vector load a lane, a group of
+// neighbours sits in neighbouring lanes (its rank takes log2 of their number shuffles), and the
+// lowest index of equals is the lowest lane of a ballot.  One of the k choices is a maximum over the
+// lane's keys, a warp reduction of integers and a ballot; the instructions of those set the time, not
+// the bytes.
+// Sums over tokens (usage, counts) are per-CTA partials joined in a fixed order: no atomics in f32.
 // Upstream (model.rs:541-556, 604-687): softmax scores, renormalised, no bias and no groups; its
 // balance loss uses mean_t(probs) (model.rs:585-590).
 #include <cuda_bf16.h>
@@ -31,12 +36,10 @@ namespace {
 
 constexpr unsigned FULL = 0xffffffffu;
 
-template <typename T>
-__device__ __forceinline__ float to_f(T v);
-template <>
-__device__ __forceinline__ float to_f<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void from_f(float& d, float v) { d = v; }
+__device__ __forceinline__ void from_f(__nv_bfloat16& d, float v) { d = __float2bfloat16(v); }
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -55,6 +58,7 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   if (v != v) return 1u;
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k); }
 __device__ __forceinline__ uint64_t order_key(double v) {
   const uint64_t u = (uint64_t)__double_as_longlong(v + 0.0);
   if (v != v) return 1u;
@@ -67,29 +71,19 @@ __device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
   return ((uint64_t)hi << 32) | lo;
 }
 
-// The warp's largest key of those with `open` bits set, and its lowest expert (index i * 32 + lane).
+// The warp's largest key, and its lowest expert's place: lane `owner`, element i (of that lane alone).
 template <typename K, int EPL>
-__device__ __forceinline__ int warp_best(const K (&key)[EPL], uint32_t open, K& best) {
-  const int lane = threadIdx.x & 31;
-  K mine = 0;
+__device__ __forceinline__ K warp_best(const K (&key)[EPL], int& owner, int& i_best) {
+  K mine = key[0];
 #pragma unroll
-  for (int i = 0; i < EPL; ++i)
-    if ((open >> i) & 1u) mine = key[i] > mine ? key[i] : mine;
-  best = warp_max_key(mine);
-  uint32_t e = 0xffffffffu;
+  for (int i = 1; i < EPL; ++i) mine = key[i] > mine ? key[i] : mine;
+  const K best = warp_max_key(mine);
+  owner = __ffs(__ballot_sync(FULL, mine == best)) - 1;
+  i_best = 0;
 #pragma unroll
   for (int i = EPL - 1; i >= 0; --i)
-    if (((open >> i) & 1u) && key[i] == best) e = i * 32 + lane;
-  return (int)__reduce_min_sync(FULL, e);
-}
-
-template <typename V, int EPL>
-__device__ __forceinline__ V of_expert(const V (&v)[EPL], int e) {
-  V r = v[0];
-#pragma unroll
-  for (int i = 1; i < EPL; ++i)
-    if ((e >> 5) == i) r = v[i];
-  return __shfl_sync(FULL, r, e & 31);
+    if (key[i] == best) i_best = i;
+  return best;
 }
 
 struct RouteShape {
@@ -97,151 +91,207 @@ struct RouteShape {
   int E, k, groups, top_groups, group_top;
   int sigmoid, renorm;
   float scale;
+  int vec;         // rows can be read EPL elements at a time
+  int lanes;       // lanes of a group where they are a power of two and its one or two best count; else 0
 };
 
-// Experts of the groups that stay, as bits of this lane's elements; b: choice values, key: their
-// order.  `close` is set when a gap on the way is no larger than `margin` times the values.
-template <typename V, typename K, int EPL>
-__device__ __forceinline__ uint32_t choose_groups(const RouteShape& s, const V (&b)[EPL], const K (&key)[EPL],
-                                                  uint32_t valid, V margin, bool& close) {
-  if (s.groups == 1) return valid;
-  const int lane = threadIdx.x & 31, n = s.E / s.groups;
-  V rank = 0;       // lane g holds group g's rank
-  for (int g = 0; g < s.groups; ++g) {
-    uint32_t open = 0;
+// EPL neighbouring logits of a row (those past E: -inf)
+template <typename LT, int EPL>
+__device__ __forceinline__ void load_row(const RouteShape& s, const LT* __restrict__ row, float (&x)[EPL]) {
+  const int e0 = (threadIdx.x & 31) * EPL;
+  if (s.vec) {
+    constexpr int BYTES = EPL * (int)sizeof(LT);
+    if (e0 < s.E) {
+      alignas(16) LT v[EPL];
+      if constexpr (BYTES >= 16) {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if ((i * 32 + lane) / n == g) open |= (1u << i) & valid;
-    V sum = 0;
-    for (int j = 0; j < min(s.group_top, n); ++j) {
-      K best;
-      const int e = warp_best<K, EPL>(key, open, best);
-      sum += of_expert<V, EPL>(b, e);
-      if ((e & 31) == lane) open &= ~(1u << (e >> 5));
+        for (int q = 0; q < BYTES / 16; ++q)
+          reinterpret_cast<uint4*>(v)[q] = __ldg(reinterpret_cast<const uint4*>(row + e0) + q);
+      } else if constexpr (BYTES == 8) {
+        *reinterpret_cast<uint2*>(v) = __ldg(reinterpret_cast<const uint2*>(row + e0));
+      } else if constexpr (BYTES == 4) {
+        *reinterpret_cast<uint32_t*>(v) = __ldg(reinterpret_cast<const uint32_t*>(row + e0));
+      } else {
+        v[0] = row[e0];
+      }
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) x[i] = to_f(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) x[i] = -INFINITY;
     }
-    if (lane == g) rank = sum;
+  } else {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) x[i] = e0 + i < s.E ? to_f(row[e0 + i]) : -INFINITY;
   }
-  const K gk[1] = {lane < s.groups ? order_key(rank) : K(0)};
-  uint32_t left = lane < s.groups;
-  uint32_t taken = 0;
+}
+
+// Scores p of the lane's experts (0 past E) and their sum over the row.
+template <int EPL>
+__device__ __forceinline__ float scores(const RouteShape& s, const float (&x)[EPL], float (&p)[EPL]) {
+  const int e0 = (threadIdx.x & 31) * EPL;
+  float sum = 0.f;
+  if (s.sigmoid) {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      p[i] = e0 + i < s.E ? 1.f / (1.f + expf(-x[i])) : 0.f;
+      sum += p[i];
+    }
+    return warp_sum(sum);
+  }
+  float mx = x[0];
+#pragma unroll
+  for (int i = 1; i < EPL; ++i) mx = fmaxf(mx, x[i]);
+  mx = warp_max(mx);
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    p[i] = e0 + i < s.E ? expf(x[i] - mx) : 0.f;
+    sum += p[i];
+  }
+  const float inv = 1.f / warp_sum(sum);
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) p[i] *= inv;
+  return 1.f;
+}
+
+// Groups of any shape, one after another: v are the values that rank them, in the order of the keys; the
+// experts of those that go lose their keys.  False when the border between the groups is closer than margin.
+template <typename V, typename K, int EPL>
+__device__ __noinline__ bool choose_any_groups(const RouteShape& s, const V (&v)[EPL], K (&key)[EPL], V margin) {
+  const int lane = threadIdx.x & 31, e0 = lane * EPL, n = s.E / s.groups;
+  V rank = 0;  // lane g: group g's
+  for (int g = 0; g < s.groups; ++g) {
+    K open[EPL];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) open[i] = (e0 + i) / n == g ? key[i] : K(0);
+    V r = 0;
+    for (int j = 0; j < min(s.group_top, n); ++j) {
+      int owner, i_best;
+      warp_best<K, EPL>(open, owner, i_best);
+      V u = 0;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i)
+        if (i == i_best) {
+          u = v[i];
+          if (lane == owner) open[i] = K(0);
+        }
+      r += __shfl_sync(FULL, u, owner);
+    }
+    if (lane == g) rank = r;
+  }
+  K gk[1] = {lane < s.groups ? order_key(rank) : K(0)};
+  uint32_t stays = 0;
   V last = 0;
+  bool clear = true;
   for (int j = 0; j <= s.top_groups && j < s.groups; ++j) {
-    K best;
-    const int g = warp_best<K, 1>(gk, left, best);
-    const V r = __shfl_sync(FULL, rank, g);
-    if (j == s.top_groups) {  // the best that goes: is it clearly behind the last that stays?
-      if (!(last - r > margin * (fabs(last) + fabs(r)))) close = true;
+    int owner, unused;
+    warp_best<K, 1>(gk, owner, unused);
+    const V r = __shfl_sync(FULL, rank, owner);
+    if (j == s.top_groups) {
+      clear = last - r > margin * (fabs(last) + fabs(r));
       break;
     }
     last = r;
-    taken |= 1u << g;
-    if (lane == g) left = 0;
+    stays |= 1u << owner;
+    if (lane == owner) gk[0] = K(0);
   }
-  uint32_t open = 0;
 #pragma unroll
   for (int i = 0; i < EPL; ++i)
-    if (((valid >> i) & 1u) && ((taken >> ((i * 32 + lane) / n)) & 1u)) open |= 1u << i;
-  return open;
+    if (e0 + i < s.E && !((stays >> ((e0 + i) / n)) & 1u)) key[i] = K(0);
+  return clear;
 }
 
-// The k best, in order: lane j holds the j-th chosen expert (k <= 32).  close: as above, unless two
-// neighbours in the order have the same logit and bias (they are equal in exact arithmetic too).  The
-// look at who comes behind the k-th goes on past such twins of it.
-template <typename V, typename K, int EPL>
-__device__ __forceinline__ int choose_experts(const RouteShape& s, const V (&b)[EPL], const K (&key)[EPL],
-                                              const float (&x)[EPL], const float (&bias)[EPL], uint32_t open, V margin,
-                                              bool exact, bool& close) {
-  const int lane = threadIdx.x & 31;
-  int mine = 0, prev = 0;
-  V last = 0;
-  for (int j = 0; j < s.k || !exact; ++j) {
-    if (j >= s.k && !__any_sync(FULL, open != 0)) break;
-    K best;
-    const int e = warp_best<K, EPL>(key, open, best);
-    if (!exact) {
-      const V v = of_expert<V, EPL>(b, e);
-      if (j > 0) {
-        const bool clear = last - v > margin * (fabs(last) + fabs(v));
-        const bool twins = !clear && of_expert<float, EPL>(x, e) == of_expert<float, EPL>(x, prev) &&
-                           of_expert<float, EPL>(bias, e) == of_expert<float, EPL>(bias, prev);
-        if (!clear && !twins) {
-          close = true;
-          break;  // the choice is made again in f64
-        }
-        if (j >= s.k && clear) break;
-      }
-      last = v;
-      prev = e;
-    }
-    if (lane == j && j < s.k) mine = e;
-    if ((e & 31) == lane) open &= ~(1u << (e >> 5));
-  }
-  return mine;
-}
-
+// The choice of one token in f64: lane j gets the j-th expert.
 template <typename LT, int EPL>
-__device__ __forceinline__ void load_scores(const RouteShape& s, const LT* __restrict__ row, float (&x)[EPL],
-                                            float (&p)[EPL], float& total) {
-  const int lane = threadIdx.x & 31;
-  float mx = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int e = lane + 32 * i;
-    x[i] = e < s.E ? to_f(row[e]) : -INFINITY;
-    mx = fmaxf(mx, x[i]);
-  }
-  if (s.sigmoid) {
-    mx = 0.f;
-  } else {
-    mx = warp_max(mx);
-  }
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    if (s.sigmoid) p[i] = 1.f / (1.f + expf(-x[i]));
-    else p[i] = expf(x[i] - mx);
-    if (lane + 32 * i >= s.E) p[i] = 0.f;
-    sum += p[i];
-  }
-  total = warp_sum(sum);
-  if (!s.sigmoid) {
-    const float inv = 1.f / total;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) p[i] *= inv;
-    total = 1.f;
-  }
-}
-
-// The choice of one token in f64.
-template <int EPL>
-__device__ __noinline__ int choose_wide(const RouteShape s, const float (&x)[EPL], const float (&bias)[EPL],
-                                        uint32_t valid, bool by_logit) {
+__device__ __noinline__ int choose_wide(const RouteShape s, const LT* __restrict__ row, const float* __restrict__ bias) {
+  const int lane = threadIdx.x & 31, e0 = lane * EPL;
+  float x[EPL];
+  load_row<LT, EPL>(s, row, x);
   double b[EPL];
   uint64_t key[EPL];
-  float mx = -INFINITY;
+  float mx = x[0];
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) mx = fmaxf(mx, x[i]);
+  for (int i = 1; i < EPL; ++i) mx = fmaxf(mx, x[i]);
   mx = warp_max(mx);
   double sum = 0.0;
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
     b[i] = s.sigmoid ? 1.0 / (1.0 + exp(-(double)x[i])) : exp((double)x[i] - (double)mx);
-    sum += ((valid >> i) & 1u) ? b[i] : 0.0;
+    sum += e0 + i < s.E ? b[i] : 0.0;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(FULL, sum, o);
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
     if (!s.sigmoid) b[i] /= sum;
-    b[i] += (double)bias[i];
-    key[i] = order_key(by_logit ? (double)x[i] : b[i]);
+    if (bias && e0 + i < s.E) b[i] += (double)bias[e0 + i];
+    key[i] = e0 + i < s.E ? order_key(bias ? b[i] : (double)x[i]) : 0ull;
   }
-  bool close = false;
-  const uint32_t open = choose_groups<double, uint64_t, EPL>(s, b, key, valid, 0.0, close);
-  return choose_experts<double, uint64_t, EPL>(s, b, key, x, bias, open, 0.0, true, close);
+  if (s.groups > 1) choose_any_groups<double, uint64_t, EPL>(s, b, key, 0.0);
+  int mine = 0;
+  for (int j = 0; j < s.k; ++j) {
+    int owner, i_best;
+    warp_best<uint64_t, EPL>(key, owner, i_best);
+    const int e = __shfl_sync(FULL, e0 + i_best, owner);
+    if (lane == j) mine = e;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (lane == owner && i == i_best) key[i] = 0ull;
+  }
+  return mine;
 }
 
-constexpr int RT_WARPS = 8;
+// Ranks of groups that fill s.lanes lanes each; the experts of those that go lose their keys.  False when
+// the border between the groups is too close for f32.
+template <int EPL>
+__device__ __forceinline__ bool choose_groups(const RouteShape& s, const float (&p)[EPL], const float (&b)[EPL],
+                                              uint32_t (&key)[EPL], bool by_logit, float margin) {
+  const int lane = threadIdx.x & 31;
+  // the two largest of the lane, then of the group's lanes (in the order of the keys)
+  uint32_t k0 = 0u, k1 = 0u;
+  float v0 = 0.f, v1 = 0.f;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    const bool first = key[i] > k0, second = key[i] > k1;
+    k1 = first ? k0 : (second ? key[i] : k1);
+    v1 = first ? v0 : (second ? (by_logit ? p[i] : b[i]) : v1);
+    k0 = first ? key[i] : k0;
+    v0 = first ? (by_logit ? p[i] : b[i]) : v0;
+  }
+  for (int o = 1; o < s.lanes; o <<= 1) {
+    const uint32_t q0 = __shfl_xor_sync(FULL, k0, o), q1 = __shfl_xor_sync(FULL, k1, o);
+    const float u0 = __shfl_xor_sync(FULL, v0, o), u1 = __shfl_xor_sync(FULL, v1, o);
+    const bool mine = k0 >= q0;  // the larger first; the second is the larger of the loser and the winner's second
+    const uint32_t lose = mine ? q0 : k0, next = mine ? k1 : q1;
+    const float lose_v = mine ? u0 : v0, next_v = mine ? v1 : u1;
+    k0 = mine ? k0 : q0;
+    v0 = mine ? v0 : u0;
+    k1 = lose > next ? lose : next;
+    v1 = lose > next ? lose_v : next_v;
+  }
+  const float rank = (s.group_top > 1 && k1 != 0u) ? v0 + v1 : v0;
+  const uint32_t gk = order_key(rank);
+  const int g = lane / s.lanes;
+  int ahead = 0;
+  for (int q = 0; q < s.groups; ++q) {
+    const uint32_t other = __shfl_sync(FULL, gk, q * s.lanes);
+    ahead += other > gk || (other == gk && q < g);
+  }
+  const bool stays = ahead < s.top_groups;
+  if (!stays) {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) key[i] = 0u;
+  }
+  if (s.top_groups == s.groups) return true;
+  // the last that stays against the best that goes (lanes past the experts: none of both)
+  const bool in = g < s.groups;
+  const uint32_t last = __reduce_min_sync(FULL, in && stays ? gk : 0xffffffffu);
+  const uint32_t best = __reduce_max_sync(FULL, in && !stays ? gk : 0u);
+  const float a = key_value(last), c = key_value(best);
+  return a - c > margin * (fabsf(a) + fabsf(c));
+}
+
+constexpr int RT_WARPS = 16;
 
 // part: per CTA [E] f32 sums of the normalised scores, then [E] int32 counts
 template <typename LT, int EPL>
@@ -249,57 +299,106 @@ __global__ void __launch_bounds__(RT_WARPS * 32) router_fwd_kernel(const LT* __r
                                                                    RouteShape s, const float* __restrict__ bias_in,
                                                                    int64_t* __restrict__ topi, float* __restrict__ topw,
                                                                    float* __restrict__ part) {
-  extern __shared__ float rt_smem[];  // [warp][E] usage, then [E] counts
+  extern __shared__ float rt_smem[];  // [warp][E] usage, [E] counts
+  __shared__ int s_e[RT_WARPS][32];
+  __shared__ float s_w[RT_WARPS][32];
   int* s_count = reinterpret_cast<int*>(rt_smem + RT_WARPS * s.E);
   for (int e = threadIdx.x; e < s.E; e += blockDim.x) s_count[e] = 0;
   __syncthreads();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, e0 = lane * EPL;
   const int64_t warps = (int64_t)gridDim.x * RT_WARPS;
   float u_acc[EPL], bias[EPL];
-  uint32_t valid = 0;
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
-    const int e = lane + 32 * i;
     u_acc[i] = 0.f;
-    bias[i] = bias_in && e < s.E ? bias_in[e] : 0.f;
-    if (e < s.E) valid |= 1u << i;
+    bias[i] = bias_in && e0 + i < s.E ? bias_in[e0 + i] : 0.f;
   }
+  const bool by_logit = bias_in == nullptr;
   // how far f32 may be off: a sigmoid's few roundings; a softmax's exponentials and E-term sum
   const float margin = s.sigmoid ? 0x1p-21f : 0x1p-17f;
   for (int64_t t = (int64_t)blockIdx.x * RT_WARPS + warp; t < s.T; t += warps) {
-    float x[EPL], p[EPL], b[EPL], total;
-    load_scores<LT, EPL>(s, logits + t * ld, x, p, total);
+    const LT* row = logits + t * ld;
+    float p[EPL], b[EPL];
     uint32_t key[EPL];
+    load_row<LT, EPL>(s, row, b);
+    const float total = scores<EPL>(s, b, p);
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      b[i] = p[i] + bias[i];
-      key[i] = order_key(bias_in ? b[i] : x[i]);
+      if (!by_logit) b[i] = p[i] + bias[i];
+      key[i] = e0 + i < s.E ? order_key(b[i]) : 0u;
     }
     bool close = false;
-    const uint32_t open = choose_groups<float, uint32_t, EPL>(s, b, key, valid, margin, close);
-    int e = choose_experts<float, uint32_t, EPL>(s, b, key, x, bias, open, margin, bias_in == nullptr, close);
-    if (close) e = choose_wide<EPL>(s, x, bias, valid, bias_in == nullptr);  // the same for every lane
-    // weights of the chosen: lane j's expert lives in lane e & 31
-    float w = 0.f;
+    if (s.groups > 1) {
+      if (s.lanes) {
+        close = !choose_groups<EPL>(s, p, b, key, by_logit, margin);
+      } else {
+        float v[EPL];
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      const float v = __shfl_sync(FULL, p[i], e & 31);
-      if ((e >> 5) == i) w = v;
+        for (int i = 0; i < EPL; ++i) v[i] = by_logit ? p[i] : b[i];
+        close = !choose_any_groups<float, uint32_t, EPL>(s, v, key, margin);
+      }
     }
-    if (lane >= s.k) w = 0.f;
+    // the k best, in order; behind the k-th the look goes on past its twins to see who comes next
+    uint32_t last = 0u;
+    int prev = 0;
+    for (int j = 0; !close && (j < s.k || !by_logit); ++j) {
+      int owner, i_best;
+      const uint32_t best = warp_best<uint32_t, EPL>(key, owner, i_best);
+      if (best == 0u) break;
+      if (!by_logit) {
+        const int e = __shfl_sync(FULL, e0 + i_best, owner);
+        if (j > 0) {
+          const float a = key_value(last), c = key_value(best);
+          const bool clear = a - c > margin * (fabsf(a) + fabsf(c));
+          // twins have the same logit and bias: they are equal in exact arithmetic too
+          if (!clear && !(to_f(row[e]) == to_f(row[prev]) && bias_in[e] == bias_in[prev])) {
+            close = true;
+            break;
+          }
+          if (j >= s.k && clear) break;
+        }
+        last = best;
+        prev = e;
+      }
+      if (lane == owner) {
+#pragma unroll
+        for (int i = 0; i < EPL; ++i)
+          if (i == i_best) {
+            key[i] = 0u;
+            if (j < s.k) {
+              s_e[warp][j] = e0 + i;
+              s_w[warp][j] = p[i];
+            }
+          }
+      }
+    }
+    if (close) {
+      const int e = choose_wide<LT, EPL>(s, row, bias_in);
+      for (int j = 0; j < s.k; ++j) {
+        const int ej = __shfl_sync(FULL, e, j);
+#pragma unroll
+        for (int i = 0; i < EPL; ++i)
+          if (e0 + i == ej) s_w[warp][j] = p[i];
+      }
+      if (lane < s.k) s_e[warp][lane] = e;
+    }
+    __syncwarp();
+    const int e = s_e[warp][lane];
+    float w = lane < s.k ? s_w[warp][lane] : 0.f;
     const float norm = s.renorm ? warp_sum(w) : 1.f;
     if (lane < s.k) {
       topi[t * s.k + lane] = e;
       topw[t * s.k + lane] = norm > 0.f ? w / norm * s.scale : 0.f;
       atomicAdd(&s_count[e], 1);
     }
+    __syncwarp();
     const float inv = total > 0.f ? 1.f / total : 0.f;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) u_acc[i] += p[i] * inv;
   }
 #pragma unroll
   for (int i = 0; i < EPL; ++i)
-    if ((valid >> i) & 1u) rt_smem[warp * s.E + lane + 32 * i] = u_acc[i];
+    if (e0 + i < s.E) rt_smem[warp * s.E + e0 + i] = u_acc[i];
   __syncthreads();
   for (int e = threadIdx.x; e < s.E; e += blockDim.x) {
     float sum = 0.f;
@@ -310,17 +409,20 @@ __global__ void __launch_bounds__(RT_WARPS * 32) router_fwd_kernel(const LT* __r
   }
 }
 
-// usage[e] = sum of the CTAs' partials / T, counts[e] = sum of theirs: 32 experts a CTA, its 8 warps
-// take CTAs in turn and are joined in order.
-__global__ void __launch_bounds__(256) router_join_kernel(const float* __restrict__ part, int blocks, int E, int64_t T,
-                                                          float* __restrict__ usage, int* __restrict__ counts) {
-  __shared__ float su[8][32];
-  __shared__ int sc[8][32];
+// usage[e] = sum of the CTAs' partials / T, counts[e] = sum of theirs: 32 experts a CTA, its warps take
+// CTAs in turn and are joined in order.
+constexpr int RJ_WARPS = 32;
+__global__ void __launch_bounds__(RJ_WARPS * 32) router_join_kernel(const float* __restrict__ part, int blocks, int E,
+                                                                    int64_t T, float* __restrict__ usage,
+                                                                    int* __restrict__ counts) {
+  __shared__ float su[RJ_WARPS][32];
+  __shared__ int sc[RJ_WARPS][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x / 32, e = blockIdx.x * 32 + lane;
   float u = 0.f;
   int c = 0;
   if (e < E) {
-    for (int b = w; b < blocks; b += 8) {
+#pragma unroll 4
+    for (int b = w; b < blocks; b += RJ_WARPS) {
       u += part[(int64_t)b * 2 * E + e];
       c += reinterpret_cast<const int*>(part)[(int64_t)b * 2 * E + E + e];
     }
@@ -330,7 +432,7 @@ __global__ void __launch_bounds__(256) router_join_kernel(const float* __restric
   __syncthreads();
   if (w == 0 && e < E) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) {
+    for (int i = 1; i < RJ_WARPS; ++i) {
       u += su[i][lane];
       c += sc[i][lane];
     }
@@ -344,78 +446,104 @@ __global__ void __launch_bounds__(RT_WARPS * 32) router_bwd_kernel(const LT* __r
                                                                    RouteShape s, const int64_t* __restrict__ topi,
                                                                    const float* __restrict__ dtopw,
                                                                    const float* __restrict__ dusage,
-                                                                   LT* __restrict__ dlogits, int64_t ldd) {
-  const int lane = threadIdx.x & 31;
+                                                                   LT* __restrict__ dlogits) {
+  extern __shared__ float rt_smem[];  // [warp][32 EPL]: gradients of the chosen scores, zero elsewhere
+  const int lane = threadIdx.x & 31, e0 = lane * EPL;
+  float* s_g = rt_smem + (threadIdx.x / 32) * 32 * EPL;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) s_g[e0 + i] = 0.f;
   const int64_t warps = (int64_t)gridDim.x * RT_WARPS;
   const float inv_t = 1.f / (float)s.T;
+  float du[EPL];
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) du[i] = dusage && e0 + i < s.E ? dusage[e0 + i] * inv_t : 0.f;
+  __syncwarp();
   for (int64_t t = (int64_t)blockIdx.x * RT_WARPS + threadIdx.x / 32; t < s.T; t += warps) {
-    float x[EPL], p[EPL], d[EPL], total;
-    load_scores<LT, EPL>(s, logits + t * ld, x, p, total);
+    // lane j: the j-th chosen expert and its weight's gradient
+    const int e = lane < s.k ? (int)topi[t * s.k + lane] : 0;
+    float g = lane < s.k ? dtopw[t * s.k + lane] * s.scale : 0.f;
+    float p[EPL], d[EPL];
+    load_row<LT, EPL>(s, logits + t * ld, d);
+    const float total = scores<EPL>(s, d, p);
     const float inv = total > 0.f ? 1.f / total : 0.f;
     float gs = 0.f;
+    if (dusage) {
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      const int e = lane + 32 * i;
-      d[i] = (dusage && e < s.E) ? dusage[e] * inv_t : 0.f;
-      gs += d[i] * p[i];
+      for (int i = 0; i < EPL; ++i) gs += du[i] * p[i];
+      gs = warp_sum(gs) * inv;
     }
-    gs = warp_sum(gs) * inv;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) d[i] = dusage ? (d[i] - gs) * inv : 0.f;
-    // lane j: the j-th chosen expert, its score and its weight's gradient
-    const int e = lane < s.k ? (int)topi[t * s.k + lane] : 0;
-    float w = 0.f;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      const float v = __shfl_sync(FULL, p[i], e & 31);
-      if ((e >> 5) == i) w = v;
-    }
-    float g = lane < s.k ? dtopw[t * s.k + lane] * s.scale : 0.f;
-    if (lane >= s.k) w = 0.f;
     if (s.renorm) {
+      // the chosen scores go the other way through the same words: to the lanes that hold the gradients
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) s_g[e0 + i] = p[i];
+      __syncwarp();
+      const float w = lane < s.k ? s_g[e] : 0.f;
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) s_g[e0 + i] = 0.f;
       const float n = warp_sum(w), gw = warp_sum(g * w);
       g = n > 0.f ? (g - gw / n) / n : 0.f;
+      __syncwarp();
     }
-    for (int j = 0; j < s.k; ++j) {
-      const int ej = __shfl_sync(FULL, e, j);
-      const float gj = __shfl_sync(FULL, g, j);
-      if ((ej & 31) == lane) {
-#pragma unroll
-        for (int i = 0; i < EPL; ++i)
-          if (i == (ej >> 5)) d[i] += gj;
-      }
-    }
+    if (lane < s.k) s_g[e] = g;
+    __syncwarp();
     float sd = 0.f;
-    if (!s.sigmoid) {
-#pragma unroll
-      for (int i = 0; i < EPL; ++i) sd += p[i] * d[i];
-      sd = warp_sum(sd);
-    }
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      const int q = lane + 32 * i;
-      if (q < s.E) {
-        const float dx = s.sigmoid ? d[i] * p[i] * (1.f - p[i]) : p[i] * (d[i] - sd);
-        if constexpr (sizeof(LT) == 4) dlogits[t * ldd + q] = dx;
-        else dlogits[t * ldd + q] = __float2bfloat16(dx);
-      }
+      d[i] = (dusage ? (du[i] - gs) * inv : 0.f) + s_g[e0 + i];
+      sd += p[i] * d[i];
     }
+    __syncwarp();
+    if (lane < s.k) s_g[e] = 0.f;
+    if (!s.sigmoid) sd = warp_sum(sd);
+    alignas(16) LT out[EPL];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) from_f(out[i], s.sigmoid ? d[i] * p[i] * (1.f - p[i]) : p[i] * (d[i] - sd));
+    LT* dst = dlogits + t * s.E + e0;  // contiguous rows
+    constexpr int BYTES = EPL * (int)sizeof(LT);
+    if (s.E % EPL == 0 && BYTES >= 4) {
+      if (e0 < s.E) {
+        if constexpr (BYTES >= 16) {
+#pragma unroll
+          for (int q = 0; q < BYTES / 16; ++q) reinterpret_cast<uint4*>(dst)[q] = reinterpret_cast<const uint4*>(out)[q];
+        } else if constexpr (BYTES == 8) {
+          *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(out);
+        } else if constexpr (BYTES == 4) {
+          *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(out);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i)
+        if (e0 + i < s.E) dst[i] = out[i];
+    }
+    __syncwarp();
   }
 }
 
 int route_grid(int64_t T) {
   const int64_t blocks = (T + RT_WARPS - 1) / RT_WARPS;
-  return (int)(blocks < 148 * 4 ? (blocks > 0 ? blocks : 1) : 148 * 4);
+  return (int)(blocks < 148 * 2 ? (blocks > 0 ? blocks : 1) : 148 * 2);
 }
 
-RouteShape route_shape(const RouteArgs& a, int64_t T, int E) {
+int route_epl(int E) {
+  int epl = 1;
+  while (epl * 32 < E) epl *= 2;
+  return epl;
+}
+
+RouteShape route_shape(const RouteArgs& a, const void* logits, int64_t ld, int elem, int64_t T, int E) {
   OXI_CHECK(E >= 1 && E <= ROUTE_MAX_EXPERTS && a.k >= 1 && a.k <= ROUTE_MAX_K, "routing: at most ", ROUTE_MAX_EXPERTS,
             " experts and k of at most ", ROUTE_MAX_K);
   OXI_CHECK(a.groups >= 1 && a.groups <= ROUTE_MAX_GROUPS && E % a.groups == 0 && a.top_groups >= 1 &&
                 a.top_groups <= a.groups && a.group_top >= 1, "routing: at most ", ROUTE_MAX_GROUPS,
             " groups of equal size, of which at least one stays");
   OXI_CHECK(a.k <= a.top_groups * (E / a.groups), "routing: k is larger than the experts that stay");
-  return {T, E, a.k, a.groups, a.top_groups, a.group_top, a.sigmoid, a.renorm, a.scale};
+  const int epl = route_epl(E), bytes = epl * elem, unit = bytes < 16 ? bytes : 16;
+  const int vec = E % epl == 0 && (reinterpret_cast<uintptr_t>(logits) % unit) == 0 && (ld * elem) % unit == 0;
+  const int n = E / a.groups, lanes = n % epl == 0 ? n / epl : 0;
+  const bool fast = lanes > 0 && (lanes & (lanes - 1)) == 0 && a.group_top <= 2;
+  return {T, E, a.k, a.groups, a.top_groups, a.group_top, a.sigmoid, a.renorm, a.scale, vec, fast ? lanes : 0};
 }
 
 }  // namespace
@@ -423,14 +551,14 @@ RouteShape route_shape(const RouteArgs& a, int64_t T, int E) {
 int64_t route_workspace(int64_t T, int E) { return (int64_t)route_grid(T) * 2 * E * 4; }
 
 #define OXI_ROUTE_EPL(F) \
-  if (E <= 32) { F(1); } else if (E <= 64) { F(2); } else if (E <= 128) { F(4); } else if (E <= 256) { F(8); } else { F(16); }
+  switch (route_epl(E)) { case 1: F(1); break; case 2: F(2); break; case 4: F(4); break; case 8: F(8); break; default: F(16); }
 
 void launch_router_fwd(const void* logits, bool bf16, int64_t ld, int64_t T, int E, const RouteArgs& a,
                        const float* bias, int64_t* topi, float* topw, float* usage, int* counts, void* workspace,
                        cudaStream_t st) {
-  const RouteShape s = route_shape(a, T, E);
+  const RouteShape s = route_shape(a, logits, ld, bf16 ? 2 : 4, T, E);
   float* part = reinterpret_cast<float*>(workspace);
-  const int grid = route_grid(T), smem = (RT_WARPS + 1) * E * 4;
+  const int grid = route_grid(T), smem = (RT_WARPS + 1) * E * 4;  // at most 35 KB
 #define OXI_RF(N)                                                                                                    \
   if (bf16)                                                                                                         \
     router_fwd_kernel<__nv_bfloat16, N><<<grid, RT_WARPS * 32, smem, st>>>(                                         \
@@ -441,24 +569,23 @@ void launch_router_fwd(const void* logits, bool bf16, int64_t ld, int64_t T, int
   OXI_ROUTE_EPL(OXI_RF)
 #undef OXI_RF
   OXI_CUDA_CHECK(cudaGetLastError());
-  router_join_kernel<<<(E + 31) / 32, 256, 0, st>>>(part, grid, E, T, usage, counts);
+  router_join_kernel<<<(E + 31) / 32, RJ_WARPS * 32, 0, st>>>(part, grid, E, T, usage, counts);
   OXI_CUDA_CHECK(cudaGetLastError());
 }
 
 void launch_router_bwd(const void* logits, bool bf16, int64_t ld, int64_t T, int E, const RouteArgs& a,
-                       const int64_t* topi, const float* dtopw, const float* dusage, void* dlogits, int64_t ldd,
-                       cudaStream_t st) {
-  const RouteShape s = route_shape(a, T, E);
+                       const int64_t* topi, const float* dtopw, const float* dusage, void* dlogits, cudaStream_t st) {
+  const RouteShape s = route_shape(a, logits, ld, bf16 ? 2 : 4, T, E);
   if (T == 0) return;
-  const int grid = route_grid(T);
+  const int grid = route_grid(T), smem = RT_WARPS * 32 * route_epl(E) * 4;  // at most 32 KB
 #define OXI_RB(N)                                                                                                    \
   if (bf16)                                                                                                         \
-    router_bwd_kernel<__nv_bfloat16, N><<<grid, RT_WARPS * 32, 0, st>>>(                                            \
+    router_bwd_kernel<__nv_bfloat16, N><<<grid, RT_WARPS * 32, smem, st>>>(                                         \
         reinterpret_cast<const __nv_bfloat16*>(logits), ld, s, topi, dtopw, dusage,                                 \
-        reinterpret_cast<__nv_bfloat16*>(dlogits), ldd);                                                            \
+        reinterpret_cast<__nv_bfloat16*>(dlogits));                                                                 \
   else                                                                                                              \
-    router_bwd_kernel<float, N><<<grid, RT_WARPS * 32, 0, st>>>(reinterpret_cast<const float*>(logits), ld, s, topi, \
-                                                                dtopw, dusage, reinterpret_cast<float*>(dlogits), ldd)
+    router_bwd_kernel<float, N><<<grid, RT_WARPS * 32, smem, st>>>(reinterpret_cast<const float*>(logits), ld, s,    \
+                                                                   topi, dtopw, dusage, reinterpret_cast<float*>(dlogits))
   OXI_ROUTE_EPL(OXI_RB)
 #undef OXI_RB
   OXI_CUDA_CHECK(cudaGetLastError());

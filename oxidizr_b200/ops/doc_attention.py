@@ -21,6 +21,7 @@ from typing import Optional
 import torch
 
 from . import reference as R
+from ._C import ext, status
 
 MAX_SEQ = 1 << 18  # DOC_MAX_SEQ of csrc/kernels_doc.h: the bit masks of a row stay in shared memory
 
@@ -58,7 +59,6 @@ def document_mask(tokens: torch.Tensor, separator: Optional[int] = None, pad: Op
     if tokens.is_cuda:
         if tokens.shape[1] > MAX_SEQ:
             raise ValueError(f"document_mask: rows of at most {MAX_SEQ} tokens, got {tokens.shape[1]}")
-        from ._C import ext
         if tokens.stride(1) != 1:
             tokens = tokens.contiguous()
         if prefix is not None and prefix.stride(1) != 1:
@@ -69,46 +69,30 @@ def document_mask(tokens: torch.Tensor, separator: Optional[int] = None, pad: Op
     return DocMask(lo, hi, None, None, causal)
 
 
-def _kernel_ok(q, k, v) -> bool:
-    if not (q.is_cuda and q.dtype == torch.bfloat16 and k.dtype == q.dtype and v.dtype == q.dtype):
-        return False
-    from ._C import ext
-    return ext().doc_attn_supported(q.shape[-1], v.shape[-1])
+MAX_HEAD = 128  # csrc/doc_attn_fwd.cu: head widths are multiples of 8 up to this
 
 
-def _check(q, k, v, scale, causal, mask, softcap, alibi):
-    B, S, Hq, D = q.shape
-    Hk = k.shape[2]
-    if k.shape != (B, S, Hk, D) or v.shape[:3] != (B, S, Hk) or Hk == 0 or Hq % Hk:
-        raise ValueError(f"attention: q {list(q.shape)}, k {list(k.shape)}, v {list(v.shape)} do not go together")
+def _kernel_ok(t, Dqk: int, Dv: int) -> bool:
+    return (t.is_cuda and t.dtype == torch.bfloat16 and Dqk <= MAX_HEAD and Dv <= MAX_HEAD and Dqk % 8 == 0
+            and Dv % 8 == 0)
+
+
+def _check(t, B, S, Hq, scale, causal, mask, softcap, alibi):
     if not scale > 0:
         raise ValueError(f"attention: scale must be positive, got {scale}")
     if not 0 <= softcap < float("inf"):
         raise ValueError(f"attention: softcap must be a positive number, or 0 for none, got {softcap}")
     if mask is not None:
-        if mask.lo.shape != (B, S) or mask.lo.device != q.device:
+        if mask.lo.shape != (B, S) or mask.lo.device != t.device:
             raise ValueError(f"attention: the mask is for {list(mask.lo.shape)} on {mask.lo.device}, "
-                             f"q for {[B, S]} on {q.device}")
+                             f"q for {[B, S]} on {t.device}")
         if mask.causal != causal:
             raise ValueError(f"attention: causal={causal} with a mask built for causal={mask.causal}")
     if alibi is not None:
-        if alibi.shape != (Hq,) or alibi.device != q.device:
-            raise ValueError(f"attention: alibi must be one slope per query head [{Hq}] on {q.device}")
+        if alibi.shape != (Hq,) or alibi.device != t.device:
+            raise ValueError(f"attention: alibi must be one slope per query head [{Hq}] on {t.device}")
         if alibi.requires_grad:
             raise ValueError("attention: alibi slopes are constants, no gradient is computed for them")
-
-
-def _tma_view(t: torch.Tensor) -> torch.Tensor:
-    """t itself where the tensor maps can address it, else a contiguous copy.  The stride of a
-    dimension of one element is never used, and is replaced where it would not be a valid one."""
-    B, S, H, D = t.shape
-    st = list(t.stride())
-    for d in (0, 1, 2):
-        if t.shape[d] == 1:
-            st[d] = D
-    if st[3] == 1 and t.data_ptr() % 16 == 0 and all(s > 0 and s % 8 == 0 for s in st[:3]):
-        return t.as_strided(t.shape, st)
-    return t.contiguous()
 
 
 class DocAttention(torch.autograd.Function):
@@ -116,7 +100,7 @@ class DocAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, scale: float, cap: float, slopes, causal: bool, mask):
-        o, nlse2 = _fwd(q, k, v, scale, cap, slopes, causal, mask)
+        o, nlse2 = ext().doc_attn_fwd(q, k, v, scale, cap, slopes, causal, mask, status(q.device))
         ctx.save_for_backward(q, k, v, o, nlse2, slopes, *mask)
         ctx.cfg = (scale, cap, causal)
         return o
@@ -124,9 +108,9 @@ class DocAttention(torch.autograd.Function):
     @staticmethod
     def backward(ctx, do):
         q, k, v, o, nlse2, slopes, *mask = ctx.saved_tensors
-        outs = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
-        _bwd(ctx, q, k, v, o, do, nlse2, slopes, mask, [t.flatten(0, 1).flatten(1) for t in outs])
-        return (*outs, None, None, None, None, None)
+        scale, cap, causal = ctx.cfg
+        dq, dk, dv = ext().doc_attn_bwd(q, k, v, o, do, nlse2, scale, cap, slopes, causal, mask, status(q.device))
+        return dq, dk, dv, None, None, None, None, None
 
 
 class DocAttentionQKV(torch.autograd.Function):
@@ -135,39 +119,18 @@ class DocAttentionQKV(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, qkv, Hq: int, Hk: int, D: int, scale: float, cap: float, slopes, causal: bool, mask):
-        q, k, v = _heads(qkv, Hq, Hk, D)
-        o, nlse2 = _fwd(q, k, v, scale, cap, slopes, causal, mask)
+        o, nlse2 = ext().doc_attn_qkv_fwd(qkv, Hq, Hk, D, scale, cap, slopes, causal, mask, status(qkv.device))
         ctx.save_for_backward(qkv, o, nlse2, slopes, *mask)
-        ctx.cfg, ctx.heads = (scale, cap, causal), (Hq, Hk, D)
-        return o.flatten(2)
+        ctx.cfg = (Hq, Hk, D, scale, cap, causal)
+        return o
 
     @staticmethod
     def backward(ctx, do):
         qkv, o, nlse2, slopes, *mask = ctx.saved_tensors
-        Hq, Hk, D = ctx.heads
-        q, k, v = _heads(qkv, Hq, Hk, D)
-        dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        d2 = dqkv.flatten(0, 1)
-        a, b = Hq * D, (Hq + Hk) * D
-        _bwd(ctx, q, k, v, o, do.reshape(o.shape), nlse2, slopes, mask, [d2[:, :a], d2[:, a:b], d2[:, b:]])
-        return (dqkv, *[None] * 8)
-
-
-def _heads(qkv, Hq, Hk, D):
-    return (t.unflatten(-1, (-1, D)) for t in qkv.split([Hq * D, Hk * D, Hk * D], -1))
-
-
-def _fwd(q, k, v, scale, cap, slopes, causal, mask):
-    from ._C import ext, status
-    return ext().doc_attn_fwd(_tma_view(q), _tma_view(k), _tma_view(v), scale, cap, slopes, causal, list(mask),
-                              status(q.device))
-
-
-def _bwd(ctx, q, k, v, o, do, nlse2, slopes, mask, outs):
-    from ._C import ext, status
-    scale, cap, causal = ctx.cfg
-    ext().doc_attn_bwd(_tma_view(q), _tma_view(k), _tma_view(v), o, _tma_view(do), nlse2, scale, cap, slopes, causal,
-                       list(mask), *outs, status(q.device))
+        Hq, Hk, D, scale, cap, causal = ctx.cfg
+        dqkv = ext().doc_attn_qkv_bwd(qkv, Hq, Hk, D, o, do, nlse2, scale, cap, slopes, causal, mask,
+                                      status(qkv.device))
+        return dqkv, None, None, None, None, None, None, None, None
 
 
 def _reference(q, k, v, scale, causal, mask, softcap, alibi):
@@ -176,24 +139,31 @@ def _reference(q, k, v, scale, causal, mask, softcap, alibi):
     return o.transpose(1, 2)
 
 
-def _slopes(alibi):
-    return None if alibi is None else alibi.float().contiguous()
+def _options(alibi, mask):
+    return (None if alibi is None else alibi.float().contiguous()), (mask.tensors() if mask is not None else [])
 
 
 def attention(q, k, v, scale: float, causal: bool = True, mask: Optional[DocMask] = None, softcap: float = 0.0,
               alibi: Optional[torch.Tensor] = None) -> torch.Tensor:
-    _check(q, k, v, scale, causal, mask, softcap, alibi)
-    if _kernel_ok(q, k, v):
-        m = mask.tensors() if mask is not None else []
-        return DocAttention.apply(q, k, v, float(scale), float(softcap), _slopes(alibi), causal, m)
+    B, S, Hq, D = q.shape
+    Hk = k.shape[2]
+    if k.shape != (B, S, Hk, D) or v.shape[:3] != (B, S, Hk) or Hk == 0 or Hq % Hk:
+        raise ValueError(f"attention: q {list(q.shape)}, k {list(k.shape)}, v {list(v.shape)} do not go together")
+    _check(q, B, S, Hq, scale, causal, mask, softcap, alibi)
+    if _kernel_ok(q, D, v.shape[3]) and k.dtype == q.dtype and v.dtype == q.dtype:
+        slopes, m = _options(alibi, mask)
+        return DocAttention.apply(q, k, v, float(scale), float(softcap), slopes, causal, m)
     return _reference(q, k, v, scale, causal, mask, softcap, alibi)
 
 
 def attention_qkv(qkv, Hq: int, Hk: int, D: int, scale: float, causal: bool = True, mask: Optional[DocMask] = None,
                   softcap: float = 0.0, alibi: Optional[torch.Tensor] = None) -> torch.Tensor:
-    q, k, v = _heads(qkv, Hq, Hk, D)
-    _check(q, k, v, scale, causal, mask, softcap, alibi)
-    if _kernel_ok(q, k, v):
-        m = mask.tensors() if mask is not None else []
-        return DocAttentionQKV.apply(qkv, Hq, Hk, D, float(scale), float(softcap), _slopes(alibi), causal, m)
+    B, S, N = qkv.shape
+    if Hk < 1 or Hq < 1 or Hq % Hk or N != (Hq + 2 * Hk) * D:
+        raise ValueError(f"attention: qkv {list(qkv.shape)} does not hold {Hq} query and {Hk} key and value heads of {D}")
+    _check(qkv, B, S, Hq, scale, causal, mask, softcap, alibi)
+    if _kernel_ok(qkv, D, D):
+        slopes, m = _options(alibi, mask)
+        return DocAttentionQKV.apply(qkv, Hq, Hk, D, float(scale), float(softcap), slopes, causal, m)
+    q, k, v = (t.unflatten(-1, (-1, D)) for t in qkv.split([Hq * D, Hk * D, Hk * D], -1))
     return _reference(q, k, v, scale, causal, mask, softcap, alibi).flatten(2)

@@ -8,8 +8,9 @@
 //   usage  = mean over the tokens of s / sum s;  counts: how often each expert was chosen
 //
 // Without a bias the order of b is that of x, which is exact.  With one, b in f32 may order two
-// experts that are a rounding apart wrongly, so a token with a gap on the path of the choice that
-// f32 cannot vouch for is chosen again in f64 (a few tokens in a thousand).
+// experts that are a rounding apart wrongly: where f32 cannot tell which is the largest, the
+// candidates are compared in f64 (a few tokens in a thousand; a token chosen wholly in f64 took 25 us,
+// which the kernel's end had to wait for).  The same for the last group that stays.
 //
 // Backward, per token (g = d_usage / T, S = sum s):
 //   ds_j += scale (dw_j - sum_i dw_i s_i / n) / n for the chosen (n = sum of the chosen s; renorm),
@@ -52,17 +53,27 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// Unsigned keys in the order of the values; -0 is 0, NaN lies below everything, 0 is "none".
+// e^x on the special-function unit: off by |x| 2^-24 and 2^-22 of itself, a seventh of expf's instructions.
+__device__ __forceinline__ float exp_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.4426950408889634f));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Unsigned keys in the order of the values, never 0 ("none"); -0 is 0, NaN counts as -inf.
 __device__ __forceinline__ uint32_t order_key(float v) {
-  const uint32_t u = __float_as_uint(v + 0.f);
-  if (v != v) return 1u;
-  return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+  const uint32_t u = __float_as_uint(fmaxf(v, -INFINITY) + 0.f);
+  return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float((k >> 31) ? k & 0x7fffffffu : ~k); }
 __device__ __forceinline__ uint64_t order_key(double v) {
-  const uint64_t u = (uint64_t)__double_as_longlong(v + 0.0);
-  if (v != v) return 1u;
-  return (u >> 63) ? ~u : u | 0x8000000000000000ull;
+  const uint64_t u = (uint64_t)__double_as_longlong(fmax(v, -(double)INFINITY) + 0.0);
+  return u ^ ((uint64_t)((int64_t)u >> 63) | 0x8000000000000000ull);
 }
 __device__ __forceinline__ uint32_t warp_max_key(uint32_t k) { return __reduce_max_sync(FULL, k); }
 __device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
@@ -134,7 +145,7 @@ __device__ __forceinline__ float scores(const RouteShape& s, const float (&x)[EP
   if (s.sigmoid) {
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      p[i] = e0 + i < s.E ? 1.f / (1.f + expf(-x[i])) : 0.f;
+      p[i] = e0 + i < s.E ? rcp_approx(1.f + exp_approx(-x[i])) : 0.f;
       sum += p[i];
     }
     return warp_sum(sum);
@@ -145,7 +156,7 @@ __device__ __forceinline__ float scores(const RouteShape& s, const float (&x)[EP
   mx = warp_max(mx);
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
-    p[i] = e0 + i < s.E ? expf(x[i] - mx) : 0.f;
+    p[i] = e0 + i < s.E ? exp_approx(x[i] - mx) : 0.f;
     sum += p[i];
   }
   const float inv = 1.f / warp_sum(sum);
@@ -154,10 +165,11 @@ __device__ __forceinline__ float scores(const RouteShape& s, const float (&x)[EP
   return 1.f;
 }
 
-// Groups of any shape, one after another: v are the values that rank them, in the order of the keys; the
-// experts of those that go lose their keys.  False when the border between the groups is closer than margin.
+// Groups of any shape, one after another: v are the values that rank them, in the order of the keys.
+// stays: bits of the groups that stay.  False when the border between the groups is closer than margin.
 template <typename V, typename K, int EPL>
-__device__ __noinline__ bool choose_any_groups(const RouteShape& s, const V (&v)[EPL], K (&key)[EPL], V margin) {
+__device__ __forceinline__ bool choose_any_groups(const RouteShape& s, const V (&v)[EPL], const K (&key)[EPL], V margin,
+                                               uint32_t& stays) {
   const int lane = threadIdx.x & 31, e0 = lane * EPL, n = s.E / s.groups;
   V rank = 0;  // lane g: group g's
   for (int g = 0; g < s.groups; ++g) {
@@ -180,35 +192,25 @@ __device__ __noinline__ bool choose_any_groups(const RouteShape& s, const V (&v)
     if (lane == g) rank = r;
   }
   K gk[1] = {lane < s.groups ? order_key(rank) : K(0)};
-  uint32_t stays = 0;
+  stays = 0;
   V last = 0;
-  bool clear = true;
-  for (int j = 0; j <= s.top_groups && j < s.groups; ++j) {
+  for (int j = 0; j < s.groups; ++j) {
     int owner, unused;
     warp_best<K, 1>(gk, owner, unused);
     const V r = __shfl_sync(FULL, rank, owner);
-    if (j == s.top_groups) {
-      clear = last - r > margin * (fabs(last) + fabs(r));
-      break;
-    }
+    if (j == s.top_groups) return last - r > margin;
     last = r;
     stays |= 1u << owner;
     if (lane == owner) gk[0] = K(0);
   }
-#pragma unroll
-  for (int i = 0; i < EPL; ++i)
-    if (e0 + i < s.E && !((stays >> ((e0 + i) / n)) & 1u)) key[i] = K(0);
-  return clear;
+  return true;
 }
 
-// The choice of one token in f64: lane j gets the j-th expert.
+// The lane's choice values in f64.
 template <typename LT, int EPL>
-__device__ __noinline__ int choose_wide(const RouteShape s, const LT* __restrict__ row, const float* __restrict__ bias) {
-  const int lane = threadIdx.x & 31, e0 = lane * EPL;
-  float x[EPL];
-  load_row<LT, EPL>(s, row, x);
-  double b[EPL];
-  uint64_t key[EPL];
+__device__ __forceinline__ void exact_values(const RouteShape& s, const float (&x)[EPL], const float* __restrict__ bias,
+                                             double (&b)[EPL]) {
+  const int e0 = (threadIdx.x & 31) * EPL;
   float mx = x[0];
 #pragma unroll
   for (int i = 1; i < EPL; ++i) mx = fmaxf(mx, x[i]);
@@ -225,39 +227,89 @@ __device__ __noinline__ int choose_wide(const RouteShape s, const LT* __restrict
   for (int i = 0; i < EPL; ++i) {
     if (!s.sigmoid) b[i] /= sum;
     if (bias && e0 + i < s.E) b[i] += (double)bias[e0 + i];
-    key[i] = e0 + i < s.E ? order_key(bias ? b[i] : (double)x[i]) : 0ull;
   }
-  if (s.groups > 1) choose_any_groups<double, uint64_t, EPL>(s, b, key, 0.0);
-  int mine = 0;
-  for (int j = 0; j < s.k; ++j) {
-    int owner, i_best;
-    warp_best<uint64_t, EPL>(key, owner, i_best);
-    const int e = __shfl_sync(FULL, e0 + i_best, owner);
-    if (lane == j) mine = e;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (lane == owner && i == i_best) key[i] = 0ull;
-  }
-  return mine;
 }
 
-// Ranks of groups that fill s.lanes lanes each; the experts of those that go lose their keys.  False when
-// the border between the groups is too close for f32.
-template <int EPL>
-__device__ __forceinline__ bool choose_groups(const RouteShape& s, const float (&p)[EPL], const float (&b)[EPL],
-                                              uint32_t (&key)[EPL], bool by_logit, float margin) {
-  const int lane = threadIdx.x & 31;
-  // the two largest of the lane, then of the group's lanes (in the order of the keys)
-  uint32_t k0 = 0u, k1 = 0u;
-  float v0 = 0.f, v1 = 0.f;
+// The groups that stay, decided in f64.
+template <typename LT, int EPL>
+__device__ __noinline__ uint32_t exact_groups(const RouteShape s, const LT* __restrict__ row, const float* __restrict__ bias) {
+  const int e0 = (threadIdx.x & 31) * EPL;
+  float x[EPL];
+  double b[EPL];
+  uint64_t key[EPL];
+  load_row<LT, EPL>(s, row, x);
+  exact_values<LT, EPL>(s, x, bias, b);
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const bool first = key[i] > k0, second = key[i] > k1;
-    k1 = first ? k0 : (second ? key[i] : k1);
-    v1 = first ? v0 : (second ? (by_logit ? p[i] : b[i]) : v1);
-    k0 = first ? key[i] : k0;
-    v0 = first ? (by_logit ? p[i] : b[i]) : v0;
+  for (int i = 0; i < EPL; ++i) key[i] = e0 + i < s.E ? order_key(bias ? b[i] : (double)x[i]) : 0ull;
+  uint32_t stays;
+  choose_any_groups<double, uint64_t, EPL>(s, b, key, 0.0, stays);
+  return stays;
+}
+
+// The largest of the experts with keys from thr on, decided in f64; (owner, i_best) come in as f32 found it.
+template <typename LT, int EPL>
+__device__ __noinline__ void exact_best(const RouteShape s, const LT* __restrict__ row, const float* __restrict__ bias,
+                                        const uint32_t (&key)[EPL], uint32_t thr, int& owner, int& i_best) {
+  const int lane = threadIdx.x & 31, e0 = lane * EPL;
+  const int e = __shfl_sync(FULL, e0 + i_best, owner);
+  const float xb = to_f(row[e]), bb = bias[e];
+  bool other = false;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i)
+    if (key[i] >= thr) other |= to_f(row[e0 + i]) != xb || bias[e0 + i] != bb;
+  // all of one logit and bias: equal in exact arithmetic too, and f32 has found the lowest of them
+  if (!__any_sync(FULL, other)) return;
+  double b[EPL];
+  if (s.sigmoid) {
+#pragma unroll 1
+    for (int i = 0; i < EPL; ++i)
+      if (key[i] >= thr) b[i] = 1.0 / (1.0 + exp(-(double)to_f(row[e0 + i]))) + (double)bias[e0 + i];
+  } else {
+    float x[EPL];
+    load_row<LT, EPL>(s, row, x);
+    exact_values<LT, EPL>(s, x, bias, b);
   }
+  uint64_t mine = 0ull;
+  int at = 0;
+#pragma unroll 1
+  for (int i = EPL - 1; i >= 0; --i) {
+    const uint64_t k = key[i] >= thr ? order_key(b[i]) : 0ull;
+    if (k >= mine && k != 0ull) {
+      mine = k;
+      at = i;
+    }
+  }
+  const uint64_t best = warp_max_key(mine);
+  owner = __ffs(__ballot_sync(FULL, mine == best)) - 1;
+  i_best = at;
+}
+
+// The lane's two largest keys and where they are (0: none), of equals the lowest first.
+template <int EPL>
+struct Top2 {
+  uint32_t k0, k1;
+  int i0, i1;
+  bool known;  // k1 is the second largest, not only unknown
+  __device__ __forceinline__ void find(const uint32_t (&key)[EPL]) {
+    k0 = k1 = 0u;
+    i0 = i1 = 0;
+    known = true;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      const bool first = key[i] > k0, second = key[i] > k1;
+      k1 = first ? k0 : (second ? key[i] : k1);
+      i1 = first ? i0 : (second ? i : i1);
+      k0 = first ? key[i] : k0;
+      i0 = first ? i : i0;
+    }
+  }
+};
+
+// Ranks of groups that fill s.lanes lanes each, from the two largest values of each lane (k0, k1: their keys);
+// stays: whether the lane's group does.  False when the border between the groups is closer than margin.
+__device__ __forceinline__ bool choose_groups(const RouteShape& s, uint32_t k0, uint32_t k1, float v0, float v1,
+                                              float margin, bool& stays) {
+  const int lane = threadIdx.x & 31;
   for (int o = 1; o < s.lanes; o <<= 1) {
     const uint32_t q0 = __shfl_xor_sync(FULL, k0, o), q1 = __shfl_xor_sync(FULL, k1, o);
     const float u0 = __shfl_xor_sync(FULL, v0, o), u1 = __shfl_xor_sync(FULL, v1, o);
@@ -277,32 +329,27 @@ __device__ __forceinline__ bool choose_groups(const RouteShape& s, const float (
     const uint32_t other = __shfl_sync(FULL, gk, q * s.lanes);
     ahead += other > gk || (other == gk && q < g);
   }
-  const bool stays = ahead < s.top_groups;
-  if (!stays) {
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) key[i] = 0u;
-  }
+  stays = ahead < s.top_groups;
   if (s.top_groups == s.groups) return true;
   // the last that stays against the best that goes (lanes past the experts: none of both)
   const bool in = g < s.groups;
   const uint32_t last = __reduce_min_sync(FULL, in && stays ? gk : 0xffffffffu);
   const uint32_t best = __reduce_max_sync(FULL, in && !stays ? gk : 0u);
-  const float a = key_value(last), c = key_value(best);
-  return a - c > margin * (fabsf(a) + fabsf(c));
+  return key_value(last) - key_value(best) > margin;
 }
 
-constexpr int RT_WARPS = 16;
+constexpr int RT_WARPS = 8;
 
 // part: per CTA [E] f32 sums of the normalised scores, then [E] int32 counts
 template <typename LT, int EPL>
-__global__ void __launch_bounds__(RT_WARPS * 32) router_fwd_kernel(const LT* __restrict__ logits, int64_t ld,
+__global__ void __launch_bounds__(RT_WARPS * 32, EPL <= 8 ? 3 : 2) router_fwd_kernel(const LT* __restrict__ logits, int64_t ld,
                                                                    RouteShape s, const float* __restrict__ bias_in,
                                                                    int64_t* __restrict__ topi, float* __restrict__ topw,
                                                                    float* __restrict__ part) {
-  extern __shared__ float rt_smem[];  // [warp][E] usage, [E] counts
+  extern __shared__ float rt_smem[];  // [warp][32 EPL] scores of a token, at the end its sums; [E] counts
   __shared__ int s_e[RT_WARPS][32];
-  __shared__ float s_w[RT_WARPS][32];
-  int* s_count = reinterpret_cast<int*>(rt_smem + RT_WARPS * s.E);
+  float* s_p = rt_smem + (threadIdx.x / 32) * 32 * EPL;
+  int* s_count = reinterpret_cast<int*>(rt_smem + RT_WARPS * 32 * EPL);
   for (int e = threadIdx.x; e < s.E; e += blockDim.x) s_count[e] = 0;
   __syncthreads();
   const int lane = threadIdx.x & 31, warp = threadIdx.x / 32, e0 = lane * EPL;
@@ -314,8 +361,13 @@ __global__ void __launch_bounds__(RT_WARPS * 32) router_fwd_kernel(const LT* __r
     bias[i] = bias_in && e0 + i < s.E ? bias_in[e0 + i] : 0.f;
   }
   const bool by_logit = bias_in == nullptr;
-  // how far f32 may be off: a sigmoid's few roundings; a softmax's exponentials and E-term sum
-  const float margin = s.sigmoid ? 0x1p-21f : 0x1p-17f;
+  // how far apart two choice values must be for f32 to know their order, per unit of score or bias: a
+  // sigmoid is good to a few roundings, a softmax to its exponentials' and its E-term sum's
+  const float margin = s.sigmoid ? 0x1p-20f : 0x1p-17f;
+  float most = 0.f;  // largest |bias|
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) most = fmaxf(most, isinf(bias[i]) ? 0.f : fabsf(bias[i]));
+  most = warp_max(most);
   for (int64_t t = (int64_t)blockIdx.x * RT_WARPS + warp; t < s.T; t += warps) {
     const LT* row = logits + t * ld;
     float p[EPL], b[EPL];
@@ -327,64 +379,94 @@ __global__ void __launch_bounds__(RT_WARPS * 32) router_fwd_kernel(const LT* __r
       if (!by_logit) b[i] = p[i] + bias[i];
       key[i] = e0 + i < s.E ? order_key(b[i]) : 0u;
     }
-    bool close = false;
+    float apart = margin * (1.f + most);  // a sigmoid is at most 1
+    if (!s.sigmoid) {
+      float pm = p[0];
+#pragma unroll
+      for (int i = 1; i < EPL; ++i) pm = fmaxf(pm, p[i]);
+      apart = margin * (warp_max(pm) + most);
+    }
+    Top2<EPL> top;
+    top.find(key);
     if (s.groups > 1) {
+      const int n = s.E / s.groups;
+      bool stays = true, clear;
+      uint32_t bits = 0;
       if (s.lanes) {
-        close = !choose_groups<EPL>(s, p, b, key, by_logit, margin);
+        float v0 = key_value(top.k0), v1 = key_value(top.k1);
+        if (by_logit) {  // the order is that of the logits, the rank's values are the scores: as monotone
+          v0 = v1 = 0.f;
+#pragma unroll
+          for (int i = 0; i < EPL; ++i) {
+            v1 = fmaxf(v1, fminf(v0, p[i]));
+            v0 = fmaxf(v0, p[i]);
+          }
+        }
+        clear = choose_groups(s, top.k0, top.k1, v0, v1, 2.f * apart, stays);
       } else {
         float v[EPL];
 #pragma unroll
         for (int i = 0; i < EPL; ++i) v[i] = by_logit ? p[i] : b[i];
-        close = !choose_any_groups<float, uint32_t, EPL>(s, v, key, margin);
+        clear = choose_any_groups<float, uint32_t, EPL>(s, v, key, s.group_top * apart, bits);
       }
-    }
-    // the k best, in order; behind the k-th the look goes on past its twins to see who comes next
-    uint32_t last = 0u;
-    int prev = 0;
-    for (int j = 0; !close && (j < s.k || !by_logit); ++j) {
-      int owner, i_best;
-      const uint32_t best = warp_best<uint32_t, EPL>(key, owner, i_best);
-      if (best == 0u) break;
-      if (!by_logit) {
-        const int e = __shfl_sync(FULL, e0 + i_best, owner);
-        if (j > 0) {
-          const float a = key_value(last), c = key_value(best);
-          const bool clear = a - c > margin * (fabsf(a) + fabsf(c));
-          // twins have the same logit and bias: they are equal in exact arithmetic too
-          if (!clear && !(to_f(row[e]) == to_f(row[prev]) && bias_in[e] == bias_in[prev])) {
-            close = true;
-            break;
-          }
-          if (j >= s.k && clear) break;
+      if (!clear) bits = exact_groups<LT, EPL>(s, row, bias_in);
+      if (clear && s.lanes) {
+        if (!stays) {
+          top.k0 = top.k1 = 0u;
+#pragma unroll
+          for (int i = 0; i < EPL; ++i) key[i] = 0u;
         }
-        last = best;
-        prev = e;
-      }
-      if (lane == owner) {
+      } else {
 #pragma unroll
         for (int i = 0; i < EPL; ++i)
-          if (i == i_best) {
-            key[i] = 0u;
-            if (j < s.k) {
-              s_e[warp][j] = e0 + i;
-              s_w[warp][j] = p[i];
-            }
+          if (e0 + i < s.E && !((bits >> ((e0 + i) / n)) & 1u)) key[i] = 0u;
+        top.find(key);
+      }
+    }
+    // One choice is a warp maximum of the lanes' largest keys.  The lane that held it goes on to its second, and
+    // looks over its keys again only when its turn comes once more.
+    for (int j = 0; j < s.k; ++j) {
+      const uint32_t best = __reduce_max_sync(FULL, top.k0);
+      int owner = __ffs(__ballot_sync(FULL, top.k0 == best)) - 1, at = top.i0;
+      const bool given = lane == owner;
+      if (!by_logit) {
+        if (given && !top.known) top.find(key);
+        const uint32_t thr = max(order_key(key_value(best) - apart), 1u);
+        if (__any_sync(FULL, (given ? top.k1 : top.k0) >= thr)) {
+          uint32_t k[EPL];  // a copy: the keys themselves stay in registers
+          int o = owner, a = at;
+#pragma unroll
+          for (int i = 0; i < EPL; ++i) k[i] = key[i];
+          exact_best<LT, EPL>(s, row, bias_in, k, thr, o, a);
+          if (lane == o) {
+            // out of the order of the keys: it leaves them for good
+            s_e[warp][j] = e0 + a;
+#pragma unroll
+            for (int i = 0; i < EPL; ++i)
+              if (i == a) key[i] = 0u;
+            top.find(key);
           }
+          continue;
+        }
       }
-    }
-    if (close) {
-      const int e = choose_wide<LT, EPL>(s, row, bias_in);
-      for (int j = 0; j < s.k; ++j) {
-        const int ej = __shfl_sync(FULL, e, j);
+      if (given) {
+        s_e[warp][j] = e0 + at;
 #pragma unroll
         for (int i = 0; i < EPL; ++i)
-          if (e0 + i == ej) s_w[warp][j] = p[i];
+          if (i == at) key[i] = 0u;
+        top.k0 = top.k1;
+        top.i0 = top.i1;
+        top.k1 = 0u;
+        top.known = false;
+        if (top.k0 == 0u) top.find(key);
       }
-      if (lane < s.k) s_e[warp][lane] = e;
     }
+    // the scores of the chosen, by way of shared memory
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) s_p[e0 + i] = p[i];
     __syncwarp();
-    const int e = s_e[warp][lane];
-    float w = lane < s.k ? s_w[warp][lane] : 0.f;
+    const int e = lane < s.k ? s_e[warp][lane] : 0;
+    float w = lane < s.k ? s_p[e] : 0.f;
     const float norm = s.renorm ? warp_sum(w) : 1.f;
     if (lane < s.k) {
       topi[t * s.k + lane] = e;
@@ -397,13 +479,12 @@ __global__ void __launch_bounds__(RT_WARPS * 32) router_fwd_kernel(const LT* __r
     for (int i = 0; i < EPL; ++i) u_acc[i] += p[i] * inv;
   }
 #pragma unroll
-  for (int i = 0; i < EPL; ++i)
-    if (e0 + i < s.E) rt_smem[warp * s.E + e0 + i] = u_acc[i];
+  for (int i = 0; i < EPL; ++i) s_p[e0 + i] = u_acc[i];
   __syncthreads();
   for (int e = threadIdx.x; e < s.E; e += blockDim.x) {
     float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < RT_WARPS; ++w) sum += rt_smem[w * s.E + e];
+    for (int w = 0; w < RT_WARPS; ++w) sum += rt_smem[w * 32 * EPL + e];
     part[(int64_t)blockIdx.x * 2 * s.E + e] = sum;
     reinterpret_cast<int*>(part)[(int64_t)blockIdx.x * 2 * s.E + s.E + e] = s_count[e];
   }
@@ -523,7 +604,7 @@ __global__ void __launch_bounds__(RT_WARPS * 32) router_bwd_kernel(const LT* __r
 
 int route_grid(int64_t T) {
   const int64_t blocks = (T + RT_WARPS - 1) / RT_WARPS;
-  return (int)(blocks < 148 * 2 ? (blocks > 0 ? blocks : 1) : 148 * 2);
+  return (int)(blocks < 148 * 3 ? (blocks > 0 ? blocks : 1) : 148 * 3);
 }
 
 int route_epl(int E) {
@@ -558,7 +639,7 @@ void launch_router_fwd(const void* logits, bool bf16, int64_t ld, int64_t T, int
                        cudaStream_t st) {
   const RouteShape s = route_shape(a, logits, ld, bf16 ? 2 : 4, T, E);
   float* part = reinterpret_cast<float*>(workspace);
-  const int grid = route_grid(T), smem = (RT_WARPS + 1) * E * 4;  // at most 35 KB
+  const int grid = route_grid(T), smem = (RT_WARPS * 32 * route_epl(E) + E) * 4;  // at most 18 KB
 #define OXI_RF(N)                                                                                                    \
   if (bf16)                                                                                                         \
     router_fwd_kernel<__nv_bfloat16, N><<<grid, RT_WARPS * 32, smem, st>>>(                                         \
@@ -577,7 +658,7 @@ void launch_router_bwd(const void* logits, bool bf16, int64_t ld, int64_t T, int
                        const int64_t* topi, const float* dtopw, const float* dusage, void* dlogits, cudaStream_t st) {
   const RouteShape s = route_shape(a, logits, ld, bf16 ? 2 : 4, T, E);
   if (T == 0) return;
-  const int grid = route_grid(T), smem = RT_WARPS * 32 * route_epl(E) * 4;  // at most 32 KB
+  const int grid = route_grid(T), smem = RT_WARPS * 32 * route_epl(E) * 4;  // at most 16 KB
 #define OXI_RB(N)                                                                                                    \
   if (bf16)                                                                                                         \
     router_bwd_kernel<__nv_bfloat16, N><<<grid, RT_WARPS * 32, smem, st>>>(                                         \

@@ -121,6 +121,7 @@ class RouterTopK(torch.autograd.Function):
         ctx.save_for_backward(logits, topi)
         ctx.cfg = (score == "sigmoid", renorm, scale)
         ctx.mark_non_differentiable(topi, counts)
+        ctx.set_materialize_grads(False)  # no zeros for the outputs without a gradient
         return topi, topw, usage, counts
 
     @staticmethod

@@ -4,8 +4,8 @@
 // flagged run (a prompt that all of the document sees), or [a, e) without causality; a padding
 // token sees nothing and is seen by none.
 //
-// One CTA per row.  The row becomes three bit masks in shared memory (32 tokens a word, made by
-// ballots of coalesced loads): document starts, stops of a flagged run, padding.  A token's
+// One CTA per row.  The row becomes four bit masks in shared memory (32 tokens a word, made by
+// ballots of coalesced loads): document starts, stops of a flagged run, flags, padding.  A token's
 // document start is then the highest set bit at or below it: in its own word, or the last one of
 // an earlier word, found once per word by a scan over the words.  The same from the other side
 // gives the next stop.  Nothing is read twice and every global access is coalesced; the row's
@@ -65,7 +65,8 @@ __global__ void __launch_bounds__(DM_THREADS) document_mask_kernel(DmParams p) {
   uint32_t* w_start = reinterpret_cast<uint32_t*>(dm_smem);
   uint32_t* w_stop = w_start + p.words;
   uint32_t* w_pad = w_stop + p.words;
-  int* last = dm_smem + 3 * p.words;   // highest start before the word
+  uint32_t* w_flag = w_pad + p.words;
+  int* last = dm_smem + 4 * p.words;   // highest start before the word
   int* next = last + p.words;          // lowest stop after the word
   int2* bounds = reinterpret_cast<int2*>(next + p.words);  // per tile (kmin, kmax); words is even
   __shared__ int warp_part[32];
@@ -75,26 +76,37 @@ __global__ void __launch_bounds__(DM_THREADS) document_mask_kernel(DmParams p) {
   const int64_t* tok = p.tokens + b * p.ld;
   const uint8_t* pre = p.prefix ? p.prefix + b * p.ldp : nullptr;
   auto is_pad = [&](int64_t t) { return p.has_sep ? (p.has_pad && t == p.pad) : t < 0; };
-  for (int i0 = (threadIdx.x >> 5) * 32; i0 < p.words * 32; i0 += DM_THREADS) {
-    const int i = i0 + lane;
-    bool start = false, stop = false, pad = true;
-    if (i < p.S) {
-      const int64_t t = tok[i];
-      pad = is_pad(t);
-      if (i == 0) {
-        start = true;
-      } else {
-        const int64_t t1 = tok[i - 1];
-        start = p.has_sep ? (t1 == p.sep || is_pad(t1) != pad) : t != t1;
-      }
-      stop = start || (p.causal && !(pre && pre[i]));
+  // four words of a warp at a time, their loads in flight together
+  constexpr int AHEAD = 4;
+  for (int w0 = (threadIdx.x >> 5) * AHEAD; w0 < p.words; w0 += DM_THREADS / 32 * AHEAD) {
+    int64_t t[AHEAD], before[AHEAD];
+    bool flag[AHEAD];
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q) {
+      const int i = (w0 + q) * 32 + lane;
+      t[q] = i < p.S ? tok[i] : 0;
+      // the token before: the lane's to the left, the word's first looks it up
+      before[q] = i < p.S && i > 0 && lane == 0 ? tok[i - 1] : 0;
+      flag[q] = pre && i < p.S && pre[i] != 0;
     }
-    const uint32_t ws = __ballot_sync(0xffffffffu, start), wt = __ballot_sync(0xffffffffu, stop),
-                   wp = __ballot_sync(0xffffffffu, pad);
-    if (lane == 0) {
-      w_start[i0 >> 5] = ws;
-      w_stop[i0 >> 5] = wt;
-      w_pad[i0 >> 5] = wp;
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q) {
+      const int i = (w0 + q) * 32 + lane;
+      const int64_t left = __shfl_up_sync(0xffffffffu, t[q], 1), t1 = lane == 0 ? before[q] : left;
+      bool start = false, stop = false, pad = true;
+      if (i < p.S) {
+        pad = is_pad(t[q]);
+        start = i == 0 || (p.has_sep ? (t1 == p.sep || is_pad(t1) != pad) : t[q] != t1);
+        stop = start || (p.causal && !flag[q]);
+      }
+      const uint32_t ws = __ballot_sync(0xffffffffu, start), wt = __ballot_sync(0xffffffffu, stop),
+                     wp = __ballot_sync(0xffffffffu, pad), wf = __ballot_sync(0xffffffffu, flag[q]);
+      if (lane == 0 && w0 + q < p.words) {
+        w_start[w0 + q] = ws;
+        w_stop[w0 + q] = wt;
+        w_pad[w0 + q] = wp;
+        w_flag[w0 + q] = wf;
+      }
     }
   }
   __syncthreads();
@@ -150,7 +162,7 @@ __global__ void __launch_bounds__(DM_THREADS) document_mask_kernel(DmParams p) {
         lo = below ? (i & ~31) + 31 - __clz(below) : last[w];
         if (p.causal) {
           hi = i + 1;
-          if (pre && pre[lo]) hi = max(hi, next_stop(lo));
+          if ((w_flag[lo >> 5] >> (lo & 31)) & 1) hi = max(hi, next_stop(lo));
         } else {
           hi = next_stop(i);
         }
@@ -175,18 +187,29 @@ __global__ void __launch_bounds__(DM_THREADS) document_mask_kernel(DmParams p) {
     }
   }
   __syncthreads();
-  for (int t = threadIdx.x; t < p.nt; t += DM_THREADS) {
-    const int k0 = t * DA_TILE, k1 = k0 + DA_TILE;
+  // query tiles that may see a key tile: four threads a tile
+  for (int t0 = 0; t0 < p.nt; t0 += DM_THREADS / 4) {
+    const int t = t0 + threadIdx.x / 4, k0 = t * DA_TILE, k1 = k0 + DA_TILE;
     int first = p.nt, end = 0;
-    for (int q = 0; q < p.nt; ++q) {
-      const int2 r = bounds[q];
-      if (r.x < k1 && r.y > k0) {
-        first = min(first, q);
-        end = q + 1;
+    if (t < p.nt) {
+#pragma unroll 4
+      for (int q = threadIdx.x & 3; q < p.nt; q += 4) {
+        const int2 r = bounds[q];
+        if (r.x < k1 && r.y > k0) {
+          first = min(first, q);
+          end = q + 1;
+        }
       }
     }
-    p.kt[b * p.nt + t].x = end ? first : 0;
-    p.kt[b * p.nt + t].y = end;
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+      end = max(end, __shfl_xor_sync(0xffffffffu, end, o));
+    }
+    if (t < p.nt && (threadIdx.x & 3) == 0) {
+      p.kt[b * p.nt + t].x = end ? first : 0;
+      p.kt[b * p.nt + t].y = end;
+    }
   }
 }
 
@@ -214,7 +237,7 @@ void launch_document_mask(const int64_t* tokens, int64_t ld, const uint8_t* pref
   p.hi = hi;
   p.qt = reinterpret_cast<int4*>(qt);
   p.kt = reinterpret_cast<int4*>(kt);
-  const size_t smem = (size_t)p.words * 5 * sizeof(int) + (size_t)p.nt * sizeof(int2);
+  const size_t smem = (size_t)p.words * 6 * sizeof(int) + (size_t)p.nt * sizeof(int2);
   // the attribute belongs to the device's copy of the kernel: set it on whichever device this is
   if (smem > 40 * 1024)
     OXI_CUDA_CHECK(cudaFuncSetAttribute(document_mask_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));

@@ -15,8 +15,17 @@ Rules reproduced here:
 
 Extensions (all optional, ignored by the upstream parser because serde skips
 unknown keys): ``num_shared_experts``, ``init_std``, ``seed``, ``compat``,
-``ep_size``, ``moe_aux_loss``.  They are NOT part of the model-config hash, so a
-config without them hashes exactly like upstream.
+``ep_size``, ``moe_aux_loss``, and the model options
+
+* ``embed_scale``: factor of the embeddings;
+* ``doc_separator``: token id that ends a document: attention stays within documents;
+* ``attn_softcap``: scores pass through ``c tanh(./c)``; ``attn_alibi``: a bias of
+  ``-2^(-8 (h + 1) / heads) |i - j|`` on the scores of head h;
+* ``moe_score`` (``softmax`` / ``sigmoid``), ``moe_groups`` / ``moe_top_groups``, ``moe_renorm``,
+  ``moe_route_scale``: routing (``ops.api.route_topk``); ``moe_bias_rate``: a selection bias per expert that
+  moves by this much a step towards balance.
+
+They are NOT part of the model-config hash, so a config without them hashes exactly like upstream.
 """
 from __future__ import annotations
 
@@ -119,6 +128,16 @@ class ModelConfig:
     compat: Optional[str] = _f(None, kind=str)
     ep_size: Optional[int] = _f(None, kind=int)
     moe_aux_loss: Optional[str] = _f(None, kind=str)
+    embed_scale: Optional[float] = _f(None, kind=float)
+    doc_separator: Optional[int] = _f(None, kind=int)
+    attn_softcap: Optional[float] = _f(None, kind=float)
+    attn_alibi: Optional[bool] = _f(None, kind=bool)
+    moe_score: Optional[str] = _f(None, kind=str)
+    moe_groups: Optional[int] = _f(None, kind=int)
+    moe_top_groups: Optional[int] = _f(None, kind=int)
+    moe_renorm: Optional[bool] = _f(None, kind=bool)
+    moe_route_scale: Optional[float] = _f(None, kind=float)
+    moe_bias_rate: Optional[float] = _f(None, kind=float)
 
     UPSTREAM_FIELDS = (
         "name", "hidden_size", "num_layers", "num_heads", "kv_heads", "kv_latent_dim",
@@ -349,6 +368,21 @@ class LitConfig:
                   file=sys.stderr)
         if m.hidden_size % m.num_heads != 0:
             raise ConfigError("hidden_size must be divisible by num_heads")
+        if m.doc_separator is not None:
+            if m.doc_separator >= m.vocab_size:
+                raise ConfigError(f"doc_separator {m.doc_separator} is not a token of a vocabulary of {m.vocab_size}")
+            if m.mamba_layers:
+                raise ConfigError("doc_separator needs attention layers only: a Mamba layer's state would cross documents")
+        if m.attn_softcap is not None and not 0 < m.attn_softcap < math.inf:
+            raise ConfigError(f"attn_softcap must be a positive number, got {m.attn_softcap}")
+        if m.moe_score not in (None, "softmax", "sigmoid"):
+            raise ConfigError(f"moe_score must be softmax or sigmoid, got {m.moe_score!r}")
+        if m.num_experts is not None and m.experts_per_tok is not None:
+            groups, top = m.moe_groups or 1, m.moe_top_groups or m.moe_groups or 1
+            if m.num_experts % groups or not 1 <= top <= groups:
+                raise ConfigError(f"{m.num_experts} experts cannot be taken in {groups} groups of which {top} stay")
+            if not 1 <= m.experts_per_tok <= top * (m.num_experts // groups):
+                raise ConfigError(f"experts_per_tok {m.experts_per_tok} is more than the experts of {top} of {groups} groups")
 
 
 # ---------------------------------------------------------------------------

@@ -11,6 +11,31 @@ from ..ops import api
 from .common import RefModule, RopeCache, _assign, interleave_gu, normal_, split_gu, take
 
 
+class ScoreOptions:
+    """Options of a block's attention scores: a cap, and distance-bias slopes made once per device."""
+
+    def __init__(self, cfg, heads: int):
+        self.softcap = float(cfg.attn_softcap or 0.0)
+        self.alibi = bool(cfg.attn_alibi)
+        self.heads = heads
+        self._slopes = {}
+
+    def kwargs(self, mask, device) -> dict:
+        """What api.attention takes beyond its operands; empty for plain causal attention."""
+        kw = {}
+        if mask is not None:
+            kw["mask"] = mask
+        if self.softcap:
+            kw["softcap"] = self.softcap
+        if self.alibi:
+            s = self._slopes.get(device)
+            if s is None:
+                s = torch.exp2(-8.0 * torch.arange(1, self.heads + 1, dtype=torch.float32) / self.heads).to(device)
+                self._slopes[device] = s
+            kw["alibi"] = s
+        return kw
+
+
 class GQAAttention(RefModule):
     """q/k/v/o projections without bias, rotate-half RoPE over the full head
     dim, causal softmax attention with scale 1/sqrt(head_dim).
@@ -29,6 +54,7 @@ class GQAAttention(RefModule):
         self.theta = cfg.rope_theta
         self.max_seq = cfg.max_seq_len
         self.scale = 1.0 / math.sqrt(self.hd)
+        self.scores = ScoreOptions(cfg, self.nh)
         n_qkv = (self.nh + 2 * self.kvh) * self.hd
         self.w_qkv = nn.Parameter(torch.empty(n_qkv, H, device=device, dtype=dtype))
         self.o_proj = nn.Parameter(torch.empty(H, self.nh * self.hd, device=device, dtype=dtype))
@@ -37,10 +63,11 @@ class GQAAttention(RefModule):
         normal_(self.w_qkv, std, gen)
         normal_(self.o_proj, std, gen)
 
-    def forward(self, h: torch.Tensor, resid: torch.Tensor) -> torch.Tensor:
+    def forward(self, h: torch.Tensor, resid: torch.Tensor, mask=None) -> torch.Tensor:
         B, S, _ = h.shape
         cos, sin = RopeCache.get(self.hd, S, self.theta, h.device)
-        o = api.attention_rope(h, self.w_qkv, cos, sin, self.nh, self.kvh, self.hd, self.scale)
+        o = api.attention_rope(h, self.w_qkv, cos, sin, self.nh, self.kvh, self.hd, self.scale,
+                               **self.scores.kwargs(mask, h.device))
         return api.linear(o, self.o_proj, resid=resid)
 
     def export_ref(self, prefix, out):
@@ -78,6 +105,7 @@ class MLAAttention(RefModule):
         self.ql = cfg.q_latent_dim
         self.theta = cfg.rope_theta
         self.scale = 1.0 / math.sqrt(self.hd + self.dr)
+        self.scores = ScoreOptions(cfg, self.nh)
         self.n_down = self.kvl + self.ql + self.dr + self.nh * self.dr
         self.w_down = nn.Parameter(torch.empty(self.n_down, H, device=device, dtype=dtype))
         self.w_uq = nn.Parameter(torch.empty(self.nh * self.hd, self.ql, device=device, dtype=dtype))
@@ -88,7 +116,7 @@ class MLAAttention(RefModule):
         for p in (self.w_down, self.w_uq, self.w_ukv, self.o_proj):
             normal_(p, std, gen)
 
-    def forward(self, h, resid):
+    def forward(self, h, resid, mask=None):
         B, S, _ = h.shape
         nh, hd, dr = self.nh, self.hd, self.dr
         d = api.linear(h, self.w_down)
@@ -99,7 +127,7 @@ class MLAAttention(RefModule):
         cos, sin = RopeCache.get(dr, S, self.theta, h.device)
         # RoPE on the rope parts and the shared k_rope broadcast to every head, in one kernel
         q, k, v = api.mla_qkv(q_c, kv, rp, cos, sin, nh, hd, dr)
-        o = api.attention(q, k, v, self.scale, causal=True).reshape(B, S, nh * hd)
+        o = api.attention(q, k, v, self.scale, causal=True, **self.scores.kwargs(mask, h.device)).reshape(B, S, nh * hd)
         return api.linear(o, self.o_proj, resid=resid)
 
     def _splits(self):

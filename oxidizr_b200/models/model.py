@@ -4,7 +4,8 @@
 Per-layer block type follows ``ModelConfig.layer_kind`` (model.rs:795-870):
 Mamba3 / Mamba2 / Mamba1 for layers in ``mamba_layers``; otherwise MLA+MoE when
 ``kv_latent_dim`` is set, GQA+MoE when ``num_experts`` is set without MLA (an
-extension), else GQA+SwiGLU.
+extension), else GQA+SwiGLU.  With ``doc_separator`` in the config the attention layers get one document
+mask per batch, built from the token ids.
 
 ``forward(ids, targets)`` returns ``(ce_loss, aux_losses)`` using the fused
 lm_head + cross-entropy kernel (the logits are never returned);
@@ -50,9 +51,9 @@ class AttnBlock(RefModule):
         self.input_layernorm.reset_parameters()
         self.post_attention_layernorm.reset_parameters()
 
-    def forward(self, x):
+    def forward(self, x, mask=None):
         h, x = api.rmsnorm_resid(x, self.input_layernorm.weight, 1e-5)
-        x = self.self_attn(h, x)
+        x = self.self_attn(h, x, mask)
         h, x = api.rmsnorm_resid(x, self.post_attention_layernorm.weight, 1e-5)
         if self.moe is not None:
             return self.moe(h, x)
@@ -83,6 +84,8 @@ class LitGPT(RefModule):
         self.embed_tokens = nn.Parameter(torch.empty(V, H, device=device, dtype=dtype))
         self.layers = nn.ModuleList([make_block(cfg, i, device, dtype, ep_group) for i in range(cfg.num_layers)])
         self.norm = NormW(H, device=device, dtype=dtype)
+        self.embed_scale = 1.0 if cfg.embed_scale is None else float(cfg.embed_scale)
+        self.doc_separator = cfg.doc_separator
         self.lm_head = nn.Parameter(torch.empty(V, H, device=device, dtype=dtype))
         # Optional callable given the parameters a part of the forward is about to
         # use; a sharded data-parallel optimizer sets it so that the forward waits
@@ -107,12 +110,14 @@ class LitGPT(RefModule):
         gate = self._param_gate
         if gate is not None:
             gate((self.embed_tokens,))
-        x = api.embedding(ids, self.embed_tokens)
+        x = api.embedding(ids, self.embed_tokens, self.embed_scale)
+        # one mask for the attention of every layer
+        mask = None if self.doc_separator is None else api.document_mask(ids, self.doc_separator)
         aux = []
         for layer in self.layers:
             if gate is not None:
                 gate(layer.parameters())
-            x, a = layer(x)
+            x, a = layer(x) if mask is None else layer(x, mask)
             if a is not None:
                 aux.append(a)
         if gate is not None:
@@ -124,6 +129,13 @@ class LitGPT(RefModule):
         x, aux = self.hidden(ids)
         loss = api.linear_cross_entropy(x, self.lm_head, targets)
         return loss, aux
+
+    def update_route_bias(self) -> None:
+        """Move the experts' selection biases by the loads since the last call (``moe_bias_rate``)."""
+        for layer in self.layers:
+            moe = getattr(layer, "moe", None)
+            if moe is not None and moe.bias_rate:
+                moe.update_route_bias()
 
     def logits(self, ids: torch.Tensor) -> torch.Tensor:
         x, _ = self.hidden(ids)

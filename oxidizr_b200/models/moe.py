@@ -12,6 +12,9 @@ Auxiliary load-balancing loss:
   ``mean_e((mean_t p_te)^2)`` -- differentiable here (upstream detaches it);
 * ``switch``: ``E * sum_e f_e * P_e`` with f_e the routed-token fraction.
 
+The routing options of the config (sigmoid scores, a selection bias, groups, plain or scaled weights) go
+through ``api.route_topk``; the selection bias moves after each optimizer step (``update_route_bias``).
+
 Expert weights are stored stacked ([E, 2I, H] gate|up interleaved, [E, H, I])
 so a grouped GEMM can address them; ``export_ref`` writes the upstream
 per-expert names ``experts.{e}.{gate,up,down}_proj.weight``.  Several shared
@@ -60,8 +63,12 @@ def aux_from_usage(usage: torch.Tensor, counts: torch.Tensor, n_sel: int, E: int
     return usage.pow(2).mean()
 
 
-def route_with_aux(logits: torch.Tensor, k: int, E: int, kind: str):
-    """(top_idx, top_w, aux, counts): the fused router kernel on CUDA, torch ops elsewhere."""
+def route_with_aux(logits: torch.Tensor, k: int, E: int, kind: str, **options):
+    """(top_idx, top_w, aux, counts): the fused router kernel on CUDA, torch ops elsewhere.  ``options``:
+    scores, bias, groups and weights as ``api.route_topk`` takes them."""
+    if options:
+        topi, topw, usage, counts = api.route_topk(logits, k, **options)
+        return topi, topw, aux_from_usage(usage, counts, topi.numel(), E, kind), counts
     if logits.is_cuda:
         from ..ops.moe_kernels import RouterTopK, router_ok
         if router_ok(logits, k):
@@ -92,6 +99,15 @@ class MoE(RefModule):
         self.router = nn.Parameter(torch.empty(self.E, H, device=device, dtype=dtype))
         self.w_gu = nn.Parameter(torch.empty(self.E_local, 2 * self.I, H, device=device, dtype=dtype))
         self.w_down = nn.Parameter(torch.empty(self.E_local, H, self.I, device=device, dtype=dtype))
+        # routing other than the softmax, renormalised and ungrouped
+        self.route_options = {n: v for n, v in (
+            ("score", cfg.moe_score), ("groups", cfg.moe_groups), ("top_groups", cfg.moe_top_groups or cfg.moe_groups),
+            ("renorm", cfg.moe_renorm), ("scale", cfg.moe_route_scale)) if v is not None}
+        self.bias_rate = float(cfg.moe_bias_rate or 0.0)
+        if self.bias_rate:
+            # the selection bias, and the tokens each expert got since it last moved
+            self.register_buffer("route_bias", torch.zeros(self.E, dtype=torch.float32, device=device))
+            self.register_buffer("route_load", torch.zeros(self.E, dtype=torch.float32, device=device), persistent=False)
         self.n_shared = cfg.n_shared_experts
         self.shared = SwiGLU(H, self.n_shared * self.I, device, dtype) if self.n_shared > 0 else None
         # under expert parallelism the expert weights are shards, not replicas:
@@ -133,7 +149,10 @@ class MoE(RefModule):
         B, S, H = h.shape
         x = h.reshape(-1, H)
         logits = api.linear(x, self.router)
-        topi, topw, aux, counts = route_with_aux(logits, self.k, self.E, self.aux_kind)
+        options = dict(self.route_options, bias=self.route_bias) if self.bias_rate else self.route_options
+        topi, topw, aux, counts = route_with_aux(logits, self.k, self.E, self.aux_kind, **options)
+        if self.bias_rate and torch.is_grad_enabled():
+            self.route_load.add_(counts)
         if self.ep_size > 1:
             from ..parallel import ep
             if counts is not None and ep.nvlink_ok(self, x):
@@ -161,9 +180,21 @@ class MoE(RefModule):
             return self.shared(h, resid + y), aux
         return resid + y, aux
 
+    @torch.no_grad()
+    def update_route_bias(self) -> None:
+        """bias_e += rate * sign(mean load - load_e), with the loads of every data-parallel rank; then the
+        loads start again.  No host synchronisation."""
+        import torch.distributed as dist
+        if dist.is_available() and dist.is_initialized() and dist.get_world_size() > 1:
+            dist.all_reduce(self.route_load)
+        self.route_bias.add_(torch.sign(self.route_load.mean() - self.route_load), alpha=self.bias_rate)
+        self.route_load.zero_()
+
     # ------------------------------------------------------------ names
     def export_ref(self, prefix, out):
         out[prefix + "router.gate.weight"] = self.router.detach()
+        if self.bias_rate:
+            out[prefix + "router.selection_bias"] = self.route_bias.detach()
         base = self.ep_rank * self.E_local
         for e in range(self.E_local):
             g, u = split_gu(self.w_gu.detach()[e])
@@ -176,6 +207,8 @@ class MoE(RefModule):
 
     def import_ref(self, prefix, sd):
         _assign(self.router, sd, prefix + "router.gate.weight")
+        if self.bias_rate:
+            _assign(self.route_bias, sd, prefix + "router.selection_bias")
         base = self.ep_rank * self.E_local
         with torch.no_grad():
             for e in range(self.E_local):

@@ -155,6 +155,8 @@ class Trainer:
             total_ce = total_ce + ce.detach().float()
         with nvtx_range("optimizer"):
             gnorm = self.opt.step()
+        if self.cfg.model.moe_bias_rate:
+            self.model.update_route_bias()
         return total_ce / accum, gnorm
 
     def _graph_step(self, batches):

@@ -1,0 +1,126 @@
+"""The model options that use document masks, score caps, distance biases, scaled embeddings and routing,
+together, on the CPU."""
+import pytest
+import torch
+
+from oxidizr_b200.config import ConfigError, LitConfig
+from oxidizr_b200.models import build_model
+
+SEP = 3
+
+
+def config(**model):
+    m = {"name": "t", "hidden_size": 32, "num_layers": 2, "num_heads": 4, "kv_heads": 2, "num_experts": 8,
+         "experts_per_tok": 2, "intermediate_size": 16, "vocab_size": 50, "max_seq_len": 64, "rope_theta": 10000.0,
+         "dtype": "f32"}
+    m.update(model)
+    return LitConfig.from_dict({"model": m, "trainer": {
+        "learning_rate": 1e-3, "batch_size": 2, "max_steps": 1, "num_epochs": 1, "gradient_accumulation": 1,
+        "checkpoint_dir": "/tmp/oxi_packed", "log_interval": 1, "save_interval": 100, "load_balance_alpha": 0.01,
+        "group_size": 4, "beta_kl": 0.04}})
+
+
+OPTIONS = dict(doc_separator=SEP, attn_softcap=20.0, attn_alibi=True, embed_scale=32 ** 0.5, moe_score="sigmoid",
+               moe_groups=4, moe_top_groups=2, moe_route_scale=2.5, moe_bias_rate=0.01)
+LATENT = dict(kv_heads=None, kv_latent_dim=16, q_latent_dim=16, d_rope=8)
+
+
+def packed(seed):
+    g = torch.Generator().manual_seed(seed)
+    docs = [torch.randint(4, 50, (n,), generator=g) for n in (9, 1, 14, 6)]
+    row = torch.cat([torch.cat([d, torch.tensor([SEP])]) for d in docs])
+    return docs, row[None]
+
+
+@pytest.mark.parametrize("kind", [{}, LATENT])
+def test_packed_documents_are_the_documents_alone(kind):
+    """RoPE and the distance bias are relative, so a document's logits do not depend on what it is packed with."""
+    model = build_model(config(**OPTIONS, **kind).model, seed=1).double()
+    docs, row = packed(0)
+    out = model.double().logits(row).double()
+    at = 0
+    for d in docs:
+        alone = model.logits(torch.cat([d, torch.tensor([SEP])])[None]).double()
+        # the logits are formed in f32: 32 terms of about 0.02 each, and the routing weights' f32
+        assert (out[0, at:at + len(d) + 1] - alone[0]).abs().max() < 1e-4
+        at += len(d) + 1
+
+
+def test_without_the_separator_documents_do_see_each_other():
+    docs, row = packed(0)
+    model = build_model(config(**{**OPTIONS, "doc_separator": None}).model, seed=1)
+    a = model.logits(row)
+    other = row.clone()
+    other[0, 0] = 49 if int(row[0, 0]) != 49 else 48
+    assert not torch.equal(model.logits(other)[0, -5:], a[0, -5:])
+    model = build_model(config(**OPTIONS).model, seed=1)
+    assert torch.equal(model.logits(other)[0, -5:], model.logits(row)[0, -5:])
+
+
+def test_the_selection_bias_moves_towards_balance():
+    cfg = config(**OPTIONS)
+    model = build_model(cfg.model, seed=2)
+    _, row = packed(1)
+    ids = row[:, :-1].expand(2, -1)
+    loss, aux = model(ids, row[:, 1:].expand(2, -1))
+    (loss + 0.01 * torch.stack(aux).mean()).backward()
+    moe = model.layers[0].moe
+    load = moe.route_load.clone()
+    assert load.sum() == ids.numel() * 2 and (moe.route_bias == 0).all()
+    assert moe.router.grad.abs().max() > 0
+    model.update_route_bias()
+    assert torch.equal(moe.route_bias, 0.01 * torch.sign(load.mean() - load))
+    assert (moe.route_load == 0).all()
+    # not in training, no load is counted
+    with torch.no_grad():
+        model(ids, row[:, 1:].expand(2, -1))
+    assert (moe.route_load == 0).all()
+    # and the bias goes into a checkpoint and comes back
+    sd = model.export_ref()
+    other = build_model(cfg.model, seed=3)
+    other.import_ref(sd)
+    assert torch.equal(other.layers[0].moe.route_bias, moe.route_bias)
+
+
+def test_plain_options_change_nothing():
+    """A config that spells the defaults out routes and embeds as one without them.  The spelled routing forms
+    its softmax in 64 bits and rounds it once: two weights of a token apart by some steps of 2^-24, times expert
+    outputs and two layers' gains below 1 here, stay under 1e-6 in logits below 1."""
+    plain = build_model(config().model, seed=4)
+    spelled = build_model(config(moe_score="softmax", moe_groups=1, embed_scale=1.0).model, seed=4)
+    _, row = packed(2)
+    assert (plain.logits(row) - spelled.logits(row)).abs().max() < 1e-6
+
+
+def test_a_trainer_step(tmp_path):
+    from oxidizr_b200.optim import AdamW, AdamWConfig, FlatParams
+    from oxidizr_b200.trainer import Trainer
+    cfg = config(**OPTIONS)
+    model = build_model(cfg.model, seed=5)
+    opt = AdamW(FlatParams(list(model.named_parameters()), "cpu"), AdamWConfig(lr=1e-3))
+    _, row = packed(3)
+
+    class Loader:
+        def next_batch(self):
+            return row[:, :-1].expand(2, -1), row[:, 1:].expand(2, -1)
+
+        def __len__(self):
+            return 1
+
+    t = Trainer.__new__(Trainer)
+    t.cfg, t.tc, t.model, t.opt, t.loader = cfg, cfg.trainer, model, opt, Loader()
+    t.device, t.rank, t.world_size, t.global_step, t.cuda_graph = torch.device("cpu"), 0, 1, 0, False
+    before = model.layers[1].moe.route_bias.clone()
+    ce, norm = t.training_step()
+    assert torch.isfinite(ce) and torch.isfinite(norm)
+    assert not torch.equal(model.layers[1].moe.route_bias, before)
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(doc_separator=50), "vocabulary"), (dict(attn_softcap=0.0), "attn_softcap"), (dict(moe_score="relu"), "moe_score"),
+    (dict(moe_groups=3), "groups"), (dict(moe_groups=4, moe_top_groups=5), "groups"),
+    (dict(moe_groups=8, moe_top_groups=1), "experts_per_tok"),
+    (dict(doc_separator=1, mamba_layers=[0], mamba2_num_heads=8, mamba2_head_dim=8, mamba2_expand=2), "Mamba")])
+def test_config_refusals(bad, match):
+    with pytest.raises(ConfigError, match=match):
+        config(**bad)

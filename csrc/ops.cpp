@@ -5,6 +5,7 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #include <array>
+#include <atomic>
 
 #include "kernels.h"
 #include "kernels_ew.h"
@@ -473,25 +474,26 @@ oxi::DaShape da_shape(const torch::Tensor& q, const torch::Tensor& k, const torc
   return s;
 }
 
-std::vector<torch::Tensor> doc_attn_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, double scale, double cap,
-                                        c10::optional<torch::Tensor> slopes, bool causal,
-                                        std::vector<torch::Tensor> mask, torch::Tensor status) {
+// o is [B, S, Hq, Dv] or [B, S, Hq Dv]; returns the rows' softmax statistics.
+torch::Tensor da_forward(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, double scale,
+                         double cap, const c10::optional<torch::Tensor>& slopes, bool causal,
+                         const std::vector<torch::Tensor>& mask, const torch::Tensor& status, torch::Tensor& o,
+                         bool flat) {
   const oxi::DaShape s = da_shape(q, k, v, scale, cap, slopes, causal, mask);
   const auto tq = da_operand(q, q, "q"), tk = da_operand(k, q, "k"), tv = da_operand(v, q, "v");
   c10::cuda::CUDAGuard g(q.device());
-  auto o = torch::empty({s.B, s.S, s.Hq, s.Dv}, q.options());
+  o = flat ? torch::empty({s.B, s.S, (int64_t)s.Hq * s.Dv}, q.options()) : torch::empty({s.B, s.S, s.Hq, s.Dv}, q.options());
   auto nlse2 = torch::empty({s.B, s.Hq, s.S}, q.options().dtype(torch::kFloat32));
   oxi::launch_da_fwd(s, tq.d, tk.d, tv.d, {o.data_ptr(), (int64_t)s.Hq * s.Dv}, nlse2.data_ptr<float>(),
                      status_ptr(status), stream());
-  return {o, nlse2};
+  return nlse2;
 }
-std::vector<torch::Tensor> doc_attn_qkv_fwd(torch::Tensor qkv, int64_t Hq, int64_t Hk, int64_t D, double scale,
-                                            double cap, c10::optional<torch::Tensor> slopes, bool causal,
-                                            std::vector<torch::Tensor> mask, torch::Tensor status) {
-  const auto h = da_heads(qkv, Hq, Hk, D);
-  auto r = doc_attn_fwd(h[0], h[1], h[2], scale, cap, slopes, causal, mask, status);
-  r[0] = r[0].view({qkv.size(0), qkv.size(1), Hq * D});
-  return r;
+std::vector<torch::Tensor> doc_attn_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, double scale, double cap,
+                                        c10::optional<torch::Tensor> slopes, bool causal,
+                                        std::vector<torch::Tensor> mask, torch::Tensor status) {
+  torch::Tensor o;
+  auto nlse2 = da_forward(q, k, v, scale, cap, slopes, causal, mask, status, o, false);
+  return {o, nlse2};
 }
 
 void da_backward(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& o,
@@ -1374,6 +1376,162 @@ void gemm_grouped(int64_t mode, int64_t epi, torch::Tensor a, bool a_mn, torch::
 
 }  // namespace
 
+// ------------------------------------------------------------ autograd nodes
+// Operators whose GPU time at small sizes is below the host's for a node written in Python: forward and
+// backward as nodes of the C++ engine, whose backward needs no interpreter lock.
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+std::atomic<int64_t> g_node_backwards{0};  // kernel library calls that nodes made from backward passes
+
+void first_order_only(const char* what) {
+  OXI_CHECK(!at::GradMode::is_enabled(), what, ": only first derivatives (create_graph=False)");
+}
+c10::optional<torch::Tensor> maybe(const torch::Tensor& t) {
+  return t.defined() ? c10::optional<torch::Tensor>(t) : c10::nullopt;
+}
+// Slots behind the operands of an attention node: options, kept in its context.
+struct DaOptions {
+  double scale, cap;
+  bool causal;
+  torch::Tensor slopes, status;
+  std::vector<torch::Tensor> mask;
+
+  void save(AutogradContext* ctx, variable_list kept) const {
+    kept.push_back(slopes);
+    kept.insert(kept.end(), mask.begin(), mask.end());
+    ctx->save_for_backward(std::move(kept));
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["cap"] = cap;
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["status"] = status;
+  }
+  static DaOptions load(AutogradContext* ctx, const variable_list& kept, size_t at) {
+    return {ctx->saved_data["scale"].toDouble(), ctx->saved_data["cap"].toDouble(), ctx->saved_data["causal"].toBool(),
+            kept[at], ctx->saved_data["status"].toTensor(), {kept.begin() + at + 1, kept.end()}};
+  }
+};
+
+// q [B, S, Hq, Dqk], k [B, S, Hk, Dqk], v [B, S, Hk, Dv] views -> o [B, S, Hq, Dv]
+struct DocAttention : torch::autograd::Function<DocAttention> {
+  static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& q, const torch::Tensor& k,
+                               const torch::Tensor& v, const DaOptions& opt) {
+    torch::Tensor o;
+    auto nlse2 = da_forward(q, k, v, opt.scale, opt.cap, maybe(opt.slopes), opt.causal, opt.mask, opt.status, o, false);
+    opt.save(ctx, {q, k, v, o, nlse2});
+    return o;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_order_only("attention");
+    const auto t = ctx->get_saved_variables();
+    const auto opt = DaOptions::load(ctx, t, 5);
+    ++g_node_backwards;
+    auto g = doc_attn_bwd(t[0], t[1], t[2], t[3], grads[0], t[4], opt.scale, opt.cap, maybe(opt.slopes), opt.causal,
+                          opt.mask, opt.status);
+    return {g[0], g[1], g[2], torch::Tensor()};
+  }
+};
+
+// The same from the fused projection [B, S, (Hq + 2 Hk) D] -> [B, S, Hq D]; the gradient is written in the
+// projection's layout, with no assembly of slices.
+struct DocAttentionQKV : torch::autograd::Function<DocAttentionQKV> {
+  static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& qkv, int64_t Hq, int64_t Hk, int64_t D,
+                               const DaOptions& opt) {
+    const auto h = da_heads(qkv, Hq, Hk, D);
+    torch::Tensor o;
+    auto nlse2 = da_forward(h[0], h[1], h[2], opt.scale, opt.cap, maybe(opt.slopes), opt.causal, opt.mask, opt.status,
+                            o, true);
+    opt.save(ctx, {qkv, o, nlse2});
+    ctx->saved_data["heads"] = std::vector<int64_t>{Hq, Hk, D};
+    return o;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    first_order_only("attention");
+    const auto t = ctx->get_saved_variables();
+    const auto opt = DaOptions::load(ctx, t, 3);
+    const auto h = ctx->saved_data["heads"].toIntVector();
+    ++g_node_backwards;
+    auto g = doc_attn_qkv_bwd(t[0], h[0], h[1], h[2], t[1], grads[0], t[2], opt.scale, opt.cap, maybe(opt.slopes),
+                              opt.causal, opt.mask, opt.status);
+    return {g, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()};
+  }
+};
+
+struct EmbeddingLookup : torch::autograd::Function<EmbeddingLookup> {
+  static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& ids, const torch::Tensor& w, double scale,
+                               const torch::Tensor& status) {
+    const auto flat = ids.contiguous().view({-1});
+    auto out = embedding_fwd(flat, w.contiguous(), scale, status);
+    auto shape = ids.sizes().vec();
+    shape.push_back(w.size(1));
+    ctx->save_for_backward({flat});
+    ctx->saved_data["rows"] = w.size(0);
+    ctx->saved_data["scale"] = scale;
+    return out.view(shape);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto ids = ctx->get_saved_variables()[0];
+    const auto& dy = grads[0];
+    ++g_node_backwards;
+    auto dw = embedding_bwd(ids, dy.reshape({ids.numel(), dy.size(-1)}).contiguous(), ctx->saved_data["rows"].toInt(),
+                            ctx->saved_data["scale"].toDouble(), c10::nullopt);
+    return {torch::Tensor(), dw, torch::Tensor(), torch::Tensor()};
+  }
+};
+
+struct RouterTopK : torch::autograd::Function<RouterTopK> {
+  static variable_list forward(AutogradContext* ctx, const torch::Tensor& logits_, int64_t k, bool sigmoid,
+                               const c10::optional<torch::Tensor>& bias, int64_t groups, int64_t top_groups,
+                               int64_t group_top, bool renorm, double scale) {
+    const auto logits = logits_.dim() == 2 && logits_.stride(1) == 1 ? logits_ : logits_.contiguous();
+    auto r = router_fwd(logits, k, sigmoid, bias, groups, top_groups, group_top, renorm, scale);
+    ctx->save_for_backward({logits, r[0]});
+    ctx->saved_data["sigmoid"] = sigmoid;
+    ctx->saved_data["renorm"] = renorm;
+    ctx->saved_data["scale"] = scale;
+    ctx->mark_non_differentiable({r[0], r[3]});
+    ctx->set_materialize_grads(false);  // no zeros for the outputs without a gradient
+    return r;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto t = ctx->get_saved_variables();
+    const auto f32 = t[0].options().dtype(torch::kFloat32);
+    auto dtopw = grads[1].defined() ? grads[1].to(torch::kFloat32).contiguous() : torch::zeros(t[1].sizes(), f32);
+    auto du = grads[2].defined() ? grads[2].to(torch::kFloat32).contiguous() : torch::Tensor();
+    ++g_node_backwards;
+    auto dx = router_bwd(t[0], t[1], dtopw, maybe(du), ctx->saved_data["sigmoid"].toBool(),
+                         ctx->saved_data["renorm"].toBool(), ctx->saved_data["scale"].toDouble());
+    variable_list out(9);
+    out[0] = dx;
+    return out;
+  }
+};
+
+torch::Tensor doc_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, double scale, double cap,
+                            c10::optional<torch::Tensor> slopes, bool causal, std::vector<torch::Tensor> mask,
+                            torch::Tensor status) {
+  return DocAttention::apply(q, k, v, DaOptions{scale, cap, causal, slopes.value_or(torch::Tensor()), status, mask});
+}
+torch::Tensor doc_attention_qkv(torch::Tensor qkv, int64_t Hq, int64_t Hk, int64_t D, double scale, double cap,
+                                c10::optional<torch::Tensor> slopes, bool causal, std::vector<torch::Tensor> mask,
+                                torch::Tensor status) {
+  return DocAttentionQKV::apply(qkv, Hq, Hk, D,
+                                DaOptions{scale, cap, causal, slopes.value_or(torch::Tensor()), status, mask});
+}
+torch::Tensor embedding_lookup(torch::Tensor ids, torch::Tensor w, double scale, torch::Tensor status) {
+  return EmbeddingLookup::apply(ids, w, scale, status);
+}
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> router_topk(
+    torch::Tensor logits, int64_t k, bool sigmoid, c10::optional<torch::Tensor> bias, int64_t groups,
+    int64_t top_groups, int64_t group_top, bool renorm, double scale) {
+  auto r = RouterTopK::apply(logits, k, sigmoid, bias, groups, top_groups, group_top, renorm, scale);
+  return {r[0], r[1], r[2], r[3]};
+}
+
+}  // namespace
+
 // Raises through the launchers' own error path (no CUDA involved), so a test
 // can check that a failed host-side check reaches Python as an exception.
 void host_check_selftest(int64_t v) { OXI_CHECK(v == 0, "value ", v, " of ", 2.5, " ", true); }
@@ -1398,9 +1556,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("document_mask", &document_mask, "visible key ranges and tile tables of packed documents");
   m.def("doc_attn_fwd", &doc_attn_fwd, "attention over visible key ranges, forward");
   m.def("doc_attn_bwd", &doc_attn_bwd, "attention over visible key ranges, backward");
-  m.def("doc_attn_qkv_fwd", &doc_attn_qkv_fwd, "the same from a fused projection");
-  m.def("doc_attn_qkv_bwd", &doc_attn_qkv_bwd, "its gradient in the projection's layout");
+  m.def("doc_attention", &doc_attention, "attention over visible key ranges with its gradient");
+  m.def("doc_attention_qkv", &doc_attention_qkv, "the same from a fused projection");
   m.def("doc_attn_supported", [](int64_t Dqk, int64_t Dv) { return oxi::da_supported((int)Dqk, (int)Dv); });
+  m.def("embedding_lookup", &embedding_lookup, "scaled embedding lookup with its gradient");
   m.def("embedding_fwd", &embedding_fwd, "scaled embedding lookup");
   m.def("embedding_bwd", &embedding_bwd, "embedding gradient by sorted tokens");
   m.def("rope_bwd_to", &rope_bwd_to, "out-of-place RoPE backward (+ copy of the unrotated columns)");
@@ -1436,6 +1595,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ssm_scan_bwd", &ssm_scan_bwd, "Mamba2/3 selective scan backward");
   m.def("mamba1_scan_fwd", &mamba1_scan_fwd, "Mamba1 selective scan forward (saves states)");
   m.def("mamba1_scan_bwd", &mamba1_scan_bwd, "Mamba1 selective scan backward");
+  m.def("router_topk", &router_topk, "routing with its gradient");
+  m.def("node_backwards", []() { return g_node_backwards.load(); }, "library calls made by C++ nodes' backward passes");
   m.def("router_fwd", &router_fwd, "MoE router softmax + top-k + usage");
   m.def("router_bwd", &router_bwd, "MoE router backward");
   m.def("moe_permute", &moe_permute, "MoE counting-sort permutation into aligned expert segments");

@@ -63,8 +63,30 @@ class _Counter:
     LAUNCHES_PER_CALL = {"gemm_ce": 1, "adamw": 1}
 
     def __init__(self):
-        self.enabled = False
-        self.count = 0
+        self._on, self._n, self._base = False, 0, 0
+
+    @staticmethod
+    def _node_calls() -> int:
+        # calls that the extension's own autograd nodes made from their backward passes
+        return _ext._mod.node_backwards() if _ext._mod is not None else 0
+
+    @property
+    def enabled(self) -> bool:
+        return self._on
+
+    @enabled.setter
+    def enabled(self, on: bool) -> None:
+        if self._on:
+            self._n += self._node_calls() - self._base
+        self._on, self._base = bool(on), self._node_calls()
+
+    @property
+    def count(self) -> int:
+        return self._n + (self._node_calls() - self._base if self._on else 0)
+
+    @count.setter
+    def count(self, n: int) -> None:
+        self._n, self._base = n, self._node_calls()
 
     def wrap(self, mod):
         counter = self
@@ -76,8 +98,8 @@ class _Counter:
                     return fn
 
                 def call(*a, **k):
-                    if counter.enabled:
-                        counter.count += counter.LAUNCHES_PER_CALL.get(name, 1)
+                    if counter._on:
+                        counter._n += counter.LAUNCHES_PER_CALL.get(name, 1)
                     if not _DEBUG_SYNC:
                         return fn(*a, **k)
                     # debugging aid: find the first launch that faults (OXI_DEBUG_SYNC=1)

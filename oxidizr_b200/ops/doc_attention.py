@@ -11,7 +11,7 @@ and a token that sees nothing (padding) gets zeros and passes no gradient on.  W
 q, k, v and the output's gradient hold does not matter, not even NaN.
 
 bf16 CUDA tensors with head widths that are multiples of 8 up to 128 run csrc/doc_attn_fwd.cu and
-csrc/doc_attn_bwd.cu; everything else runs the statement of the same math in ``ops.reference``.
+csrc/doc_attn_bwd.cu (autograd nodes in csrc/ops.cpp, first derivatives only); everything else runs the statement of the same math in ``ops.reference``.
 """
 from __future__ import annotations
 
@@ -95,44 +95,6 @@ def _check(t, B, S, Hq, scale, causal, mask, softcap, alibi):
             raise ValueError("attention: alibi slopes are constants, no gradient is computed for them")
 
 
-class DocAttention(torch.autograd.Function):
-    """q [B, S, Hq, Dqk], k [B, S, Hk, Dqk], v [B, S, Hk, Dv] views -> o [B, S, Hq, Dv]."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, scale: float, cap: float, slopes, causal: bool, mask):
-        o, nlse2 = ext().doc_attn_fwd(q, k, v, scale, cap, slopes, causal, mask, status(q.device))
-        ctx.save_for_backward(q, k, v, o, nlse2, slopes, *mask)
-        ctx.cfg = (scale, cap, causal)
-        return o
-
-    @staticmethod
-    def backward(ctx, do):
-        q, k, v, o, nlse2, slopes, *mask = ctx.saved_tensors
-        scale, cap, causal = ctx.cfg
-        dq, dk, dv = ext().doc_attn_bwd(q, k, v, o, do, nlse2, scale, cap, slopes, causal, mask, status(q.device))
-        return dq, dk, dv, None, None, None, None, None
-
-
-class DocAttentionQKV(torch.autograd.Function):
-    """The same from the fused projection [B, S, (Hq + 2 Hk) D] -> [B, S, Hq D]; the gradient is
-    written in the projection's layout, with no assembly of slices."""
-
-    @staticmethod
-    def forward(ctx, qkv, Hq: int, Hk: int, D: int, scale: float, cap: float, slopes, causal: bool, mask):
-        o, nlse2 = ext().doc_attn_qkv_fwd(qkv, Hq, Hk, D, scale, cap, slopes, causal, mask, status(qkv.device))
-        ctx.save_for_backward(qkv, o, nlse2, slopes, *mask)
-        ctx.cfg = (Hq, Hk, D, scale, cap, causal)
-        return o
-
-    @staticmethod
-    def backward(ctx, do):
-        qkv, o, nlse2, slopes, *mask = ctx.saved_tensors
-        Hq, Hk, D, scale, cap, causal = ctx.cfg
-        dqkv = ext().doc_attn_qkv_bwd(qkv, Hq, Hk, D, o, do, nlse2, scale, cap, slopes, causal, mask,
-                                      status(qkv.device))
-        return dqkv, None, None, None, None, None, None, None, None
-
-
 def _reference(q, k, v, scale, causal, mask, softcap, alibi):
     lo, hi = (mask.lo, mask.hi) if mask is not None else R.plain_ranges(q.shape[0], q.shape[1], causal, q.device)
     o = R.attention_ranges(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), scale, lo, hi, softcap, alibi)
@@ -152,7 +114,7 @@ def attention(q, k, v, scale: float, causal: bool = True, mask: Optional[DocMask
     _check(q, B, S, Hq, scale, causal, mask, softcap, alibi)
     if _kernel_ok(q, D, v.shape[3]) and k.dtype == q.dtype and v.dtype == q.dtype:
         slopes, m = _options(alibi, mask)
-        return DocAttention.apply(q, k, v, float(scale), float(softcap), slopes, causal, m)
+        return ext().doc_attention(q, k, v, scale, softcap, slopes, causal, m, status(q.device))
     return _reference(q, k, v, scale, causal, mask, softcap, alibi)
 
 
@@ -164,6 +126,6 @@ def attention_qkv(qkv, Hq: int, Hk: int, D: int, scale: float, causal: bool = Tr
     _check(qkv, B, S, Hq, scale, causal, mask, softcap, alibi)
     if _kernel_ok(qkv, D, D):
         slopes, m = _options(alibi, mask)
-        return DocAttentionQKV.apply(qkv, Hq, Hk, D, float(scale), float(softcap), slopes, causal, m)
+        return ext().doc_attention_qkv(qkv, Hq, Hk, D, scale, softcap, slopes, causal, m, status(qkv.device))
     q, k, v = (t.unflatten(-1, (-1, D)) for t in qkv.split([Hq * D, Hk * D, Hk * D], -1))
     return _reference(q, k, v, scale, causal, mask, softcap, alibi).flatten(2)

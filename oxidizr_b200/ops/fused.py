@@ -77,12 +77,9 @@ def _c(t: torch.Tensor) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------- embedding
-class Embedding(torch.autograd.Function):
-    """w[ids] * scale; the gradient sums each row's tokens in f32 in their order, by sorting them
-    (csrc/embed.cu), so it is the same from run to run."""
-
+class _EmbeddingMainGrad(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, ids, w, scale: float = 1.0):
+    def forward(ctx, ids, w, scale: float):
         ids_f = _c(ids.reshape(-1))
         out = ext().embedding_fwd(ids_f, _c(w), scale, status(w.device))
         ctx.save_for_backward(ids_f)
@@ -93,13 +90,22 @@ class Embedding(torch.autograd.Function):
     def backward(ctx, dy):
         (ids,) = ctx.saved_tensors
         w = ctx.w
-        dy = _c(dy.reshape(-1, w.shape[1]))
-        mg = getattr(w, "main_grad", None)
-        if mg is not None:
-            ext().embedding_bwd(ids, dy, w.shape[0], ctx.scale, mg.view(w.shape))
-            _ready(w)
-            return None, None, None
-        return None, ext().embedding_bwd(ids, dy, w.shape[0], ctx.scale, None), None
+        ext().embedding_bwd(ids, _c(dy.reshape(ids.numel(), w.shape[1])), w.shape[0], ctx.scale,
+                            w.main_grad.view(w.shape))
+        _ready(w)
+        return None, None, None
+
+
+class Embedding:
+    """w[ids] * scale; the gradient sums each row's tokens in f32 in their order, by sorting them
+    (csrc/embed.cu), so it is the same from run to run.  Without ``main_grad`` on w the node is the one in
+    csrc/ops.cpp."""
+
+    @staticmethod
+    def apply(ids, w, scale: float = 1.0):
+        if getattr(w, "main_grad", None) is not None:
+            return _EmbeddingMainGrad.apply(ids, w, scale)
+        return ext().embedding_lookup(ids, w, scale, status(w.device))
 
 
 # ------------------------------------------------------------------- norms

@@ -104,32 +104,17 @@ def grouped_ok(x: torch.Tensor, w_gu: torch.Tensor) -> bool:
             and hasattr(ext(), "gemm_grouped"))
 
 
-class RouterTopK(torch.autograd.Function):
+class RouterTopK:
     """The router of csrc/router.cu: scores, choice, weights, mean normalised score and counts.
 
-    Returns ``(topi [T,k] int64, topw [T,k] f32, usage [E] f32, counts [E] int32)``; ``usage`` and
-    ``topw`` carry gradients.  The options are those of ``ops.api.route_topk``.
+    ``apply`` returns ``(topi [T,k] int64, topw [T,k] f32, usage [E] f32, counts [E] int32)``; ``usage`` and
+    ``topw`` carry gradients (an autograd node in csrc/ops.cpp).  The options are those of ``ops.api.route_topk``.
     """
 
     @staticmethod
-    def forward(ctx, logits, k: int, score: str = "softmax", bias=None, groups: int = 1, top_groups: int = 1,
-                group_top: int = 2, renorm: bool = True, scale: float = 1.0):
-        if logits.stride(1) != 1:
-            logits = logits.contiguous()
-        topi, topw, usage, counts = ext().router_fwd(logits, int(k), score == "sigmoid", bias, groups, top_groups,
-                                                     group_top, renorm, scale)
-        ctx.save_for_backward(logits, topi)
-        ctx.cfg = (score == "sigmoid", renorm, scale)
-        ctx.mark_non_differentiable(topi, counts)
-        ctx.set_materialize_grads(False)  # no zeros for the outputs without a gradient
-        return topi, topw, usage, counts
-
-    @staticmethod
-    def backward(ctx, _dtopi, dtopw, dusage, _dcounts):
-        logits, topi = ctx.saved_tensors
-        dtopw = torch.zeros(topi.shape, device=topi.device) if dtopw is None else dtopw.float().contiguous()
-        du = None if dusage is None else dusage.float().contiguous()
-        return ext().router_bwd(logits, topi, dtopw, du, *ctx.cfg), *[None] * 8
+    def apply(logits, k: int, score: str = "softmax", bias=None, groups: int = 1, top_groups: int = 1,
+              group_top: int = 2, renorm: bool = True, scale: float = 1.0):
+        return ext().router_topk(logits, k, score == "sigmoid", bias, groups, top_groups, group_top, renorm, scale)
 
 
 ROUTE_MAX_EXPERTS, ROUTE_MAX_K, ROUTE_MAX_GROUPS = 512, 32, 32  # csrc/kernels_moe.h

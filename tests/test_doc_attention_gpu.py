@@ -321,3 +321,49 @@ def test_refusals_on_the_gpu():
         api.attention(q[:, :8], k[:, :8], v[:, :8], 0.25, mask=m)
     with pytest.raises(ValueError, match="slope"):
         api.attention(q, k, v, 0.25, mask=m, alibi=torch.ones(2))
+
+
+def test_graph_is_kept_and_second_derivatives_are_refused():
+    torch.manual_seed(3)
+    qkv = torch.randn(2, 70, 3 * 64, device="cuda").bfloat16().requires_grad_()
+    o = api.attention_qkv(qkv, 1, 1, 64, 0.125, softcap=20.0)
+    do = torch.randn_like(o)
+    a, = torch.autograd.grad(o, qkv, do, retain_graph=True)
+    b, = torch.autograd.grad(o, qkv, do, retain_graph=True)
+    assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="first derivatives"):
+        torch.autograd.grad(o, qkv, do, create_graph=True)
+    q, k, v = (t.unflatten(-1, (1, 64)) for t in qkv.split(64, -1))
+    o2 = api.attention(q, k, v, 0.125, softcap=20.0)
+    assert torch.equal(o2.flatten(2), o)
+    c, = torch.autograd.grad(o2, qkv, do.view_as(o2))
+    assert torch.equal(a, c)
+    with torch.no_grad():
+        assert not api.attention(q, k, v, 0.125, softcap=20.0).requires_grad
+
+
+def test_only_some_operands_want_gradients():
+    torch.manual_seed(4)
+    q, k, v = (torch.randn(1, 90, 2, 64, device="cuda").bfloat16() for _ in range(3))
+    do = torch.randn_like(q)
+    for t in (q, k, v):
+        t.requires_grad_()
+    full = torch.autograd.grad(api.attention(q, k, v, 0.125, softcap=5.0), (q, k, v), do)
+    k.requires_grad_(False)
+    part = torch.autograd.grad(api.attention(q, k, v, 0.125, softcap=5.0), (q, v), do)
+    assert torch.equal(part[0], full[0]) and torch.equal(part[1], full[2])
+
+
+def test_launches_of_backward_passes_are_counted():
+    from oxidizr_b200.ops._C import launch_counter
+    qkv = torch.randn(1, 70, 3 * 64, device="cuda").bfloat16().requires_grad_()
+    launch_counter.count = 0
+    launch_counter.enabled = True
+    try:
+        api.attention_qkv(qkv, 1, 1, 64, 0.125, softcap=20.0).sum().backward()
+    finally:
+        launch_counter.enabled = False
+    n = launch_counter.count
+    assert n == 2
+    api.attention_qkv(qkv, 1, 1, 64, 0.125, softcap=20.0).sum().backward()
+    assert launch_counter.count == n

@@ -14,7 +14,7 @@
 // the m of the steps before it, so that its exponentials wait for no maximum, and the maximum found
 // meanwhile moves m (and rescales O in TMEM) for the next step when it is more than 8 above.  Only
 // where it is more than 60 above, or a row sees its first keys, is the step's own maximum used.
-// Scores capped at up to 60 log 2 need no maximum at all: m = 0.
+// Scores capped at up to 60 log 2 need no maximum at all: m = 0 (unless a negative slope adds to them).
 // Steps outside the bounds of the query tile's ranges are not loaded or computed; a step that is
 // wholly visible to a warp's 32 rows is computed without a mask.
 // Warps: 0 TMA, 1 MMA + TMEM owner, 2..5 softmax and output.
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const float slope2 = ALIBI ? __ldg(p.slopes + h) * LOG2E : 0.f;
     const float C = ALIBI ? 1.f : p.c_log2;
-    const bool bounded = CAP && p.c_log2 <= 60.f;
+    const bool bounded = CAP && p.c_log2 <= 60.f && slope2 >= 0.f;
     float m = bounded ? 0.f : -INFINITY, m_next = m, l = 0.f;
     bool ok = true;
     // O times 2^(m - m_new), m = m_new; O belongs to the product of step i - 1 until it completes.  Called

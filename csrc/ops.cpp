@@ -410,7 +410,7 @@ std::vector<torch::Tensor> document_mask(torch::Tensor tokens, c10::optional<tor
   return {lo, hi, qt, kt};
 }
 
-// An operand [B, S, H, D] that tensor maps can address, t itself or a contiguous copy.  The stride of a
+// An operand [B, S, H, D] that tensor maps can address, t itself or a copy.  The stride of a
 // dimension of one element is never used and need not be a valid one.
 struct DaOperand {
   torch::Tensor t;
@@ -423,7 +423,7 @@ DaOperand da_operand(const torch::Tensor& t, const torch::Tensor& like, const ch
   r.t = t;
   bool ok = t.stride(3) == 1 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
   for (int i = 0; i < 3 && ok; ++i) ok = t.size(i) == 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0);
-  if (!ok) r.t = t.contiguous();
+  if (!ok) r.t = t.clone(at::MemoryFormat::Contiguous);  // contiguous() would keep a misaligned base
   int64_t st[3];
   for (int i = 0; i < 3; ++i) st[i] = r.t.size(i) == 1 ? 8 : r.t.stride(i);
   r.d = {r.t.data_ptr(), st[0], st[1], st[2]};
@@ -450,7 +450,7 @@ oxi::DaShape da_shape(const torch::Tensor& q, const torch::Tensor& k, const torc
   s.Dqk = (int)q.size(3); s.Dv = (int)v.size(3);
   OXI_CHECK(k.size(0) == s.B && v.size(0) == s.B && k.size(1) == s.S && v.size(1) == s.S && v.size(2) == s.Hk &&
                 k.size(3) == s.Dqk, "attention: q, k, v do not go together");
-  OXI_CHECK(s.Hk > 0 && s.Hq % s.Hk == 0, "attention: query heads must be a multiple of key heads");
+  OXI_CHECK(s.Hk > 0 && s.Hq > 0 && s.Hq % s.Hk == 0, "attention: query heads must be a multiple of key heads");
   s.scale = (float)scale;
   s.cap = (float)cap;
   s.causal = causal;
@@ -464,7 +464,7 @@ oxi::DaShape da_shape(const torch::Tensor& q, const torch::Tensor& k, const torc
     const int64_t nt = (s.S + oxi::DA_TILE - 1) / oxi::DA_TILE;
     for (size_t i = 0; i < 4; ++i) {
       const auto& m = mask[i];
-      OXI_CHECK(m.device() == q.device() && m.scalar_type() == torch::kInt32 && m.is_contiguous() &&
+      OXI_CHECK(m.defined() && m.device() == q.device() && m.scalar_type() == torch::kInt32 && m.is_contiguous() &&
                     m.numel() == (i < 2 ? (int64_t)s.B * s.S : (int64_t)s.B * nt * 4),
                 "attention: the mask was built for another batch or device");
     }

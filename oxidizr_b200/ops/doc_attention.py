@@ -86,6 +86,8 @@ def _check(t, B, S, Hq, scale, causal, mask, softcap, alibi):
         if mask.lo.shape != (B, S) or mask.lo.device != t.device:
             raise ValueError(f"attention: the mask is for {list(mask.lo.shape)} on {mask.lo.device}, "
                              f"q for {[B, S]} on {t.device}")
+        if mask.lo.is_cuda and (mask.qt is None or mask.kt is None):
+            raise ValueError("attention: the mask has no tile tables; document_mask makes them")
         if mask.causal != causal:
             raise ValueError(f"attention: causal={causal} with a mask built for causal={mask.causal}")
     if alibi is not None:
@@ -109,7 +111,7 @@ def attention(q, k, v, scale: float, causal: bool = True, mask: Optional[DocMask
               alibi: Optional[torch.Tensor] = None) -> torch.Tensor:
     B, S, Hq, D = q.shape
     Hk = k.shape[2]
-    if k.shape != (B, S, Hk, D) or v.shape[:3] != (B, S, Hk) or Hk == 0 or Hq % Hk:
+    if k.shape != (B, S, Hk, D) or v.shape[:3] != (B, S, Hk) or Hk < 1 or Hq < 1 or Hq % Hk:
         raise ValueError(f"attention: q {list(q.shape)}, k {list(k.shape)}, v {list(v.shape)} do not go together")
     _check(q, B, S, Hq, scale, causal, mask, softcap, alibi)
     if _kernel_ok(q, D, v.shape[3]) and k.dtype == q.dtype and v.dtype == q.dtype:

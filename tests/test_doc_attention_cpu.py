@@ -180,3 +180,13 @@ def test_the_extension_refuses_with_exceptions():
         e.document_mask(torch.zeros(1, 4, dtype=torch.int64), None, None, None, True)
     with pytest.raises((RuntimeError, ValueError)):
         e.doc_attn_fwd(x, x, x, 0.1, 0.0, None, True, [], st)
+    with pytest.raises(RuntimeError):
+        e.doc_attention(x, x, x, 0.1, 0.0, None, True, [], st)
+    with pytest.raises(RuntimeError):
+        e.doc_attention_qkv(x.flatten(2), 1, 1, 8, 0.1, 0.0, None, True, [], st)
+
+
+def test_no_heads_are_refused():
+    k = torch.zeros(1, 4, 2, 8)
+    with pytest.raises(ValueError, match="do not go together"):
+        api.attention(torch.zeros(1, 4, 0, 8), k, k, 0.1, softcap=1.0)

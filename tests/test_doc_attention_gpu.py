@@ -367,3 +367,31 @@ def test_launches_of_backward_passes_are_counted():
     assert n == 2
     api.attention_qkv(qkv, 1, 1, 64, 0.125, softcap=20.0).sum().backward()
     assert launch_counter.count == n
+
+
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+def test_negative_slopes(cap):
+    """A bias that grows with the distance: scores far above the cap, whose sums must not overflow."""
+    S = 400
+    m = api.document_mask(torch.zeros(1, S, dtype=torch.int64, device="cuda"))
+    slopes = torch.tensor([-1.0, 0.5], device="cuda")
+    q, k, v, do = inputs(1, S, 2, 1, 64, 64, seed=11)
+    got = run(q, k, v, do, 0.125, mask=m, softcap=cap, alibi=slopes)
+    check(got, oracle(q, k, v, do, 0.125, m, cap, slopes))
+    finish()
+
+
+def test_operands_off_the_alignment():
+    """Contiguous operands whose first element is not at a multiple of 16 bytes are copied."""
+    q, k, v, do = inputs(2, 130, 2, 2, 64, 64, seed=12)
+    want = run(q, k, v, do, 0.125, softcap=20.0)
+
+    def shifted(t):
+        buf = torch.empty(t.numel() + 3, dtype=t.dtype, device="cuda")
+        buf[3:].copy_(t.detach().reshape(-1))
+        return buf[3:].view(t.shape)
+
+    got = run(*(shifted(t).requires_grad_() for t in (q, k, v)), shifted(do), 0.125, softcap=20.0)
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    finish()

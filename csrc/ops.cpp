@@ -402,8 +402,10 @@ std::vector<torch::Tensor> document_mask(torch::Tensor tokens, c10::optional<tor
   }
   const int64_t nt = (S + oxi::DA_TILE - 1) / oxi::DA_TILE;
   auto opt = torch::TensorOptions().dtype(torch::kInt32).device(tokens.device());
-  auto lo = torch::empty({B, S}, opt), hi = torch::empty({B, S}, opt);
-  auto qt = torch::empty({B, nt, 4}, opt), kt = torch::empty({B, nt, 4}, opt);
+  // one allocation: the host's time is what a short batch costs
+  auto all = torch::empty({B * (8 * nt + 2 * S)}, opt);
+  auto qt = all.as_strided({B, nt, 4}, {4 * nt, 4, 1}, 0), kt = all.as_strided({B, nt, 4}, {4 * nt, 4, 1}, 4 * B * nt);
+  auto lo = all.as_strided({B, S}, {S, 1}, 8 * B * nt), hi = all.as_strided({B, S}, {S, 1}, 8 * B * nt + B * S);
   oxi::launch_document_mask(tokens.data_ptr<int64_t>(), tokens.stride(0), pre, ldp, (int)B, (int)S,
                             separator.has_value(), separator.value_or(0), pad.has_value(), pad.value_or(0), causal,
                             lo.data_ptr<int>(), hi.data_ptr<int>(), qt.data_ptr<int>(), kt.data_ptr<int>(), stream());

@@ -395,3 +395,30 @@ def test_operands_off_the_alignment():
     for a, b in zip(got, want):
         assert torch.equal(a, b)
     finish()
+
+
+@pytest.mark.parametrize("S", [4097, 8192, 12417, 33000])
+@pytest.mark.parametrize("mean", [30, 5000, 10 ** 6])
+def test_ranges_across_slices(S, mean):
+    """Documents, prompts and padding that reach over several CTAs' slices of a row, and none that do."""
+    from oxidizr_b200.ops import reference as R
+    doc, flags = layout(3, S, mean, S + mean)
+    long = torch.arange(S, device="cuda").expand(3, S) < torch.tensor([[S], [S // 2], [4096]], device="cuda")
+    for prefix, causal in ((None, True), (None, False), (flags, True), (long, True), (~long, True)):
+        m = api.document_mask(doc, prefix=prefix, causal=causal)
+        lo, hi = R.document_ranges(doc, prefix=prefix, causal=causal)
+        assert torch.equal(m.lo, lo) and torch.equal(m.hi, hi)
+        nt = (S + 127) // 128
+        pad = nt * 128 - S
+        some = torch.nn.functional.pad(hi > lo, (0, pad)).view(3, nt, 128)
+        a = torch.nn.functional.pad(lo, (0, pad)).view(3, nt, 128)
+        e = torch.nn.functional.pad(hi, (0, pad)).view(3, nt, 128)
+        kmin = a.masked_fill(~some, 2 ** 31 - 1).amin(-1) * some.any(-1)
+        kmax = e.masked_fill(~some, 0).amax(-1)
+        assert torch.equal(m.qt[..., 0], kmin.int()) and torch.equal(m.qt[..., 1], kmax)
+        k0 = torch.arange(nt, device="cuda") * 128
+        sees = (kmin[:, :, None] < k0 + 128) & (kmax[:, :, None] > k0)  # [B, query tile, key tile]
+        n = torch.arange(nt, device="cuda")[:, None]
+        end = torch.where(sees, n + 1, 0).amax(1)
+        first = torch.where(sees, n, nt).amin(1) * (end > 0)
+        assert torch.equal(m.kt[..., 0], first.int()) and torch.equal(m.kt[..., 1], end.int())

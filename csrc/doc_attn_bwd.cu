@@ -245,7 +245,11 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
       }
     }
     asm volatile("bar.sync 1, 512;" ::: "memory");  // delta's rows; reached by every softmax warp
+    // keys that all of the warp's rows see, and that any does
     const int all_lo = __reduce_max_sync(0xffffffffu, vis.begin), all_hi = __reduce_min_sync(0xffffffffu, vis.end);
+    const bool sees = vis.end > vis.begin;
+    const int any_lo = __reduce_min_sync(0xffffffffu, sees ? vis.begin : INT_MAX);
+    const int any_hi = __reduce_max_sync(0xffffffffu, sees ? vis.end : 0);
     const uint32_t s_addr = TM_S + mine * DQ_KEYS + lane_base + half * 32;
     const uint32_t dp_addr = TM_DP + mine * DQ_KEYS + lane_base + half * 32;
     const float ndl = s_row[r];
@@ -257,6 +261,14 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
       const bool padded = tile_has_pad(p, b, k0 / DA_TILE);
       if (!mbar_wait(&s_full[mine], ph, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
+      if (k0 >= any_hi || k0 + 32 <= any_lo) {  // nothing here is seen by the warp's rows
+        if (!mbar_wait(&dp_full[mine], ph, abort_flag, p.status)) { ok = false; break; }
+        tc_fence_after();
+        uint32_t zero[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) zero[e] = 0u;
+        tmem_st16(dp_addr, zero);
+      } else {
       uint64_t x[16], f[CAP ? 16 : 1];  // scores, then P; the cap's derivative
       tmem_ld_pairs(s_addr, x);
       const bool masked = !(all_lo <= k0 && k0 + 32 <= all_hi);
@@ -303,6 +315,7 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
       };
       if (masked) gradients(std::true_type{});
       else gradients(std::false_type{});
+      }
       // S_i has read K_i: rows of padding become zero before the dQ product reads them
       if (padded)
         zero_pad_rows<L::KBQ, DQ_KEYS>(sK + (i % L::ST) * L::K_BYTES, p, b, (kr.begin + i) * DQ_KEYS, half * 128 + r, 256);
@@ -581,8 +594,20 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
       if (!mbar_wait(&vec_full[st], u & 1, abort_flag, p.status) ||
           !mbar_wait(&s_full[mine], ph, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
+      bool hidden = false;  // none of the warp's queries sees any of its keys
+      if (masked) {
+        const int w0 = kt * DA_TILE + quarter * 32, q = q0 + half * 32 + lane;
+        const int* range = reinterpret_cast<const int*>(s_vec + st * L::VEC + half * 32 + lane);
+        const int lo = p.lo ? range[2 * KV_QUERIES] : 0;
+        const int hi = p.lo ? range[3 * KV_QUERIES] : (q < p.S ? (p.causal ? q + 1 : p.S) : 0);
+        hidden = !__any_sync(0xffffffffu, lo < w0 + 32 && hi > w0);
+      }
       uint64_t x[16];  // scores, then P times the cap's derivative
       uint32_t pk[16];
+      if (hidden) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) pk[e] = 0u;
+      } else {
       tmem_ld_pairs(s_addr, x);
       auto probabilities = [&](auto near, auto some_hidden) {
         constexpr bool HIDDEN = decltype(some_hidden)::value;
@@ -632,6 +657,7 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
       const bool near = CAP && warp_near(x, p.x_scale);
       if (masked) near ? probabilities(std::true_type{}, std::true_type{}) : probabilities(std::false_type{}, std::true_type{});
       else near ? probabilities(std::true_type{}, std::false_type{}) : probabilities(std::false_type{}, std::false_type{});
+      }
       tmem_st16(s_addr, pk);
       if (padded) {
         if (!mbar_wait(&q_full[st], u & 1, abort_flag, p.status)) { ok = false; break; }
@@ -663,7 +689,8 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
           }
         }
       };
-      if (masked) gradients(std::true_type{});
+      if (hidden) {}  // pk is zero
+      else if (masked) gradients(std::true_type{});
       else gradients(std::false_type{});
       tmem_st16(dp_addr, pk);
       tc_wait_st();

@@ -174,6 +174,10 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
     const TileRange vis = key_range(p, b, qpos);
     // keys that all rows of the warp see
     const int all_lo = __reduce_max_sync(0xffffffffu, vis.begin), all_hi = __reduce_min_sync(0xffffffffu, vis.end);
+    // keys that any of them sees
+    const bool sees = vis.end > vis.begin;
+    const int any_lo = __reduce_min_sync(0xffffffffu, sees ? vis.begin : INT_MAX);
+    const int any_hi = __reduce_max_sync(0xffffffffu, sees ? vis.end : 0);
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const float slope2 = ALIBI ? __ldg(p.slopes + h) * LOG2E : 0.f;
     const float C = ALIBI ? 1.f : p.c_log2;
@@ -208,6 +212,12 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
       if (!mbar_wait(&s_full[i & 1], (i >> 1) & 1, abort_flag, p.status)) { ok = false; break; }
       tc_fence_after();
       if (!bounded && __any_sync(0xffffffffu, m_next > m) && !move(i, m_next)) { ok = false; break; }
+      if (k0 >= any_hi || k0 + FW_KEYS <= any_lo) {  // nothing here is seen by the warp's rows
+        uint32_t zero[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) zero[e] = 0u;
+        tmem_st32(s_addr, zero);
+      } else {
       uint64_t x[2][16];
       {
         uint32_t w[2][32];
@@ -277,6 +287,7 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
       tmem_st16(s_addr + 16, pk[1]);
       const float2 rsum = unpack2(add2(add2(rs[0], rs[1]), add2(rs[2], rs[3])));
       l += rsum.x + rsum.y;
+      }
       if (padded) {
         // V_i has landed before its product may read it; rows of padding become zero
         if (!mbar_wait(&v_full[i % L::VST], (i / L::VST) & 1, abort_flag, p.status)) { ok = false; break; }

@@ -4,6 +4,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 
 #include "gemm_kernel.cuh"
@@ -348,10 +349,15 @@ inline void da_check(const DaShape& s) {
                 (s.lo != nullptr) == (s.kt != nullptr), "ranges and tile tables come together");
 }
 
-// Shared memory attribute of a kernel, set before every launch: it belongs to the current device.
+// Shared memory attribute of a kernel, set once for each device that launches it.
 template <typename K>
-inline void da_smem(K kern, int bytes) {
+inline void da_smem(K kern, int bytes, std::atomic<uint64_t>& devices) {
+  int dev;
+  OXI_CUDA_CHECK(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
+  if (devices.load(std::memory_order_relaxed) & bit) return;
   OXI_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  devices.fetch_or(bit, std::memory_order_relaxed);
 }
 
 }  // namespace

@@ -808,8 +808,9 @@ void launch_bwd_t(const BwdArgs& a) {
                     tdq = da_tmap_out(a.dq, s.B, s.S, s.Hq, s.Dqk);
   auto kq = da_dq_kernel<DQP, DVP, CAP, ALIBI>;
   auto kkv = da_dkv_kernel<DQP, DVP, CAP, ALIBI>;
-  da_smem(kq, DaDqSmem<DQP, DVP>::TOTAL);
-  da_smem(kkv, DaDkvSmem<DQP, DVP>::TOTAL);
+  static std::atomic<uint64_t> dq_devices{0}, dkv_devices{0};
+  da_smem(kq, DaDqSmem<DQP, DVP>::TOTAL, dq_devices);
+  da_smem(kkv, DaDkvSmem<DQP, DVP>::TOTAL, dkv_devices);
   kq<<<dim3(s.Hq, s.B, p.nt), DA_GROUPS_THREADS, DaDqSmem<DQP, DVP>::TOTAL, a.st>>>(tq, tk64, tv64, td, tdq, p, a.o, a.dout,
                                                                                     a.nlse2, a.ndelta);
   OXI_CUDA_CHECK(cudaGetLastError());

@@ -327,7 +327,8 @@ void launch_fwd_t(const DaShape& s, const DaTensor& q, const DaTensor& k, const 
   const CUtensorMap tq = da_tmap(q, s.B, s.S, s.Hq, s.Dqk), tk = da_tmap(k, s.B, s.S, s.Hk, s.Dqk, FW_KEYS),
                     tv = da_tmap(v, s.B, s.S, s.Hk, s.Dv, FW_KEYS), to = da_tmap_out(o, s.B, s.S, s.Hq, s.Dv);
   auto kern = da_fwd_kernel<DQP, DVP, CAP, ALIBI>;
-  da_smem(kern, L::TOTAL);
+  static std::atomic<uint64_t> devices{0};
+  da_smem(kern, L::TOTAL, devices);
   const dim3 grid(s.Hq, s.B, (s.S + DA_TILE - 1) / DA_TILE);
   kern<<<grid, FW_THREADS, L::TOTAL, st>>>(tq, tk, tv, to, da_params(s, status), nlse2);
   OXI_CUDA_CHECK(cudaGetLastError());

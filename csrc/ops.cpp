@@ -1420,6 +1420,7 @@ struct DaOptions {
 struct DocAttention : torch::autograd::Function<DocAttention> {
   static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& q, const torch::Tensor& k,
                                const torch::Tensor& v, const DaOptions& opt) {
+    at::AutoDispatchBelowADInplaceOrView below;  // nothing here is recorded
     torch::Tensor o;
     auto nlse2 = da_forward(q, k, v, opt.scale, opt.cap, maybe(opt.slopes), opt.causal, opt.mask, opt.status, o, false);
     opt.save(ctx, {q, k, v, o, nlse2});
@@ -1427,6 +1428,7 @@ struct DocAttention : torch::autograd::Function<DocAttention> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     first_order_only("attention");
+    at::AutoDispatchBelowADInplaceOrView below;
     const auto t = ctx->get_saved_variables();
     const auto opt = DaOptions::load(ctx, t, 5);
     ++g_node_backwards;
@@ -1441,6 +1443,7 @@ struct DocAttention : torch::autograd::Function<DocAttention> {
 struct DocAttentionQKV : torch::autograd::Function<DocAttentionQKV> {
   static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& qkv, int64_t Hq, int64_t Hk, int64_t D,
                                const DaOptions& opt) {
+    at::AutoDispatchBelowADInplaceOrView below;  // nothing here is recorded
     const auto h = da_heads(qkv, Hq, Hk, D);
     torch::Tensor o;
     auto nlse2 = da_forward(h[0], h[1], h[2], opt.scale, opt.cap, maybe(opt.slopes), opt.causal, opt.mask, opt.status,
@@ -1451,6 +1454,7 @@ struct DocAttentionQKV : torch::autograd::Function<DocAttentionQKV> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     first_order_only("attention");
+    at::AutoDispatchBelowADInplaceOrView below;
     const auto t = ctx->get_saved_variables();
     const auto opt = DaOptions::load(ctx, t, 3);
     const auto h = ctx->saved_data["heads"].toIntVector();
@@ -1464,6 +1468,7 @@ struct DocAttentionQKV : torch::autograd::Function<DocAttentionQKV> {
 struct EmbeddingLookup : torch::autograd::Function<EmbeddingLookup> {
   static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& ids, const torch::Tensor& w, double scale,
                                const torch::Tensor& status) {
+    at::AutoDispatchBelowADInplaceOrView below;  // nothing here is recorded
     const auto flat = ids.contiguous().view({-1});
     auto out = embedding_fwd(flat, w.contiguous(), scale, status);
     auto shape = ids.sizes().vec();
@@ -1487,6 +1492,7 @@ struct RouterTopK : torch::autograd::Function<RouterTopK> {
   static variable_list forward(AutogradContext* ctx, const torch::Tensor& logits_, int64_t k, bool sigmoid,
                                const c10::optional<torch::Tensor>& bias, int64_t groups, int64_t top_groups,
                                int64_t group_top, bool renorm, double scale) {
+    at::AutoDispatchBelowADInplaceOrView below;  // nothing here is recorded
     const auto logits = logits_.dim() == 2 && logits_.stride(1) == 1 ? logits_ : logits_.contiguous();
     auto r = router_fwd(logits, k, sigmoid, bias, groups, top_groups, group_top, renorm, scale);
     ctx->save_for_backward({logits, r[0]});

@@ -111,6 +111,7 @@ class _Counter:
                     except RuntimeError as e:
                         raise RuntimeError(f"oxidizr kernel call {name!r} failed: {e}") from e
                     return r
+                self.__dict__[name] = call  # the next call of this name does not come here
                 return call
 
             def __dir__(self):

@@ -272,11 +272,14 @@ __device__ __forceinline__ void tma_store_4d(const void* tmap, const void* smem_
                "r"(smem_u32(smem_src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
                : "memory");
 }
-// one block of 64 columns (kb, of `width` columns) of rows 32 * quarter .. from token pos
+// one block of 64 columns (kb, of `width` columns) of rows 32 * quarter .. from token pos.  LOW: also what
+// rounding the values to bf16 leaves over, as bf16, by way of stage_lo to tmap_lo
+template <bool LOW = false>
 __device__ __forceinline__ void store_block(uint8_t* stage, uint32_t taddr, int kb, int width, int quarter, float f,
-                                            bool zero, bool nan, const void* tmap, int head, int pos, int S, int b) {
+                                            bool zero, bool nan, const void* tmap, int head, int pos, int S, int b,
+                                            uint8_t* stage_lo = nullptr, const void* tmap_lo = nullptr) {
   const int lane = threadIdx.x & 31;
-  uint8_t* slab = stage + kb * (DA_TILE * 128) + quarter * (32 * 128);
+  const int at = kb * (DA_TILE * 128) + quarter * (32 * 128);
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     uint32_t w[32];
@@ -284,19 +287,26 @@ __device__ __forceinline__ void store_block(uint8_t* stage, uint32_t taddr, int 
     tc_wait_ld();
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      uint32_t u[4];
+      uint32_t u[4], lo[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        u[e] = pack_bf16(__uint_as_float(w[q * 8 + 2 * e]) * f, __uint_as_float(w[q * 8 + 2 * e + 1]) * f);
-        if (zero) u[e] = nan ? 0x7fff7fffu : 0u;
+        const float x = __uint_as_float(w[q * 8 + 2 * e]) * f, y = __uint_as_float(w[q * 8 + 2 * e + 1]) * f;
+        u[e] = pack_bf16(x, y);
+        lo[e] = LOW ? pack_bf16(x - __uint_as_float(u[e] << 16), y - __uint_as_float(u[e] & 0xffff0000u)) : 0u;
+        if (zero) {
+          u[e] = nan ? 0x7fff7fffu : 0u;
+          lo[e] = 0u;
+        }
       }
-      sw128_store16(slab, lane, c * 4 + q, make_uint4(u[0], u[1], u[2], u[3]));
+      sw128_store16(stage + at, lane, c * 4 + q, make_uint4(u[0], u[1], u[2], u[3]));
+      if (LOW) sw128_store16(stage_lo + at, lane, c * 4 + q, make_uint4(lo[0], lo[1], lo[2], lo[3]));
     }
   }
   fence_proxy_async_smem();
   __syncwarp();
   if (lane == 0 && kb * 64 < width && pos + quarter * 32 < S) {
-    tma_store_4d(tmap, slab, kb * 64, head, pos + quarter * 32, b);
+    tma_store_4d(tmap, stage + at, kb * 64, head, pos + quarter * 32, b);
+    if (LOW) tma_store_4d(tmap_lo, stage_lo + at, kb * 64, head, pos + quarter * 32, b);
     bulk_commit();
   }
 }

@@ -11,9 +11,12 @@
 // Both keep their accumulators in TMEM and feed dS (and P^T) to the tensor cores from TMEM, written by
 // the softmax warps over the scores they were computed from.
 //
-// delta is formed in the dQ kernel, from the rounded o, and is off by what that rounding does.  The
-// row's sum of P (dP - delta) would be zero with the true one: the dQ kernel adds it up as it goes,
-// and the dK / dV kernel behind it gets the corrected delta.
+// delta is formed in the dQ kernel, from o.  Where one key has most of a row's weight, dP - delta is what
+// two nearly equal numbers leave, so an error of delta counts many times: with o rounded to bf16, dQ was
+// 0.6 % off (2-norm) for documents of a few tokens with sharp scores, where the roundings of dS and dQ make
+// 0.24 %.  With o in two bf16 (o + o_lo) and the forward's mean taken with one set of weights it is 0.27 %.
+// The row's sum of P (dP - delta) would be zero with the true delta: the dQ kernel adds it up as it goes,
+// and the dK / dV kernel behind it gets the corrected one.
 #include "doc_attn.cuh"
 
 namespace oxi {
@@ -66,7 +69,7 @@ template <int DQP, int DVP, bool CAP, bool ALIBI>
 __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
     da_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
-                 const __grid_constant__ CUtensorMap tmDQ, DaParams p, DaTensor o_in, DaTensor do_in,
+                 const __grid_constant__ CUtensorMap tmDQ, DaParams p, DaTensor o_in, DaTensor olo_in,
                  const float* __restrict__ nlse2, float* __restrict__ ndelta) {
   using L = DaDqSmem<DQP, DVP>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -206,19 +209,19 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
     const bool in = qpos < p.S;
     const int64_t vi = ((int64_t)b * p.Hq + h) * p.S + qpos;
     const float nls = in ? __ldg(nlse2 + vi) : -INFINITY;
-    // minus delta of 8 rows a warp, 16 bytes a lane: 2 rows at a time
+    // minus delta of 8 rows a warp, 16 bytes a lane: 2 rows at a time; dO is in shared memory
     {
       const __nv_bfloat16* op = reinterpret_cast<const __nv_bfloat16*>(o_in.ptr) + b * o_in.sb + h * o_in.sh;
-      const __nv_bfloat16* dp = reinterpret_cast<const __nv_bfloat16*>(do_in.ptr) + b * do_in.sb + h * do_in.sh;
-      const int c = (lane & 15) * 8, row0 = (warp - 2) * 8 + (lane >> 4);
-      uint4 x[4], y[4];
+      const __nv_bfloat16* lp = reinterpret_cast<const __nv_bfloat16*>(olo_in.ptr) + b * olo_in.sb + h * olo_in.sh;
+      const int chunk = lane & 15, row0 = (warp - 2) * 8 + (lane >> 4);
+      uint4 x[4], xl[4];
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int64_t pos = qt * DA_TILE + row0 + 2 * g;
-        x[g] = y[g] = make_uint4(0, 0, 0, 0);
-        if (pos < p.S && c < p.Dv) {
-          x[g] = __ldg(reinterpret_cast<const uint4*>(op + pos * o_in.ss + c));
-          y[g] = __ldg(reinterpret_cast<const uint4*>(dp + pos * do_in.ss + c));
+        x[g] = xl[g] = make_uint4(0, 0, 0, 0);
+        if (pos < p.S && chunk * 8 < p.Dv) {
+          x[g] = __ldg(reinterpret_cast<const uint4*>(op + pos * o_in.ss + chunk * 8));
+          xl[g] = __ldg(reinterpret_cast<const uint4*>(lp + pos * olo_in.ss + chunk * 8));
         }
       }
       if (!mbar_wait(q_full, 0, abort_flag, p.status)) ok = false;
@@ -232,16 +235,21 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
       }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const uint32_t xw[4] = {x[g].x, x[g].y, x[g].z, x[g].w}, yw[4] = {y[g].x, y[g].y, y[g].z, y[g].w};
+        const int row = row0 + 2 * g;
+        uint4 y = make_uint4(0, 0, 0, 0);
+        if (chunk < DVP / 8)
+          y = *reinterpret_cast<const uint4*>(sDO + (chunk >> 3) * L::QBLK + row * 128 + (((chunk & 7) ^ (row & 7)) << 4));
+        const uint32_t xw[4] = {x[g].x, x[g].y, x[g].z, x[g].w}, lw[4] = {xl[g].x, xl[g].y, xl[g].z, xl[g].w},
+                       yw[4] = {y.x, y.y, y.z, y.w};
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float2 a = unpack_bf16(xw[e]), d = unpack_bf16(yw[e]);
-          sum = fmaf(a.x, d.x, fmaf(a.y, d.y, sum));
+          const float2 a = unpack_bf16(xw[e]), l = unpack_bf16(lw[e]), d = unpack_bf16(yw[e]);
+          sum = fmaf(a.x + l.x, d.x, fmaf(a.y + l.y, d.y, sum));
         }
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if ((lane & 15) == 0) s_row[row0 + 2 * g] = -sum;
+        if (chunk == 0) s_row[row] = -sum;
       }
     }
     asm volatile("bar.sync 1, 512;" ::: "memory");  // delta's rows; reached by every softmax warp
@@ -789,7 +797,7 @@ inline CUtensorMap part_tmap(float* ptr, int64_t planes, int S, int D) {
 
 struct BwdArgs {
   DaShape s;
-  DaTensor q, k, v, o, dout;
+  DaTensor q, k, v, o, o_lo, dout;
   const float* nlse2;
   float *ndelta, *part;
   DaOut dq, dk, dv;
@@ -811,7 +819,7 @@ void launch_bwd_t(const BwdArgs& a) {
   static std::atomic<uint64_t> dq_devices{0}, dkv_devices{0};
   da_smem(kq, DaDqSmem<DQP, DVP>::TOTAL, dq_devices);
   da_smem(kkv, DaDkvSmem<DQP, DVP>::TOTAL, dkv_devices);
-  kq<<<dim3(s.Hq, s.B, p.nt), DA_GROUPS_THREADS, DaDqSmem<DQP, DVP>::TOTAL, a.st>>>(tq, tk64, tv64, td, tdq, p, a.o, a.dout,
+  kq<<<dim3(s.Hq, s.B, p.nt), DA_GROUPS_THREADS, DaDqSmem<DQP, DVP>::TOTAL, a.st>>>(tq, tk64, tv64, td, tdq, p, a.o, a.o_lo,
                                                                                     a.nlse2, a.ndelta);
   OXI_CUDA_CHECK(cudaGetLastError());
   const int splits = da_bwd_splits(s.B, s.S, s.Hq, s.Hk);
@@ -848,17 +856,17 @@ int da_bwd_splits(int B, int S, int Hq, int Hk) {
 }
 
 void launch_da_bwd(const DaShape& s, const DaTensor& q, const DaTensor& k, const DaTensor& v, const DaTensor& o,
-                   const DaTensor& dout, const float* nlse2, float* ndelta, float* part, const DaOut& dq, const DaOut& dk,
+                   const DaTensor& o_lo, const DaTensor& dout, const float* nlse2, float* ndelta, float* part, const DaOut& dq, const DaOut& dk,
                    const DaOut& dv, int* status, cudaStream_t st) {
   if (s.B == 0 || s.S == 0 || s.Hq == 0) return;
   da_check(s);
   for (const DaOut* t : {&dq, &dk, &dv})
     OXI_CHECK((reinterpret_cast<uintptr_t>(t->ptr) & 15) == 0 && t->ld % 8 == 0, "16-byte aligned gradient rows");
-  for (const DaTensor* t : {&o, &dout})
+  for (const DaTensor* t : {&o, &o_lo, &dout})
     OXI_CHECK((reinterpret_cast<uintptr_t>(t->ptr) & 15) == 0 && t->sb % 8 == 0 && t->ss % 8 == 0 && t->sh % 8 == 0,
               "16-byte aligned rows of the output and its gradient");
   OXI_CHECK(da_bwd_splits(s.B, s.S, s.Hq, s.Hk) == 1 || part != nullptr, "attention backward needs its parts' workspace");
-  const BwdArgs a{s, q, k, v, o, dout, nlse2, ndelta, part, dq, dk, dv, status, st};
+  const BwdArgs a{s, q, k, v, o, o_lo, dout, nlse2, ndelta, part, dq, dk, dv, status, st};
   if (s.Dqk <= 64 && s.Dv <= 64) launch_bwd_d<64, 64>(a);
   else if (s.Dv <= 64) launch_bwd_d<128, 64>(a);
   else launch_bwd_d<128, 128>(a);

@@ -14,6 +14,10 @@
 // the m of the steps before it, so that its exponentials wait for no maximum, and the maximum found
 // meanwhile moves m (and rescales O in TMEM) for the next step when it is more than 8 above.  Only
 // where it is more than 60 above, or a row sees its first keys, is the step's own maximum used.
+// O is divided by the sum of the rounded P: it is then a true mean of the v_j, with weights a rounding off,
+// and where one key has nearly all the weight its rounding cancels.  The backward's delta lives on that (see
+// doc_attn_bwd.cu); its P takes the sum of P itself.  For a backward, what rounding o to bf16 leaves over is
+// kept as a second bf16 (o_lo).
 // Scores capped at up to 60 log 2 need no maximum at all: m = 0 (unless a negative slope adds to them).
 // Steps outside the bounds of the query tile's ranges are not loaded or computed; a step that is
 // wholly visible to a warp's 32 rows is computed without a mask.
@@ -43,8 +47,8 @@ struct DaFwdSmem {
 template <int DQP, int DVP, bool CAP, bool ALIBI>
 __global__ void __launch_bounds__(FW_THREADS, 2)
     da_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, DaParams p,
-                  float* __restrict__ nlse2) {
+                  const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
+                  const __grid_constant__ CUtensorMap tmOlo, DaParams p, float* __restrict__ nlse2, bool want_lo) {
   using L = DaFwdSmem<DQP, DVP>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -182,7 +186,7 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
     const float slope2 = ALIBI ? __ldg(p.slopes + h) * LOG2E : 0.f;
     const float C = ALIBI ? 1.f : p.c_log2;
     const bool bounded = CAP && p.c_log2 <= 60.f && slope2 >= 0.f;
-    float m = bounded ? 0.f : -INFINITY, m_next = m, l = 0.f;
+    float m = bounded ? 0.f : -INFINITY, m_next = m, l = 0.f, lr = 0.f;  // sums of P and of the rounded P
     bool ok = true;
     // O times 2^(m - m_new), m = m_new; O belongs to the product of step i - 1 until it completes.  Called
     // behind S_i, which was issued after the product of step i - 2: pv_done's parity can only mean i - 1.
@@ -190,6 +194,7 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
       const float alpha = m_new == m ? 1.f : ex2_approx(m - m_new);  // 2^-inf = 0 at a row's first keys
       m = m_new;
       l *= alpha;
+      lr *= alpha;
       if (i == 0) return true;
       if (!mbar_wait(pv_done, (i - 1) & 1, abort_flag, p.status)) return false;
       tc_fence_after();
@@ -263,9 +268,10 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const uint64_t pp = ex2_2(fma2(x[c][e], cc, mref));
-            rs[e & 3] = add2(rs[e & 3], pp);
             const float2 v = unpack2(pp);
             pk[c][e] = pack_bf16(v.x, v.y);
+            rs[e & 1] = add2(rs[e & 1], pp);
+            rs[2 + (e & 1)] = add2(rs[2 + (e & 1)], f2(pk[c][e] << 16, pk[c][e] & 0xffff0000u));
           }
       };
       exponentials();
@@ -285,8 +291,9 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
       }
       tmem_st16(s_addr, pk[0]);
       tmem_st16(s_addr + 16, pk[1]);
-      const float2 rsum = unpack2(add2(add2(rs[0], rs[1]), add2(rs[2], rs[3])));
-      l += rsum.x + rsum.y;
+      const float2 exact = unpack2(add2(rs[0], rs[1])), rounded = unpack2(add2(rs[2], rs[3]));
+      l += exact.x + exact.y;
+      lr += rounded.x + rounded.y;
       }
       if (padded) {
         // V_i has landed before its product may read it; rows of padding become zero
@@ -301,12 +308,18 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
     if (ok && n > 0 && !mbar_wait(o_done, 0, abort_flag, p.status)) ok = false;
     if (ok) {
       tc_fence_after();
-      // a row that sees no key is zero; one whose scores are NaN stays NaN.  Q's tile is free by now
-      const bool some = l > 0.f;
+      // a row that sees no key is zero; one whose scores are NaN stays NaN.  the tiles in shared memory are free
+      const bool some = lr > 0.f;
+      const float inv = some ? 1.f / lr : 0.f;
+      static_assert(L::KBV * L::QBLK <= L::KST * L::K_BYTES, "o_lo is staged in K's ring");
 #pragma unroll 1
-      for (int kb = 0; kb < L::KBV; ++kb)
-        store_block(sQ, TM_O + lane_base, kb, p.Dv, quarter, some ? 1.f / l : 0.f, !some, l != l, &tmO, h, qt * DA_TILE,
-                    p.S, b);
+      for (int kb = 0; kb < L::KBV; ++kb) {
+        if (want_lo)
+          store_block<true>(sQ, TM_O + lane_base, kb, p.Dv, quarter, inv, !some, l != l, &tmO, h, qt * DA_TILE, p.S, b, sK,
+                            &tmOlo);
+        else
+          store_block(sQ, TM_O + lane_base, kb, p.Dv, quarter, inv, !some, l != l, &tmO, h, qt * DA_TILE, p.S, b);
+      }
       if (qpos < p.S) nlse2[((int64_t)b * p.Hq + h) * p.S + qpos] = l == 0.f ? -INFINITY : -(m + log2f(l));
       if (lane == 0) bulk_wait_read<0>();
     }
@@ -322,27 +335,28 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
 
 template <int DQP, int DVP, bool CAP, bool ALIBI>
 void launch_fwd_t(const DaShape& s, const DaTensor& q, const DaTensor& k, const DaTensor& v, const DaOut& o,
-                  float* nlse2, int* status, cudaStream_t st) {
+                  const DaOut& o_lo, float* nlse2, int* status, cudaStream_t st) {
   using L = DaFwdSmem<DQP, DVP>;
   const CUtensorMap tq = da_tmap(q, s.B, s.S, s.Hq, s.Dqk), tk = da_tmap(k, s.B, s.S, s.Hk, s.Dqk, FW_KEYS),
-                    tv = da_tmap(v, s.B, s.S, s.Hk, s.Dv, FW_KEYS), to = da_tmap_out(o, s.B, s.S, s.Hq, s.Dv);
+                    tv = da_tmap(v, s.B, s.S, s.Hk, s.Dv, FW_KEYS), to = da_tmap_out(o, s.B, s.S, s.Hq, s.Dv),
+                    tlo = o_lo.ptr ? da_tmap_out(o_lo, s.B, s.S, s.Hq, s.Dv) : to;
   auto kern = da_fwd_kernel<DQP, DVP, CAP, ALIBI>;
   static std::atomic<uint64_t> devices{0};
   da_smem(kern, L::TOTAL, devices);
   const dim3 grid(s.Hq, s.B, (s.S + DA_TILE - 1) / DA_TILE);
-  kern<<<grid, FW_THREADS, L::TOTAL, st>>>(tq, tk, tv, to, da_params(s, status), nlse2);
+  kern<<<grid, FW_THREADS, L::TOTAL, st>>>(tq, tk, tv, to, tlo, da_params(s, status), nlse2, o_lo.ptr != nullptr);
   OXI_CUDA_CHECK(cudaGetLastError());
 }
 
 template <int DQP, int DVP>
 void launch_fwd_d(const DaShape& s, const DaTensor& q, const DaTensor& k, const DaTensor& v, const DaOut& o,
-                  float* nlse2, int* status, cudaStream_t st) {
+                  const DaOut& o_lo, float* nlse2, int* status, cudaStream_t st) {
   if (s.cap > 0.f)
-    s.slopes ? launch_fwd_t<DQP, DVP, true, true>(s, q, k, v, o, nlse2, status, st)
-             : launch_fwd_t<DQP, DVP, true, false>(s, q, k, v, o, nlse2, status, st);
+    s.slopes ? launch_fwd_t<DQP, DVP, true, true>(s, q, k, v, o, o_lo, nlse2, status, st)
+             : launch_fwd_t<DQP, DVP, true, false>(s, q, k, v, o, o_lo, nlse2, status, st);
   else
-    s.slopes ? launch_fwd_t<DQP, DVP, false, true>(s, q, k, v, o, nlse2, status, st)
-             : launch_fwd_t<DQP, DVP, false, false>(s, q, k, v, o, nlse2, status, st);
+    s.slopes ? launch_fwd_t<DQP, DVP, false, true>(s, q, k, v, o, o_lo, nlse2, status, st)
+             : launch_fwd_t<DQP, DVP, false, false>(s, q, k, v, o, o_lo, nlse2, status, st);
 }
 
 }  // namespace
@@ -352,14 +366,15 @@ bool da_supported(int Dqk, int Dv) {
 }
 
 void launch_da_fwd(const DaShape& s, const DaTensor& q, const DaTensor& k, const DaTensor& v, const DaOut& o,
-                   float* nlse2, int* status, cudaStream_t st) {
+                   const DaOut& o_lo, float* nlse2, int* status, cudaStream_t st) {
   if (s.B == 0 || s.S == 0 || s.Hq == 0) return;
   da_check(s);
-  OXI_CHECK((reinterpret_cast<uintptr_t>(o.ptr) & 15) == 0 && o.ld % 8 == 0, "16-byte aligned output rows");
+  for (const DaOut* t : {&o, &o_lo})
+    OXI_CHECK((reinterpret_cast<uintptr_t>(t->ptr) & 15) == 0 && t->ld % 8 == 0, "16-byte aligned output rows");
   // kernels for widths of up to 64 and 128 columns: narrower heads are padded with zero columns
-  if (s.Dqk <= 64 && s.Dv <= 64) launch_fwd_d<64, 64>(s, q, k, v, o, nlse2, status, st);
-  else if (s.Dv <= 64) launch_fwd_d<128, 64>(s, q, k, v, o, nlse2, status, st);
-  else launch_fwd_d<128, 128>(s, q, k, v, o, nlse2, status, st);
+  if (s.Dqk <= 64 && s.Dv <= 64) launch_fwd_d<64, 64>(s, q, k, v, o, o_lo, nlse2, status, st);
+  else if (s.Dv <= 64) launch_fwd_d<128, 64>(s, q, k, v, o, o_lo, nlse2, status, st);
+  else launch_fwd_d<128, 128>(s, q, k, v, o, o_lo, nlse2, status, st);
 }
 
 }  // namespace oxi

@@ -476,36 +476,35 @@ oxi::DaShape da_shape(const torch::Tensor& q, const torch::Tensor& k, const torc
   return s;
 }
 
-// o is [B, S, Hq, Dv] or [B, S, Hq Dv]; returns the rows' softmax statistics.
-torch::Tensor da_forward(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, double scale,
-                         double cap, const c10::optional<torch::Tensor>& slopes, bool causal,
-                         const std::vector<torch::Tensor>& mask, const torch::Tensor& status, torch::Tensor& o,
-                         bool flat) {
+// o is [B, S, Hq, Dv], or [B, S, Hq Dv] when flat; o_lo, for a backward, is what its rounding left over; nlse2 the
+// rows' softmax statistics.
+struct DaForward {
+  torch::Tensor o, o_lo, nlse2;
+};
+DaForward da_forward(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, double scale, double cap,
+                     const c10::optional<torch::Tensor>& slopes, bool causal, const std::vector<torch::Tensor>& mask,
+                     const torch::Tensor& status, bool flat, bool train) {
   const oxi::DaShape s = da_shape(q, k, v, scale, cap, slopes, causal, mask);
   const auto tq = da_operand(q, q, "q"), tk = da_operand(k, q, "k"), tv = da_operand(v, q, "v");
   c10::cuda::CUDAGuard g(q.device());
-  o = flat ? torch::empty({s.B, s.S, (int64_t)s.Hq * s.Dv}, q.options()) : torch::empty({s.B, s.S, s.Hq, s.Dv}, q.options());
-  auto nlse2 = torch::empty({s.B, s.Hq, s.S}, q.options().dtype(torch::kFloat32));
-  oxi::launch_da_fwd(s, tq.d, tk.d, tv.d, {o.data_ptr(), (int64_t)s.Hq * s.Dv}, nlse2.data_ptr<float>(),
-                     status_ptr(status), stream());
-  return nlse2;
+  const int64_t ld = (int64_t)s.Hq * s.Dv;
+  DaForward r;
+  r.o = flat ? torch::empty({s.B, s.S, ld}, q.options()) : torch::empty({s.B, s.S, s.Hq, s.Dv}, q.options());
+  if (train) r.o_lo = torch::empty(r.o.sizes(), q.options());
+  r.nlse2 = torch::empty({s.B, s.Hq, s.S}, q.options().dtype(torch::kFloat32));
+  oxi::launch_da_fwd(s, tq.d, tk.d, tv.d, {r.o.data_ptr(), ld}, {train ? r.o_lo.data_ptr() : nullptr, ld},
+                     r.nlse2.data_ptr<float>(), status_ptr(status), stream());
+  return r;
 }
-std::vector<torch::Tensor> doc_attn_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, double scale, double cap,
-                                        c10::optional<torch::Tensor> slopes, bool causal,
-                                        std::vector<torch::Tensor> mask, torch::Tensor status) {
-  torch::Tensor o;
-  auto nlse2 = da_forward(q, k, v, scale, cap, slopes, causal, mask, status, o, false);
-  return {o, nlse2};
-}
-
 void da_backward(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& o,
-                 const torch::Tensor& dout, const torch::Tensor& nlse2, double scale, double cap,
+                 const torch::Tensor& o_lo, const torch::Tensor& dout, const torch::Tensor& nlse2, double scale, double cap,
                  const c10::optional<torch::Tensor>& slopes, bool causal, const std::vector<torch::Tensor>& mask,
                  const oxi::DaOut& dq, const oxi::DaOut& dk, const oxi::DaOut& dv, const torch::Tensor& status) {
   const oxi::DaShape s = da_shape(q, k, v, scale, cap, slopes, causal, mask);
   const auto tq = da_operand(q, q, "q"), tk = da_operand(k, q, "k"), tv = da_operand(v, q, "v"),
-             to = da_operand(o, q, "o"), td = da_operand(dout, q, "the output's gradient");
-  OXI_CHECK(o.sizes() == dout.sizes() && o.size(0) == s.B && o.size(1) == s.S && o.size(2) == s.Hq &&
+             to = da_operand(o, q, "o"), tl = da_operand(o_lo, q, "o_lo"),
+             td = da_operand(dout, q, "the output's gradient");
+  OXI_CHECK(o.sizes() == dout.sizes() && o_lo.sizes() == dout.sizes() && o.size(0) == s.B && o.size(1) == s.S && o.size(2) == s.Hq &&
                 o.size(3) == s.Dv, "attention backward: o and its gradient must be [B, S, Hq, Dv]");
   OXI_CHECK(nlse2.device() == q.device() && nlse2.scalar_type() == torch::kFloat32 && nlse2.is_contiguous() &&
                 nlse2.numel() == (int64_t)s.B * s.Hq * s.S, "attention backward: nlse2");
@@ -513,11 +512,11 @@ void da_backward(const torch::Tensor& q, const torch::Tensor& k, const torch::Te
   const int splits = oxi::da_bwd_splits(s.B, s.S, s.Hq, s.Hk);
   torch::Tensor part;
   if (splits > 1) part = torch::empty({splits, (int64_t)s.B * s.Hk * s.S, s.Dqk + s.Dv}, nlse2.options());
-  oxi::launch_da_bwd(s, tq.d, tk.d, tv.d, to.d, td.d, nlse2.data_ptr<float>(), ndelta.data_ptr<float>(),
+  oxi::launch_da_bwd(s, tq.d, tk.d, tv.d, to.d, tl.d, td.d, nlse2.data_ptr<float>(), ndelta.data_ptr<float>(),
                      splits > 1 ? part.data_ptr<float>() : nullptr, dq, dk, dv, status_ptr(status), stream());
 }
 std::vector<torch::Tensor> doc_attn_bwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor o,
-                                        torch::Tensor dout, torch::Tensor nlse2, double scale, double cap,
+                                        torch::Tensor o_lo, torch::Tensor dout, torch::Tensor nlse2, double scale, double cap,
                                         c10::optional<torch::Tensor> slopes, bool causal,
                                         std::vector<torch::Tensor> mask, torch::Tensor status) {
   OXI_CHECK(q.is_cuda() && q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "attention: q, k, v must be CUDA [B, S, H, D]");
@@ -525,11 +524,11 @@ std::vector<torch::Tensor> doc_attn_bwd(torch::Tensor q, torch::Tensor k, torch:
   auto dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), q.options()),
        dv = torch::empty(v.sizes(), q.options());
   auto out = [](torch::Tensor& t) { return oxi::DaOut{t.data_ptr(), t.size(2) * t.size(3)}; };
-  da_backward(q, k, v, o, dout, nlse2, scale, cap, slopes, causal, mask, out(dq), out(dk), out(dv), status);
+  da_backward(q, k, v, o, o_lo, dout, nlse2, scale, cap, slopes, causal, mask, out(dq), out(dk), out(dv), status);
   return {dq, dk, dv};
 }
 torch::Tensor doc_attn_qkv_bwd(torch::Tensor qkv, int64_t Hq, int64_t Hk, int64_t D, torch::Tensor o,
-                               torch::Tensor dout, torch::Tensor nlse2, double scale, double cap,
+                               torch::Tensor o_lo, torch::Tensor dout, torch::Tensor nlse2, double scale, double cap,
                                c10::optional<torch::Tensor> slopes, bool causal, std::vector<torch::Tensor> mask,
                                torch::Tensor status) {
   const auto h = da_heads(qkv, Hq, Hk, D);
@@ -539,7 +538,8 @@ torch::Tensor doc_attn_qkv_bwd(torch::Tensor qkv, int64_t Hq, int64_t Hk, int64_
   auto dqkv = torch::empty(qkv.sizes(), qkv.options());
   const int64_t ld = qkv.size(2);
   auto* base = reinterpret_cast<uint16_t*>(dqkv.data_ptr());
-  da_backward(h[0], h[1], h[2], o.unflatten(2, {Hq, D}), dout.unflatten(2, {Hq, D}), nlse2, scale, cap, slopes, causal,
+  da_backward(h[0], h[1], h[2], o.unflatten(2, {Hq, D}), o_lo.unflatten(2, {Hq, D}),
+              dout.unflatten(2, {Hq, D}), nlse2, scale, cap, slopes, causal,
               mask, {base, ld}, {base + Hq * D, ld}, {base + (Hq + Hk) * D, ld}, status);
   return dqkv;
 }
@@ -1400,6 +1400,7 @@ struct DaOptions {
   bool causal;
   torch::Tensor slopes, status;
   std::vector<torch::Tensor> mask;
+  bool train;  // a backward may follow
 
   void save(AutogradContext* ctx, variable_list kept) const {
     kept.push_back(slopes);
@@ -1412,7 +1413,7 @@ struct DaOptions {
   }
   static DaOptions load(AutogradContext* ctx, const variable_list& kept, size_t at) {
     return {ctx->saved_data["scale"].toDouble(), ctx->saved_data["cap"].toDouble(), ctx->saved_data["causal"].toBool(),
-            kept[at], ctx->saved_data["status"].toTensor(), {kept.begin() + at + 1, kept.end()}};
+            kept[at], ctx->saved_data["status"].toTensor(), {kept.begin() + at + 1, kept.end()}, true};
   }
 };
 
@@ -1421,18 +1422,17 @@ struct DocAttention : torch::autograd::Function<DocAttention> {
   static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& q, const torch::Tensor& k,
                                const torch::Tensor& v, const DaOptions& opt) {
     at::AutoDispatchBelowADInplaceOrView below;  // nothing here is recorded
-    torch::Tensor o;
-    auto nlse2 = da_forward(q, k, v, opt.scale, opt.cap, maybe(opt.slopes), opt.causal, opt.mask, opt.status, o, false);
-    opt.save(ctx, {q, k, v, o, nlse2});
-    return o;
+    auto r = da_forward(q, k, v, opt.scale, opt.cap, maybe(opt.slopes), opt.causal, opt.mask, opt.status, false, opt.train);
+    opt.save(ctx, {q, k, v, r.o, r.o_lo, r.nlse2});
+    return r.o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     first_order_only("attention");
     at::AutoDispatchBelowADInplaceOrView below;
     const auto t = ctx->get_saved_variables();
-    const auto opt = DaOptions::load(ctx, t, 5);
+    const auto opt = DaOptions::load(ctx, t, 6);
     ++g_node_backwards;
-    auto g = doc_attn_bwd(t[0], t[1], t[2], t[3], grads[0], t[4], opt.scale, opt.cap, maybe(opt.slopes), opt.causal,
+    auto g = doc_attn_bwd(t[0], t[1], t[2], t[3], t[4], grads[0], t[5], opt.scale, opt.cap, maybe(opt.slopes), opt.causal,
                           opt.mask, opt.status);
     return {g[0], g[1], g[2], torch::Tensor()};
   }
@@ -1445,21 +1445,20 @@ struct DocAttentionQKV : torch::autograd::Function<DocAttentionQKV> {
                                const DaOptions& opt) {
     at::AutoDispatchBelowADInplaceOrView below;  // nothing here is recorded
     const auto h = da_heads(qkv, Hq, Hk, D);
-    torch::Tensor o;
-    auto nlse2 = da_forward(h[0], h[1], h[2], opt.scale, opt.cap, maybe(opt.slopes), opt.causal, opt.mask, opt.status,
-                            o, true);
-    opt.save(ctx, {qkv, o, nlse2});
+    auto r = da_forward(h[0], h[1], h[2], opt.scale, opt.cap, maybe(opt.slopes), opt.causal, opt.mask, opt.status, true,
+                        opt.train);
+    opt.save(ctx, {qkv, r.o, r.o_lo, r.nlse2});
     ctx->saved_data["heads"] = std::vector<int64_t>{Hq, Hk, D};
-    return o;
+    return r.o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     first_order_only("attention");
     at::AutoDispatchBelowADInplaceOrView below;
     const auto t = ctx->get_saved_variables();
-    const auto opt = DaOptions::load(ctx, t, 3);
+    const auto opt = DaOptions::load(ctx, t, 4);
     const auto h = ctx->saved_data["heads"].toIntVector();
     ++g_node_backwards;
-    auto g = doc_attn_qkv_bwd(t[0], h[0], h[1], h[2], t[1], grads[0], t[2], opt.scale, opt.cap, maybe(opt.slopes),
+    auto g = doc_attn_qkv_bwd(t[0], h[0], h[1], h[2], t[1], t[2], grads[0], t[3], opt.scale, opt.cap, maybe(opt.slopes),
                               opt.causal, opt.mask, opt.status);
     return {g, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()};
   }
@@ -1520,13 +1519,15 @@ struct RouterTopK : torch::autograd::Function<RouterTopK> {
 torch::Tensor doc_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, double scale, double cap,
                             c10::optional<torch::Tensor> slopes, bool causal, std::vector<torch::Tensor> mask,
                             torch::Tensor status) {
-  return DocAttention::apply(q, k, v, DaOptions{scale, cap, causal, slopes.value_or(torch::Tensor()), status, mask});
+  const bool train = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad());
+  return DocAttention::apply(q, k, v, DaOptions{scale, cap, causal, slopes.value_or(torch::Tensor()), status, mask, train});
 }
 torch::Tensor doc_attention_qkv(torch::Tensor qkv, int64_t Hq, int64_t Hk, int64_t D, double scale, double cap,
                                 c10::optional<torch::Tensor> slopes, bool causal, std::vector<torch::Tensor> mask,
                                 torch::Tensor status) {
+  const bool train = at::GradMode::is_enabled() && qkv.requires_grad();
   return DocAttentionQKV::apply(qkv, Hq, Hk, D,
-                                DaOptions{scale, cap, causal, slopes.value_or(torch::Tensor()), status, mask});
+                                DaOptions{scale, cap, causal, slopes.value_or(torch::Tensor()), status, mask, train});
 }
 torch::Tensor embedding_lookup(torch::Tensor ids, torch::Tensor w, double scale, torch::Tensor status) {
   return EmbeddingLookup::apply(ids, w, scale, status);
@@ -1562,11 +1563,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("logits"), py::arg("V"), py::arg("lse"), py::arg("targets"), py::arg("gscale"), py::arg("inv_count"),
         py::arg("col0") = 0);
   m.def("document_mask", &document_mask, "visible key ranges and tile tables of packed documents");
-  m.def("doc_attn_fwd", &doc_attn_fwd, "attention over visible key ranges, forward");
-  m.def("doc_attn_bwd", &doc_attn_bwd, "attention over visible key ranges, backward");
   m.def("doc_attention", &doc_attention, "attention over visible key ranges with its gradient");
   m.def("doc_attention_qkv", &doc_attention_qkv, "the same from a fused projection");
-  m.def("doc_attn_supported", [](int64_t Dqk, int64_t Dv) { return oxi::da_supported((int)Dqk, (int)Dv); });
   m.def("embedding_lookup", &embedding_lookup, "scaled embedding lookup with its gradient");
   m.def("embedding_fwd", &embedding_fwd, "scaled embedding lookup");
   m.def("embedding_bwd", &embedding_bwd, "embedding gradient by sorted tokens");

@@ -178,8 +178,6 @@ def test_the_extension_refuses_with_exceptions():
     st = torch.zeros(16, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="document_mask"):
         e.document_mask(torch.zeros(1, 4, dtype=torch.int64), None, None, None, True)
-    with pytest.raises((RuntimeError, ValueError)):
-        e.doc_attn_fwd(x, x, x, 0.1, 0.0, None, True, [], st)
     with pytest.raises(RuntimeError):
         e.doc_attention(x, x, x, 0.1, 0.0, None, True, [], st)
     with pytest.raises(RuntimeError):

@@ -422,3 +422,20 @@ def test_ranges_across_slices(S, mean):
         end = torch.where(sees, n + 1, 0).amax(1)
         first = torch.where(sees, n, nt).amin(1) * (end > 0)
         assert torch.equal(m.kt[..., 0], first.int()) and torch.equal(m.kt[..., 1], end.int())
+
+
+@pytest.mark.parametrize("mean,cap", [(1.5, 0.0), (3, 20.0), (12, 0.0), (100, 50.0), (700, 20.0)])
+def test_sharp_scores_keep_the_gradients(mean, cap):
+    """Rows with one dominant key, whose dP - delta nearly cancels.  In the 2-norm a gradient is off by the rounding
+    of its bf16 terms and its own, each at most 2^-8 / sqrt 3 of a value (rms): 0.82 x 2^-8 together, and the rest
+    of 2^-8 for the forward's rounded weights."""
+    B, S = 2, 900
+    q, k, v, do = inputs(B, S, 4, 2, 64, 64, seed=int(mean * 10), sharp=2.0)
+    doc = layout(B, S, mean, int(mean), pad=False)[0] if mean > 2 else torch.arange(S, device="cuda").expand(B, S) * 2 // 3
+    m = api.document_mask(doc)
+    got = run(q, k, v, do, 0.125, mask=m, softcap=cap)
+    want = oracle(q, k, v, do, 0.125, m, cap, None)
+    check(got, want)
+    for name, x, (y, _) in zip(("o", "dq", "dk", "dv"), got, want):
+        assert (x.double() - y).norm() <= HALF * y.norm(), name
+    finish()

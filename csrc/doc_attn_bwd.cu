@@ -706,7 +706,8 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&ds_full[mine]);
     }
-    if (ok && n > 0 && !mbar_wait(all_done, 0, abort_flag, p.status)) ok = false;
+    // K's and V's tiles are where the gradients are staged: without a step, their copies may still be on their way
+    if (ok && !mbar_wait(n > 0 ? all_done : kv_full, 0, abort_flag, p.status)) ok = false;
     if (ok) {
       tc_fence_after();
       // every product has completed and every copy landed: shared memory is free for the output tiles

@@ -305,7 +305,8 @@ __global__ void __launch_bounds__(FW_THREADS, 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[i & 1]);
     }
-    if (ok && n > 0 && !mbar_wait(o_done, 0, abort_flag, p.status)) ok = false;
+    // Q's tile is where the output is staged: without a step, its copy may still be on its way
+    if (ok && !mbar_wait(n > 0 ? o_done : q_full, 0, abort_flag, p.status)) ok = false;
     if (ok) {
       tc_fence_after();
       // a row that sees no key is zero; one whose scores are NaN stays NaN.  the tiles in shared memory are free

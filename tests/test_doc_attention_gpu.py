@@ -439,3 +439,22 @@ def test_sharp_scores_keep_the_gradients(mean, cap):
     for name, x, (y, _) in zip(("o", "dq", "dk", "dv"), got, want):
         assert (x.double() - y).norm() <= HALF * y.norm(), name
     finish()
+
+
+@pytest.mark.parametrize("D,Dv", [(64, 64), (96, 64), (128, 128)])
+def test_tiles_of_padding_alone(D, Dv):
+    """Tiles with nothing to compute: their zeros are staged where operands land, which must have landed."""
+    B, S = 16, 2048
+    q, k, v, do = inputs(B, S, 4, 4, D, Dv, seed=21)
+    doc = torch.where(torch.arange(S, device="cuda") < 200, 0, -1).expand(B, S)
+    m = api.document_mask(doc)
+    first = None
+    for _ in range(20):
+        got = run(q, k, v, do, D ** -0.5, mask=m)
+        for x in got:
+            assert not x[:, 200:].any()
+        if first is None:
+            first = got
+        for x, y in zip(got, first):
+            assert torch.equal(x, y)
+    finish()

@@ -562,7 +562,10 @@ __global__ void __launch_bounds__(RT_WARPS * 32) router_bwd_kernel(const LT* __r
       __syncwarp();
 #pragma unroll
       for (int i = 0; i < EPL; ++i) s_g[e0 + i] = 0.f;
-      const float n = warp_sum(w), gw = warp_sum(g * w);
+      // of the gradients' differences from the first one's: what they have in common (all of it, for one expert)
+      // cancels without a rounding
+      g -= __shfl_sync(FULL, g, 0);
+      const float n = warp_sum(w), gw = warp_sum(lane < s.k ? g * w : 0.f);
       g = n > 0.f ? (g - gw / n) / n : 0.f;
       __syncwarp();
     }

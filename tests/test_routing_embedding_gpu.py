@@ -266,3 +266,18 @@ def test_embedding_empty_and_captured():
         for a, b in zip(out, ref):
             assert torch.equal(a, b)
     finish()
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E", [2, 40, 256])
+def test_one_renormalised_expert(E, score):
+    """Its weight is the scale whatever the logits: what reaches them is the usage's gradient alone, to f32's accuracy."""
+    T = 4000
+    g = torch.Generator(device="cuda").manual_seed(E)
+    x = torch.randn(T, E, generator=g, device="cuda")
+    dw, du = torch.randn(T, 1, generator=g, device="cuda"), torch.randn(E, generator=g, device="cuda")
+    got, want = route_both(x, 1, dw, du, score=score, scale=2.5)
+    # per element an f32 chain of 64 steps over parts that are at most a few times the result's size, in the 2-norm
+    assert (got[4].double() - want[4]).norm() <= 256 * F32 * want[4].norm()
+    got, _ = route_both(x, 1, dw, torch.zeros_like(du), score=score, scale=2.5)
+    assert not got[4].any()

@@ -3,6 +3,7 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <array>
 #include <atomic>
@@ -1388,8 +1389,14 @@ using torch::autograd::variable_list;
 
 std::atomic<int64_t> g_node_backwards{0};  // kernel library calls that nodes made from backward passes
 
-void first_order_only(const char* what) {
-  OXI_CHECK(!at::GradMode::is_enabled(), what, ": only first derivatives (create_graph=False)");
+// Gradients that are recorded (create_graph) become nodes that raise when they are differentiated.
+variable_list first_order_only(variable_list grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list in;
+  for (auto& g : grads) in.push_back(g.defined() ? g.detach().requires_grad_(true) : g);
+  auto raise = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " has first derivatives only",
+                                                               (int64_t)in.size());
+  return (*raise)(std::move(in));
 }
 c10::optional<torch::Tensor> maybe(const torch::Tensor& t) {
   return t.defined() ? c10::optional<torch::Tensor>(t) : c10::nullopt;
@@ -1427,7 +1434,9 @@ struct DocAttention : torch::autograd::Function<DocAttention> {
     return r.o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    first_order_only("attention");
+    return first_order_only(gradients(ctx, grads), "attention");
+  }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     at::AutoDispatchBelowADInplaceOrView below;
     const auto t = ctx->get_saved_variables();
     const auto opt = DaOptions::load(ctx, t, 6);
@@ -1452,7 +1461,9 @@ struct DocAttentionQKV : torch::autograd::Function<DocAttentionQKV> {
     return r.o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    first_order_only("attention");
+    return first_order_only(gradients(ctx, grads), "attention");
+  }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     at::AutoDispatchBelowADInplaceOrView below;
     const auto t = ctx->get_saved_variables();
     const auto opt = DaOptions::load(ctx, t, 4);
@@ -1478,6 +1489,10 @@ struct EmbeddingLookup : torch::autograd::Function<EmbeddingLookup> {
     return out.view(shape);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return first_order_only(gradients(ctx, grads), "embedding");
+  }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
+    at::AutoDispatchBelowADInplaceOrView below;
     const auto ids = ctx->get_saved_variables()[0];
     const auto& dy = grads[0];
     ++g_node_backwards;
@@ -1503,6 +1518,10 @@ struct RouterTopK : torch::autograd::Function<RouterTopK> {
     return r;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    return first_order_only(gradients(ctx, grads), "routing");
+  }
+  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
+    at::AutoDispatchBelowADInplaceOrView below;
     const auto t = ctx->get_saved_variables();
     const auto f32 = t[0].options().dtype(torch::kFloat32);
     auto dtopw = grads[1].defined() ? grads[1].to(torch::kFloat32).contiguous() : torch::zeros(t[1].sizes(), f32);

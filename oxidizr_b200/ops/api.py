@@ -195,20 +195,22 @@ def attention(q, k, v, scale: float, causal: bool = True, mask=None, softcap: fl
     """q [B, S, Hq, Dqk], k [B, S, Hk, Dqk], v [B, S, Hk, Dv] -> [B, S, Hq, Dv].  ``mask`` from
     document_mask, ``softcap`` c: scores pass through c tanh(./c), ``alibi`` f32 [Hq]: slopes of a bias
     -slope |i - j| added after the cap."""
+    from .doc_attention import attention as _doc, takes_plain
     if mask is None and not softcap and alibi is None:
-        from .attention import attention as _att
-        return _att(q, k, v, scale, causal)
-    from .doc_attention import attention as _doc
+        same = k.dtype == v.dtype == q.dtype and k.shape == (*q.shape[:2], k.shape[2], q.shape[3]) and v.shape[:3] == k.shape[:3]
+        if not (same and takes_plain(q, q.shape[2], k.shape[2], q.shape[3], v.shape[3], scale)):
+            from .attention import attention as _att
+            return _att(q, k, v, scale, causal)
     return _doc(q, k, v, scale, causal, mask, softcap or 0.0, alibi)
 
 
 def attention_qkv(qkv, Hq: int, Hk: int, D: int, scale: float, causal: bool = True, mask=None, softcap: float = 0.0,
                   alibi=None):
     """``attention`` from the fused [B, S, (Hq + 2 Hk) D] projection; returns [B, S, Hq D]."""
-    if mask is None and not softcap and alibi is None:
+    from .doc_attention import attention_qkv as _doc, takes_plain
+    if mask is None and not softcap and alibi is None and not takes_plain(qkv, Hq, Hk, D, D, scale):
         from .attention import attention_qkv as _aq
         return _aq(qkv, Hq, Hk, D, scale, causal)
-    from .doc_attention import attention_qkv as _doc
     return _doc(qkv, Hq, Hk, D, scale, causal, mask, softcap or 0.0, alibi)
 
 

@@ -331,8 +331,10 @@ def test_graph_is_kept_and_second_derivatives_are_refused():
     a, = torch.autograd.grad(o, qkv, do, retain_graph=True)
     b, = torch.autograd.grad(o, qkv, do, retain_graph=True)
     assert torch.equal(a, b)
+    a2, = torch.autograd.grad(o, qkv, do, create_graph=True)
+    assert torch.equal(a, a2)
     with pytest.raises(RuntimeError, match="first derivatives"):
-        torch.autograd.grad(o, qkv, do, create_graph=True)
+        a2.float().sum().backward()
     q, k, v = (t.unflatten(-1, (1, 64)) for t in qkv.split(64, -1))
     o2 = api.attention(q, k, v, 0.125, softcap=20.0)
     assert torch.equal(o2.flatten(2), o)
@@ -457,4 +459,21 @@ def test_tiles_of_padding_alone(D, Dv):
             first = got
         for x, y in zip(got, first):
             assert torch.equal(x, y)
+    finish()
+
+
+@pytest.mark.parametrize("S", [1, 2, 3, 130, 700])
+@pytest.mark.parametrize("causal", [True, False])
+def test_plain_attention_runs_the_same_kernels(S, causal):
+    """Without a mask, a cap or slopes too, both entry points."""
+    q, k, v, do = inputs(2, S, 4, 2, 64, 64, seed=S)
+    lo = torch.zeros(2, S, dtype=torch.int64, device="cuda")
+    hi = torch.arange(1, S + 1, device="cuda").expand(2, S) if causal else torch.full((2, S), S, device="cuda")
+    m = type("M", (), {"lo": lo, "hi": hi})
+    got = run(q, k, v, do, 0.125, causal=causal)
+    check(got, oracle(q, k, v, do, 0.125, m, 0.0, None))
+    qkv = torch.cat([t.flatten(2) for t in (q, k, v)], -1).requires_grad_()
+    o = api.attention_qkv(qkv, 4, 2, 64, 0.125, causal=causal)
+    g, = torch.autograd.grad(o, qkv, do.flatten(2))
+    assert torch.equal(o, got[0].flatten(2)) and torch.equal(g, torch.cat([t.flatten(2) for t in got[1:]], -1))
     finish()

@@ -289,11 +289,9 @@ template <int EPL>
 struct Top2 {
   uint32_t k0, k1;
   int i0, i1;
-  bool known;  // k1 is the second largest, not only unknown
   __device__ __forceinline__ void find(const uint32_t (&key)[EPL]) {
     k0 = k1 = 0u;
     i0 = i1 = 0;
-    known = true;
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
       const bool first = key[i] > k0, second = key[i] > k1;
@@ -302,6 +300,13 @@ struct Top2 {
       k0 = first ? key[i] : k0;
       i0 = first ? i : i0;
     }
+  }
+  // the next two, in the same order, behind the key `last` at place `at`
+  __device__ __forceinline__ void find_behind(const uint32_t (&key)[EPL], uint32_t last, int at) {
+    uint32_t rest[EPL];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) rest[i] = key[i] < last || (key[i] == last && i > at) ? key[i] : 0u;
+    find(rest);
   }
 };
 
@@ -336,6 +341,37 @@ __device__ __forceinline__ bool choose_groups(const RouteShape& s, uint32_t k0, 
   const uint32_t last = __reduce_min_sync(FULL, in && stays ? gk : 0xffffffffu);
   const uint32_t best = __reduce_max_sync(FULL, in && !stays ? gk : 0u);
   return key_value(last) - key_value(best) > margin;
+}
+
+// The k choices of a token with a near tie, one after another, each among the experts that f32 cannot tell from
+// the best; open: bits of the lane's experts that take part.
+template <typename LT, int EPL>
+__device__ __noinline__ void careful_choice(const RouteShape s, const LT* __restrict__ row, const float* __restrict__ bias,
+                                            uint32_t open, float apart, int* __restrict__ chosen) {
+  const int lane = threadIdx.x & 31, e0 = lane * EPL;
+  uint32_t key[EPL];
+  {
+    float x[EPL], p[EPL];
+    load_row<LT, EPL>(s, row, x);
+    scores<EPL>(s, x, p);
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) key[i] = (open >> i) & 1u ? order_key(p[i] + bias[e0 + i]) : 0u;
+  }
+  for (int j = 0; j < s.k; ++j) {
+    int owner, at;
+    const uint32_t best = warp_best<uint32_t, EPL>(key, owner, at);
+    const uint32_t thr = max(order_key(key_value(best) - apart), 1u);
+    int near = 0;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) near += key[i] >= thr;
+    if (__reduce_add_sync(FULL, near) > 1) exact_best<LT, EPL>(s, row, bias, key, thr, owner, at);
+    if (lane == owner) {
+      chosen[j] = e0 + at;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i)
+        if (i == at) key[i] = 0u;
+    }
+  }
 }
 
 constexpr int RT_WARPS = 8;
@@ -424,41 +460,31 @@ __global__ void __launch_bounds__(RT_WARPS * 32, EPL <= 8 ? 3 : 2) router_fwd_ke
       }
     }
     // One choice is a warp maximum of the lanes' largest keys.  The lane that held it goes on to its second, and
-    // looks over its keys again only when its turn comes once more.
+    // looks over its keys again only when its turn comes once more.  With a bias the values that follow one
+    // another, the first that is not chosen among them, are compared afterwards: where two are too close for
+    // f32 to order, the token is done again with care.
+    uint32_t mine = 0u, after = 0u;  // lane j: the j-th best key; the first that is left
     for (int j = 0; j < s.k; ++j) {
       const uint32_t best = __reduce_max_sync(FULL, top.k0);
-      int owner = __ffs(__ballot_sync(FULL, top.k0 == best)) - 1, at = top.i0;
-      const bool given = lane == owner;
-      if (!by_logit) {
-        if (given && !top.known) top.find(key);
-        const uint32_t thr = max(order_key(key_value(best) - apart), 1u);
-        if (__any_sync(FULL, (given ? top.k1 : top.k0) >= thr)) {
-          uint32_t k[EPL];  // a copy: the keys themselves stay in registers
-          int o = owner, a = at;
-#pragma unroll
-          for (int i = 0; i < EPL; ++i) k[i] = key[i];
-          exact_best<LT, EPL>(s, row, bias_in, k, thr, o, a);
-          if (lane == o) {
-            // out of the order of the keys: it leaves them for good
-            s_e[warp][j] = e0 + a;
-#pragma unroll
-            for (int i = 0; i < EPL; ++i)
-              if (i == a) key[i] = 0u;
-            top.find(key);
-          }
-          continue;
-        }
-      }
-      if (given) {
+      if (lane == j) mine = best;
+      if (lane == __ffs(__ballot_sync(FULL, top.k0 == best)) - 1) {
+        const int at = top.i0;
         s_e[warp][j] = e0 + at;
-#pragma unroll
-        for (int i = 0; i < EPL; ++i)
-          if (i == at) key[i] = 0u;
         top.k0 = top.k1;
         top.i0 = top.i1;
         top.k1 = 0u;
-        top.known = false;
-        if (top.k0 == 0u) top.find(key);
+        if (top.k0 == 0u) top.find_behind(key, best, at);
+      }
+    }
+    if (!by_logit) {
+      after = __reduce_max_sync(FULL, top.k0);
+      const uint32_t next = __shfl_down_sync(FULL, mine, 1), behind = lane == s.k - 1 ? after : next;
+      const bool near = lane < s.k && behind != 0u && !(key_value(mine) - key_value(behind) > apart);
+      if (__any_sync(FULL, near)) {
+        uint32_t open = 0u;
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) open |= key[i] != 0u ? 1u << i : 0u;
+        careful_choice<LT, EPL>(s, row, bias_in, open, apart, s_e[warp]);
       }
     }
     // the scores of the chosen, by way of shared memory

@@ -22,6 +22,11 @@
 namespace oxi {
 namespace {
 
+// A row that sees one key has no gradient through its score.  That is exact here, not what rounding leaves: the dQ
+// kernel takes its P as zero, and marks it for the dK / dV kernel with this NaN in place of delta (arithmetic
+// makes no such NaN).
+constexpr uint32_t LONE_KEY = 0x7fc0a5a5u;
+
 // ------------------------------------------------------------------ dQ
 constexpr int DQ_KEYS = 64;
 constexpr int DA_GROUPS_THREADS = 64 + 512;  // TMA warp, MMA warp, two groups of 8 softmax warps
@@ -208,7 +213,8 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
     const TileRange vis = key_range(p, b, qpos);
     const bool in = qpos < p.S;
     const int64_t vi = ((int64_t)b * p.Hq + h) * p.S + qpos;
-    const float nls = in ? __ldg(nlse2 + vi) : -INFINITY;
+    const bool lone = vis.end - vis.begin == 1;
+    const float nls = in && !lone ? __ldg(nlse2 + vi) : -INFINITY;
     // minus delta of 8 rows a warp, 16 bytes a lane: 2 rows at a time; dO is in shared memory
     {
       const __nv_bfloat16* op = reinterpret_cast<const __nv_bfloat16*>(o_in.ptr) + b * o_in.sb + h * o_in.sh;
@@ -338,7 +344,7 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
     if (ok) {
       tc_fence_after();
       if (sub == 0 && in)
-        ndelta[vi] = ndl - ((s_row[DA_TILE + r] + s_row[2 * DA_TILE + r]) + (s_row[3 * DA_TILE + r] + s_row[4 * DA_TILE + r]));
+        ndelta[vi] = lone ? __uint_as_float(LONE_KEY) : ndl - ((s_row[DA_TILE + r] + s_row[2 * DA_TILE + r]) + (s_row[3 * DA_TILE + r] + s_row[4 * DA_TILE + r]));
       // Q's tile in shared memory is free by now
       if (sub < L::KBQ)
         store_block(sQ, TM_DQ + lane_base, sub, p.Dqk, quarter, p.scale, n == 0, false, &tmDQ, h, qt * DA_TILE, p.S, b);
@@ -686,12 +692,13 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
           const float4 d4 = vec[KV_QUERIES / 4 + e / 2];
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
-            const uint64_t ds = mul2(x[e + g], add2(d[e + g], g ? f2(d4.z, d4.w) : f2(d4.x, d4.y)));
+            const float2 nd = g ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y);
+            const uint64_t ds = mul2(x[e + g], add2(d[e + g], f2(nd.x, nd.y)));
             float2 u = unpack2(ds);
-            if (decltype(some_hidden)::value) {  // a hidden pair adds nothing, whatever dP is
+            if (decltype(some_hidden)::value) {  // a hidden pair adds nothing, whatever dP is; nor does a lone key
               const float2 w = unpack2(x[e + g]);
-              u.x = w.x == 0.f ? 0.f : u.x;
-              u.y = w.y == 0.f ? 0.f : u.y;
+              u.x = w.x == 0.f || __float_as_uint(nd.x) == LONE_KEY ? 0.f : u.x;
+              u.y = w.y == 0.f || __float_as_uint(nd.y) == LONE_KEY ? 0.f : u.y;
             }
             pk[e + g] = pack_bf16(u.x, u.y);
           }

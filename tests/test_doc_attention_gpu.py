@@ -477,3 +477,17 @@ def test_plain_attention_runs_the_same_kernels(S, causal):
     g, = torch.autograd.grad(o, qkv, do.flatten(2))
     assert torch.equal(o, got[0].flatten(2)) and torch.equal(g, torch.cat([t.flatten(2) for t in got[1:]], -1))
     finish()
+
+
+@pytest.mark.parametrize("S,causal", [(1, True), (1, False), (300, True)])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+def test_one_key_gets_no_gradient_through_its_score(S, causal, cap):
+    """A softmax over one key is constant: dQ and dK are zeros, not what rounding leaves."""
+    q, k, v, do = inputs(2, S, 4, 2, 64, 32, seed=31)
+    masks = [api.document_mask(torch.arange(S, device="cuda").expand(2, S), causal=causal)] + ([None] if S == 1 else [])
+    for m in masks:
+        o, dq, dk, dv = run(q, k, v, do, 0.125, mask=m, softcap=cap, causal=causal)
+        assert torch.equal(o, v.repeat_interleave(2, 2)) and not dq.any() and not dk.any()
+        want = do.double().unflatten(2, (2, 2)).sum(3)
+        assert ((dv.double() - want).abs() <= HALF * want.abs() + 2 * (HALF + REST) * do.double().unflatten(2, (2, 2)).abs().sum(3)).all()
+    finish()

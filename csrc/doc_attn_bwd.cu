@@ -11,6 +11,15 @@
 // Both keep their accumulators in TMEM and feed dS (and P^T) to the tensor cores from TMEM, written by
 // the softmax warps over the scores they were computed from.
 //
+// What bounds them: the products of a dQ step (128 queries x 64 keys, 128-wide heads) take 788 clocks, of a dK / dV
+// step 1044, and the softmax warps' instructions about as long; the two overlap through the alternating groups.  One
+// dense causal row of 8192 tokens, 16 / 4 heads of 128: dQ 369 us (1118 TFLOP/s of its own three products), dK and dV
+// 481 us (1143 of its four); with a cap of 50, whose tanh and derivative are instructions, 480 and 556 us; heads of 64:
+// 286 and 393 us (16 / 16 heads).  8 x 2048 tokens in documents of 700, capped: 241 and 230 us.  16 x 1024 tokens in
+// documents of 300, heads of 96 and 64: 104 and 113 us, half of it a CTA's start and end (4 us, one CTA a SM).
+//
+// P and dS are rounded to bf16 for the tensor cores (2^-8 of each term at most, with random signs over the keys of a
+// row); statistics, delta and accumulators are f32.
 // delta is formed in the dQ kernel, from o.  Where one key has most of a row's weight, dP - delta is what
 // two nearly equal numbers leave, so an error of delta counts many times: with o rounded to bf16, dQ was
 // 0.6 % off (2-norm) for documents of a few tokens with sharp scores, where the roundings of dS and dQ make
@@ -344,7 +353,9 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
     if (ok) {
       tc_fence_after();
       if (sub == 0 && in)
-        ndelta[vi] = lone ? __uint_as_float(LONE_KEY) : ndl - ((s_row[DA_TILE + r] + s_row[2 * DA_TILE + r]) + (s_row[3 * DA_TILE + r] + s_row[4 * DA_TILE + r]));
+        ndelta[vi] = lone ? __uint_as_float(LONE_KEY)
+                          : ndl - ((s_row[DA_TILE + r] + s_row[2 * DA_TILE + r]) +
+                                   (s_row[3 * DA_TILE + r] + s_row[4 * DA_TILE + r]));
       // Q's tile in shared memory is free by now
       if (sub < L::KBQ)
         store_block(sQ, TM_DQ + lane_base, sub, p.Dqk, quarter, p.scale, n == 0, false, &tmDQ, h, qt * DA_TILE, p.S, b);

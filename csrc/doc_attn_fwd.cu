@@ -22,6 +22,14 @@
 // Steps outside the bounds of the query tile's ranges are not loaded or computed; a step that is
 // wholly visible to a warp's 32 rows is computed without a mask.
 // Warps: 0 TMA, 1 MMA + TMEM owner, 2..5 softmax and output.
+//
+// What bounds it: a step's products take 652 clocks (128-wide heads), its 8192 exponentials 512 of the
+// special-function unit, and neither runs alone: 1100 clocks a step.  One dense causal row of 8192 tokens, 16 / 4
+// heads: 261 us of width 128 (1054 TFLOP/s), 239 us of width 64 (575; the exponentials alone take 120 us at
+// the unit's rate), 406 us of width 128 under a cap of 50.  8 x 2048 tokens in documents of 700 with that cap: 185 us;
+// 16 x 1024 in documents of 300, 96- and 64-wide heads: 58 us, of which a CTA's six steps are the smaller part
+// (start, first loads and output take 4 us, which the other CTA of the SM covers only while it computes).
+// Tried and slower: eight softmax warps that halve a row (they exchange maxima and sums at each step).
 #include "doc_attn.cuh"
 
 namespace oxi {

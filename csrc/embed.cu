@@ -14,6 +14,14 @@
 //      columns; what belongs wholly to the block is written, a segment's part at the block's edge
 //      goes to the workspace.
 //   3. join: the parts of a segment that spans blocks are added in their order.
+// The rows that no token names are zeroed first, by a memset of the whole gradient: it runs at the memory's rate and
+// is most of what a large vocabulary costs.
+//
+// 16384 tokens, 128354 x 2048 bf16: forward 15 us, memset 87, sort 20.5 (two passes of 9 bits over one cluster of 8
+// CTAs: latency), reduce 32 (134 MB read, 4.2 TB/s), join 17 (one token is a twentieth of the batch: its parts are one
+// warp's chain); 689 MB in 167 us.  256 tokens, 100315 x 128 f32: 2, 10, 12, 12 and 2 us, less than the host takes.
+// Tried and no faster: zeroing in the sort's launch by other clusters, zeroing last and only what no token names,
+// rows of 2 or 4 steps ahead, blocks of 8 or 16 rows.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>

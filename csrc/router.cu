@@ -8,9 +8,11 @@
 //   usage  = mean over the tokens of s / sum s;  counts: how often each expert was chosen
 //
 // Without a bias the order of b is that of x, which is exact.  With one, b in f32 may order two
-// experts that are a rounding apart wrongly: where f32 cannot tell which is the largest, the
-// candidates are compared in f64 (a few tokens in a thousand; a token chosen wholly in f64 took 25 us,
-// which the kernel's end had to wait for).  The same for the last group that stays.
+// experts that are a rounding apart wrongly.  So the finished list of choices is looked over: where two
+// that follow one another are closer than f32 can tell, the token's choices are made again, one by one,
+// those that f32 cannot tell from the best compared in f64 (a few tokens in a thousand; a token chosen
+// wholly in f64 took 25 us, which the kernel's end had to wait for).  The same for the last group that
+// stays.
 //
 // Backward, per token (g = d_usage / T, S = sum s):
 //   ds_j += scale (dw_j - sum_i dw_i s_i / n) / n for the chosen (n = sum of the chosen s; renorm),
@@ -20,7 +22,9 @@
 // neighbours sits in neighbouring lanes (its rank takes log2 of their number shuffles), and the
 // lowest index of equals is the lowest lane of a ballot.  One of the k choices is a maximum over the
 // lane's keys, a warp reduction of integers and a ballot; the instructions of those set the time, not
-// the bytes.
+// the bytes.  32768 tokens x 256 experts in 8 groups, sigmoid with a bias, bf16: forward 56 us (16.8 MB of
+// logits are 2.6 us), backward 18 us (33.6 MB, 1.9 TB/s), join 4 us; 16384 x 64: 13, 7 and 4 us.  Looking for a near
+// tie at each choice, 68 and 19 us.
 // Sums over tokens (usage, counts) are per-CTA partials joined in a fixed order: no atomics in f32.
 // Upstream (model.rs:541-556, 604-687): softmax scores, renormalised, no bias and no groups; its
 // balance loss uses mean_t(probs) (model.rs:585-590).

@@ -369,7 +369,7 @@ class LitConfig:
         if m.hidden_size % m.num_heads != 0:
             raise ConfigError("hidden_size must be divisible by num_heads")
         if m.doc_separator is not None:
-            if m.doc_separator >= m.vocab_size:
+            if not 0 <= m.doc_separator < m.vocab_size:
                 raise ConfigError(f"doc_separator {m.doc_separator} is not a token of a vocabulary of {m.vocab_size}")
             if m.mamba_layers:
                 raise ConfigError("doc_separator needs attention layers only: a Mamba layer's state would cross documents")
@@ -377,7 +377,9 @@ class LitConfig:
             raise ConfigError(f"attn_softcap must be a positive number, got {m.attn_softcap}")
         if m.moe_score not in (None, "softmax", "sigmoid"):
             raise ConfigError(f"moe_score must be softmax or sigmoid, got {m.moe_score!r}")
-        if m.num_experts is not None and m.experts_per_tok is not None:
+        if m.moe_bias_rate is not None and not 0 <= m.moe_bias_rate < math.inf:
+            raise ConfigError(f"moe_bias_rate must not be negative, got {m.moe_bias_rate}")
+        if m.num_experts is not None and m.experts_per_tok is not None and (m.moe_groups or m.moe_top_groups):
             groups, top = m.moe_groups or 1, m.moe_top_groups or m.moe_groups or 1
             if m.num_experts % groups or not 1 <= top <= groups:
                 raise ConfigError(f"{m.num_experts} experts cannot be taken in {groups} groups of which {top} stay")

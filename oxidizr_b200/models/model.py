@@ -130,12 +130,24 @@ class LitGPT(RefModule):
         loss = api.linear_cross_entropy(x, self.lm_head, targets)
         return loss, aux
 
+    @torch.no_grad()
     def update_route_bias(self) -> None:
-        """Move the experts' selection biases by the loads since the last call (``moe_bias_rate``)."""
-        for layer in self.layers:
-            moe = getattr(layer, "moe", None)
-            if moe is not None and moe.bias_rate:
-                moe.update_route_bias()
+        """Move the experts' selection biases by the loads since the last call (``moe_bias_rate``), those of every
+        data-parallel rank: one all-reduce for all layers."""
+        import torch.distributed as dist
+        moes = [layer.moe for layer in self.layers if getattr(layer, "moe", None) is not None and layer.moe.bias_rate]
+        if not moes:
+            return
+        loads = torch.stack([m.route_load for m in moes])
+        if dist.is_available() and dist.is_initialized() and dist.get_world_size() > 1:
+            if loads.is_cuda and dist.get_backend() == "gloo":
+                total = loads.cpu()
+                dist.all_reduce(total)
+                loads.copy_(total)
+            else:
+                dist.all_reduce(loads)
+        for m, load in zip(moes, loads):
+            m.move_route_bias(load)
 
     def logits(self, ids: torch.Tensor) -> torch.Tensor:
         x, _ = self.hidden(ids)

@@ -13,7 +13,7 @@ Auxiliary load-balancing loss:
 * ``switch``: ``E * sum_e f_e * P_e`` with f_e the routed-token fraction.
 
 The routing options of the config (sigmoid scores, a selection bias, groups, plain or scaled weights) go
-through ``api.route_topk``; the selection bias moves after each optimizer step (``update_route_bias``).
+through ``api.route_topk``; the selection bias moves after each optimizer step (``LitGPT.update_route_bias``).
 
 Expert weights are stored stacked ([E, 2I, H] gate|up interleaved, [E, H, I])
 so a grouped GEMM can address them; ``export_ref`` writes the upstream
@@ -181,13 +181,9 @@ class MoE(RefModule):
         return resid + y, aux
 
     @torch.no_grad()
-    def update_route_bias(self) -> None:
-        """bias_e += rate * sign(mean load - load_e), with the loads of every data-parallel rank; then the
-        loads start again.  No host synchronisation."""
-        import torch.distributed as dist
-        if dist.is_available() and dist.is_initialized() and dist.get_world_size() > 1:
-            dist.all_reduce(self.route_load)
-        self.route_bias.add_(torch.sign(self.route_load.mean() - self.route_load), alpha=self.bias_rate)
+    def move_route_bias(self, load: torch.Tensor) -> None:
+        """bias_e += rate * sign(mean load - load_e); then the loads start again.  No host synchronisation."""
+        self.route_bias.add_(torch.sign(load.mean() - load), alpha=self.bias_rate)
         self.route_load.zero_()
 
     # ------------------------------------------------------------ names

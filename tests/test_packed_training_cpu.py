@@ -117,10 +117,33 @@ def test_a_trainer_step(tmp_path):
 
 
 @pytest.mark.parametrize("bad,match", [
-    (dict(doc_separator=50), "vocabulary"), (dict(attn_softcap=0.0), "attn_softcap"), (dict(moe_score="relu"), "moe_score"),
+    (dict(doc_separator=50), "vocabulary"), (dict(doc_separator=-1), "doc_separator"), (dict(moe_bias_rate=-1.0), "moe_bias_rate"), (dict(attn_softcap=0.0), "attn_softcap"), (dict(moe_score="relu"), "moe_score"),
     (dict(moe_groups=3), "groups"), (dict(moe_groups=4, moe_top_groups=5), "groups"),
     (dict(moe_groups=8, moe_top_groups=1), "experts_per_tok"),
     (dict(doc_separator=1, mamba_layers=[0], mamba2_num_heads=8, mamba2_head_dim=8, mamba2_expand=2), "Mamba")])
 def test_config_refusals(bad, match):
     with pytest.raises(ConfigError, match=match):
         config(**bad)
+
+
+def _balance_rank(rank, store, out):
+    import torch.distributed as dist
+    dist.init_process_group("gloo", init_method=f"file://{store}", rank=rank, world_size=2)
+    model = build_model(config(**OPTIONS).model, seed=6)
+    _, row = packed(10 + rank)
+    loss, _ = model(row[:, :-1], row[:, 1:])
+    loads = [layer.moe.route_load.clone() for layer in model.layers]
+    model.update_route_bias()
+    torch.save((loads, [layer.moe.route_bias for layer in model.layers]), f"{out}.{rank}")
+    dist.destroy_process_group()
+
+
+def test_ranks_move_the_bias_by_their_common_load(tmp_path):
+    import torch.multiprocessing as mp
+    out = str(tmp_path / "out")
+    mp.start_processes(_balance_rank, args=(str(tmp_path / "store"), out), nprocs=2, start_method="spawn")
+    (l0, b0), (l1, b1) = (torch.load(f"{out}.{r}") for r in range(2))
+    assert any(not torch.equal(x, y) for x, y in zip(l0, l1))
+    for x, y, u, v in zip(l0, l1, b0, b1):
+        total = x + y
+        assert torch.equal(u, v) and torch.equal(u, 0.01 * torch.sign(total.mean() - total))

@@ -491,3 +491,30 @@ def test_one_key_gets_no_gradient_through_its_score(S, causal, cap):
         want = do.double().unflatten(2, (2, 2)).sum(3)
         assert ((dv.double() - want).abs() <= HALF * want.abs() + 2 * (HALF + REST) * do.double().unflatten(2, (2, 2)).abs().sum(3)).all()
     finish()
+
+
+def test_offsets_past_31_bits():
+    """The last row of a batch of 2.4e9 elements gives what it gives alone."""
+    B, S, H, D = 24, 8192, 32, 128
+    qkv = torch.empty(B, S, 3 * H * D, dtype=torch.bfloat16, device="cuda").normal_().requires_grad_()
+    doc = (torch.arange(S, device="cuda") // 200).expand(B, S)
+    do = torch.empty(B, S, H * D, dtype=torch.bfloat16, device="cuda").normal_()
+    o = api.attention_qkv(qkv, H, H, D, D ** -0.5, mask=api.document_mask(doc))
+    g, = torch.autograd.grad(o, qkv, do)
+    one = qkv.detach()[-1:].clone().requires_grad_()
+    o1 = api.attention_qkv(one, H, H, D, D ** -0.5, mask=api.document_mask(doc[-1:]))
+    g1, = torch.autograd.grad(o1, one, do[-1:])
+    assert torch.equal(o[-1:], o1) and torch.equal(g[-1:], g1)
+    finish()
+
+
+def test_nothing_to_attend():
+    """No tokens, and no rows."""
+    for B, S in ((2, 0), (0, 5)):
+        m = api.document_mask(torch.zeros(B, S, dtype=torch.int64, device="cuda"))
+        assert m.lo.shape == (B, S)
+        q, k, v, do = inputs(B, S, 2, 1, 64, 64)
+        for kw in (dict(mask=m), dict(softcap=5.0), {}):
+            for x, y in zip(run(q, k, v, do, 0.125, **kw), (q, q, k, v)):
+                assert x.shape == y.shape
+    finish()

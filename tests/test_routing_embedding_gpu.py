@@ -281,3 +281,27 @@ def test_one_renormalised_expert(E, score):
     assert (got[4].double() - want[4]).norm() <= 256 * F32 * want[4].norm()
     got, _ = route_both(x, 1, dw, torch.zeros_like(du), score=score, scale=2.5)
     assert not got[4].any()
+
+
+def test_embedding_offsets_past_31_bits():
+    """Rows of a table of 2.3e9 elements, the last of them too."""
+    V, H = 1_150_000, 2048
+    w = torch.empty(V, H, dtype=torch.bfloat16, device="cuda").normal_().requires_grad_()
+    ids = torch.tensor([[V - 1, 0, V - 1, 1_100_000]], device="cuda")
+    y = api.embedding(ids, w)
+    assert torch.equal(y, w.detach()[ids])
+    dy = torch.randn(1, 4, H, device="cuda").bfloat16()
+    g, = torch.autograd.grad(y, w, dy)
+    want = (dy[0, 0].float() + dy[0, 2].float()).bfloat16()
+    assert torch.equal(g[V - 1], want) and torch.equal(g[0], dy[0, 1]) and torch.equal(g[1_100_000], dy[0, 3])
+    assert int((g != 0).any(1).sum()) == 3
+    finish()
+
+
+def test_routing_of_no_tokens():
+    x = torch.zeros(0, 16, device="cuda").requires_grad_()
+    topi, topw, usage, counts = api.route_topk(x, 2)
+    assert topi.shape == topw.shape == (0, 2) and not usage.any() and not counts.any()
+    g, = torch.autograd.grad(topw.sum() + usage.sum(), x)
+    assert g.shape == x.shape
+    finish()

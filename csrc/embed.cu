@@ -19,7 +19,8 @@
 //
 // 16384 tokens, 128354 x 2048 bf16: forward 15 us, memset 87, sort 20.5 (two passes of 9 bits over one cluster of 8
 // CTAs: latency), reduce 32 (134 MB read, 4.2 TB/s), join 17 (one token is a twentieth of the batch: its parts are one
-// warp's chain); 689 MB in 167 us.  256 tokens, 100315 x 128 f32: 2, 10, 12, 12 and 2 us, less than the host takes.
+// warp's chain); 689 MB in 167 us.  256 tokens, 100315 x 128 f32: forward 2 us, memset 10, the sum
+// without a sort 4, less than the host takes.
 // Tried and no faster: zeroing in the sort's launch by other clusters, zeroing last and only what no token names,
 // rows of 2 or 4 steps ahead, blocks of 8 or 16 rows.
 #include <cooperative_groups.h>
@@ -292,6 +293,64 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const int* __restri
   put_row<TO, N, ACC>(dw, id, H, c, acc, scale);
 }
 
+// -------------------------------------------------------------------- few tokens
+// Without a sort: the warp of an id's first token adds the rows of all of its tokens, in order.  Every warp looks at
+// every id (in shared memory, 32 at a time), and one token that is most of the batch is one warp's chain, so this is
+// for few tokens, where the sort's launches are what counts.  256 tokens of 2048 bf16, 1000 rows: 5 us (with the sort 26, three more
+// launches), and the host's part falls from 33 to 11 us; with one token that is 70 % of the batch 38 us, as long as the
+// sort's kernels and launches (37).  Of 512 tokens that one took 77 us.
+constexpr int EB_FEW = 256;
+
+template <typename TI, typename TO, int N, bool ACC>
+__global__ void __launch_bounds__(256) embedding_few_kernel(const int64_t* __restrict__ ids, const TI* __restrict__ dy,
+                                                            TO* dw, int T, int64_t V, int H, float scale) {
+  __shared__ int s_id[EB_FEW];
+  for (int i = threadIdx.x; i < EB_FEW; i += 256) {
+    const int64_t id = i < T ? ids[i] : -1;
+    s_id[i] = id >= 0 && id < V ? (int)id : -1;
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 31, t = blockIdx.x * 8 + threadIdx.x / 32, c = (blockIdx.y * 32 + lane) * N;
+  if (t >= T) return;
+  const int id = s_id[t];
+  if (id < 0) return;
+  for (int p0 = 0; p0 < t; p0 += 32)
+    if (__any_sync(0xffffffffu, p0 + lane < t && s_id[p0 + lane] == id)) return;
+  float acc[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  for (int p0 = t & ~31; p0 < T; p0 += 32) {
+    uint32_t here = __ballot_sync(0xffffffffu, p0 + lane >= t && s_id[p0 + lane] == id);
+    while (here) {  // eight rows in flight
+      float v[8][N];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const int p = here ? p0 + __ffs(here) - 1 : -1;
+        here &= here - 1;
+        if (p >= 0 && c < H) {
+          Cols<TI, N>::load(dy + (int64_t)p * H + c, v[q]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i) v[q][i] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] += v[q][i];
+    }
+  }
+  if (c < H) put_row<TO, N, ACC>(dw, id, H, c, acc, scale);
+}
+
+template <typename TI, typename TO, int N, bool ACC>
+void launch_few(const int64_t* ids, const void* dy, void* dw, int T, int64_t V, int H, float scale, cudaStream_t st) {
+  const dim3 grid((unsigned)((T + 7) / 8), (unsigned)((H + 32 * N - 1) / (32 * N)));
+  embedding_few_kernel<TI, TO, N, ACC><<<grid, 256, 0, st>>>(ids, reinterpret_cast<const TI*>(dy),
+                                                             reinterpret_cast<TO*>(dw), T, V, H, scale);
+  OXI_CUDA_CHECK(cudaGetLastError());
+}
+
 int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 template <typename TI, typename TO, int N, bool ACC>
@@ -328,6 +387,7 @@ void launch_embedding_fwd(const int64_t* ids, const void* w, void* out, bool bf1
 }
 
 int64_t embedding_bwd_workspace(int64_t T, int H) {
+  if (T <= EB_FEW) return 0;
   const int64_t blocks = (T + EB_ROWS - 1) / EB_ROWS;
   return 4 * round_up(T * 4, 256) + (blocks > 1 ? blocks * 2 * (int64_t)H * 4 : 0);
 }
@@ -338,6 +398,18 @@ void launch_embedding_bwd(const int64_t* ids, const void* dy, bool bf16, void* d
   OXI_CHECK(T < (1LL << 31) && V < (1LL << 27), "embedding gradient: fewer than 2^31 tokens and 2^27 rows");
   if (!accumulate) OXI_CUDA_CHECK(cudaMemsetAsync(dw, 0, (size_t)V * H * (bf16 ? 2 : 4), st));
   if (T == 0) return;
+  const bool vec = H % 8 == 0 && aligned16(dy) && aligned16(dw);
+  if (T <= EB_FEW) {
+#define OXI_EF(TI, TO, ACC)                                                                  \
+  do {                                                                                      \
+    if (vec) launch_few<TI, TO, 8, ACC>(ids, dy, dw, (int)T, V, H, scale, st);               \
+    else launch_few<TI, TO, 1, ACC>(ids, dy, dw, (int)T, V, H, scale, st);                   \
+  } while (0)
+    if (accumulate) { if (bf16) OXI_EF(__nv_bfloat16, float, true); else OXI_EF(float, float, true); }
+    else { if (bf16) OXI_EF(__nv_bfloat16, __nv_bfloat16, false); else OXI_EF(float, float, false); }
+#undef OXI_EF
+    return;
+  }
   SortParams s;
   s.ids = ids;
   s.V = V;
@@ -372,7 +444,6 @@ void launch_embedding_bwd(const int64_t* ids, const void* dy, bool bf16, void* d
   OXI_CUDA_CHECK(cudaLaunchKernelEx(&cfg, embedding_sort_kernel, s));
   const int* key = s.key[(s.passes - 1) & 1];
   const int* pos = s.pos[(s.passes - 1) & 1];
-  const bool vec = H % 8 == 0 && aligned16(dy) && aligned16(dw);
 #define OXI_ER(TI, TO, ACC)                                                                                 \
   do {                                                                                                     \
     if (vec) launch_reduce<TI, TO, 8, ACC>(key, pos, dy, dw, part, (int)T, (int)V, H, scale, st);           \

@@ -305,3 +305,26 @@ def test_routing_of_no_tokens():
     g, = torch.autograd.grad(topw.sum() + usage.sum(), x)
     assert g.shape == x.shape
     finish()
+
+
+@pytest.mark.parametrize("T", [1, 31, 33, 255, 256, 257, 500])
+@pytest.mark.parametrize("H,dt", [(40, torch.bfloat16), (256, torch.float32), (7, torch.float32)])
+@pytest.mark.parametrize("hot", [0.0, 0.8])
+def test_embedding_of_few_tokens(T, H, dt, hot):
+    """Either side of the size where the gradient sorts, with one token that is most of the batch; new and added to."""
+    from oxidizr_b200.ops._C import ext
+    V = 90
+    g = torch.Generator(device="cuda").manual_seed(T + H)
+    ids = torch.randint(0, V, (T,), generator=g, device="cuda")
+    ids = torch.where(torch.rand(T, generator=g, device="cuda") < hot, 5, ids)
+    dy = torch.randn(T, H, generator=g, device="cuda").to(dt)
+    want = torch.zeros(V, H, dtype=torch.float64, device="cuda").index_add_(0, ids, dy.double())
+    size = torch.zeros_like(want).index_add_(0, ids, dy.double().abs())
+    got = ext().embedding_bwd(ids, dy, V, 2.0, None)
+    step = BF16 if dt == torch.bfloat16 else F32
+    # a sum of up to T terms in f32, the scale and the rounding of the type
+    assert ((got.double() - 2 * want).abs() <= step * 2 * want.abs() + (T + 4) * F32 * 2 * size + 1e-30).all()
+    acc = torch.ones(V, H, device="cuda")
+    ext().embedding_bwd(ids, dy, V, 2.0, acc)
+    assert ((acc.double() - 1 - 2 * want).abs() <= (T + 6) * F32 * (1 + 2 * size)).all()
+    assert torch.equal(acc[size.sum(1) == 0], torch.ones_like(acc[size.sum(1) == 0]))

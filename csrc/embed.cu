@@ -18,7 +18,7 @@
 // is most of what a large vocabulary costs.
 //
 // 16384 tokens, 128354 x 2048 bf16: forward 15 us, memset 87, sort 20.5 (two passes of 9 bits over one cluster of 8
-// CTAs: latency), reduce 32 (134 MB read, 4.2 TB/s), join 17 (one token is a twentieth of the batch: its parts are one
+// CTAs: latency), reduce 32 (67 MB read, some 40 written: 3.3 TB/s), join 17 (one token is a twentieth of the batch: its parts are one
 // warp's chain); 689 MB in 167 us.  256 tokens, 100315 x 128 f32: forward 2 us, memset 10, the sum
 // without a sort 4, less than the host takes.
 // Tried and no faster: zeroing in the sort's launch by other clusters, zeroing last and only what no token names,

@@ -17,6 +17,7 @@
 // 481 us (1143 of its four); with a cap of 50, whose tanh and derivative are instructions, 480 and 556 us; heads of 64:
 // 286 and 393 us (16 / 16 heads).  8 x 2048 tokens in documents of 700, capped: 241 and 230 us.  16 x 1024 tokens in
 // documents of 300, heads of 96 and 64: 104 and 113 us, half of it a CTA's start and end (4 us, one CTA a SM).
+// Tried and no faster: dK / dV's CTAs started under dQ's last wave (a programmatic launch).
 //
 // P and dS are rounded to bf16 for the tensor cores (2^-8 of each term at most, with random signs over the keys of a
 // row); statistics, delta and accumulators are f32.
@@ -831,7 +832,8 @@ void launch_bwd_t(const BwdArgs& a) {
   const CUtensorMap tq = da_tmap(a.q, s.B, s.S, s.Hq, s.Dqk), td = da_tmap(a.dout, s.B, s.S, s.Hq, s.Dv),
                     tk = da_tmap(a.k, s.B, s.S, s.Hk, s.Dqk), tv = da_tmap(a.v, s.B, s.S, s.Hk, s.Dv),
                     tk64 = da_tmap(a.k, s.B, s.S, s.Hk, s.Dqk, DQ_KEYS), tv64 = da_tmap(a.v, s.B, s.S, s.Hk, s.Dv, DQ_KEYS),
-                    tq64 = da_tmap(a.q, s.B, s.S, s.Hq, s.Dqk, KV_QUERIES), td64 = da_tmap(a.dout, s.B, s.S, s.Hq, s.Dv, KV_QUERIES),
+                    tq64 = da_tmap(a.q, s.B, s.S, s.Hq, s.Dqk, KV_QUERIES),
+                    td64 = da_tmap(a.dout, s.B, s.S, s.Hq, s.Dv, KV_QUERIES),
                     tdq = da_tmap_out(a.dq, s.B, s.S, s.Hq, s.Dqk);
   auto kq = da_dq_kernel<DQP, DVP, CAP, ALIBI>;
   auto kkv = da_dkv_kernel<DQP, DVP, CAP, ALIBI>;
@@ -875,8 +877,8 @@ int da_bwd_splits(int B, int S, int Hq, int Hk) {
 }
 
 void launch_da_bwd(const DaShape& s, const DaTensor& q, const DaTensor& k, const DaTensor& v, const DaTensor& o,
-                   const DaTensor& o_lo, const DaTensor& dout, const float* nlse2, float* ndelta, float* part, const DaOut& dq, const DaOut& dk,
-                   const DaOut& dv, int* status, cudaStream_t st) {
+                   const DaTensor& o_lo, const DaTensor& dout, const float* nlse2, float* ndelta, float* part,
+                   const DaOut& dq, const DaOut& dk, const DaOut& dv, int* status, cudaStream_t st) {
   if (s.B == 0 || s.S == 0 || s.Hq == 0) return;
   da_check(s);
   for (const DaOut* t : {&dq, &dk, &dv})

@@ -18,8 +18,8 @@
 // is most of what a large vocabulary costs.
 //
 // 16384 tokens, 128354 x 2048 bf16: forward 15 us, memset 87, sort 20.5 (two passes of 9 bits over one cluster of 8
-// CTAs: latency), reduce 32 (67 MB read, some 40 written: 3.3 TB/s), join 17 (one token is a twentieth of the batch: its parts are one
-// warp's chain); 689 MB in 167 us.  256 tokens, 100315 x 128 f32: forward 2 us, memset 10, the sum
+// CTAs: latency), reduce 32 (67 MB read, some 40 written: 3.3 TB/s), join 17 (one token is a twentieth of the batch:
+// its parts are one warp's chain); 689 MB in 167 us.  256 tokens, 100315 x 128 f32: forward 2 us, memset 10, the sum
 // without a sort 4, less than the host takes.
 // Tried and no faster: zeroing in the sort's launch by other clusters, zeroing last and only what no token names,
 // rows of 2 or 4 steps ahead, blocks of 8 or 16 rows.
@@ -296,9 +296,9 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const int* __restri
 // -------------------------------------------------------------------- few tokens
 // Without a sort: the warp of an id's first token adds the rows of all of its tokens, in order.  Every warp looks at
 // every id (in shared memory, 32 at a time), and one token that is most of the batch is one warp's chain, so this is
-// for few tokens, where the sort's launches are what counts.  256 tokens of 2048 bf16, 1000 rows: 5 us (with the sort 26, three more
-// launches), and the host's part falls from 33 to 11 us; with one token that is 70 % of the batch 38 us, as long as the
-// sort's kernels and launches (37).  Of 512 tokens that one took 77 us.
+// for few tokens, where the sort's launches are what counts.  256 tokens of 2048 bf16, 1000 rows: 5 us (with the sort
+// 26, three more launches), and the host's part falls from 33 to 11 us; with one token that is 70 % of the batch 38 us,
+// as long as the sort's kernels and launches (37).  Of 512 tokens that one took 77 us.
 constexpr int EB_FEW = 256;
 
 template <typename TI, typename TO, int N, bool ACC>

@@ -38,14 +38,14 @@ struct DaShape {
   const int *lo, *hi, *qt, *kt;  // all or none
 };
 bool da_supported(int Dqk, int Dv);
-// o [B*S, Hq*Dv] bf16, o_lo (null, or for a backward) what the rounding left over; nlse2 [B, Hq, S] f32: minus log2 of the row's sum of 2^score (-inf for a row that sees
-// nothing), what the backward adds to a score
+// o [B*S, Hq*Dv] bf16; o_lo (null, or for a backward) what its rounding left over; nlse2 [B, Hq, S] f32: minus log2
+// of the row's sum of 2^score (-inf for a row that sees nothing), what the backward adds to a score
 void launch_da_fwd(const DaShape& s, const DaTensor& q, const DaTensor& k, const DaTensor& v, const DaOut& o,
                    const DaOut& o_lo, float* nlse2, int* status, cudaStream_t st);
 // dq, dk, dv from dout [B, S, Hq, Dv].  ndelta [B, Hq, S] f32 is scratch, and part too: with
 // da_bwd_splits > 1 that many f32 [B, Hk, S, Dv] and then [B, Hk, S, Dqk].
 int da_bwd_splits(int B, int S, int Hq, int Hk);
 void launch_da_bwd(const DaShape& s, const DaTensor& q, const DaTensor& k, const DaTensor& v, const DaTensor& o,
-                   const DaTensor& o_lo, const DaTensor& dout, const float* nlse2, float* ndelta, float* part, const DaOut& dq, const DaOut& dk,
-                   const DaOut& dv, int* status, cudaStream_t st);
+                   const DaTensor& o_lo, const DaTensor& dout, const float* nlse2, float* ndelta, float* part,
+                   const DaOut& dq, const DaOut& dk, const DaOut& dv, int* status, cudaStream_t st);
 }  // namespace oxi

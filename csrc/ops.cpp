@@ -505,8 +505,8 @@ void da_backward(const torch::Tensor& q, const torch::Tensor& k, const torch::Te
   const auto tq = da_operand(q, q, "q"), tk = da_operand(k, q, "k"), tv = da_operand(v, q, "v"),
              to = da_operand(o, q, "o"), tl = da_operand(o_lo, q, "o_lo"),
              td = da_operand(dout, q, "the output's gradient");
-  OXI_CHECK(o.sizes() == dout.sizes() && o_lo.sizes() == dout.sizes() && o.size(0) == s.B && o.size(1) == s.S && o.size(2) == s.Hq &&
-                o.size(3) == s.Dv, "attention backward: o and its gradient must be [B, S, Hq, Dv]");
+  OXI_CHECK(o.sizes() == dout.sizes() && o_lo.sizes() == dout.sizes() && o.size(0) == s.B && o.size(1) == s.S &&
+                o.size(2) == s.Hq && o.size(3) == s.Dv, "attention backward: o and its gradient must be [B, S, Hq, Dv]");
   OXI_CHECK(nlse2.device() == q.device() && nlse2.scalar_type() == torch::kFloat32 && nlse2.is_contiguous() &&
                 nlse2.numel() == (int64_t)s.B * s.Hq * s.S, "attention backward: nlse2");
   auto ndelta = torch::empty_like(nlse2);

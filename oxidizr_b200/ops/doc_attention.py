@@ -11,7 +11,8 @@ and a token that sees nothing (padding) gets zeros and passes no gradient on.  W
 q, k, v and the output's gradient hold does not matter, not even NaN.
 
 bf16 CUDA tensors with head widths that are multiples of 8 up to 128 run csrc/doc_attn_fwd.cu and
-csrc/doc_attn_bwd.cu (autograd nodes in csrc/ops.cpp, first derivatives only); everything else runs the statement of the same math in ``ops.reference``.
+csrc/doc_attn_bwd.cu (autograd nodes in csrc/ops.cpp, first derivatives only); everything else runs the
+statement of the same math in ``ops.reference``.
 """
 from __future__ import annotations
 

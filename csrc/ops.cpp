@@ -1479,11 +1479,11 @@ struct EmbeddingLookup : torch::autograd::Function<EmbeddingLookup> {
   static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& ids, const torch::Tensor& w, double scale,
                                const torch::Tensor& status) {
     at::AutoDispatchBelowADInplaceOrView below;  // nothing here is recorded
-    const auto flat = ids.contiguous().view({-1});
-    auto out = embedding_fwd(flat, w.contiguous(), scale, status);
+    auto out = embedding_fwd(ids.contiguous().view({-1}), w.contiguous(), scale, status);
     auto shape = ids.sizes().vec();
     shape.push_back(w.size(1));
-    ctx->save_for_backward({flat});
+    // ids themselves: a view made here has a version of its own, and would not see that they were overwritten
+    ctx->save_for_backward({ids});
     ctx->saved_data["rows"] = w.size(0);
     ctx->saved_data["scale"] = scale;
     return out.view(shape);
@@ -1493,7 +1493,7 @@ struct EmbeddingLookup : torch::autograd::Function<EmbeddingLookup> {
   }
   static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const auto ids = ctx->get_saved_variables()[0];
+    const auto ids = ctx->get_saved_variables()[0].contiguous().view({-1});
     const auto& dy = grads[0];
     ++g_node_backwards;
     auto dw = embedding_bwd(ids, dy.reshape({ids.numel(), dy.size(-1)}).contiguous(), ctx->saved_data["rows"].toInt(),

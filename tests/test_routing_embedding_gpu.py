@@ -328,3 +328,31 @@ def test_embedding_of_few_tokens(T, H, dt, hot):
     ext().embedding_bwd(ids, dy, V, 2.0, acc)
     assert ((acc.double() - 1 - 2 * want).abs() <= (T + 6) * F32 * (1 + 2 * size)).all()
     assert torch.equal(acc[size.sum(1) == 0], torch.ones_like(acc[size.sum(1) == 0]))
+
+
+@pytest.mark.parametrize("main_grad", [False, True])
+@pytest.mark.parametrize("shape", [(3, 50), (700,)])
+def test_ids_overwritten_before_the_backward(shape, main_grad):
+    """Ids in a buffer that the next batch is copied into: the gradient of the old batch is refused, not scattered to the
+    new one's rows."""
+    ids = torch.randint(0, 30, shape, device="cuda")
+    for view in (ids, ids.t()) if len(shape) == 2 else (ids, ids[::2]):
+        w = torch.nn.Parameter(torch.randn(30, 16, device="cuda").bfloat16())
+        if main_grad:
+            w.main_grad = torch.zeros(30, 16, device="cuda")
+        y = api.embedding(view, w)
+        ids.copy_(ids.flip(0))
+        # (ids that are not contiguous may have been copied: then the old batch's rows are what they get)
+        if view.is_contiguous() or not main_grad:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.sum().backward()
+    finish()
+
+
+def test_outputs_overwritten_before_the_backward():
+    x = torch.randn(40, 16, device="cuda", requires_grad=True)
+    topi, topw, _, _ = api.route_topk(x, 3)
+    topi.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        topw.sum().backward()
+    finish()

@@ -16,7 +16,7 @@
 //
 // Backward, per token (g = d_usage / T, S = sum s):
 //   ds_j += scale (dw_j - sum_i dw_i s_i / n) / n for the chosen (n = sum of the chosen s; renorm),
-//   ds   += (g - sum_e g_e s_e / S) / S,  then dx = s (ds - sum s ds) or ds s (1 - s).
+//   ds   += (g - sum_e g_e s_e / S) / S,  then dx = s (ds - sum s ds) or ds s(x) s(-x) (sigmoid).
 //
 // A lane holds EPL neighbouring experts, so that a row is one vector load a lane, a group of
 // neighbours sits in neighbouring lanes (its rank takes log2 of their number shuffles), and the
@@ -601,18 +601,27 @@ __global__ void __launch_bounds__(RT_WARPS * 32) router_bwd_kernel(const LT* __r
     }
     if (lane < s.k) s_g[e] = g;
     __syncwarp();
-    float sd = 0.f;
+    alignas(16) LT out[EPL];
+    if (s.sigmoid) {
+      // 1 - p is the sigmoid of -x: the difference would be rounding alone for large x, and zero from x = 17 on
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      d[i] = (dusage ? (du[i] - gs) * inv : 0.f) + s_g[e0 + i];
-      sd += p[i] * d[i];
+      for (int i = 0; i < EPL; ++i) {
+        const float ds = (dusage ? (du[i] - gs) * inv : 0.f) + s_g[e0 + i];
+        from_f(out[i], ds * p[i] * rcp_approx(1.f + exp_approx(d[i])));
+      }
+    } else {
+      float sd = 0.f;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) {
+        d[i] = (dusage ? (du[i] - gs) * inv : 0.f) + s_g[e0 + i];
+        sd += p[i] * d[i];
+      }
+      sd = warp_sum(sd);
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) from_f(out[i], p[i] * (d[i] - sd));
     }
     __syncwarp();
     if (lane < s.k) s_g[e] = 0.f;
-    if (!s.sigmoid) sd = warp_sum(sd);
-    alignas(16) LT out[EPL];
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) from_f(out[i], s.sigmoid ? d[i] * p[i] * (1.f - p[i]) : p[i] * (d[i] - sd));
     LT* dst = dlogits + t * s.E + e0;  // contiguous rows
     constexpr int BYTES = EPL * (int)sizeof(LT);
     if (s.E % EPL == 0 && BYTES >= 4) {

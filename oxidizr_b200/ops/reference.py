@@ -334,6 +334,24 @@ def adamw_step(p, g, m, v, step: int, lr: float, beta1=0.9, beta2=0.999, eps=1e-
 
 
 # ----------------------------------------------------------------- routing
+class _Sigmoid(torch.autograd.Function):
+    """Sigmoid with the derivative s(x) s(-x): formed as s (1 - s) it is rounding alone where s is close to 1."""
+
+    @staticmethod
+    def forward(ctx, x):
+        ctx.save_for_backward(x)
+        return torch.sigmoid(x)
+
+    @staticmethod
+    def backward(ctx, dy):
+        (x,) = ctx.saved_tensors
+        return dy * sigmoid(x) * sigmoid(-x)
+
+
+def sigmoid(x: torch.Tensor) -> torch.Tensor:
+    return _Sigmoid.apply(x)
+
+
 def route_topk(logits: torch.Tensor, k: int, score: str = "softmax", bias: Optional[torch.Tensor] = None,
                groups: int = 1, top_groups: int = 1, group_top: int = 2, renorm: bool = True, scale: float = 1.0):
     """Top-k routing (model.rs:541-556 is softmax scores without bias and groups): the choice in f64, where
@@ -341,7 +359,7 @@ def route_topk(logits: torch.Tensor, k: int, score: str = "softmax", bias: Optio
     T, E = logits.shape
 
     def scores(x):
-        return torch.softmax(x, -1) if score == "softmax" else torch.sigmoid(x)
+        return torch.softmax(x, -1) if score == "softmax" else sigmoid(x)
 
     with torch.no_grad():
         x = logits.detach().double()

@@ -103,3 +103,16 @@ def test_the_extension_refuses_with_exceptions():
         e.router_fwd(w, 2, False, None, 1, 1, 2, True, 1.0)
     with pytest.raises(RuntimeError, match="router logits"):
         e.router_bwd(w, torch.zeros(4, 2, dtype=torch.int64), torch.zeros(4, 2), None, False, True, 1.0)
+
+
+def test_gradient_of_saturated_sigmoids():
+    """s (1 - s) is 1e-7 at 16 and 9e-14 at 30: not zero, and not what rounding s to f32 leaves of 1 - s."""
+    x = torch.tensor([[16.0, 20.0, 30.0, -30.0, 12.0]], requires_grad=True)
+    topw = api.route_topk(x, 4, "sigmoid", renorm=False)[1]
+    (g,) = torch.autograd.grad(topw.sum(), x)
+    e = torch.exp(-x.detach().double().abs())
+    # -30 is the one that is not chosen; an exponential, two quotients and a product in f32
+    assert ((g.double() - (e / (1 + e) ** 2).index_fill(1, torch.tensor([3]), 0.0)).abs() <= 8 * 2 ** -24 * e).all()
+    # and the second derivative is that of the formula
+    wide = x.detach().double().requires_grad_(True)
+    assert torch.autograd.gradgradcheck(lambda v: api.route_topk(v / 8, 4, "sigmoid", renorm=False)[1], (wide,))

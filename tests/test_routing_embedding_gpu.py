@@ -356,3 +356,32 @@ def test_outputs_overwritten_before_the_backward():
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         topw.sum().backward()
     finish()
+
+
+@pytest.mark.parametrize("E,k", [(6, 2), (64, 8), (200, 8)])
+@pytest.mark.parametrize("renorm", [True, False])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_gradient_of_saturated_sigmoids(E, k, renorm, dt):
+    """Logits out to 30, where s is 1 to f32 and 1 - s is not nothing: the gradient is held relative to s (1 - s)."""
+    T, scale = 300, 2.5
+    g = torch.Generator(device="cuda").manual_seed(E)
+    x = ((torch.rand(T, E, generator=g, device="cuda") * 2 - 1) * 30).to(dt)
+    x[::7] = x[::7].abs()  # tokens with positive logits alone
+    dw, du = torch.randn(T, k, generator=g, device="cuda"), torch.randn(E, generator=g, device="cuda")
+    got, want = route_both(x, k, dw, du, score="sigmoid", renorm=renorm, scale=scale)
+    assert torch.equal(got[0], want[0])
+    s, q = torch.sigmoid(x.double()), torch.sigmoid(-x.double())
+    S = s.sum(-1, keepdim=True)
+    sel = s.gather(1, want[0])
+    n = sel.sum(-1, keepdim=True) if renorm else torch.ones_like(S)
+    a = dw.double().abs() * scale / n
+    # renormalised, of differences from the first gradient: up to twice each, and their mean
+    a = 2 * a + 2 * (a * sel).sum(-1, keepdim=True) / n if renorm else a
+    part = torch.zeros_like(s).scatter_add_(1, want[0], a)
+    u = du.double().abs() / T
+    part = part + (u + (u * s).sum(-1, keepdim=True) / S) / S
+    # e^x is off by |x| + 4 steps of f32, in s or in 1 - s and in the sums of s; quotients, products and sums 40 more
+    tol = (2 * 30 + 48) * F32 * s * q * part
+    step = BF16 if dt == torch.bfloat16 else F32
+    assert ((got[4].double() - want[4]).abs() <= step * want[4].abs() + tol + 1e-30).all()
+    finish()

@@ -229,19 +229,32 @@ void check_embedding(const torch::Tensor& ids, const torch::Tensor& w, const cha
             "embedding: ids must be contiguous int64 on the same device");
 }
 
-torch::Tensor embedding_fwd(torch::Tensor ids, torch::Tensor w, double scale, torch::Tensor status) {
+// (rows, order): the tokens' order for embedding_bwd with train (undefined where that needs none)
+std::pair<torch::Tensor, torch::Tensor> embedding_fwd_train(torch::Tensor ids, torch::Tensor w, double scale,
+                                                            torch::Tensor status, bool train) {
   check_embedding(ids, w, "w");
   c10::cuda::CUDAGuard g(w.device());
-  auto out = torch::empty({ids.numel(), w.size(1)}, w.options());
+  const int64_t T = ids.numel(), n = train ? oxi::embedding_order_bytes(T, w.size(0)) : 0;
+  const auto bytes = torch::TensorOptions().dtype(torch::kUInt8).device(w.device());
+  torch::Tensor out = torch::empty({T, w.size(1)}, w.options()), order, scratch;
+  if (n > 0 && w.size(1) > 0) {
+    order = torch::empty({n}, bytes);
+    scratch = torch::empty({n}, bytes);
+  }
   oxi::launch_embedding_fwd(ids.data_ptr<int64_t>(), w.data_ptr(), out.data_ptr(),
-                            w.scalar_type() == torch::kBFloat16, ids.numel(), w.size(0), (int)w.size(1), (float)scale,
-                            status_ptr(status), stream());
-  return out;
+                            w.scalar_type() == torch::kBFloat16, T, w.size(0), (int)w.size(1), (float)scale,
+                            status_ptr(status), order.defined() ? order.data_ptr() : nullptr,
+                            order.defined() ? scratch.data_ptr() : nullptr, stream());
+  return {out, order};
+}
+torch::Tensor embedding_fwd(torch::Tensor ids, torch::Tensor w, double scale, torch::Tensor status) {
+  return embedding_fwd_train(ids, w, scale, status, false).first;
 }
 
-// The gradient [V, H] of the looked-up rows: a new tensor of dy's type, or added to acc (f32 [V, H]).
+// The gradient [V, H] of the looked-up rows: a new tensor of dy's type, or added to acc (f32 [V, H]).  order: what
+// embedding_fwd_train made of the same ids and V, if it did.
 torch::Tensor embedding_bwd(torch::Tensor ids, torch::Tensor dy, int64_t V, double scale,
-                            c10::optional<torch::Tensor> acc) {
+                            c10::optional<torch::Tensor> acc, c10::optional<torch::Tensor> order) {
   check_embedding(ids, dy, "dy");
   c10::cuda::CUDAGuard g(dy.device());
   const int64_t T = ids.numel(), H = dy.size(1);
@@ -256,10 +269,15 @@ torch::Tensor embedding_bwd(torch::Tensor ids, torch::Tensor dy, int64_t V, doub
   } else {
     dw = torch::empty({V, H}, dy.options());
   }
-  auto ws = torch::empty({oxi::embedding_bwd_workspace(T, (int)H)},
+  const bool ordered = order.has_value() && order->defined();
+  OXI_CHECK(!ordered || (order->device() == dy.device() && order->scalar_type() == torch::kUInt8 &&
+                         order->is_contiguous() && order->numel() == oxi::embedding_order_bytes(T, V)),
+            "embedding gradient: the order is of other ids");
+  auto ws = torch::empty({oxi::embedding_bwd_workspace(T, (int)H, ordered)},
                          torch::TensorOptions().dtype(torch::kUInt8).device(dy.device()));
-  oxi::launch_embedding_bwd(ids.data_ptr<int64_t>(), dy.data_ptr(), dy.scalar_type() == torch::kBFloat16,
-                            dw.data_ptr(), add, T, V, (int)H, (float)scale, ws.data_ptr(), stream());
+  oxi::launch_embedding_bwd(ids.data_ptr<int64_t>(), ordered ? order->data_ptr() : nullptr, dy.data_ptr(),
+                            dy.scalar_type() == torch::kBFloat16, dw.data_ptr(), add, T, V, (int)H, (float)scale,
+                            ws.data_ptr(), stream());
   return dw;
 }
 
@@ -1477,13 +1495,13 @@ struct DocAttentionQKV : torch::autograd::Function<DocAttentionQKV> {
 
 struct EmbeddingLookup : torch::autograd::Function<EmbeddingLookup> {
   static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& ids, const torch::Tensor& w, double scale,
-                               const torch::Tensor& status) {
+                               const torch::Tensor& status, bool train) {
     at::AutoDispatchBelowADInplaceOrView below;  // nothing here is recorded
-    auto out = embedding_fwd(ids.contiguous().view({-1}), w.contiguous(), scale, status);
+    auto [out, order] = embedding_fwd_train(ids.contiguous().view({-1}), w.contiguous(), scale, status, train);
     auto shape = ids.sizes().vec();
     shape.push_back(w.size(1));
     // ids themselves: a view made here has a version of its own, and would not see that they were overwritten
-    ctx->save_for_backward({ids});
+    ctx->save_for_backward({ids, order});
     ctx->saved_data["rows"] = w.size(0);
     ctx->saved_data["scale"] = scale;
     return out.view(shape);
@@ -1493,12 +1511,13 @@ struct EmbeddingLookup : torch::autograd::Function<EmbeddingLookup> {
   }
   static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const auto ids = ctx->get_saved_variables()[0].contiguous().view({-1});
+    const auto saved = ctx->get_saved_variables();
+    const auto ids = saved[0].contiguous().view({-1});
     const auto& dy = grads[0];
     ++g_node_backwards;
     auto dw = embedding_bwd(ids, dy.reshape({ids.numel(), dy.size(-1)}).contiguous(), ctx->saved_data["rows"].toInt(),
-                            ctx->saved_data["scale"].toDouble(), c10::nullopt);
-    return {torch::Tensor(), dw, torch::Tensor(), torch::Tensor()};
+                            ctx->saved_data["scale"].toDouble(), c10::nullopt, maybe(saved[1]));
+    return {torch::Tensor(), dw, torch::Tensor(), torch::Tensor(), torch::Tensor()};
   }
 };
 
@@ -1549,7 +1568,7 @@ torch::Tensor doc_attention_qkv(torch::Tensor qkv, int64_t Hq, int64_t Hk, int64
                                 DaOptions{scale, cap, causal, slopes.value_or(torch::Tensor()), status, mask, train});
 }
 torch::Tensor embedding_lookup(torch::Tensor ids, torch::Tensor w, double scale, torch::Tensor status) {
-  return EmbeddingLookup::apply(ids, w, scale, status);
+  return EmbeddingLookup::apply(ids, w, scale, status, at::GradMode::is_enabled() && w.requires_grad());
 }
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> router_topk(
     torch::Tensor logits, int64_t k, bool sigmoid, c10::optional<torch::Tensor> bias, int64_t groups,
@@ -1586,7 +1605,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("doc_attention_qkv", &doc_attention_qkv, "the same from a fused projection");
   m.def("embedding_lookup", &embedding_lookup, "scaled embedding lookup with its gradient");
   m.def("embedding_fwd", &embedding_fwd, "scaled embedding lookup");
-  m.def("embedding_bwd", &embedding_bwd, "embedding gradient by sorted tokens");
+  m.def("embedding_fwd_train", &embedding_fwd_train, "the same, and the tokens' order for its gradient");
+  m.def("embedding_bwd", &embedding_bwd, "embedding gradient by sorted tokens", py::arg("ids"), py::arg("dy"),
+        py::arg("V"), py::arg("scale"), py::arg("acc"), py::arg("order") = py::none());
   m.def("rope_bwd_to", &rope_bwd_to, "out-of-place RoPE backward (+ copy of the unrotated columns)");
   m.def("rope_bwd", &rope_bwd, "in-place inverse rotate-half RoPE");
   m.def("sqsum", &sqsum, "sum of squares (atomically added into out)");

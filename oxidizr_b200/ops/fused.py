@@ -81,17 +81,17 @@ class _EmbeddingMainGrad(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, w, scale: float):
         ids_f = _c(ids.reshape(-1))
-        out = ext().embedding_fwd(ids_f, _c(w), scale, status(w.device))
-        ctx.save_for_backward(ids_f)
+        out, order = ext().embedding_fwd_train(ids_f, _c(w), scale, status(w.device), ctx.needs_input_grad[1])
+        ctx.save_for_backward(ids_f, order)
         ctx.w, ctx.scale = w, scale
         return out.view(*ids.shape, w.shape[1])
 
     @staticmethod
     def backward(ctx, dy):
-        (ids,) = ctx.saved_tensors
+        ids, order = ctx.saved_tensors
         w = ctx.w
         ext().embedding_bwd(ids, _c(dy.reshape(ids.numel(), w.shape[1])), w.shape[0], ctx.scale,
-                            w.main_grad.view(w.shape))
+                            w.main_grad.view(w.shape), order)
         _ready(w)
         return None, None, None
 

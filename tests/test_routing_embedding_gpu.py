@@ -385,3 +385,74 @@ def test_gradient_of_saturated_sigmoids(E, k, renorm, dt):
     step = BF16 if dt == torch.bfloat16 else F32
     assert ((got[4].double() - want[4]).abs() <= step * want[4].abs() + tol + 1e-30).all()
     finish()
+
+
+@pytest.mark.parametrize("T,V,H", [(1024, 700, 40), (1025, 1, 36), (1500, 3, 7), (5000, 128354, 64), (20000, 2 ** 18 + 1, 8),
+                                   (70000, 511, 24), (300001, 40000, 8)])
+@pytest.mark.parametrize("hot", [0.0, 0.6, 1.0])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_embedding_order_made_beside_the_lookup(T, V, H, hot, dt):
+    """The tokens' order of a lookup that trains, and of a gradient that makes its own: the same bits; ids outside the
+    rows, one token that is most of the batch, sums of thousands of parts."""
+    from oxidizr_b200.ops._C import ext, read_status
+    g = torch.Generator(device="cuda").manual_seed(T + H)
+    ids = torch.randint(0, V, (T,), generator=g, device="cuda")
+    ids = torch.where(torch.rand(T, generator=g, device="cuda") < hot, V // 2, ids)
+    ids[::97] = torch.tensor([-1, V], device="cuda").repeat(T)[:ids[::97].numel()]
+    there = (ids >= 0) & (ids < V)
+    w = torch.randn(V, H, generator=g, device="cuda").to(dt).requires_grad_(True)
+    dy = torch.randn(T, H, generator=g, device="cuda").to(dt)
+    y, other = api.embedding(ids, w, scale=2.0), api.embedding(ids.flip(0), w)
+    assert read_status("cuda") == 3  # the ids outside
+    assert torch.equal(y[there], (w.detach()[ids[there]].float() * 2.0).to(dt)) and not y[~there].any()
+    (dw,) = torch.autograd.grad(y, w, dy, retain_graph=True)
+    (again,) = torch.autograd.grad(y, w, dy)
+    assert torch.equal(dw, again) and torch.equal(dw, ext().embedding_bwd(ids, dy, V, 2.0, None))
+    want = torch.zeros(V, H, dtype=torch.float64, device="cuda").index_add_(0, ids[there], dy[there].double())
+    size = torch.zeros_like(want).index_add_(0, ids[there], dy[there].double().abs())
+    step = BF16 if dt == torch.bfloat16 else F32
+    # runs of up to 32 terms, one sum of their parts, the scale and the rounding of the type
+    steps = 32 + T // 32 + 4
+    assert ((dw.double() - 2 * want).abs() <= step * 2 * want.abs() + steps * F32 * 2 * size + 1e-30).all()
+    (dw,) = torch.autograd.grad(other, w, dy.flip(0))
+    assert ((dw.double() - want).abs() <= step * want.abs() + steps * F32 * size + 1e-30).all()
+    # added to an optimizer's buffer: bit for bit the same each time
+    p = torch.nn.Parameter(w.detach().clone())
+    got = []
+    for _ in range(2):
+        p.main_grad = torch.ones(V, H, device="cuda")
+        api.embedding(ids, p, scale=2.0).backward(dy)
+        got.append(p.main_grad)
+    assert torch.equal(*got) and read_status("cuda") == 3
+    assert ((got[0].double() - 1 - 2 * want).abs() <= F32 * (1 + 2 * want.abs()) + steps * F32 * 2 * size).all()
+    finish()
+
+
+def test_embedding_of_many_tokens_captured_and_on_another_stream():
+    T, V, H = 3000, 500, 64
+    g = torch.Generator(device="cuda").manual_seed(9)
+    ids = [torch.randint(0, V, (T,), generator=g, device="cuda") for _ in range(2)]
+    w = torch.randn(V, H, generator=g, device="cuda").bfloat16().requires_grad_(True)
+    dy = torch.randn(T, H, generator=g, device="cuda").bfloat16()
+
+    def step(i):
+        y = api.embedding(i, w)
+        return [y.detach(), *torch.autograd.grad(y, w, dy)]
+
+    want = [step(i) for i in ids]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = step(ids[0])
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, b) for a, b in zip(other, want[0]))
+    static = ids[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(static)
+    for k in (1, 0, 1):
+        static.copy_(ids[k])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want[k]))
+    finish()

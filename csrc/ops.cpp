@@ -1504,22 +1504,49 @@ struct EmbeddingLookup : torch::autograd::Function<EmbeddingLookup> {
     ctx->save_for_backward({ids, order});
     ctx->saved_data["rows"] = w.size(0);
     ctx->saved_data["scale"] = scale;
+    ctx->saved_data["status"] = status;
     return out.view(shape);
   }
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    return first_order_only(gradients(ctx, grads), "embedding");
-  }
-  static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
+  static variable_list backward(AutogradContext* ctx, variable_list grads);
+};
+
+// The lookup's gradient.  Linear in dy, and its derivative is the lookup again: derivatives of any order.
+struct EmbeddingGradient : torch::autograd::Function<EmbeddingGradient> {
+  static torch::Tensor sum(const torch::Tensor& dy, const torch::Tensor& ids, const c10::optional<torch::Tensor>& order,
+                           int64_t rows, double scale) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const auto saved = ctx->get_saved_variables();
-    const auto ids = saved[0].contiguous().view({-1});
-    const auto& dy = grads[0];
     ++g_node_backwards;
-    auto dw = embedding_bwd(ids, dy.reshape({ids.numel(), dy.size(-1)}).contiguous(), ctx->saved_data["rows"].toInt(),
-                            ctx->saved_data["scale"].toDouble(), c10::nullopt, maybe(saved[1]));
-    return {torch::Tensor(), dw, torch::Tensor(), torch::Tensor(), torch::Tensor()};
+    return embedding_bwd(ids.contiguous().view({-1}), dy.reshape({ids.numel(), dy.size(-1)}).contiguous(), rows, scale,
+                         c10::nullopt, order);
+  }
+  static torch::Tensor forward(AutogradContext* ctx, const torch::Tensor& dy, const torch::Tensor& ids,
+                               const c10::optional<torch::Tensor>& order, int64_t rows, double scale,
+                               const torch::Tensor& status) {
+    ctx->save_for_backward({ids});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["status"] = status;
+    return sum(dy, ids, order, rows, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const bool train = at::GradMode::is_enabled() && grads[0].requires_grad();
+    variable_list out(6);
+    out[0] = EmbeddingLookup::apply(ctx->get_saved_variables()[0], grads[0], ctx->saved_data["scale"].toDouble(),
+                                    ctx->saved_data["status"].toTensor(), train);
+    return out;
   }
 };
+
+variable_list EmbeddingLookup::backward(AutogradContext* ctx, variable_list grads) {
+  const auto saved = ctx->get_saved_variables();
+  const int64_t rows = ctx->saved_data["rows"].toInt();
+  const double scale = ctx->saved_data["scale"].toDouble();
+  const auto order = maybe(saved[1]);
+  variable_list out(5);
+  out[1] = at::GradMode::is_enabled()
+               ? EmbeddingGradient::apply(grads[0], saved[0], order, rows, scale, ctx->saved_data["status"].toTensor())
+               : EmbeddingGradient::sum(grads[0], saved[0], order, rows, scale);
+  return out;
+}
 
 struct RouterTopK : torch::autograd::Function<RouterTopK> {
   static variable_list forward(AutogradContext* ctx, const torch::Tensor& logits_, int64_t k, bool sigmoid,

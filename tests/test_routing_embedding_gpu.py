@@ -456,3 +456,25 @@ def test_embedding_of_many_tokens_captured_and_on_another_stream():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want[k]))
     finish()
+
+
+@pytest.mark.parametrize("T", [6, 1500])
+def test_embedding_differentiated_twice(T):
+    """A penalty on the gradient's size: its derivative by what came back, which is a lookup, and by the weights."""
+    V, H, scale = 40, 8, 3.0
+    g = torch.Generator(device="cuda").manual_seed(T)
+    ids = torch.randint(0, V, (T,), generator=g, device="cuda")
+    w = torch.randn(V, H, generator=g, device="cuda")
+
+    def penalty(look, w):
+        y = look(w)
+        (dw,) = torch.autograd.grad((y * y * y).sum(), w, create_graph=True)
+        assert dw.requires_grad
+        return torch.autograd.grad((dw * dw).sum(), w)[0]
+
+    got = penalty(lambda w: api.embedding(ids, w, scale=scale), w.clone().requires_grad_(True))
+    want = penalty(lambda w: w[ids] * scale, w.double().requires_grad_(True))
+    # sums of up to n rows that are products of a few rounded factors, twice; all terms of a row have one sign each
+    n = int(torch.bincount(ids, minlength=V).max())
+    assert ((got.double() - want).abs() <= (2 * n + 24) * F32 * want.abs()).all()
+    finish()

@@ -131,9 +131,10 @@ class LitGPT(RefModule):
         return loss, aux
 
     @torch.no_grad()
-    def update_route_bias(self) -> None:
+    def update_route_bias(self, updated: Optional[torch.Tensor] = None) -> None:
         """Move the experts' selection biases by the loads since the last call (``moe_bias_rate``), those of every
-        data-parallel rank: one all-reduce for all layers."""
+        data-parallel rank: one all-reduce for all layers.  ``updated`` (a device bool): where it is false the biases stay
+        and the loads are dropped, as the optimizer dropped the gradients."""
         import torch.distributed as dist
         moes = [layer.moe for layer in self.layers if getattr(layer, "moe", None) is not None and layer.moe.bias_rate]
         if not moes:
@@ -147,7 +148,7 @@ class LitGPT(RefModule):
             else:
                 dist.all_reduce(loads)
         for m, load in zip(moes, loads):
-            m.move_route_bias(load)
+            m.move_route_bias(load, updated)
 
     def logits(self, ids: torch.Tensor) -> torch.Tensor:
         x, _ = self.hidden(ids)

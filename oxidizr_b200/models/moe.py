@@ -26,6 +26,8 @@ token dispatch/combine goes through :mod:`oxidizr_b200.parallel.ep`.
 """
 from __future__ import annotations
 
+from typing import Optional
+
 import torch
 import torch.nn.functional as F
 from torch import nn
@@ -181,9 +183,13 @@ class MoE(RefModule):
         return resid + y, aux
 
     @torch.no_grad()
-    def move_route_bias(self, load: torch.Tensor) -> None:
-        """bias_e += rate * sign(mean load - load_e); then the loads start again.  No host synchronisation."""
-        self.route_bias.add_(torch.sign(load.mean() - load), alpha=self.bias_rate)
+    def move_route_bias(self, load: torch.Tensor, updated: Optional[torch.Tensor] = None) -> None:
+        """bias_e += rate * sign(mean load - load_e) (where ``updated``); then the loads start again.  No host
+        synchronisation."""
+        move = torch.sign(load.mean() - load)
+        if updated is not None:
+            move = torch.where(updated, move, torch.zeros_like(move))
+        self.route_bias.add_(move, alpha=self.bias_rate)
         self.route_load.zero_()
 
     # ------------------------------------------------------------ names

@@ -183,6 +183,11 @@ class AdamW:
     def grad_norm_tensor(self) -> torch.Tensor:
         return self._norm
 
+    def updated(self) -> torch.Tensor:
+        """Whether the last step moved the weights, as a device bool [1]: a non-finite gradient norm (or an
+        expert-parallel layer over its capacity) skips the update and leaves a NaN coefficient."""
+        return torch.isfinite(self._coef)
+
     def step(self, grad_scale: float = 1.0) -> torch.Tensor:
         """One update; returns the pre-clip global grad norm as a device scalar."""
         f, c = self.flat, self.cfg
@@ -217,6 +222,7 @@ class AdamW:
             self._norm.copy_(nrm.reshape(1))
             if not bool(torch.isfinite(nrm)):
                 # as on the device: a non-finite gradient norm skips the update
+                self._coef.fill_(float("nan"))
                 f.zero_grad()
                 if self.local is not None:
                     self.local.flat.zero_grad()
@@ -224,6 +230,7 @@ class AdamW:
             coef = 1.0
             if c.max_grad_norm and nrm.item() > c.max_grad_norm:
                 coef = c.max_grad_norm / (nrm.item() + 1e-6)
+            self._coef.fill_(coef * grad_scale)
             g = g * coef
             if self.local is not None:
                 self.local.update(torch.tensor(coef * grad_scale, dtype=torch.float32), t)

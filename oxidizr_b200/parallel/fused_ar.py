@@ -261,6 +261,10 @@ class ShardedDDPAdamW:
     def lr(self) -> float:
         return self.cfg.lr
 
+    def updated(self) -> torch.Tensor:
+        """Whether the last step moved the weights (a device bool [1]); a skipped update leaves a NaN coefficient."""
+        return torch.isfinite(self._coef)
+
     def _skip_word(self):
         """Expert-parallel over-capacity flag of this step (skips the update), if any."""
         if self.local is None:

@@ -156,7 +156,8 @@ class Trainer:
         with nvtx_range("optimizer"):
             gnorm = self.opt.step()
         if self.cfg.model.moe_bias_rate:
-            self.model.update_route_bias()
+            # a step that the optimizer skipped moves no bias either; no host sync
+            self.model.update_route_bias(self.opt.updated() if hasattr(self.opt, "updated") else None)
         return total_ce / accum, gnorm
 
     def _graph_step(self, batches):

@@ -147,3 +147,45 @@ def test_ranks_move_the_bias_by_their_common_load(tmp_path):
     for x, y, u, v in zip(l0, l1, b0, b1):
         total = x + y
         assert torch.equal(u, v) and torch.equal(u, 0.01 * torch.sign(total.mean() - total))
+
+
+class Batches:
+    def __init__(self, row, copies=2):
+        self.row, self.copies = row, copies
+
+    def next_batch(self):
+        return self.row[:, :-1].expand(self.copies, -1), self.row[:, 1:].expand(self.copies, -1)
+
+
+def trainer_of(cfg, model, opt, row):
+    from oxidizr_b200.trainer import Trainer
+    t = Trainer.__new__(Trainer)
+    t.cfg, t.tc, t.model, t.opt, t.loader = cfg, cfg.trainer, model, opt, Batches(row)
+    t.device, t.rank, t.world_size, t.global_step, t.cuda_graph = torch.device("cpu"), 0, 1, 0, False
+    return t
+
+
+def test_a_skipped_step_moves_no_bias():
+    """A gradient that is not finite: the optimizer leaves the weights, and the biases stay with them."""
+    from oxidizr_b200.optim import AdamW, AdamWConfig, FlatParams
+    cfg = config(**OPTIONS)
+    model = build_model(cfg.model, seed=5)
+    opt = AdamW(FlatParams(list(model.named_parameters()), "cpu"), AdamWConfig(lr=1e-3))
+    t = trainer_of(cfg, model, opt, packed(3)[1])
+    t.training_step()
+    assert bool(opt.updated())
+    biases = [layer.moe.route_bias.clone() for layer in model.layers]
+    assert any(b.any() for b in biases)
+    weights = opt.flat.flat.clone()
+    head = model.lm_head.detach().clone()
+    with torch.no_grad():
+        model.lm_head[5] = float("nan")
+    _, norm = t.training_step()
+    assert not torch.isfinite(norm) and not bool(opt.updated())
+    for layer, b in zip(model.layers, biases):
+        assert torch.equal(layer.moe.route_bias, b) and not layer.moe.route_load.any()
+    with torch.no_grad():
+        model.lm_head.copy_(head)
+    assert torch.equal(opt.flat.flat, weights)
+    t.training_step()
+    assert bool(opt.updated()) and any(not torch.equal(layer.moe.route_bias, b) for layer, b in zip(model.layers, biases))

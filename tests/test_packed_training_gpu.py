@@ -118,3 +118,49 @@ def test_captured_step():
     # (a near tie in the choice may fall the other way after those: the biases agree but for single steps of it)
     a, b = eager.layers[0].moe.route_bias, model.layers[0].moe.route_bias
     assert (a != 0).any() and (a - b).abs().max() <= 4 * 2 * 1e-3
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_skipped_step_moves_no_bias(captured):
+    """A gradient norm that is not finite skips the update on the device; the selection biases stay too, with no host sync."""
+    from oxidizr_b200.optim import AdamW, AdamWConfig, FlatParams
+    model = build_model(config(), device="cuda", seed=3)
+    opt = AdamW(FlatParams(list(model.named_parameters()), "cuda"), AdamWConfig(lr=1e-3))
+    ids = batch(5)
+
+    def train():
+        loss, aux = model(ids[:, :-1], ids[:, 1:])
+        (loss.float() + 0.01 * torch.stack([a.float() for a in aux]).mean()).backward()
+        opt.step()
+        model.update_route_bias(opt.updated())
+
+    run = train
+    if captured:
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            train()
+            train()
+        torch.cuda.current_stream().wait_stream(s)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            train()
+        run = graph.replay
+    run()
+    torch.cuda.synchronize()
+    assert bool(opt.updated())
+    biases = [layer.moe.route_bias.clone() for layer in model.layers]
+    keep = model.norm.weight.detach().clone()
+    with torch.no_grad():
+        model.norm.weight.fill_(float("nan"))
+    run()
+    torch.cuda.synchronize()
+    assert not bool(opt.updated())
+    for layer, b in zip(model.layers, biases):
+        assert b.any() and torch.equal(layer.moe.route_bias, b) and not layer.moe.route_load.any()
+    with torch.no_grad():
+        model.norm.weight.copy_(keep)
+    run()
+    torch.cuda.synchronize()
+    assert bool(opt.updated())
+    assert any(not torch.equal(layer.moe.route_bias, b) for layer, b in zip(model.layers, biases))

@@ -23,7 +23,8 @@ unknown keys): ``num_shared_experts``, ``init_std``, ``seed``, ``compat``,
   ``-2^(-8 (h + 1) / heads) |i - j|`` on the scores of head h;
 * ``moe_score`` (``softmax`` / ``sigmoid``), ``moe_groups`` / ``moe_top_groups``, ``moe_renorm``,
   ``moe_route_scale``: routing (``ops.api.route_topk``); ``moe_bias_rate``: a selection bias per expert that
-  moves by this much a step towards balance.
+  moves by this much a step towards balance (a checkpoint without biases starts them at zero; one with biases keeps
+  them, where they were, in a config without the rate).
 
 They are NOT part of the model-config hash, so a config without them hashes exactly like upstream.
 """

@@ -106,9 +106,10 @@ class MoE(RefModule):
             ("score", cfg.moe_score), ("groups", cfg.moe_groups), ("top_groups", cfg.moe_top_groups or cfg.moe_groups),
             ("renorm", cfg.moe_renorm), ("scale", cfg.moe_route_scale)) if v is not None}
         self.bias_rate = float(cfg.moe_bias_rate or 0.0)
+        # the selection bias (without a rate: none, or that of a checkpoint, which stays), and the tokens each expert got
+        # since it last moved
+        self.register_buffer("route_bias", torch.zeros(self.E, dtype=torch.float32, device=device) if self.bias_rate else None)
         if self.bias_rate:
-            # the selection bias, and the tokens each expert got since it last moved
-            self.register_buffer("route_bias", torch.zeros(self.E, dtype=torch.float32, device=device))
             self.register_buffer("route_load", torch.zeros(self.E, dtype=torch.float32, device=device), persistent=False)
         self.n_shared = cfg.n_shared_experts
         self.shared = SwiGLU(H, self.n_shared * self.I, device, dtype) if self.n_shared > 0 else None
@@ -151,7 +152,7 @@ class MoE(RefModule):
         B, S, H = h.shape
         x = h.reshape(-1, H)
         logits = api.linear(x, self.router)
-        options = dict(self.route_options, bias=self.route_bias) if self.bias_rate else self.route_options
+        options = self.route_options if self.route_bias is None else dict(self.route_options, bias=self.route_bias)
         topi, topw, aux, counts = route_with_aux(logits, self.k, self.E, self.aux_kind, **options)
         if self.bias_rate and torch.is_grad_enabled():
             self.route_load.add_(counts)
@@ -195,7 +196,7 @@ class MoE(RefModule):
     # ------------------------------------------------------------ names
     def export_ref(self, prefix, out):
         out[prefix + "router.gate.weight"] = self.router.detach()
-        if self.bias_rate:
+        if self.route_bias is not None:
             out[prefix + "router.selection_bias"] = self.route_bias.detach()
         base = self.ep_rank * self.E_local
         for e in range(self.E_local):
@@ -209,8 +210,16 @@ class MoE(RefModule):
 
     def import_ref(self, prefix, sd):
         _assign(self.router, sd, prefix + "router.gate.weight")
-        if self.bias_rate:
-            _assign(self.route_bias, sd, prefix + "router.selection_bias")
+        key = prefix + "router.selection_bias"
+        if key in sd:
+            # a model routes as it was trained to, whether its biases move on or not
+            if self.route_bias is None:
+                self.route_bias = torch.zeros(self.E, dtype=torch.float32, device=self.router.device)
+            _assign(self.route_bias, sd, key)
+        elif self.bias_rate:
+            self.route_bias.zero_()  # trained without: they start where a new model's do
+        else:
+            self.route_bias = None
         base = self.ep_rank * self.E_local
         with torch.no_grad():
             for e in range(self.E_local):

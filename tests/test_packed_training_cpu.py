@@ -189,3 +189,36 @@ def test_a_skipped_step_moves_no_bias():
     assert torch.equal(opt.flat.flat, weights)
     t.training_step()
     assert bool(opt.updated()) and any(not torch.equal(layer.moe.route_bias, b) for layer, b in zip(model.layers, biases))
+
+
+def test_selection_biases_and_checkpoints():
+    """The option is turned on in a run that began without it, and off in one that had it: the first starts from zero
+    biases, the second goes on routing with those it has."""
+    plain, moving = config(**{**OPTIONS, "moe_bias_rate": None}), config(**OPTIONS)
+    old = build_model(plain.model, seed=7)
+    assert not any("selection_bias" in k for k in old.export_ref())
+    new = build_model(moving.model, seed=8)
+    with torch.no_grad():
+        new.layers[0].moe.route_bias.fill_(9.0)
+    new.import_ref(old.export_ref())
+    _, row = packed(4)
+    assert not new.layers[0].moe.route_bias.any()
+    # (zero biases choose by s where none choose by the logits: the same order, and all else is the same)
+    assert torch.equal(new.logits(row), old.logits(row))
+    with torch.no_grad():
+        for layer in new.layers:
+            layer.moe.route_bias.copy_(torch.linspace(-1, 1, 8))
+    want = new.logits(row)
+    assert not torch.equal(want, old.logits(row))
+    old.import_ref(new.export_ref())
+    assert torch.equal(old.logits(row), want)
+    loss, _ = old(row[:, :-1], row[:, 1:])
+    loss.backward()
+    old.update_route_bias()
+    assert torch.equal(old.layers[0].moe.route_bias, torch.linspace(-1, 1, 8))  # they stay
+    again = build_model(plain.model, seed=9)
+    again.import_ref(old.export_ref())  # and go into the next checkpoint
+    assert torch.equal(again.logits(row), want)
+    new = build_model(plain.model, seed=7)
+    again.import_ref(new.export_ref())
+    assert again.layers[0].moe.route_bias is None

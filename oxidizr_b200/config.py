@@ -380,6 +380,12 @@ class LitConfig:
             raise ConfigError(f"moe_score must be softmax or sigmoid, got {m.moe_score!r}")
         if m.moe_bias_rate is not None and not 0 <= m.moe_bias_rate < math.inf:
             raise ConfigError(f"moe_bias_rate must not be negative, got {m.moe_bias_rate}")
+        for name in ("embed_scale", "moe_route_scale"):
+            if getattr(m, name) is not None and not math.isfinite(getattr(m, name)):
+                raise ConfigError(f"{name} must be a finite number, got {getattr(m, name)}")
+        for name in ("moe_groups", "moe_top_groups"):
+            if getattr(m, name) is not None and getattr(m, name) < 1:
+                raise ConfigError(f"{name} must be at least 1, got {getattr(m, name)}")
         if m.num_experts is not None and m.experts_per_tok is not None and (m.moe_groups or m.moe_top_groups):
             groups, top = m.moe_groups or 1, m.moe_top_groups or m.moe_groups or 1
             if m.num_experts % groups or not 1 <= top <= groups:

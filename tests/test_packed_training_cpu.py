@@ -222,3 +222,13 @@ def test_selection_biases_and_checkpoints():
     new = build_model(plain.model, seed=7)
     again.import_ref(new.export_ref())
     assert again.layers[0].moe.route_bias is None
+
+
+@pytest.mark.parametrize("bad,match", [
+    (dict(moe_groups=0), "moe_groups"), (dict(moe_groups=-2), "moe_groups"), (dict(moe_groups=4, moe_top_groups=0), "moe_top_groups"),
+    (dict(moe_top_groups=0), "moe_top_groups"), (dict(moe_route_scale=float("nan")), "moe_route_scale"),
+    (dict(moe_route_scale=float("inf")), "moe_route_scale"), (dict(embed_scale=float("nan")), "embed_scale"),
+    (dict(embed_scale=-float("inf")), "embed_scale")])
+def test_config_refuses_what_the_first_forward_would_fail_on(bad, match):
+    with pytest.raises(ConfigError, match=match):
+        config(**bad)

@@ -1564,7 +1564,32 @@ struct RouterTopK : torch::autograd::Function<RouterTopK> {
     return r;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    return first_order_only(gradients(ctx, grads), "routing");
+    return at::GradMode::is_enabled() ? recorded(ctx, grads) : gradients(ctx, grads);
+  }
+  // A gradient that may be differentiated: the same formulas in operations that record theirs, for the choice as it is.
+  static variable_list recorded(AutogradContext* ctx, const variable_list& grads) {
+    const auto t = ctx->get_saved_variables();
+    variable_list out(9), outputs, d_outputs;
+    const auto x = t[0].to(torch::kFloat32);
+    const bool sigmoid = ctx->saved_data["sigmoid"].toBool();
+    // (not the library's sigmoid, whose derivative s (1 - s) is rounding alone where s is close to 1)
+    const auto s = sigmoid ? torch::exp(torch::log_sigmoid(x)) : torch::softmax(x, -1);
+    if (grads[1].defined()) {
+      auto w = s.gather(1, t[1]);
+      if (ctx->saved_data["renorm"].toBool()) {
+        const auto n = w.sum(-1, true), some = n.gt(0);
+        w = torch::where(some, w / torch::where(some, n, torch::ones_like(n)), torch::zeros_like(w));
+      }
+      outputs.push_back(w * ctx->saved_data["scale"].toDouble());
+      d_outputs.push_back(grads[1].to(torch::kFloat32));
+    }
+    if (grads[2].defined() && x.size(0) > 0) {
+      outputs.push_back((s / s.sum(-1, true)).mean(0));
+      d_outputs.push_back(grads[2].to(torch::kFloat32));
+    }
+    out[0] = outputs.empty() ? torch::zeros_like(t[0])
+                             : torch::autograd::grad(outputs, {t[0]}, d_outputs, /*retain_graph=*/true, /*create_graph=*/true)[0];
+    return out;
   }
   static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     at::AutoDispatchBelowADInplaceOrView below;

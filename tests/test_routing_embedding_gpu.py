@@ -478,3 +478,31 @@ def test_embedding_differentiated_twice(T):
     n = int(torch.bincount(ids, minlength=V).max())
     assert ((got.double() - want).abs() <= (2 * n + 24) * F32 * want.abs()).all()
     finish()
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,k,renorm", [(8, 2, True), (300, 20, True), (300, 20, False)])
+def test_routing_differentiated_twice(E, k, renorm, score):
+    """A penalty on the router's gradient, differentiated by the logits and by what came back."""
+    T = 33
+    g = torch.Generator(device="cuda").manual_seed(E)
+    x, dw, du = (torch.randn(*s, generator=g, device="cuda") for s in ((T, E), (T, k), (E,)))
+
+    def second(route, x, dw, du):
+        x, dw, du = (t.clone().requires_grad_(True) for t in (x, dw, du))
+        topi, topw, usage, _ = route(x * 1.0)
+        (dx,) = torch.autograd.grad((topw, usage), x, (dw, du), create_graph=True)
+        return [dx.detach(), *torch.autograd.grad((dx * dx).sum(), (x, dw, du))]
+
+    kw = dict(score=score, renorm=renorm, scale=1.5)
+    got = second(lambda v: api.route_topk(v, k, **kw), x, dw, du)
+    want = second(lambda v: R.route_topk(v, k, score, None, 1, 1, 2, renorm, 1.5), *(t.double() for t in (x, dw, du)))
+    for a, b in zip(got, want):
+        # f32 sums of E terms and their derivatives, in the 2-norm
+        assert (a.double() - b).norm() <= (E + 64) * F32 * b.norm()
+    # the gradient that is recorded is the one that is not
+    leaf = x.clone().requires_grad_(True)
+    out = api.route_topk(leaf, k, **kw)
+    (plain,) = torch.autograd.grad((out[1], out[2]), leaf, (dw, du))
+    assert (plain - got[0]).norm() <= (E + 64) * F32 * plain.norm()
+    finish()

@@ -198,7 +198,8 @@ def attention(q, k, v, scale: float, causal: bool = True, mask=None, softcap: fl
     from .doc_attention import attention as _doc, takes_plain
     if mask is None and not softcap and alibi is None:
         same = k.dtype == v.dtype == q.dtype and k.shape == (*q.shape[:2], k.shape[2], q.shape[3]) and v.shape[:3] == k.shape[:3]
-        if not (same and takes_plain(q, q.shape[2], k.shape[2], q.shape[3], v.shape[3], scale)):
+        train = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+        if not (same and takes_plain(q, q.shape[2], k.shape[2], q.shape[3], v.shape[3], scale, causal, train)):
             from .attention import attention as _att
             return _att(q, k, v, scale, causal)
     return _doc(q, k, v, scale, causal, mask, softcap or 0.0, alibi)
@@ -208,7 +209,8 @@ def attention_qkv(qkv, Hq: int, Hk: int, D: int, scale: float, causal: bool = Tr
                   alibi=None):
     """``attention`` from the fused [B, S, (Hq + 2 Hk) D] projection; returns [B, S, Hq D]."""
     from .doc_attention import attention_qkv as _doc, takes_plain
-    if mask is None and not softcap and alibi is None and not takes_plain(qkv, Hq, Hk, D, D, scale):
+    if mask is None and not softcap and alibi is None and not takes_plain(
+            qkv, Hq, Hk, D, D, scale, causal, torch.is_grad_enabled() and qkv.requires_grad):
         from .attention import attention_qkv as _aq
         return _aq(qkv, Hq, Hk, D, scale, causal)
     return _doc(qkv, Hq, Hk, D, scale, causal, mask, softcap or 0.0, alibi)

@@ -78,14 +78,28 @@ def _kernel_ok(t, Dqk: int, Dv: int) -> bool:
             and Dv % 8 == 0)
 
 
-def takes_plain(t, Hq: int, Hk: int, Dqk: int, Dv: int, scale: float) -> bool:
-    """Plain attention of [B, S, ...] operands of t's type, causal or not, goes to these kernels wherever they take its
-    shapes: they are faster than csrc/flash_attn.cu at every length (forward and backward of 8 x 2048 tokens, 16 query
-    and 4 key heads of 128: 151 and 518 us, there 188 and 745; of 4 x 64 tokens 12 and 58 us, there 25 and 80), add no
-    gradient with atomics, and keep more of dQ and dK in short rows (off by 0.3 % for 2 tokens, there 0.45 %)."""
+# Rows of up to this many tokens, by head widths: (causal, both ways)
+_FLASH_ROWS = {(64, 64): (384, 200), (96, 64): (256, 200), (128, 64): (200, 128), (128, 128): (200, 128)}
+_FLASH_CTAS = 10 * 148
+
+
+def takes_plain(t, Hq: int, Hk: int, Dqk: int, Dv: int, scale: float, causal: bool, train: bool) -> bool:
+    """Whether plain attention of [B, S, ...] operands of t's type goes to these kernels rather than to
+    csrc/flash_attn.cu (of the widths in _FLASH_ROWS) or PyTorch.
+
+    They are the faster ones but for many short rows: forward and backward of 8 x 2048 tokens, 16 query and 8 key heads of
+    128, 658 us, there 890; of 12 x 1000 tokens, 16 heads of 64, 341 and 363; but of 192 x 64 tokens 298 and 239, of
+    61 x 200 265 and 224, of 32 x 384 241 and 228, because a CTA of the two backward kernels takes 4 us to start and end,
+    and such rows give it little to do between.  Few such CTAs, under ten times the SMs, take less than the host
+    needs for the call, which is a third less here (89 and 133 us).  Without a gradient the two differ below 64 tokens:
+    768 x 16 take 189 and 173 us.  These kernels add no gradient with atomics, and keep more of dQ and dK in short
+    rows (off by 0.3 % for 2 tokens, there 0.45 %; one token alone gets the exact zeros that it has here)."""
     B, S = t.shape[:2]
-    return (scale > 0 and S > 0 and 0 < Hk <= Hq <= 65535 and Hq % Hk == 0 and 0 < B <= 65535
-            and _kernel_ok(t, Dqk, Dv))
+    if not (scale > 0 and S > 0 and 0 < Hk <= Hq <= 65535 and Hq % Hk == 0 and 0 < B <= 65535 and _kernel_ok(t, Dqk, Dv)):
+        return False
+    rows = _FLASH_ROWS.get((Dqk, Dv))
+    short = rows is not None and 1 < S <= ((rows[0] if causal else rows[1]) if train else 64)
+    return not (short and B * Hq * ((S + 127) // 128) >= _FLASH_CTAS)
 
 
 def _check(t, B, S, Hq, scale, causal, mask, softcap, alibi):

@@ -542,3 +542,33 @@ def test_two_streams_at_once():
         for x, y in zip(r, want[i % 2]):
             assert torch.equal(x, y)
     finish()
+
+
+@pytest.mark.parametrize("D,Dv,S,causal", [(64, 64, 16, True), (64, 64, 300, True), (64, 64, 130, False), (96, 64, 64, True),
+                                           (128, 64, 100, True), (128, 128, 128, False)])
+def test_many_short_rows(D, Dv, S, causal):
+    """Plain attention whose rows are too short for the backward's CTAs runs the kernels that are faster there: the same
+    mathematics on either side of the rule's border."""
+    from oxidizr_b200.ops.doc_attention import takes_plain
+    H, B = 8, -(-10 * 148 // (8 * ((S + 127) // 128)))
+    q, k, v, do = inputs(B, S, H, H, D, Dv, seed=S)
+    scale = D ** -0.5
+    many = (H, H, D, Dv, scale, causal, True)
+    assert not takes_plain(q, *many) and takes_plain(q[1:], *many)
+    assert takes_plain(q, *many[:-1], False) == (S > 64)
+    lo = torch.zeros(B, S, dtype=torch.int64, device="cuda")
+    hi = torch.arange(1, S + 1, device="cuda").expand(B, S) if causal else torch.full((B, S), S, device="cuda")
+    for first in (0, 1):
+        x = [t[first:] for t in (q, k, v, do)]
+        got = run(*x, scale, causal=causal)
+        check(got, oracle(*x, scale, type("M", (), {"lo": lo[first:], "hi": hi[first:]}), 0.0, None))
+        if D == Dv:
+            qkv = torch.cat([t.flatten(2) for t in x[:3]], -1).requires_grad_()
+            o = api.attention_qkv(qkv, H, H, D, scale, causal=causal)
+            g, = torch.autograd.grad(o, qkv, x[3].flatten(2))
+            assert torch.equal(o, got[0].flatten(2))
+            check([*(t.unflatten(2, (H, D)) for t in g.split(H * D, -1))], oracle(
+                *x, scale, type("M", (), {"lo": lo[first:], "hi": hi[first:]}), 0.0, None)[1:])
+    with torch.no_grad():
+        check([api.attention(q, k, v, scale, causal=causal)], oracle(q, k, v, do, scale, type("M", (), {"lo": lo, "hi": hi}), 0.0, None))
+    finish()

@@ -572,3 +572,19 @@ def test_many_short_rows(D, Dv, S, causal):
     with torch.no_grad():
         check([api.attention(q, k, v, scale, causal=causal)], oracle(q, k, v, do, scale, type("M", (), {"lo": lo, "hi": hi}), 0.0, None))
     finish()
+
+
+@pytest.mark.parametrize("D,Dv,Hq,Hk", [(96, 64, 3, 3), (128, 64, 4, 1), (128, 128, 4, 2), (40, 32, 2, 2), (64, 128, 2, 1)])
+@pytest.mark.parametrize("mean,cap,alibi", [(3, 0.0, False), (12, 20.0, True), (100, 0.0, True), (700, 50.0, False)])
+def test_sharp_scores_keep_the_gradients_at_every_width(D, Dv, Hq, Hk, mean, cap, alibi):
+    """In the 2-norm, as above: delta from the two-part output (from o as it is rounded, dQ would be off by 1.5 x 2^-8)."""
+    B, S = 2, 700
+    q, k, v, do = inputs(B, S, Hq, Hk, D, Dv, seed=D + mean, sharp=2.0 * (64 / D) ** 0.25)
+    slopes = torch.tensor([0.3, 0.05, 0.01, 0.0], device="cuda")[:Hq] if alibi else None
+    m = api.document_mask(layout(B, S, mean, mean, pad=False)[0])
+    got = run(q, k, v, do, D ** -0.5, mask=m, softcap=cap, alibi=slopes)
+    want = oracle(q, k, v, do, D ** -0.5, m, cap, slopes)
+    check(got, want)
+    for name, x, (y, _) in zip(("o", "dq", "dk", "dv"), got, want):
+        assert (x.double() - y).norm() <= HALF * y.norm(), name
+    finish()

@@ -232,3 +232,48 @@ def test_selection_biases_and_checkpoints():
 def test_config_refuses_what_the_first_forward_would_fail_on(bad, match):
     with pytest.raises(ConfigError, match=match):
         config(**bad)
+
+
+def _expert_rank(rank, store, out):
+    import torch.distributed as dist
+    from oxidizr_b200.models.moe import MoE
+    dist.init_process_group("gloo", init_method=f"file://{store}", rank=rank, world_size=2)
+    worst = 0.0
+    for options in (OPTIONS, dict(OPTIONS, moe_score="softmax", moe_renorm=False, moe_groups=2, moe_top_groups=1)):
+        cfg = config(**options).model
+        sharded, whole = MoE(cfg, "cpu", torch.float64, ep_group=dist.group.WORLD), MoE(cfg, "cpu", torch.float64)
+        for m in (sharded, whole):
+            m.reset_parameters(0.3, torch.Generator().manual_seed(11))
+            m.route_bias.copy_(torch.linspace(-0.3, 0.3, 8))
+        g = torch.Generator().manual_seed(20 + rank)
+        x, resid, dy = (torch.randn(1, 37, 32, generator=g, dtype=torch.float64) for _ in range(3))
+        leaves = [x.clone().requires_grad_(True) for _ in range(2)]
+        for m, leaf in zip((sharded, whole), leaves):
+            y, aux = m(leaf, resid)
+            ((y * dy).sum() + aux).backward()
+            m.result = y.detach()
+        for p in (whole.w_gu, whole.w_down):  # an expert's gradient is the sum over the ranks that send it tokens
+            dist.all_reduce(p.grad)
+        mine = slice(4 * rank, 4 * rank + 4)
+        for a, b in ((sharded.result, whole.result), (leaves[0].grad, leaves[1].grad), (sharded.router.grad, whole.router.grad),
+                     (sharded.w_gu.grad, whole.w_gu.grad[mine]), (sharded.w_down.grad, whole.w_down.grad[mine]),
+                     (sharded.route_load, whole.route_load)):
+            worst = max(worst, float((a - b).abs().max() / b.abs().max()))
+        loads = [m.route_load.clone() for m in (sharded,)]
+        dist.all_reduce(loads[0])
+        sharded.move_route_bias(loads[0])
+        biases = [torch.zeros(8) for _ in range(2)]
+        dist.all_gather(biases, sharded.route_bias.float())
+        assert torch.equal(*biases) and not torch.equal(biases[0], whole.route_bias.float())
+    torch.save(worst, f"{out}.{rank}")
+    dist.destroy_process_group()
+
+
+def test_routing_options_with_experts_on_two_ranks(tmp_path):
+    """Grouped, biased and scaled routing in the sharded layer and in the whole one: sums of the same terms in 64 bits but
+    for the weights, which both take from the same f32 router."""
+    import torch.multiprocessing as mp
+    out = str(tmp_path / "out")
+    mp.start_processes(_expert_rank, args=(str(tmp_path / "store"), out), nprocs=2, start_method="spawn")
+    for r in range(2):
+        assert torch.load(f"{out}.{r}") < 1e-6

@@ -164,3 +164,22 @@ def test_a_skipped_step_moves_no_bias(captured):
     torch.cuda.synchronize()
     assert bool(opt.updated())
     assert any(not torch.equal(layer.moe.route_bias, b) for layer, b in zip(model.layers, biases))
+
+
+@pytest.mark.parametrize("kind", [{}, LATENT])
+def test_gradients_outside_the_experts_are_near_the_stated_math(kind):
+    """The bound that twenty roundings to bf16 in a row give, 20 x 2^-8 of a gradient's norm: of the parameters that every
+    token passes through, whose gradients a changed choice of experts (4 of 600 tokens) reaches through a residual."""
+    model = build_model(config(**kind), device="cuda", seed=2)
+    wide = build_model(config(dtype="f32", **kind), seed=2)
+    wide.import_ref({k: v.float().cpu() for k, v in model.export_ref().items()})
+    ids = batch(1)
+    grads, ref = step(model, ids)[1], step(wide, ids.cpu())[1]
+    seen = 0
+    for n, g in grads.items():
+        if ".moe." not in n:
+            r = ref[n].cuda()
+            assert (g.float() - r).norm() <= 20 * 2 ** -8 * r.norm(), (n, ((g.float() - r).norm() / r.norm()).item())
+            seen += 1
+    assert seen >= 8
+    torch.cuda.synchronize()

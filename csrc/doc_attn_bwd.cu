@@ -12,15 +12,19 @@
 // the softmax warps over the scores they were computed from.
 //
 // What bounds them: the products of a dQ step (128 queries x 64 keys, 128-wide heads) take 788 clocks, of a dK / dV
-// step 1044, and the softmax warps' instructions about as long; the two overlap through the alternating groups.  One
+// step 1310 (S and dP have their A operand in shared memory there), and the softmax warps' instructions about as
+// long; the two overlap through the alternating groups.  dK / dV keeps to 96 registers, which the 18 warps leave a
+// thread, and spills 16 to 172 bytes for it, most under a cap.  One
 // dense causal row of 8192 tokens, 16 / 4 heads of 128: dQ 369 us (1118 TFLOP/s of its own three products), dK and dV
 // 481 us (1143 of its four); with a cap of 50, whose tanh and derivative are instructions, 480 and 556 us; heads of 64:
 // 286 and 393 us (16 / 16 heads).  8 x 2048 tokens in documents of 700, capped: 241 and 230 us.  16 x 1024 tokens in
-// documents of 300, heads of 96 and 64: 104 and 113 us, half of it a CTA's start and end (4 us, one CTA a SM).
+// documents of 300, heads of 96 and 64: 104 and 112 us, 40 % of it starts and ends of CTAs (4 of 10 us, one CTA a SM): of
+// rows as short as that without a mask, many at a time, flash_attn.cu's backward is the faster one.
 // Tried and no faster: dK / dV's CTAs started under dQ's last wave (a programmatic launch).
 //
 // P and dS are rounded to bf16 for the tensor cores (2^-8 of each term at most, with random signs over the keys of a
-// row); statistics, delta and accumulators are f32.
+// row); statistics, delta and accumulators are f32.  The gradients are 0.23 to 0.24 % off in the 2-norm, where products of
+// f32 and one rounding of the result to bf16 leave 0.166 %.
 // delta is formed in the dQ kernel, from o.  Where one key has most of a row's weight, dP - delta is what
 // two nearly equal numbers leave, so an error of delta counts many times: with o rounded to bf16, dQ was
 // 0.6 % off (2-norm) for documents of a few tokens with sharp scores, where the roundings of dS and dQ make
@@ -686,6 +690,7 @@ __global__ void __launch_bounds__(DA_GROUPS_THREADS, 1)
       }
       tmem_st16(s_addr, pk);
       if (padded) {
+        // (dP^T may still be reading dO: only the columns of padded queries can differ, and those are not used)
         if (!mbar_wait(&q_full[st], u & 1, abort_flag, p.status)) { ok = false; break; }
         zero_pad_rows<L::KBV, KV_QUERIES>(sDO + st * L::DO_BYTES, p, b, q0, half * 128 + r, 256);
         zero_pad_rows<L::KBQ, KV_QUERIES>(sQ + st * L::Q_BYTES, p, b, q0, half * 128 + r, 256);

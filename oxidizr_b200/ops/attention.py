@@ -1,7 +1,9 @@
 """Causal attention entry points.
 
-CUDA: the sm_100a flash-attention kernels (``csrc/flash_attn.cu``) when built;
-CPU: the materialised reference (model.rs:362-377).
+What ``ops.doc_attention.takes_plain`` does not take.  CUDA: the sm_100a flash-attention kernels
+(``csrc/flash_attn.cu``) for head widths of 64, 96 / 64, 128 / 64 and 128 (many short rows), PyTorch's attention for
+widths past 128, for those that are not multiples of 8 and for other types; CPU: the materialised reference
+(model.rs:362-377).
 Layout: q/k [B, S, H, Dqk], v [B, S, Hk, Dv] (GQA when Hk < Hq; Dqk > Dv for
 multi-head latent attention), output [B, S, Hq, Dv].
 """
@@ -46,7 +48,7 @@ def attention_cuda(q, k, v, scale: float, causal: bool = True):
     if native_ok(q.shape[-1], v.shape[-1]) and q.dtype == torch.bfloat16:
         from .flash import FlashAttention
         return FlashAttention.apply(q, k, v, scale, causal)
-    # library attention, used only until the native kernel is present
+    # widths and types that no kernel here takes
     out = torch.nn.functional.scaled_dot_product_attention(
         q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=causal, scale=scale,
         enable_gqa=k.shape[2] != q.shape[2])

@@ -93,6 +93,7 @@ __global__ void __launch_bounds__(FA_THREADS, 2)
   uint64_t* v_full = bars + 7;    // [3]
   uint64_t* v_empty = bars + 10;  // [3]
   uint64_t* s_full = bars + 13;   // [2]
+  uint64_t* o_done = bars + 15;   // the last PV
   uint64_t* p_full = bars + 17;
   uint64_t* pv_done = bars + 18;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
@@ -123,6 +124,7 @@ __global__ void __launch_bounds__(FA_THREADS, 2)
     for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1);
     mbar_init(p_full, 8);
     mbar_init(pv_done, 1);
+    mbar_init(o_done, 1);
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
@@ -211,6 +213,7 @@ __global__ void __launch_bounds__(FA_THREADS, 2)
                         (j | kk) != 0);
         tc_commit(pv_done);
         tc_commit(&v_empty[vs]);
+        if (j + 1 == nk) tc_commit(o_done);
       }
     }
     __syncwarp();
@@ -285,8 +288,8 @@ __global__ void __launch_bounds__(FA_THREADS, 2)
       const bool rescale_warp = __any_sync(0xffffffffu, move && j > 0);
       m = m_new;
       if (j > 0 && rescale_warp) {
-        // O is owned by the previous PV MMA until it completes (PV_j cannot have
-        // completed yet, so the parity wait cannot skip a phase)
+        // O is owned by the previous PV MMA until it completes.  The parity can only mean that one: PV_j has not been
+        // issued, and S_j, which is complete, was issued behind PV_{j-2}
         if (!mbar_wait(pv_done, (j - 1) & 1, abort_flag, p.status)) {
           ok = false;
           continue;
@@ -326,7 +329,9 @@ __global__ void __launch_bounds__(FA_THREADS, 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(p_full);
     }
-    if (ok && !mbar_wait(pv_done, (nk - 1) & 1, abort_flag, p.status)) ok = false;
+    // a barrier of its own: while the last PV but one is still running, pv_done's parity is that of the one before it,
+    // and a wait for the last would end at once
+    if (ok && !mbar_wait(o_done, 0, abort_flag, p.status)) ok = false;
     s_lsum[half * 128 + r] = l;
     asm volatile("bar.sync 1, 256;" ::: "memory");  // reached by every softmax warp
     if (ok) {

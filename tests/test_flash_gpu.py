@@ -168,3 +168,26 @@ def test_attention_rope_fused_backward(hd, B, S, Hq, Hk, H):
     for name, sl in (("q", slice(0, Hq * hd)), ("k", slice(Hq * hd, (Hq + Hk) * hd)), ("v", slice((Hq + Hk) * hd, N))):
         e = _rel(w.grad[sl], wr.grad[sl])
         assert e < 3e-2, (name, e)
+
+
+@pytest.mark.parametrize("D,Dv", [(64, 64), (96, 64), (128, 64), (128, 128)])
+@pytest.mark.parametrize("B,S", [(185, 128), (92, 256), (46, 512)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_forward_repeats_itself_under_load(B, S, D, Dv, causal):
+    """Two CTAs an SM and few key tiles each: the output waits for the last product, whatever the other CTA does to the
+    one before it."""
+    from oxidizr_b200.ops.flash import FlashAttention
+    g = torch.Generator(device="cuda").manual_seed(B)
+    q, k, v = (torch.randn(B, S, 8, d, generator=g, device="cuda").bfloat16() for d in (D, D, Dv))
+    with torch.no_grad():
+        first = FlashAttention.apply(q, k, v, D ** -0.5, causal)
+        for _ in range(40):
+            assert torch.equal(FlashAttention.apply(q, k, v, D ** -0.5, causal), first)
+    s = torch.einsum("bihd,bjhd->bhij", q.double(), k.double()) * D ** -0.5
+    if causal:
+        s = s.masked_fill(torch.ones(S, S, device="cuda", dtype=torch.bool).triu(1), float("-inf"))
+    p = torch.softmax(s, -1)
+    want, size = torch.einsum("bhij,bjhd->bihd", p, v.double()), torch.einsum("bhij,bjhd->bihd", p, v.double().abs())
+    # the weights and the output rounded to bf16, their sum not: 2^-8 of the terms twice and of the value, 2^-11 for f32
+    assert ((first.double() - want).abs() <= 2.0 ** -8 * want.abs() + (2.0 ** -7 + 2.0 ** -11) * size).all()
+    torch.cuda.synchronize()

@@ -504,7 +504,7 @@ int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 template <typename TI, typename TO, int N, bool ACC>
 void launch_reduce(const int2* pair, const void* dy, void* dw, float* part, int T, int V, int H,
                    float scale, cudaStream_t st) {
-  const int64_t blocks = (T + EB_ROWS - 1) / EB_ROWS;
+  const int64_t blocks = ((int64_t)T + EB_ROWS - 1) / EB_ROWS;
   const dim3 grid((unsigned)((blocks + 7) / 8), (unsigned)((H + 32 * N - 1) / (32 * N)));
   embedding_reduce_kernel<TI, TO, N, ACC><<<grid, 256, 0, st>>>(pair, reinterpret_cast<const TI*>(dy),
                                                                 reinterpret_cast<TO*>(dw), part, T, V, H, scale);

@@ -199,7 +199,7 @@ def attention(q, k, v, scale: float, causal: bool = True, mask=None, softcap: fl
     if mask is None and not softcap and alibi is None:
         same = k.dtype == v.dtype == q.dtype and k.shape == (*q.shape[:2], k.shape[2], q.shape[3]) and v.shape[:3] == k.shape[:3]
         train = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
-        if not (same and takes_plain(q, q.shape[2], k.shape[2], q.shape[3], v.shape[3], scale, causal, train)):
+        if not (same and takes_plain(q, q.shape[2], k.shape[2], q.shape[3], v.shape[3], scale, causal, train, (k, v))):
             from .attention import attention as _att
             return _att(q, k, v, scale, causal)
     return _doc(q, k, v, scale, causal, mask, softcap or 0.0, alibi)

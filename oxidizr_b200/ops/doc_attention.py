@@ -83,8 +83,14 @@ _FLASH_ROWS = {(64, 64): (384, 200), (96, 64): (256, 200), (128, 64): (200, 128)
 _FLASH_CTAS = 10 * 148
 
 
-def takes_plain(t, Hq: int, Hk: int, Dqk: int, Dv: int, scale: float, causal: bool, train: bool) -> bool:
-    """Whether plain attention of [B, S, ...] operands of t's type goes to these kernels rather than to
+def _flash_layout(t) -> bool:
+    """Rows that csrc/flash_attn.cu's tensor maps can address, as they are or copied; these kernels' operands are copied
+    wherever they need be."""
+    return t.data_ptr() % 16 == 0 and t.stride(-1) == 1 and all(s % 8 == 0 for s in t.stride()[:-1])
+
+
+def takes_plain(t, Hq: int, Hk: int, Dqk: int, Dv: int, scale: float, causal: bool, train: bool, others=()) -> bool:
+    """Whether plain attention of [B, S, ...] operands of t's type (t and the others) goes to these kernels rather than to
     csrc/flash_attn.cu (of the widths in _FLASH_ROWS) or PyTorch.
 
     They are the faster ones but for many short rows: forward and backward of 8 x 2048 tokens, 16 query and 8 key heads of
@@ -99,7 +105,7 @@ def takes_plain(t, Hq: int, Hk: int, Dqk: int, Dv: int, scale: float, causal: bo
         return False
     rows = _FLASH_ROWS.get((Dqk, Dv))
     short = rows is not None and 1 < S <= ((rows[0] if causal else rows[1]) if train else 64)
-    return not (short and B * Hq * ((S + 127) // 128) >= _FLASH_CTAS)
+    return not (short and B * Hq * ((S + 127) // 128) >= _FLASH_CTAS and all(map(_flash_layout, (t, *others))))
 
 
 def _check(t, B, S, Hq, scale, causal, mask, softcap, alibi):

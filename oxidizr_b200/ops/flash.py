@@ -23,6 +23,20 @@ def _fwd(q2, k2, v2, B, S, Hq, Hk, D, scale, causal, Dv=None):
     return o, lse
 
 
+def _first_order_only(*grads):
+    """Gradients that are recorded (create_graph) raise when they are differentiated."""
+    if not torch.is_grad_enabled():
+        return grads
+    return [torch._C._functions.DelayedError(b"attention has first derivatives only", 1)(g.detach().requires_grad_())
+            for g in grads]
+
+
+def _rows(t):
+    """Rows that a tensor map can address: contiguous, from a multiple of 16 bytes on."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _bwd(q2, k2, v2, o, lse, do2, dq, dk, dv, B, S, Hq, Hk, D, scale, causal, Dv=None, rope=None):
     """rope = (cos, sin) tables: q and k were rotate-half RoPE outputs and dq / dk come
     back as the gradients of the unrotated q and k."""
@@ -51,14 +65,12 @@ class FlashAttentionQKV(torch.autograd.Function):
     def backward(ctx, do):
         qkv2, o, lse = ctx.saved_tensors
         B, S, Hq, Hk, D, scale, causal = ctx.cfg
-        do2 = do.reshape(B * S, Hq * D)
-        if not do2.is_contiguous():
-            do2 = do2.contiguous()
+        do2 = _rows(do.reshape(B * S, Hq * D))
         dqkv = torch.empty_like(qkv2)
         q2, k2, v2 = qkv2[:, :Hq * D], qkv2[:, Hq * D:(Hq + Hk) * D], qkv2[:, (Hq + Hk) * D:]
         _bwd(q2, k2, v2, o, lse, do2, dqkv[:, :Hq * D], dqkv[:, Hq * D:(Hq + Hk) * D], dqkv[:, (Hq + Hk) * D:],
              B, S, Hq, Hk, D, scale, causal)
-        return dqkv.view(B, S, -1), None, None, None, None, None
+        return *_first_order_only(dqkv.view(B, S, -1)), None, None, None, None, None
 
 
 class FlashAttention(torch.autograd.Function):
@@ -80,9 +92,9 @@ class FlashAttention(torch.autograd.Function):
     def backward(ctx, do):
         q2, k2, v2, o, lse = ctx.saved_tensors
         B, S, Hq, Hk, D, Dv, scale, causal = ctx.cfg
-        do2 = do.reshape(B * S, Hq * Dv).contiguous()
+        do2 = _rows(do.reshape(B * S, Hq * Dv))
         dq = torch.empty(B * S, Hq * D, dtype=q2.dtype, device=q2.device)
         dk = torch.empty(B * S, Hk * D, dtype=q2.dtype, device=q2.device)
         dv = torch.empty(B * S, Hk * Dv, dtype=q2.dtype, device=q2.device)
         _bwd(q2, k2, v2, o, lse, do2, dq, dk, dv, B, S, Hq, Hk, D, scale, causal, Dv)
-        return dq.view(B, S, Hq, D), dk.view(B, S, Hk, D), dv.view(B, S, Hk, Dv), None, None
+        return *_first_order_only(dq.view(B, S, Hq, D), dk.view(B, S, Hk, D), dv.view(B, S, Hk, Dv)), None, None

@@ -588,3 +588,43 @@ def test_sharp_scores_keep_the_gradients_at_every_width(D, Dv, Hq, Hk, mean, cap
     for name, x, (y, _) in zip(("o", "dq", "dk", "dv"), got, want):
         assert (x.double() - y).norm() <= HALF * y.norm(), name
     finish()
+
+
+@pytest.mark.parametrize("S,D", [(2, 64), (3, 128), (40, 64)])
+def test_many_short_rows_of_any_layout(S, D):
+    """Operands and gradients off the alignment, of odd strides and expanded: on either side of the rule's border, as
+    without it.  Second derivatives are refused by both."""
+    H = 8
+    for B in (200, 30):
+        q, k, v, do = inputs(B, S, H, H, D, D, seed=S)
+        scale = D ** -0.5
+        want = run(q, k, v, do, scale)
+        hi = torch.arange(1, S + 1, device="cuda").expand(B, S)
+        m = type("M", (), {"lo": torch.zeros_like(hi), "hi": hi})
+        ref = oracle(q, k, v, do, scale, m, 0.0, None)
+        check(want, ref)
+
+        def off(t, by):
+            buf = torch.empty(t.numel() + by, dtype=t.dtype, device="cuda")
+            buf[by:].copy_(t.reshape(-1))
+            return buf[by:].view(t.shape)
+
+        check(run(off(q, 3), k, v, do, scale), ref)
+        check(run(q, k, v, off(do, 1), scale), ref)
+        wide = torch.zeros(B, S, H, D + 1, device="cuda").bfloat16()
+        wide[..., :D] = v
+        check(run(q, k, wide[..., :D], do, scale), ref)
+        heads = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v)]
+        check(run(*heads, do, scale), ref)
+        qkv = off(torch.cat([t.flatten(2) for t in (q, k, v)], -1), 5).requires_grad_()
+        o = api.attention_qkv(qkv, H, H, D, scale)
+        (g,) = torch.autograd.grad(o, qkv, off(do.flatten(2), 7))
+        check([o.unflatten(2, (H, D)), *(t.unflatten(2, (H, D)) for t in g.split(H * D, -1))], ref)
+        leaf = q.detach().requires_grad_(True)
+        one = torch.ones((), device="cuda", dtype=torch.bfloat16).expand(B, S, H, D)
+        (g,) = torch.autograd.grad(api.attention(leaf, k, v, scale), leaf, one)
+        check([g], [oracle(q, k, v, one, scale, m, 0.0, None)[1]])
+        (g,) = torch.autograd.grad(api.attention(leaf, k, v, scale), leaf, do, create_graph=True)
+        with pytest.raises(RuntimeError, match="first derivatives|once_differentiable"):
+            g.float().sum().backward()
+    finish()

@@ -1549,13 +1549,13 @@ variable_list EmbeddingLookup::backward(AutogradContext* ctx, variable_list grad
 }
 
 struct RouterTopK : torch::autograd::Function<RouterTopK> {
+  static torch::Tensor rows(const torch::Tensor& t) { return t.dim() == 2 && t.stride(1) == 1 ? t : t.contiguous(); }
   static variable_list forward(AutogradContext* ctx, const torch::Tensor& logits_, int64_t k, bool sigmoid,
                                const c10::optional<torch::Tensor>& bias, int64_t groups, int64_t top_groups,
                                int64_t group_top, bool renorm, double scale) {
     at::AutoDispatchBelowADInplaceOrView below;  // nothing here is recorded
-    const auto logits = logits_.dim() == 2 && logits_.stride(1) == 1 ? logits_ : logits_.contiguous();
-    auto r = router_fwd(logits, k, sigmoid, bias, groups, top_groups, group_top, renorm, scale);
-    ctx->save_for_backward({logits, r[0]});
+    auto r = router_fwd(rows(logits_), k, sigmoid, bias, groups, top_groups, group_top, renorm, scale);
+    ctx->save_for_backward({logits_, r[0]});
     ctx->saved_data["sigmoid"] = sigmoid;
     ctx->saved_data["renorm"] = renorm;
     ctx->saved_data["scale"] = scale;
@@ -1598,7 +1598,7 @@ struct RouterTopK : torch::autograd::Function<RouterTopK> {
     auto dtopw = grads[1].defined() ? grads[1].to(torch::kFloat32).contiguous() : torch::zeros(t[1].sizes(), f32);
     auto du = grads[2].defined() ? grads[2].to(torch::kFloat32).contiguous() : torch::Tensor();
     ++g_node_backwards;
-    auto dx = router_bwd(t[0], t[1], dtopw, maybe(du), ctx->saved_data["sigmoid"].toBool(),
+    auto dx = router_bwd(rows(t[0]), t[1], dtopw, maybe(du), ctx->saved_data["sigmoid"].toBool(),
                          ctx->saved_data["renorm"].toBool(), ctx->saved_data["scale"].toDouble());
     variable_list out(9);
     out[0] = dx;

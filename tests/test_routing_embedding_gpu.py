@@ -506,3 +506,21 @@ def test_routing_differentiated_twice(E, k, renorm, score):
     (plain,) = torch.autograd.grad((out[1], out[2]), leaf, (dw, du))
     assert (plain - got[0]).norm() <= (E + 64) * F32 * plain.norm()
     finish()
+
+
+def test_routing_of_other_layouts_differentiated_twice():
+    """Logits whose rows are not contiguous, which the kernel takes as a copy."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x, dw = torch.randn(12, 30, generator=g, device="cuda"), torch.randn(30, 3, generator=g, device="cuda")
+
+    def second(x, route):
+        x = x.clone().requires_grad_(True)
+        w = route(x.t())[1]
+        (dx,) = torch.autograd.grad(w, x, dw.to(x.dtype), create_graph=True)
+        return dx.detach(), torch.autograd.grad((dx * dx).sum(), x)[0]
+
+    got = second(x, lambda v: api.route_topk(v, 3, "sigmoid"))
+    want = second(x.double(), lambda v: R.route_topk(v, 3, "sigmoid"))
+    for a, b in zip(got, want):
+        assert (a.double() - b).norm() <= 80 * F32 * b.norm()
+    finish()

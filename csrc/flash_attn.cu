@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(FA_THREADS, 2)
       for (int kb = 0; kb < KBQ; ++kb) tma_load_2d(sQ + kb * FA_BM * 128, &tmQ, q_full, h * DQ + kb * 64, row0 + q0);
       // K_j runs ahead of V_j: K stages free up when S_j completes, V stages
       // when PV_j completes, so K loads are issued as early as possible.
-      int jv = 0;
+      int jk = 0, jv = 0;  // tiles asked for
       for (int j = 0; j < nk && ok; ++j) {
         const int ks = j % L::KST, ku = j / L::KST;
         if (!mbar_wait(&k_empty[ks], (ku & 1) ^ 1, abort_flag, p.status)) { ok = false; break; }
@@ -158,6 +158,7 @@ __global__ void __launch_bounds__(FA_THREADS, 2)
         for (int kb = 0; kb < KBQ; ++kb)
           tma_load_2d(sK + ks * L::K_BYTES + kb * FA_BNF * 128, &tmK, &k_full[ks], hk * DQ + kb * 64,
                       row0 + j * FA_BNF);
+        jk = j + 1;
         // issue every V load whose stage is already free (never more than one behind K)
         while (jv <= j) {
           const int vs = jv % L::VST, vu = jv / L::VST;
@@ -171,9 +172,13 @@ __global__ void __launch_bounds__(FA_THREADS, 2)
           ++jv;
         }
       }
-      // drain: wait for every copy issued to land before leaving
+      // after a failed wait: leave no copy in flight into shared memory
       if (!ok) {
         mbar_wait(q_full, 0, nullptr, p.status);
+        for (int j = max(0, jk - L::KST); j < jk; ++j)
+          mbar_wait(&k_full[j % L::KST], (j / L::KST) & 1, nullptr, p.status);
+        for (int j = max(0, jv - L::VST); j < jv; ++j)
+          mbar_wait(&v_full[j % L::VST], (j / L::VST) & 1, nullptr, p.status);
       }
     }
     __syncwarp();

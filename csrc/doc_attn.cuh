@@ -4,7 +4,6 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
-#include <atomic>
 #include <climits>
 
 #include "gemm_kernel.cuh"
@@ -357,17 +356,6 @@ inline void da_check(const DaShape& s) {
   OXI_CHECK(s.B <= 65535 && s.Hq <= 65535, "batch and heads of at most 65535");
   OXI_CHECK((s.lo != nullptr) == (s.hi != nullptr) && (s.lo != nullptr) == (s.qt != nullptr) &&
                 (s.lo != nullptr) == (s.kt != nullptr), "ranges and tile tables come together");
-}
-
-// Shared memory attribute of a kernel, set once for each device that launches it.
-template <typename K>
-inline void da_smem(K kern, int bytes, std::atomic<uint64_t>& devices) {
-  int dev;
-  OXI_CUDA_CHECK(cudaGetDevice(&dev));
-  const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
-  if (devices.load(std::memory_order_relaxed) & bit) return;
-  OXI_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  devices.fetch_or(bit, std::memory_order_relaxed);
 }
 
 }  // namespace

@@ -843,8 +843,8 @@ void launch_bwd_t(const BwdArgs& a) {
   auto kq = da_dq_kernel<DQP, DVP, CAP, ALIBI>;
   auto kkv = da_dkv_kernel<DQP, DVP, CAP, ALIBI>;
   static std::atomic<uint64_t> dq_devices{0}, dkv_devices{0};
-  da_smem(kq, DaDqSmem<DQP, DVP>::TOTAL, dq_devices);
-  da_smem(kkv, DaDkvSmem<DQP, DVP>::TOTAL, dkv_devices);
+  set_smem_once(kq, DaDqSmem<DQP, DVP>::TOTAL, dq_devices);
+  set_smem_once(kkv, DaDkvSmem<DQP, DVP>::TOTAL, dkv_devices);
   kq<<<dim3(s.Hq, s.B, p.nt), DA_GROUPS_THREADS, DaDqSmem<DQP, DVP>::TOTAL, a.st>>>(tq, tk64, tv64, td, tdq, p, a.o, a.o_lo,
                                                                                     a.nlse2, a.ndelta);
   OXI_CUDA_CHECK(cudaGetLastError());

@@ -352,7 +352,7 @@ void launch_fwd_t(const DaShape& s, const DaTensor& q, const DaTensor& k, const 
                     tlo = o_lo.ptr ? da_tmap_out(o_lo, s.B, s.S, s.Hq, s.Dv) : to;
   auto kern = da_fwd_kernel<DQP, DVP, CAP, ALIBI>;
   static std::atomic<uint64_t> devices{0};
-  da_smem(kern, L::TOTAL, devices);
+  set_smem_once(kern, L::TOTAL, devices);
   const dim3 grid(s.Hq, s.B, (s.S + DA_TILE - 1) / DA_TILE);
   kern<<<grid, FW_THREADS, L::TOTAL, st>>>(tq, tk, tv, to, tlo, da_params(s, status), nlse2, o_lo.ptr != nullptr);
   OXI_CUDA_CHECK(cudaGetLastError());

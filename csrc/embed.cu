@@ -535,7 +535,8 @@ void launch_sort(const int64_t* ids, int64_t T, int64_t V, int2* pair, int2* scr
   int ctas = 1;
   while (ctas < ES_MAX_CTAS && (int64_t)ctas * ES_THREADS < T) ctas *= 2;
   const int smem = (ES_WARPS * (ES_DIGITS + 1) + 2 * ES_DIGITS) * (int)sizeof(int);
-  OXI_CUDA_CHECK(cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  static std::atomic<uint64_t> devices{0};
+  set_smem_once(embedding_sort_kernel, smem, devices);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(ES_THREADS);

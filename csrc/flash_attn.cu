@@ -393,11 +393,8 @@ void launch_fa_fwd_t(const void* q, int64_t ldq, const void* k, int64_t ldk, con
   p.lse = lse;
   p.status = status;
   auto kern = fa_fwd_kernel<DQ, DV>;
-  static bool attr = false;
-  if (!attr) {
-    OXI_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
-    attr = true;
-  }
+  static std::atomic<uint64_t> devices{0};
+  set_smem_once(kern, L::TOTAL, devices);
   dim3 grid(Hq, B, (S + FA_BM - 1) / FA_BM);
   kern<<<grid, FA_THREADS, L::TOTAL, st>>>(tq, tk, tv, p);
   OXI_CUDA_CHECK(cudaGetLastError());
@@ -948,11 +945,8 @@ void launch_fa_bwd_t(const void* q, int64_t ldq, const void* k, int64_t ldk, con
   p.rope_sin = rope_sin;
   p.status = status;
   auto kern = fa_bwd_kernel<DQ, DV>;
-  static bool attr = false;
-  if (!attr) {
-    OXI_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::TOTAL));
-    attr = true;
-  }
+  static std::atomic<uint64_t> devices{0};
+  set_smem_once(kern, L::TOTAL, devices);
   dim3 grid(Hk, B, (S + 127) / 128);
   kern<<<grid, FA_BWD_THREADS, L::TOTAL, st>>>(tq, tk, tv, tdo, tdq, p);
   OXI_CUDA_CHECK(cudaGetLastError());

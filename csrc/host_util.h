@@ -1,6 +1,8 @@
 // Host-side error helpers shared by the torch-free launchers.
 #pragma once
 #include <cuda_runtime.h>
+#include <atomic>
+#include <cstdint>
 #include <cstdio>
 #include <type_traits>
 #include <stdexcept>
@@ -55,3 +57,16 @@ template <typename... Args>
     cudaError_t _e = (expr);                                                                        \
     if (_e != cudaSuccess) ::oxi::fail(__FILE__, __LINE__, "CUDA error: ", cudaGetErrorString(_e)); \
   } while (0)
+
+namespace oxi {
+// Shared memory attribute of a kernel, set once for each device that launches it (a bit of `devices` each).
+template <typename K>
+inline void set_smem_once(K kern, int bytes, std::atomic<uint64_t>& devices) {
+  int dev;
+  OXI_CUDA_CHECK(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
+  if (devices.load(std::memory_order_relaxed) & bit) return;
+  OXI_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  devices.fetch_or(bit, std::memory_order_relaxed);
+}
+}  // namespace oxi

@@ -97,8 +97,8 @@ class _EmbeddingMainGrad(torch.autograd.Function):
 
 
 class Embedding:
-    """w[ids] * scale; the gradient sums each row's tokens in f32 in their order, by sorting them
-    (csrc/embed.cu), so it is the same from run to run.  Without ``main_grad`` on w the node is the one in
+    """w[ids] * scale; the gradient sums each row's tokens in f32, in stretches whose order the ids and their number
+    decide (csrc/embed.cu), so it is the same from run to run.  Without ``main_grad`` on w the node is the one in
     csrc/ops.cpp."""
 
     @staticmethod
